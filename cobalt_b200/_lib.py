@@ -48,7 +48,7 @@ class CobaltStagedInput(Structure):
 
 
 IN_PLAIN, IN_GLU, IN_ADDNORM = 0, 1, 2
-EUNSUPPORTED = -7
+ETIMEOUT, EUNSUPPORTED = -5, -7
 
 
 class CobaltError(RuntimeError):
@@ -109,6 +109,14 @@ EXPORTS = {
     "cobalt_attn_decode_fused": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_int, c_int, c_int,
                                          c_int, c_int, c_float, c_int, c_int64, c_void_p]),
     "cobalt_attn_decode_fused_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "cobalt_kv4_tile_bytes": (c_size_t, [c_int]),
+    "cobalt_kv4_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                  c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p]),
+    "cobalt_kv4_read": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "cobalt_kv4_attend_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "cobalt_kv4_attend": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                  c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    "cobalt_kv4_status": (c_int, [c_void_p, POINTER(c_uint32)]),
     "cobalt_allreduce_peer": (c_int, [c_void_p, c_int, c_int, c_size_t, c_size_t, c_size_t, c_void_p, c_int, c_void_p,
                                       c_void_p]),
     "cobalt_device_status": (c_int, [c_void_p, c_void_p, POINTER(c_uint32)]),

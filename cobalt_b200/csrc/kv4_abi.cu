@@ -1,0 +1,151 @@
+// C ABI of the 4-bit KV cache: argument validation and launches.  See include/cobalt_b200.h.
+#include "kv4_kernels.cuh"
+
+using namespace cb;
+
+namespace {
+
+constexpr int MAX_DEVICES = 64;
+
+int sm_count(int* n) {
+    static int sms[MAX_DEVICES], major[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
+    if (dev < 0 || dev >= MAX_DEVICES) return COBALT_EINVAL;
+    if (!sms[dev]) {
+        if (cudaDeviceGetAttribute(&major[dev], cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return COBALT_ELAUNCH;
+        int count = 0;
+        if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return COBALT_ELAUNCH;
+        sms[dev] = count;
+    }
+    if (major[dev] != 10) return COBALT_EARCH;
+    *n = sms[dev];
+    return COBALT_OK;
+}
+// the status word of the current device (part of the library's image: nothing is allocated)
+uint32_t* status_word() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, g_kv4_status) == cudaSuccess ? (uint32_t*)p : nullptr;
+}
+int launched() { return cudaGetLastError() == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH; }
+bool dim_ok(int D) { return D > 0 && D % KV4_GROUP == 0 && D <= KV4_GROUP * KV4_MAX_GROUPS; }
+
+// The cache of a call, or why it cannot be one.  Rows (tokens of all sequences) are a grid dimension and an int in the kernels.
+int make_cache(Kv4Cache* c, const void* tiles, int64_t seq_stride, const int64_t* positions, int64_t pos_stride, int n_seq, int T, int n_kv, int D,
+               int n_slots) {
+    if (!tiles || !positions || ((uintptr_t)tiles & 15) || ((uintptr_t)positions & 7) || pos_stride < 0) return COBALT_EINVAL;
+    if (n_seq <= 0 || T <= 0 || n_kv <= 0 || n_slots <= 0 || !dim_ok(D)) return COBALT_EINVAL;
+    if ((int64_t)n_seq * T > 0x3FFFFFFFll || n_kv > 0xFFFF || n_slots > 0x3FFFFFFF) return COBALT_ETOOBIG;
+    c->n_kv = n_kv;
+    c->n_slots = n_slots;
+    c->n_tiles = (n_slots + KV4_TILE - 1) / KV4_TILE;
+    const int64_t one = (int64_t)n_kv * c->n_tiles * kv4_tile_bytes(D / KV4_GROUP);
+    if (seq_stride < 0 || (seq_stride & 15) || (n_seq > 1 && seq_stride < one)) return COBALT_EINVAL;
+    c->tiles = (uint8_t*)const_cast<void*>(tiles);
+    c->seq_stride = seq_stride;
+    return COBALT_OK;
+}
+// rows of bf16 that are read four bytes at a time
+bool rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 3) && !(ld & 1) && ld >= width; }
+
+}  // namespace
+
+#define KV4_DISPATCH(D, CALL)                    \
+    switch ((D) / KV4_GROUP) {                   \
+        case 1: { constexpr int G = 1; CALL; } break; \
+        case 2: { constexpr int G = 2; CALL; } break; \
+        case 3: { constexpr int G = 3; CALL; } break; \
+        default: { constexpr int G = 4; CALL; } break; \
+    }
+
+extern "C" {
+
+size_t cobalt_kv4_tile_bytes(int head_dim) { return dim_ok(head_dim) ? (size_t)kv4_tile_bytes(head_dim / KV4_GROUP) : 0; }
+
+int cobalt_kv4_append(const void* k, int64_t ld_k, const void* v, int64_t ld_v, const void* q, int64_t ld_q, void* q_out, int64_t ld_q_out,
+                      const int64_t* positions, int64_t pos_seq_stride, void* tiles, int64_t tiles_seq_stride, int n_seq, int T, int n_heads,
+                      int n_kv_heads, int head_dim, int n_slots, const float* inv_freq, const void* q_norm_w, const void* k_norm_w, float eps,
+                      void* stream) {
+    Kv4AppendParams P = {};
+    int rc = make_cache(&P.cache, tiles, tiles_seq_stride, positions, pos_seq_stride, n_seq, T, n_kv_heads, head_dim, n_slots);
+    if (rc) return rc;
+    if (!rows_ok(k, ld_k, (int64_t)n_kv_heads * head_dim) || !rows_ok(v, ld_v, (int64_t)n_kv_heads * head_dim)) return COBALT_EINVAL;
+    if (q && (n_heads <= 0 || !rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !rows_ok(q_out, ld_q_out, (int64_t)n_heads * head_dim))) return COBALT_EINVAL;
+    if (q_norm_w && !q) return COBALT_EINVAL;
+    if (((uintptr_t)inv_freq | (uintptr_t)q_norm_w | (uintptr_t)k_norm_w) & 3) return COBALT_EINVAL;
+    int sms = 0;
+    if ((rc = sm_count(&sms))) return rc;
+    P.k = (const uint16_t*)k; P.v = (const uint16_t*)v; P.q = (const uint16_t*)q; P.q_out = (uint16_t*)q_out;
+    P.ld_k = ld_k; P.ld_v = ld_v; P.ld_q = ld_q; P.ld_qo = ld_q_out;
+    P.positions = (const long long*)positions;
+    P.pos_stride = pos_seq_stride;
+    P.T = T; P.n_heads = q ? n_heads : 0;
+    P.inv_freq = inv_freq;
+    P.q_norm = (const uint16_t*)q_norm_w; P.k_norm = (const uint16_t*)k_norm_w;
+    P.eps = eps;
+    const int rows = n_seq * T, items = 2 * n_kv_heads + P.n_heads, warps = KV4_THREADS / 32;
+    // few rows: the heads of a row are spread over blocks until the GPU has about two blocks per SM
+    const int most = (items + warps - 1) / warps, want = (2 * sms + rows - 1) / rows;
+    const dim3 grid((unsigned)rows, (unsigned)(want < most ? want : most));
+    KV4_DISPATCH(head_dim, (kv4_append_kernel<G><<<grid, KV4_THREADS, 0, (cudaStream_t)stream>>>(P)));
+    return launched();
+}
+
+int cobalt_kv4_read(const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride, void* k, void* v, int n_seq,
+                    int T, int n_kv_heads, int head_dim, int n_slots, void* stream) {
+    Kv4Cache C;
+    int rc = make_cache(&C, tiles, tiles_seq_stride, positions, pos_seq_stride, n_seq, T, n_kv_heads, head_dim, n_slots);
+    if (rc) return rc;
+    if (!k || !v || (((uintptr_t)k | (uintptr_t)v) & 3)) return COBALT_EINVAL;
+    int sms = 0;
+    if ((rc = sm_count(&sms))) return rc;
+    const long long items = (long long)n_seq * T * n_kv_heads, blocks = (items + KV4_THREADS / 32 - 1) / (KV4_THREADS / 32);
+    if (blocks > 0x7FFFFFFFll) return COBALT_ETOOBIG;
+    KV4_DISPATCH(head_dim, (kv4_read_kernel<G><<<(unsigned)blocks, KV4_THREADS, 0, (cudaStream_t)stream>>>(
+                               C, (const long long*)positions, pos_seq_stride, T, items, (uint16_t*)k, (uint16_t*)v)));
+    return launched();
+}
+
+size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots) {
+    (void)n_seq; (void)T; (void)n_heads; (void)n_kv_heads; (void)head_dim; (void)n_slots;
+    return 0;
+}
+
+int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
+                      void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks, float scale,
+                      void* scratch, size_t scratch_bytes, void* stream) {
+    Kv4AttendParams P = {};
+    int rc = make_cache(&P.cache, tiles, tiles_seq_stride, positions, pos_seq_stride, n_seq, T, n_kv_heads, head_dim, n_slots);
+    if (rc) return rc;
+    if (n_heads <= 0 || n_heads % n_kv_heads != 0 || window < 0 || sinks < 0) return COBALT_EINVAL;
+    if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
+    (void)scratch; (void)scratch_bytes;
+    int sms = 0;
+    if ((rc = sm_count(&sms))) return rc;
+    P.q = (const uint16_t*)q; P.ld_q = ld_q;
+    P.positions = (const long long*)positions;
+    P.pos_stride = pos_seq_stride;
+    P.out = (uint16_t*)out;
+    P.n_seq = n_seq; P.T = T; P.n_heads = n_heads; P.rep = n_heads / n_kv_heads;
+    P.window = window; P.sinks = sinks;
+    P.scale = scale;
+    const long long items = (long long)n_seq * T * n_heads, blocks = (items + KV4_THREADS / 32 - 1) / (KV4_THREADS / 32);
+    if (blocks > 0x7FFFFFFFll) return COBALT_ETOOBIG;
+    KV4_DISPATCH(head_dim, (kv4_attend_rows_kernel<G><<<(unsigned)blocks, KV4_THREADS, 0, (cudaStream_t)stream>>>(P, items)));
+    return launched();
+}
+
+int cobalt_kv4_status(void* stream, uint32_t* status_out) {
+    if (!status_out) return COBALT_EINVAL;
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc) return rc;
+    uint32_t* word = status_word();
+    if (!word) return COBALT_ELAUNCH;
+    if (cudaMemcpyAsync(status_out, word, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
+    if (cudaMemsetAsync(word, 0, 4, (cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
+    if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
+    return *status_out == 0 ? COBALT_OK : COBALT_ETIMEOUT;
+}
+
+}  // extern "C"

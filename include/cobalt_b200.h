@@ -337,6 +337,44 @@ int cobalt_attn_prompt(const void* q, const void* k_cache, const void* v_cache, 
                        int n_heads, int n_kv_heads, int head_dim, int n_slots, int max_ctx, int window, float scale, int n_seq,
                        int64_t cache_seq_stride, void* status, void* stream);
 
+/* KV cache in 4 bits.  64 neighbouring channels of one slot of one KV head are a group: x = (c - z) * s, codes c in 0..15,
+ * s = bf16((max - min) / 15), z = fp16(-min / s), c = clamp(rint(x / s + z), 0, 15); a constant group takes s = bf16(|min| / 256); a group
+ * with a value that is not finite, or with a range beyond fp32, reads as NaN.  32 slots of one KV head are a tile, one piece of
+ * cobalt_kv4_tile_bytes(head_dim) = 36 * head_dim bytes (0: head_dim is not 64, 128, 192 or 256), G = head_dim / 64:
+ *     K codes [G][32 slots][32 B] (channel 2b in the low half of byte b) | V codes [G][16 slot pairs][8 chunks of 8 channels][2 slots][4 B],
+ *     chunk g of pair p at place g ^ ((p & 2) << 1) | K [32 slots][G] { fp16 zero, bf16 scale } | V scale [32 slots][G] bf16 |
+ *     V zero [G][32 slots] fp16
+ * A cache is [sequence][KV head][ceil(n_slots / 32) tiles], 16-byte aligned, sequences tiles_seq_stride bytes apart (a multiple of 16).
+ * Every byte of a fresh cache is irrelevant: a slot is only read by tokens at or behind its position.
+ *
+ * All calls: n_seq sequences of T tokens, row seq * T + t; positions[seq * pos_seq_stride + t] (pos_seq_stride 0: the same for every
+ * sequence) is read on the device.
+ *   cobalt_kv4_append : k and v [rows] x ld (elements, even; 4-byte aligned), n_kv_heads * head_dim values each, into the slots at
+ *                       their positions (outside [0, n_slots): not stored; the positions of one sequence must differ).  k first gets
+ *                       the per-head norm of cobalt_rope_kv() if k_norm_w is given and its rotation if inv_freq is; so does q (may be NULL) with
+ *                       q_norm_w, into q_out (may be q).  v is stored as it is.
+ *   cobalt_kv4_read   : the slots at the positions, as bf16 [rows][n_kv_heads][head_dim]; a position outside [0, n_slots) reads as zeros.
+ *   cobalt_kv4_attend : grouped-query attention of the tokens (q [rows] x ld_q, rotated) over the cache, out [rows][n_heads * head_dim]
+ *                       (16-byte aligned).  A token at position p sees slot j < n_slots if j <= p and (window == 0 or j > p - window or
+ *                       j < sinks); one that sees none (p < 0: padding) gets zeros.  Scores, softmax and sums in fp32, one rounding
+ *                       at the end.  scratch: cobalt_kv4_attend_scratch_bytes() (0: none needed), 256-byte aligned, contents irrelevant;
+ *                       calls that may overlap on the GPU need buffers of their own.
+ *   cobalt_kv4_status : 0, or the code of the first bounded wait of an attend call on the current device that gave up since the
+ *                       last question (its rows are then not written).  Synchronises `stream`; not during capture.
+ * The reference holds its cache in bf16 and has no counterpart. */
+size_t cobalt_kv4_tile_bytes(int head_dim);
+int cobalt_kv4_append(const void* k, int64_t ld_k, const void* v, int64_t ld_v, const void* q, int64_t ld_q, void* q_out, int64_t ld_q_out,
+                      const int64_t* positions, int64_t pos_seq_stride, void* tiles, int64_t tiles_seq_stride, int n_seq, int T, int n_heads,
+                      int n_kv_heads, int head_dim, int n_slots, const float* inv_freq, const void* q_norm_w, const void* k_norm_w, float eps,
+                      void* stream);
+int cobalt_kv4_read(const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride, void* k, void* v, int n_seq,
+                    int T, int n_kv_heads, int head_dim, int n_slots, void* stream);
+size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots);
+int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
+                      void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks, float scale,
+                      void* scratch, size_t scratch_bytes, void* stream);
+int cobalt_kv4_status(void* stream, uint32_t* status_out);
+
 /* All-reduce (sum) of the fp32 partial outputs of a row-parallel layer over peer memory, for tensor-parallel decode
  * (the reference has no distributed code; this replaces the NCCL all-reduce that would follow cobalt_linear_f32).
  * Every rank owns one symmetric buffer mapped into all processes: [staging: slot_stride bytes][slot 0: world rows of
