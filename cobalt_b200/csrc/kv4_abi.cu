@@ -48,6 +48,54 @@ int make_cache(Kv4Cache* c, const void* tiles, int64_t seq_stride, const int64_t
 // rows of bf16 that are read four bytes at a time
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 3) && !(ld & 1) && ld >= width; }
 
+struct AttendCfg {
+    int cols, nb, col_tiles, grid;
+    size_t joins_off, scratch;
+};
+// Columns are spread evenly over the fewest tiles of 8 * nb that a warp's registers hold; CTAs fill the GPU once, each with a warp's tile
+// of slots per warp at least.
+AttendCfg attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, int sms) {
+    AttendCfg c;
+    const int G = D / KV4_GROUP;
+    c.cols = n_heads / n_kv * T;
+    const int eights = (c.cols + 7) / 8;
+    c.col_tiles = (eights + ka_max_nb(G) - 1) / ka_max_nb(G);
+    c.nb = (eights + c.col_tiles - 1) / c.col_tiles;
+    c.col_tiles = (eights + c.nb - 1) / c.nb;
+    const double tiles = (double)n_seq * c.col_tiles * n_kv * ((n_slots + KV4_TILE - 1) / KV4_TILE);
+    const double most = (double)sms * ka_ctas_per_sm(G, c.nb), need = tiles / KA_MIN_TILES;
+    c.grid = (int)(need < 1 ? 1 : need < most ? need + 0.999 : most);
+    c.joins_off = (size_t)c.grid * 2 * ka_state_floats(G, c.nb) * 128;
+    c.scratch = c.joins_off + (size_t)c.grid * sizeof(int4);
+    return c;
+}
+template <int G, int NB>
+int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c, cudaStream_t st) {
+    static bool configured[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(kv4_attend_kernel<G, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_smem_bytes(G, NB)) != cudaSuccess)
+            return COBALT_ELAUNCH;
+        configured[dev] = true;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)c.grid);
+    cfg.blockDim = dim3(KA_THREADS);
+    cfg.dynamicSmemBytes = ka_smem_bytes(G, NB);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kv4_attend_kernel<G, NB>, P, W) != cudaSuccess) return COBALT_ELAUNCH;
+    cfg.gridDim = dim3((unsigned)c.grid, NB, G);
+    cfg.blockDim = dim3(32 * KC_WARPS);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<G, NB>, P, W) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+}
+
 }  // namespace
 
 #define KV4_DISPATCH(D, CALL)                    \
@@ -107,8 +155,9 @@ int cobalt_kv4_read(const void* tiles, int64_t tiles_seq_stride, const int64_t* 
 }
 
 size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots) {
-    (void)n_seq; (void)T; (void)n_heads; (void)n_kv_heads; (void)head_dim; (void)n_slots;
-    return 0;
+    int sms = 0;
+    if (n_seq <= 0 || T <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_slots <= 0 || !dim_ok(head_dim) || sm_count(&sms)) return 0;
+    return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms).scratch;
 }
 
 int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
@@ -119,20 +168,34 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     if (rc) return rc;
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || window < 0 || sinks < 0) return COBALT_EINVAL;
     if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
-    (void)scratch; (void)scratch_bytes;
+    if ((int64_t)n_heads / n_kv_heads * T > 0x3FFFFFFFll) return COBALT_ETOOBIG;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
+    const AttendCfg c = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms);
+    if ((int64_t)n_seq * c.col_tiles > 0x3FFFFFFFll) return COBALT_ETOOBIG;
+    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < c.scratch) return COBALT_ESCRATCH;
     P.q = (const uint16_t*)q; P.ld_q = ld_q;
     P.positions = (const long long*)positions;
     P.pos_stride = pos_seq_stride;
     P.out = (uint16_t*)out;
     P.n_seq = n_seq; P.T = T; P.n_heads = n_heads; P.rep = n_heads / n_kv_heads;
     P.window = window; P.sinks = sinks;
-    P.scale = scale;
-    const long long items = (long long)n_seq * T * n_heads, blocks = (items + KV4_THREADS / 32 - 1) / (KV4_THREADS / 32);
-    if (blocks > 0x7FFFFFFFll) return COBALT_ETOOBIG;
-    KV4_DISPATCH(head_dim, (kv4_attend_rows_kernel<G><<<(unsigned)blocks, KV4_THREADS, 0, (cudaStream_t)stream>>>(P, items)));
-    return launched();
+    P.scale_log2 = scale * 1.44269504f;
+    Kv4Work W;
+    W.cols = c.cols;
+    W.col_tiles = c.col_tiles;
+    W.partial = (float*)scratch;
+    W.joins = (int4*)((uint8_t*)scratch + c.joins_off);
+    switch (head_dim / KV4_GROUP * 10 + c.nb) {
+        case 11: return launch_attend<1, 1>(P, W, c, (cudaStream_t)stream);
+        case 12: return launch_attend<1, 2>(P, W, c, (cudaStream_t)stream);
+        case 13: return launch_attend<1, 3>(P, W, c, (cudaStream_t)stream);
+        case 14: return launch_attend<1, 4>(P, W, c, (cudaStream_t)stream);
+        case 21: return launch_attend<2, 1>(P, W, c, (cudaStream_t)stream);
+        case 22: return launch_attend<2, 2>(P, W, c, (cudaStream_t)stream);
+        case 31: return launch_attend<3, 1>(P, W, c, (cudaStream_t)stream);
+        default: return launch_attend<4, 1>(P, W, c, (cudaStream_t)stream);
+    }
 }
 
 int cobalt_kv4_status(void* stream, uint32_t* status_out) {

@@ -244,65 +244,594 @@ struct Kv4AttendParams {
     uint16_t* out;                                                     // [n_seq * T][n_heads * D]
     int n_seq, T, n_heads, rep;
     int window, sinks;
-    float scale;
+    float scale_log2;                                                  // scale * log2(e)
 };
 
-// A slot is visible for a token at `pos` if it is not behind it, and inside the window or among the first slots.
-__device__ __forceinline__ bool kv4_visible(long long slot, long long pos, int window, int sinks) {
-    return slot <= pos && (window <= 0 || slot > pos - window || slot < sinks);
+// The slots that a token sees: j <= hi and (j >= lo or j < sinks); hi = -1: none.
+struct Kv4Range { int lo, hi; };
+__device__ __forceinline__ Kv4Range kv4_range(const Kv4AttendParams& P, int seq, int tok) {
+    const long long pos = P.positions[seq * P.pos_stride + tok];
+    Kv4Range r;
+    r.hi = pos < 0 ? -1 : (int)min(pos, (long long)P.cache.n_slots - 1);
+    r.lo = P.window > 0 ? (int)max(0ll, min(pos - P.window + 1, (long long)P.cache.n_slots)) : 0;
+    return r;
+}
+// The tiles that some token of a range sees, in order (i < n_sink: tile i, else first + i - n_sink; at least one, so that a row that
+// sees nothing gets its zeros), and what of a tile needs no mask.
+struct Kv4Tiles {
+    int n, n_sink, first;
+    int hi_max, lo_min, hi_min, lo_max;
+    __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
+};
+__device__ __forceinline__ Kv4Tiles kv4_tiles(const Kv4AttendParams& P, int seq, int tok0, int tok1) {
+    Kv4Tiles e;
+    e.hi_max = -1; e.lo_min = 0x7FFFFFFF; e.hi_min = 0x7FFFFFFF; e.lo_max = 0;
+    for (int t = tok0; t <= tok1; ++t) {
+        const Kv4Range r = kv4_range(P, seq, t);
+        e.hi_max = max(e.hi_max, r.hi);
+        e.hi_min = min(e.hi_min, r.hi);
+        e.lo_max = max(e.lo_max, r.lo);
+        if (r.lo <= r.hi) e.lo_min = min(e.lo_min, r.lo);
+    }
+    const int tiles = (e.hi_max + KV4_TILE) / KV4_TILE;                // of slots 0 .. hi_max
+    e.n_sink = (min(P.sinks, e.hi_max + 1) + KV4_TILE - 1) / KV4_TILE;
+    e.first = e.lo_min > e.hi_max ? tiles : e.lo_min / KV4_TILE;
+    if (e.first <= e.n_sink) e.first = e.n_sink = 0;
+    e.n = max(1, e.n_sink + tiles - e.first);
+    if (e.n_sink + tiles - e.first <= 0) e.first = e.n_sink = 0;
+    return e;
 }
 
-// One warp per (row, query head), one slot at a time; running maximum and sum of exponentials.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ float f16_to_float(uint32_t bits) { return __half2float(__ushort_as_half((uint16_t)bits)); }
+
+// Few rows per KV head (decode, proposed tokens): the columns of a tile product are (token, query head) pairs of one KV head, eight to an
+// n of mma.m16n8k16, and both contractions have the cache as their A operand, so no row of the tensor core is wasted:
+//     S^T [32 slots x 8] = K [32 x D] Q^T,        O^T [D x 8] += V^T [D x 32] P^T.
+// A code is an operand as it is: a nibble in the low bits of a 16-bit float is the subnormal c * 2^-24, exactly, one nibble further up it is
+// 16 times that (the queries' channels, or the result's rows, take the 1/16).  Expanding eight codes is one shift and four ands;
+// scales and zeros never touch a code:
+//     S = sum_g s_g ( sum_{d in g} q c  -  z_g sum_{d in g} q ),        O_g = sum_j (P_j s_jg) c_j  -  sum_j (P_j s_jg) z_jg,
+// the last sum through the tensor core too (z is an fp16 operand), so that both sums carry the same rounded weights: with many
+// slots of nearly equal weight they cancel down to the mean, and a rounding of one alone would show.
+// Queries are scaled by a power of two into the upper range of fp16, which holds every bf16 significand; so are the weights P s, by
+// the largest scale seen so far: fp16 weights (2^-11), everything else fp32.  A running maximum per column, moved only when a score
+// exceeds it by 2^8 (fp16 weights have that room), keeps the rescaling of O out of the loop.
+//
+// A warp owns a ring of tiles, one bulk copy each, and walks every 4th tile of its CTA's range alone.  The list of all (sequence, columns,
+// KV head, tile) is cut into equal ranges, one per CTA, whatever the lengths of the sequences are; a CTA joins its warps' states at
+// the end of every head, and heads that lie in several CTAs are joined by kv4_combine_kernel.
+constexpr int KA_WARPS = 4, KA_THREADS = 32 * KA_WARPS;
+constexpr int KA_STAGES = 2;
+constexpr int KA_MIN_TILES = 4;                                        // per CTA: one per warp
+constexpr int ka_max_nb(int G) { return G == 1 ? 4 : G == 2 ? 2 : 1; } // groups of eight columns a warp holds
+constexpr int ka_ctas_per_sm(int G, int NB) { return NB == 1 ? (G <= 2 ? 4 : G == 3 ? 3 : 2) : G * NB <= 2 ? 3 : 2; }
+constexpr int ka_state_floats(int G, int NB) { return NB * (16 * G + 4); }      // per lane: O, reference and sum of two columns
+constexpr size_t ka_smem_bytes(int G, int NB) {
+    return (size_t)KA_WARPS * KA_STAGES * kv4_tile_bytes(G) + 2 * (size_t)ka_state_floats(G, NB) * 128 + KA_WARPS * KA_STAGES * 8 + 128;
+}
+static_assert(ka_smem_bytes(4, 1) * 2 <= 227 * 1024 - 2048, "at least two CTAs per SM");
+
+struct Kv4Work {
+    int cols, col_tiles;                                               // rep * T columns per KV head, in tiles of 8 * NB
+    float* partial;                                                    // [CTA][2][floats][32 lanes]
+    int4* joins;                                                       // [CTA]: head that begins in this CTA and ends in a later one
+};
+
+// State of a segment (one KV head, one tile of columns): lane (g, t) has columns 2t, 2t + 1 and channels 8g .. 8g + 7 of every group:
+// o[16 G]: group, channel pair m, { channel 2m col 0, 2m col 1, 2m + 1 col 0, 2m + 1 col 1 }; reference and sum of both columns.
+// In memory [4 + 16 G][32 lanes]: references, sums, o.
 template <int G>
-__global__ void __launch_bounds__(KV4_THREADS) kv4_attend_rows_kernel(const Kv4AttendParams P, long long items) {
-    constexpr int D = 64 * G;
-    const long long item = (long long)blockIdx.x * (KV4_THREADS / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (item >= items) return;
-    const long long row = item / P.n_heads;
-    const int head = (int)(item - row * P.n_heads), seq = (int)(row / P.T), t = (int)(row - (long long)seq * P.T);
-    const long long pos = P.positions[seq * P.pos_stride + t];
-    const int last = (int)min(pos, (long long)P.cache.n_slots - 1);
-    bool any = false;
-    float q[G][2], o[G][2];
+struct Kv4State {
+    float o[16 * G], ref[2], sum[2];
+    __device__ __forceinline__ void store(float* p, int lane) const {
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(P.q + row * P.ld_q + (size_t)head * D + 64 * g + 2 * lane);
-        q[g][0] = __uint_as_float(w << 16);
-        q[g][1] = __uint_as_float(w & 0xFFFF0000u);
-        o[g][0] = o[g][1] = 0.0f;
+        for (int c = 0; c < 2; ++c) { p[c * 32 + lane] = ref[c]; p[(2 + c) * 32 + lane] = sum[c]; }
+#pragma unroll
+        for (int i = 0; i < 16 * G; ++i) p[(4 + i) * 32 + lane] = o[i];
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j <= last; ++j) {
-        if (!kv4_visible(j, pos, P.window, P.sinks)) {
-            j = (int)max((long long)j, min((long long)last, pos - P.window));          // on to the window
-            continue;
-        }
-        any = true;
-        const uint8_t* tile = P.cache.tile(seq, head / P.rep, j, G);
-        float x = 0.0f;
+    // p: references and sums, po: values (of G groups out of those in memory)
+    __device__ __forceinline__ void join(const float* p, const float* po, int lane) {
+        float mine[2], other[2];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float2 k = kv4_key(tile, G, g, j % KV4_TILE, lane);
-            x = fmaf(q[g][0], k.x, fmaf(q[g][1], k.y, x));
+        for (int c = 0; c < 2; ++c) {
+            const float r = p[c * 32 + lane], top = fmaxf(ref[c], r), base = top == -INFINITY ? 0.0f : top;
+            mine[c] = ex2(ref[c] - base);
+            other[c] = ex2(r - base);
+            ref[c] = top;
+            sum[c] = sum[c] * mine[c] + p[(2 + c) * 32 + lane] * other[c];
         }
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, s);
-        x *= P.scale;
-        const float nm = fmaxf(m, x), base = nm == -INFINITY ? 0.0f : nm, keep = expf(m - base), p = expf(x - base);
-        m = nm;
-        l = l * keep + p;
+        for (int i = 0; i < 16 * G; ++i) o[i] = o[i] * mine[i & 1] + po[i * 32 + lane] * other[i & 1];
+    }
+    __device__ __forceinline__ void join(const float* p, int lane) { join(p, p + 4 * 32, lane); }
+};
+template <int G>
+__device__ __forceinline__ void kv4_write_out(const Kv4AttendParams& P, const Kv4State<G>& st, int seq, int kvh, int col0, int cols, int D, int first_group, int lane) {
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float2 v = kv4_value(tile, G, g, j % KV4_TILE, lane);
-            o[g][0] = fmaf(p, v.x, o[g][0] * keep);
-            o[g][1] = fmaf(p, v.y, o[g][1] * keep);
+    for (int c = 0; c < 2; ++c) {
+        const int col = col0 + 2 * t + c;
+        if (col >= cols) continue;
+        const int tok = col / P.rep, head = kvh * P.rep + col % P.rep;
+        const Kv4Range r = kv4_range(P, seq, tok);
+        const bool any = r.hi >= 0 && (r.lo <= r.hi || P.sinks > 0);
+        const float inv = 1.0f / st.sum[c];
+        uint16_t* dst = P.out + (((long long)seq * P.T + tok) * P.n_heads + head) * D + 64 * first_group + 8 * g;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            uint32_t w[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) w[m] = any ? pack_bf16x2(st.o[16 * gr + 4 * m + c] * inv, st.o[16 * gr + 4 * m + 2 + c] * inv) : 0u;
+            *reinterpret_cast<uint4*>(dst + 64 * gr) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-    // a row that sees nothing is zero
+}
+
+template <int G, int NB>
+__global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_kernel(const Kv4AttendParams P, const Kv4Work W) {
+    constexpr int D = 64 * G, TILE = kv4_tile_bytes(G);
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint8_t* ring = smem + warp * (KA_STAGES * TILE);
+    float* region = reinterpret_cast<float*>(smem + KA_WARPS * KA_STAGES * TILE);
+    const uint32_t bar0 = smem_u32(region + 2 * ka_state_floats(G, NB) * 32) + warp * KA_STAGES * 8;
+    long long* scan = reinterpret_cast<long long*>(reinterpret_cast<uint8_t*>(region + 2 * ka_state_floats(G, NB) * 32) + KA_WARPS * KA_STAGES * 8);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (lane == 0) {
+        for (int s = 0; s < KA_STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
+        mbar_fence_init();
+        fence_proxy_async();
+    }
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // ---- this CTA's range of the list of tiles: entries (sequence, tile of columns), each n_kv heads of n tiles
+    const int n_kv = P.cache.n_kv, entries = P.n_seq * W.col_tiles;
+    auto entry = [&](int e) {
+        const int seq = e / W.col_tiles, c0 = (e - seq * W.col_tiles) * 8 * NB;
+        return kv4_tiles(P, seq, c0 / P.rep, (min(c0 + 8 * NB, W.cols) - 1) / P.rep);
+    };
+    long long mine = 0;
+    for (int e = threadIdx.x; e < entries; e += KA_THREADS) mine += entry(e).n;
+    long long total = mine;
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-        *reinterpret_cast<uint32_t*>(P.out + item * D + 64 * g + 2 * lane) = any ? pack_bf16x2(o[g][0] / l, o[g][1] / l) : 0u;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    if (lane == 0) scan[warp] = total;
+    __syncthreads();
+    total = n_kv * (scan[0] + scan[1] + scan[2] + scan[3]);
+    const long long per = max((long long)KA_MIN_TILES, (total + gridDim.x - 1) / gridDim.x);
+    const long long start = blockIdx.x * per, end = min(total, start + per);
+    if (threadIdx.x == 0) W.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (start >= end) return;
+    // the entry in which the range begins: prefix sums, as many entries at a time as there are threads
+    int e_first = 0;
+    long long e_at = 0;
+    for (int c0 = 0; c0 < entries; c0 += KA_THREADS) {
+        const int e = c0 + threadIdx.x;
+        const long long n = entries <= KA_THREADS ? mine * n_kv : e < entries ? (long long)entry(e).n * n_kv : 0;
+        long long up = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xFFFFFFFFu, up, o);
+            if (lane >= o) up += v;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = up;
+        __syncthreads();
+        long long before = e_at;
+        for (int w = 0; w < warp; ++w) before += scan[w];
+        before += up - n;
+        const bool here = n > 0 && before <= start && start < before + n;
+        e_at += scan[0] + scan[1] + scan[2] + scan[3];
+        if (__syncthreads_or(here)) {
+            if (here) { scan[4] = e; scan[5] = before; }
+            __syncthreads();
+            e_first = (int)scan[4];
+            e_at = scan[5];
+            break;
+        }
+    }
+
+    struct Cursor { int e, kvh, i; Kv4Tiles k; };
+    auto forward = [&](Cursor& c, int by) {                            // the caller stays inside the range
+        c.i += by;
+        while (c.i >= c.k.n) {
+            c.i -= c.k.n;
+            if (++c.kvh == n_kv) {
+                c.kvh = 0;
+                c.k = entry(++c.e);
+            }
+        }
+    };
+    Cursor at;
+    at.e = e_first;
+    at.k = entry(e_first);
+    at.kvh = (int)((start - e_at) / at.k.n);
+    at.i = (int)((start - e_at) - (long long)at.kvh * at.k.n);
+    Cursor ahead = at;                                                 // the next tile to fetch
+    int to_fetch = (int)((end - start - warp + KA_WARPS - 1) / KA_WARPS), fetched = 0, used = 0;
+    if (to_fetch > 0 && warp > 0) forward(ahead, warp);
+    auto fetch = [&]() {
+        if (fetched == to_fetch) return;
+        if (lane == 0) {
+            const int s = fetched % KA_STAGES;
+            const uint8_t* src = P.cache.tiles + (long long)(ahead.e / W.col_tiles) * P.cache.seq_stride +
+                                 ((long long)ahead.kvh * P.cache.n_tiles + ahead.k.tile(ahead.i)) * TILE;
+            mbar_arrive_expect_tx(bar0 + 8 * s, TILE);
+            bulk_g2s(smem_u32(ring + s * TILE), src, TILE, bar0 + 8 * s);
+        }
+        if (++fetched < to_fetch) forward(ahead, KA_WARPS);
+    };
+#pragma unroll
+    for (int s = 0; s < KA_STAGES; ++s) fetch();
+
+    bool healthy = true;
+    for (long long i = start; i < end;) {
+        const int here = (int)min((long long)(at.k.n - at.i), end - i);            // tiles of this head in this CTA
+        const int seq = at.e / W.col_tiles, col0 = (at.e - seq * W.col_tiles) * 8 * NB;
+        // ---- queries as B operands: column g of every group of eight, channels 16t .. 16t + 15 of every group of 64
+        uint32_t qf[NB][G][8];
+        float qs[NB][G][2], fac[NB][2];
+        Kv4Range range[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int col = col0 + 8 * nb + g;
+            float x[G][16], top = 0.0f;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                uint32_t w[8] = {};
+                if (col < W.cols) {
+                    const uint16_t* src = P.q + ((long long)seq * P.T + col / P.rep) * P.ld_q + (at.kvh * P.rep + col % P.rep) * D + 64 * gr + 16 * t;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) w[k] = __ldg(reinterpret_cast<const uint32_t*>(src) + k);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { x[gr][2 * k] = __uint_as_float(w[k] << 16); x[gr][2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u); }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(fabsf(x[gr][k]))));     // a NaN stays on top
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) top = __uint_as_float(max(__float_as_uint(top), __shfl_xor_sync(0xFFFFFFFFu, __float_as_uint(top), o)));
+            const int ex = max(-112, (int)(__float_as_uint(top) >> 23) - 127);     // largest magnitude in [2^ex, 2^(ex + 1))
+            const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);     // exact: a power of two
+            // (queries that are not finite, or beyond 2^117, give no number)
+            const float my_fac = ex <= 117 ? P.scale_log2 * __uint_as_float((uint32_t)(ex + 10 + 127) << 23) : __uint_as_float(0x7FC00000u);
+            float my_sum[G];
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                float s = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) { x[gr][k] *= up; s += x[gr][k]; }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+                my_sum[gr] = s * 0x1p-24f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int d = 8 * j + 2 * h;
+                        qf[nb][gr][4 * j + 2 * h] = pack_f16x2(x[gr][d], x[gr][d + 4]);
+                        qf[nb][gr][4 * j + 2 * h + 1] = pack_f16x2(x[gr][d + 1] * 0.0625f, x[gr][d + 5] * 0.0625f);
+                    }
+            }
+            // what the scores of columns 2t, 2t + 1 need
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                fac[nb][c] = __shfl_sync(0xFFFFFFFFu, my_fac, 4 * (2 * t + c));
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) qs[nb][gr][c] = __shfl_sync(0xFFFFFFFFu, my_sum[gr], 4 * (2 * t + c));
+                const int cc = col0 + 8 * nb + 2 * t + c;
+                range[nb][c] = cc < W.cols ? kv4_range(P, seq, cc / P.rep) : Kv4Range{0, 0x7FFFFFFF};
+            }
+        }
+        float o[NB][G][4][4], zero[NB][G][4], ref[NB][2], sum[NB][2], up_v[G];      // up_v: power of two that the weights are scaled by
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) up_v[gr] = 0x1p126f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) { ref[nb][c] = -INFINITY; sum[nb][c] = 0.0f; }
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    zero[nb][gr][k] = 0.0f;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) o[nb][gr][m][k] = 0.0f;
+                }
+        }
+
+        for (int k = (warp - (int)(i - start)) & (KA_WARPS - 1); k < here && healthy; k += KA_WARPS) {
+            const int s = used % KA_STAGES;
+            healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE));
+            if (!healthy) break;
+            ++used;
+            const uint8_t* tile = ring + s * TILE;
+            const int j0 = at.k.tile(at.i + k) * KV4_TILE;
+            const bool whole = j0 + KV4_TILE - 1 <= at.k.hi_min && (j0 >= at.k.lo_max || j0 + KV4_TILE <= P.sinks);
+
+            // ---- scores of slots 16 b + g (and + 8), columns 2t, 2t + 1
+            float x[NB][2][4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[nb][b][r] = 0.0f;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    float acc[NB][4];
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[nb][r] = 0.0f;
+                    const uint2 ka = *reinterpret_cast<const uint2*>(tile + kv4_k_row(G, gr, 16 * b + g) + 8 * t);
+                    const uint2 kb = *reinterpret_cast<const uint2*>(tile + kv4_k_row(G, gr, 16 * b + g + 8) + 8 * t);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t wa = (j ? ka.y : ka.x) >> (8 * h), wb = (j ? kb.y : kb.x) >> (8 * h);
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+                                mma_f16(acc[nb], wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, qf[nb][gr][4 * j + 2 * h],
+                                        qf[nb][gr][4 * j + 2 * h + 1]);
+                        }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t m = *reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, gr, 16 * b + g + 8 * r));
+                        const float sc = __uint_as_float(m & 0xFFFF0000u), z = f16_to_float(m & 0xFFFFu);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) x[nb][b][2 * r + c] = fmaf(sc, fmaf(-z, qs[nb][gr][c], acc[nb][2 * r + c]), x[nb][b][2 * r + c]);
+                    }
+                }
+            }
+            // ---- value scales of the same slots, times what brings the largest seen below 2^7
+            float vs[G][2][2];
+            bool move = false;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr)
+                        vs[gr][b][r] = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, gr, 16 * b + g + 8 * r)) << 16);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[nb][b][r] *= fac[nb][r & 1];
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int j = j0 + 16 * b + g + 8 * r;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                if (j > range[nb][c].hi || (j < range[nb][c].lo && j >= P.sinks)) x[nb][b][2 * r + c] = -INFINITY;
+                        if (j > at.k.hi_max || (j < at.k.lo_min && j >= P.sinks))                  // nobody sees it: it may hold anything
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) vs[gr][b][r] = 0.0f;
+                    }
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    move |= fmaxf(fmaxf(x[nb][0][c], x[nb][0][c + 2]), fmaxf(x[nb][1][c], x[nb][1][c + 2])) > ref[nb][c] + 8.0f;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) move |= fmaxf(fmaxf(vs[gr][0][0], vs[gr][0][1]), fmaxf(vs[gr][1][0], vs[gr][1][1])) * up_v[gr] >= 128.0f;
+            if (__any_sync(0xFFFFFFFFu, move)) {                       // new references
+                float down_v[G];
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) top = fmaxf(top, vs[gr][b][r]);                // a NaN stays out
+                    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
+                    const int ex = max(-120, (int)(bits >> 23) - 127);
+                    const float up = fminf(up_v[gr], __uint_as_float((uint32_t)(6 - ex + 127) << 23));
+                    down_v[gr] = up_v[gr] == up ? 1.0f : up * __uint_as_float((uint32_t)(254 - (__float_as_uint(up_v[gr]) >> 23)) << 23);
+                    up_v[gr] = up;
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float f[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float top = fmaxf(fmaxf(x[nb][0][c], x[nb][0][c + 2]), fmaxf(x[nb][1][c], x[nb][1][c + 2]));
+#pragma unroll
+                        for (int s2 = 4; s2 < 32; s2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s2));
+                        top = fmaxf(top, ref[nb][c]);
+                        f[c] = ref[nb][c] == top ? 1.0f : ex2(ref[nb][c] - top);
+                        ref[nb][c] = top;
+                        sum[nb][c] *= f[c];
+                    }
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            zero[nb][gr][r] *= f[r & 1] * down_v[gr];
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) o[nb][gr][m][r] *= f[r & 1] * down_v[gr];
+                        }
+                }
+            }
+            // ---- weights, and weights times scales as B operands (columns by slots: the transpose of how the scores lie)
+            uint32_t pf[NB][G][4];
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) vs[gr][b][r] *= up_v[gr];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float base0 = ref[nb][0] == -INFINITY ? 0.0f : ref[nb][0], base1 = ref[nb][1] == -INFINITY ? 0.0f : ref[nb][1];
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float p0 = ex2(x[nb][b][2 * r] - base0), p1 = ex2(x[nb][b][2 * r + 1] - base1);
+                        const bool h0 = !whole && x[nb][b][2 * r] == -INFINITY, h1 = !whole && x[nb][b][2 * r + 1] == -INFINITY;
+                        sum[nb][0] += p0;
+                        sum[nb][1] += p1;
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr)
+                            pf[nb][gr][2 * b + r] = transpose_8x8(pack_f16x2(h0 ? 0.0f : p0 * vs[gr][b][r], h1 ? 0.0f : p1 * vs[gr][b][r]));
+                    }
+            }
+            // ---- values: slots 2t, 2t + 1 of every eight, channels 8g .. 8g + 7 of every group
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t w[2][2];                                  // [eight slots][channels 0..3, 4..7] of the even (low half) and odd slot
+                    uint32_t z[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int slot = 16 * b + 8 * r + 2 * t;
+                        const uint2 v = *reinterpret_cast<const uint2*>(tile + kv4_v_chunk(G, gr, slot, g));
+                        w[r][0] = __byte_perm(v.x, v.y, 0x5410);
+                        w[r][1] = __byte_perm(v.x, v.y, 0x7632);
+                        z[r] = *reinterpret_cast<const uint32_t*>(tile + kv4_v_zero(G, gr, slot));
+                        if (!whole) {
+                            const int j = j0 + slot;
+                            if (j > at.k.hi_max || (j < at.k.lo_min && j >= P.sinks)) z[r] &= 0xFFFF0000u;
+                            if (j + 1 > at.k.hi_max || (j + 1 < at.k.lo_min && j + 1 >= P.sinks)) z[r] &= 0x0000FFFFu;
+                        }
+                    }
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        mma_f16(zero[nb][gr], z[0], z[0], z[1], z[1], pf[nb][gr][2 * b], pf[nb][gr][2 * b + 1]);
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const uint32_t wa = w[0][m >> 1] >> (8 * (m & 1)), wb = w[1][m >> 1] >> (8 * (m & 1));
+                            mma_f16(o[nb][gr][m], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu, wb & 0x00F000F0u, pf[nb][gr][2 * b],
+                                    pf[nb][gr][2 * b + 1]);
+                        }
+                    }
+                }
+            __syncwarp();
+            fetch();
+        }
+
+        // ---- join the warps' states; first to plain fp32 values and whole sums
+        const bool complete = at.i == 0 && here == at.k.n;
+        Kv4State<G> st[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float v = sum[nb][c];
+#pragma unroll
+                for (int s2 = 4; s2 < 32; s2 <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, s2);
+                st[nb].sum[c] = v;
+                st[nb].ref[c] = ref[nb][c];
+            }
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                const float down = __uint_as_float((254u - (__float_as_uint(up_v[gr]) >> 23)) << 23);
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        st[nb].o[16 * gr + 4 * m + r] = fmaf(o[nb][gr][m][r], r < 2 ? 0x1p24f : 0x1p20f, -zero[nb][gr][r & 1]) * down;
+            }
+        }
+        healthy = __syncthreads_and(healthy);
+        if (healthy) {
+            if (warp >= 2)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) st[nb].store(region + ((warp - 2) * NB + nb) * (16 * G + 4) * 32, lane);
+            __syncthreads();
+            if (warp < 2)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) st[nb].join(region + (warp * NB + nb) * (16 * G + 4) * 32, lane);
+            __syncthreads();
+            if (warp == 1)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) st[nb].store(region + nb * (16 * G + 4) * 32, lane);
+            __syncthreads();
+            if (warp == 0) {
+                float* to = W.partial + (blockIdx.x * 2ll + (i > start ? 1 : 0)) * ka_state_floats(G, NB) * 32;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    st[nb].join(region + nb * (16 * G + 4) * 32, lane);
+                    if (complete) kv4_write_out<G>(P, st[nb], seq, at.kvh, col0 + 8 * nb, W.cols, D, 0, lane);
+                    else st[nb].store(to + nb * (16 * G + 4) * 32, lane);
+                }
+                if (at.i == 0 && here < at.k.n && lane == 0) {               // it begins here and goes on
+                    const long long rest = at.k.n - at.i - here;
+                    W.joins[blockIdx.x] = make_int4(at.e, at.kvh, i > start ? 1 : 0, (int)((rest + per - 1) / per));
+                }
+            }
+            __syncthreads();
+        } else {
+            break;
+        }
+        i += here;
+        if (i < end) forward(at, here);
+    }
+    for (; used < fetched; ++used)                                     // (after a wait that gave up) no copy may land behind the CTA's end
+        mbar_wait_bounded(bar0 + 8 * (used % KA_STAGES), (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE);
+}
+
+// Heads that lie in several CTAs of kv4_attend_kernel: block (b, y, z) joins eight columns and a group of channels of the head that begins in
+// CTA b.  Its states are slot 1 (or 0: the CTA began with it) of CTA b and slot 0 of the CTAs behind.
+constexpr int KC_WARPS = 8;
+template <int G, int NB>
+__global__ void __launch_bounds__(32 * KC_WARPS) kv4_combine_kernel(const Kv4AttendParams P, const Kv4Work W) {
+    __shared__ float region[KC_WARPS][20][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 j = W.joins[blockIdx.x];
+    if (j.x < 0) return;
+    const int nb = blockIdx.y, gr = blockIdx.z, seq = j.x / W.col_tiles, col0 = (j.x - seq * W.col_tiles) * 8 * NB + 8 * nb;
+    Kv4State<1> st;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st.o[i] = 0.0f;
+    st.ref[0] = st.ref[1] = -INFINITY;
+    st.sum[0] = st.sum[1] = 0.0f;
+#pragma unroll 2
+    for (int k = warp; k <= j.w; k += KC_WARPS) {
+        const float* p = W.partial + ((long long)(blockIdx.x + k) * 2 + (k == 0 ? j.z : 0)) * ka_state_floats(G, NB) * 32 + nb * (16 * G + 4) * 32;
+        st.join(p, p + (4 + 16 * gr) * 32, lane);
+    }
+    st.store(&region[warp][0][0], lane);
+    __syncthreads();
+    if (warp == 0) {
+        for (int w = 1; w < min(KC_WARPS, j.w + 1); ++w) st.join(&region[w][0][0], lane);
+        kv4_write_out<1>(P, st, seq, j.y, col0, W.cols, 64 * G, gr, lane);
+    }
 }
 
 }  // namespace cb
