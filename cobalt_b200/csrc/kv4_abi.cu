@@ -50,24 +50,28 @@ bool rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_
 
 struct AttendCfg {
     int cols, nb, col_tiles, grid;
+    bool split;
     size_t joins_off, scratch;
 };
-// Columns are spread evenly over the fewest tiles of 8 * nb that a warp's registers hold; CTAs fill the GPU once, each with a warp's tile
-// of slots per warp at least.
-AttendCfg attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, int sms) {
-    AttendCfg c;
+// Columns are spread evenly over the fewest tiles of 8 * nb that a warp's registers hold.  CTAs fill the GPU once, each with a tile of slots
+// per warp at least; or a CTA per head, where there are that many.
+int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, int sms, AttendCfg* c) {
     const int G = D / KV4_GROUP;
-    c.cols = n_heads / n_kv * T;
-    const int eights = (c.cols + 7) / 8;
-    c.col_tiles = (eights + ka_max_nb(G) - 1) / ka_max_nb(G);
-    c.nb = (eights + c.col_tiles - 1) / c.col_tiles;
-    c.col_tiles = (eights + c.nb - 1) / c.nb;
-    const double tiles = (double)n_seq * c.col_tiles * n_kv * ((n_slots + KV4_TILE - 1) / KV4_TILE);
-    const double most = (double)sms * ka_ctas_per_sm(G, c.nb), need = tiles / KA_MIN_TILES;
-    c.grid = (int)(need < 1 ? 1 : need < most ? need + 0.999 : most);
-    c.joins_off = (size_t)c.grid * 2 * ka_state_floats(G, c.nb) * 128;
-    c.scratch = c.joins_off + (size_t)c.grid * sizeof(int4);
-    return c;
+    const int64_t cols = (int64_t)(n_heads / n_kv) * T;
+    if (cols > 0x3FFFFFFFll) return COBALT_ETOOBIG;
+    c->cols = (int)cols;
+    const int eights = (c->cols + 7) / 8;
+    c->col_tiles = (eights + ka_max_nb(G) - 1) / ka_max_nb(G);
+    c->nb = (eights + c->col_tiles - 1) / c->col_tiles;
+    c->col_tiles = (eights + c->nb - 1) / c->nb;
+    const double all = (double)n_seq * c->col_tiles * n_kv, tiles = all * ((n_slots + KV4_TILE - 1) / KV4_TILE);
+    c->split = (int64_t)n_seq * c->col_tiles <= KA_ENTRIES && tiles < 1e9;
+    const double most = (double)sms * ka_ctas_per_sm(G, c->nb), need = tiles / KA_MIN_TILES;
+    if (!c->split && all > 2e9) return COBALT_ETOOBIG;
+    c->grid = (int)(!c->split ? all : need < 1 ? 1 : need < most ? need + 0.999 : most);
+    c->joins_off = (size_t)c->grid * 2 * ka_state_floats(G, c->nb) * 128;
+    c->scratch = c->split ? c->joins_off + (size_t)c->grid * sizeof(int4) : 0;
+    return COBALT_OK;
 }
 template <int G, int NB>
 int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c, cudaStream_t st) {
@@ -90,6 +94,7 @@ int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, kv4_attend_kernel<G, NB>, P, W) != cudaSuccess) return COBALT_ELAUNCH;
+    if (!c.split) return COBALT_OK;
     cfg.gridDim = dim3((unsigned)c.grid, NB, G);
     cfg.blockDim = dim3(32 * KC_WARPS);
     cfg.dynamicSmemBytes = 0;
@@ -157,7 +162,8 @@ int cobalt_kv4_read(const void* tiles, int64_t tiles_seq_stride, const int64_t* 
 size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots) {
     int sms = 0;
     if (n_seq <= 0 || T <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_slots <= 0 || !dim_ok(head_dim) || sm_count(&sms)) return 0;
-    return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms).scratch;
+    AttendCfg c;
+    return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms, &c) ? 0 : c.scratch;
 }
 
 int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
@@ -167,13 +173,12 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     int rc = make_cache(&P.cache, tiles, tiles_seq_stride, positions, pos_seq_stride, n_seq, T, n_kv_heads, head_dim, n_slots);
     if (rc) return rc;
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || window < 0 || sinks < 0) return COBALT_EINVAL;
-    if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
-    if ((int64_t)n_heads / n_kv_heads * T > 0x3FFFFFFFll) return COBALT_ETOOBIG;
+    if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || ((uintptr_t)q & 15) || (ld_q & 7) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
-    const AttendCfg c = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms);
-    if ((int64_t)n_seq * c.col_tiles > 0x3FFFFFFFll) return COBALT_ETOOBIG;
-    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < c.scratch) return COBALT_ESCRATCH;
+    AttendCfg c;
+    if ((rc = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms, &c))) return rc;
+    if (c.split && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < c.scratch)) return COBALT_ESCRATCH;
     P.q = (const uint16_t*)q; P.ld_q = ld_q;
     P.positions = (const long long*)positions;
     P.pos_stride = pos_seq_stride;
@@ -184,6 +189,7 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     Kv4Work W;
     W.cols = c.cols;
     W.col_tiles = c.col_tiles;
+    W.split = c.split;
     W.partial = (float*)scratch;
     W.joins = (int4*)((uint8_t*)scratch + c.joins_off);
     switch (head_dim / KV4_GROUP * 10 + c.nb) {

@@ -14,6 +14,7 @@
 // shared-memory reads free of bank conflicts.
 #pragma once
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "common.cuh"
 #include "staged_input.cuh"
 
@@ -256,29 +257,33 @@ __device__ __forceinline__ Kv4Range kv4_range(const Kv4AttendParams& P, int seq,
     r.lo = P.window > 0 ? (int)max(0ll, min(pos - P.window + 1, (long long)P.cache.n_slots)) : 0;
     return r;
 }
-// The tiles that some token of a range sees, in order (i < n_sink: tile i, else first + i - n_sink; at least one, so that a row that
-// sees nothing gets its zeros), and what of a tile needs no mask.
-struct Kv4Tiles {
-    int n, n_sink, first;
-    int hi_max, lo_min, hi_min, lo_max;
-    __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
-};
-__device__ __forceinline__ Kv4Tiles kv4_tiles(const Kv4AttendParams& P, int seq, int tok0, int tok1) {
-    Kv4Tiles e;
-    e.hi_max = -1; e.lo_min = 0x7FFFFFFF; e.hi_min = 0x7FFFFFFF; e.lo_max = 0;
+// What a range of tokens sees: the slots between the bounds of all of them, and those between the bounds that bind every one.
+struct Kv4Span { int hi_max, lo_min, hi_min, lo_max; };
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4AttendParams& P, int seq, int tok0, int tok1) {
+    Kv4Span s = {-1, 0x7FFFFFFF, 0x7FFFFFFF, 0};
     for (int t = tok0; t <= tok1; ++t) {
         const Kv4Range r = kv4_range(P, seq, t);
-        e.hi_max = max(e.hi_max, r.hi);
-        e.hi_min = min(e.hi_min, r.hi);
-        e.lo_max = max(e.lo_max, r.lo);
-        if (r.lo <= r.hi) e.lo_min = min(e.lo_min, r.lo);
+        s.hi_max = max(s.hi_max, r.hi);
+        s.hi_min = min(s.hi_min, r.hi);
+        s.lo_max = max(s.lo_max, r.lo);
+        if (r.lo <= r.hi) s.lo_min = min(s.lo_min, r.lo);
     }
-    const int tiles = (e.hi_max + KV4_TILE) / KV4_TILE;                // of slots 0 .. hi_max
-    e.n_sink = (min(P.sinks, e.hi_max + 1) + KV4_TILE - 1) / KV4_TILE;
-    e.first = e.lo_min > e.hi_max ? tiles : e.lo_min / KV4_TILE;
+    return s;
+}
+// The tiles that hold a slot some token sees, in order: i < n_sink: tile i, else first + i - n_sink.  At least one, so that a row
+// that sees nothing gets its zeros.
+struct Kv4Tiles {
+    int n, n_sink, first;
+    __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
+};
+__device__ __forceinline__ Kv4Tiles kv4_tiles(const Kv4Span& s, int sinks) {
+    Kv4Tiles e;
+    const int tiles = (s.hi_max + KV4_TILE) / KV4_TILE;                // of slots 0 .. hi_max
+    e.n_sink = (min(sinks, s.hi_max + 1) + KV4_TILE - 1) / KV4_TILE;
+    e.first = min(tiles, s.lo_min / KV4_TILE);
     if (e.first <= e.n_sink) e.first = e.n_sink = 0;
-    e.n = max(1, e.n_sink + tiles - e.first);
-    if (e.n_sink + tiles - e.first <= 0) e.first = e.n_sink = 0;
+    e.n = e.n_sink + tiles - e.first;
+    if (e.n == 0) { e.n = 1; e.first = 0; }
     return e;
 }
 
@@ -291,6 +296,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {       // d = a b
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -300,6 +309,30 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     uint32_t d;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
+}
+// the words, and the bf16 values, of a slot's G groups (aligned to their own size where G is a power of two)
+template <int G>
+__device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[G]) {
+    if (G == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[G - 1] = v.y; }
+    else if (G == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1 % G] = v.y; w[2 % G] = v.z; w[3 % G] = v.w; }
+    else {
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) w[gr] = reinterpret_cast<const uint32_t*>(p)[gr];
+    }
+}
+template <int G>
+__device__ __forceinline__ void kv4_halves(const uint8_t* p, float (&f)[G]) {
+    if (G % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < G / 2; ++k) {
+            const uint32_t v = reinterpret_cast<const uint32_t*>(p)[k];
+            f[(2 * k) % G] = __uint_as_float(v << 16);
+            f[(2 * k + 1) % G] = __uint_as_float(v & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) f[gr] = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[gr] << 16);
+    }
 }
 __device__ __forceinline__ float f16_to_float(uint32_t bits) { return __half2float(__ushort_as_half((uint16_t)bits)); }
 
@@ -318,20 +351,23 @@ __device__ __forceinline__ float f16_to_float(uint32_t bits) { return __half2flo
 //
 // A warp owns a ring of tiles, one bulk copy each, and walks every 4th tile of its CTA's range alone.  The list of all (sequence, columns,
 // KV head, tile) is cut into equal ranges, one per CTA, whatever the lengths of the sequences are; a CTA joins its warps' states at
-// the end of every head, and heads that lie in several CTAs are joined by kv4_combine_kernel.
+// the end of every head, and heads that lie in several CTAs are joined by kv4_combine_kernel.  Above KA_ENTRIES (sequence, columns) pairs there
+// are heads enough to fill the GPU: a CTA takes one head each, and nothing is joined across CTAs.
 constexpr int KA_WARPS = 4, KA_THREADS = 32 * KA_WARPS;
 constexpr int KA_STAGES = 2;
 constexpr int KA_MIN_TILES = 4;                                        // per CTA: one per warp
+constexpr int KA_ENTRIES = 256;
 constexpr int ka_max_nb(int G) { return G == 1 ? 4 : G == 2 ? 2 : 1; } // groups of eight columns a warp holds
 constexpr int ka_ctas_per_sm(int G, int NB) { return NB == 1 ? (G <= 2 ? 4 : G == 3 ? 3 : 2) : G * NB <= 2 ? 3 : 2; }
 constexpr int ka_state_floats(int G, int NB) { return NB * (16 * G + 4); }      // per lane: O, reference and sum of two columns
 constexpr size_t ka_smem_bytes(int G, int NB) {
-    return (size_t)KA_WARPS * KA_STAGES * kv4_tile_bytes(G) + 2 * (size_t)ka_state_floats(G, NB) * 128 + KA_WARPS * KA_STAGES * 8 + 128;
+    return (size_t)KA_WARPS * KA_STAGES * kv4_tile_bytes(G) + 2 * (size_t)ka_state_floats(G, NB) * 128 + KA_WARPS * KA_STAGES * 8 + KA_ENTRIES * 20 + 64;
 }
 static_assert(ka_smem_bytes(4, 1) * 2 <= 227 * 1024 - 2048, "at least two CTAs per SM");
 
 struct Kv4Work {
     int cols, col_tiles;                                               // rep * T columns per KV head, in tiles of 8 * NB
+    bool split;                                                        // ranges of the list (else a CTA per head)
     float* partial;                                                    // [CTA][2][floats][32 lanes]
     int4* joins;                                                       // [CTA]: head that begins in this CTA and ends in a later one
 };
@@ -388,13 +424,15 @@ __device__ __forceinline__ void kv4_write_out(const Kv4AttendParams& P, const Kv
 
 template <int G, int NB>
 __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_kernel(const Kv4AttendParams P, const Kv4Work W) {
-    constexpr int D = 64 * G, TILE = kv4_tile_bytes(G);
+    constexpr int D = 64 * G, TILE = kv4_tile_bytes(G), STATE = (16 * G + 4) * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t* ring = smem + warp * (KA_STAGES * TILE);
     float* region = reinterpret_cast<float*>(smem + KA_WARPS * KA_STAGES * TILE);
-    const uint32_t bar0 = smem_u32(region + 2 * ka_state_floats(G, NB) * 32) + warp * KA_STAGES * 8;
-    long long* scan = reinterpret_cast<long long*>(reinterpret_cast<uint8_t*>(region + 2 * ka_state_floats(G, NB) * 32) + KA_WARPS * KA_STAGES * 8);
+    int4* spans = reinterpret_cast<int4*>(region + 2 * NB * STATE);
+    int* before = reinterpret_cast<int*>(spans + KA_ENTRIES);          // tiles (of one head) of the entries before
+    int* scan = before + KA_ENTRIES;
+    const uint32_t bar0 = smem_u32(scan + 8) + warp * KA_STAGES * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (lane == 0) {
         for (int s = 0; s < KA_STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
@@ -404,90 +442,100 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
     __syncwarp();
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- this CTA's range of the list of tiles: entries (sequence, tile of columns), each n_kv heads of n tiles
-    const int n_kv = P.cache.n_kv, entries = P.n_seq * W.col_tiles;
-    auto entry = [&](int e) {
-        const int seq = e / W.col_tiles, c0 = (e - seq * W.col_tiles) * 8 * NB;
-        return kv4_tiles(P, seq, c0 / P.rep, (min(c0 + 8 * NB, W.cols) - 1) / P.rep);
-    };
-    long long mine = 0;
-    for (int e = threadIdx.x; e < entries; e += KA_THREADS) mine += entry(e).n;
-    long long total = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-    if (lane == 0) scan[warp] = total;
-    __syncthreads();
-    total = n_kv * (scan[0] + scan[1] + scan[2] + scan[3]);
-    const long long per = max((long long)KA_MIN_TILES, (total + gridDim.x - 1) / gridDim.x);
-    const long long start = blockIdx.x * per, end = min(total, start + per);
-    if (threadIdx.x == 0) W.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    if (start >= end) return;
-    // the entry in which the range begins: prefix sums, as many entries at a time as there are threads
-    int e_first = 0;
-    long long e_at = 0;
+    // ---- the entries (sequence, tile of columns) and their tiles; this CTA's range of the list: every entry is `heads` heads of n tiles
+    const int n_kv = P.cache.n_kv;
+    const int entry0 = W.split ? 0 : (gridDim.x - 1 - blockIdx.x) / n_kv;              // (last tokens first: their rows are the longest)
+    const int head0 = W.split ? 0 : (gridDim.x - 1 - blockIdx.x) % n_kv;
+    const int entries = W.split ? P.n_seq * W.col_tiles : 1, heads = W.split ? n_kv : 1;
+    int total = 0;
+#pragma unroll 1
     for (int c0 = 0; c0 < entries; c0 += KA_THREADS) {
         const int e = c0 + threadIdx.x;
-        const long long n = entries <= KA_THREADS ? mine * n_kv : e < entries ? (long long)entry(e).n * n_kv : 0;
-        long long up = n;
+        int n = 0;
+        if (e < entries) {
+            const int seq = (entry0 + e) / W.col_tiles, col = ((entry0 + e) - seq * W.col_tiles) * 8 * NB;
+            const Kv4Span sp = kv4_span(P, seq, col / P.rep, (min(col + 8 * NB, W.cols) - 1) / P.rep);
+            spans[e] = make_int4(sp.hi_max, sp.lo_min, sp.hi_min, sp.lo_max);
+            n = kv4_tiles(sp, P.sinks).n;
+        }
+        int up = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xFFFFFFFFu, up, o);
+            const int v = __shfl_up_sync(0xFFFFFFFFu, up, o);
             if (lane >= o) up += v;
         }
-        __syncthreads();
         if (lane == 31) scan[warp] = up;
         __syncthreads();
-        long long before = e_at;
-        for (int w = 0; w < warp; ++w) before += scan[w];
-        before += up - n;
-        const bool here = n > 0 && before <= start && start < before + n;
-        e_at += scan[0] + scan[1] + scan[2] + scan[3];
-        if (__syncthreads_or(here)) {
-            if (here) { scan[4] = e; scan[5] = before; }
-            __syncthreads();
-            e_first = (int)scan[4];
-            e_at = scan[5];
-            break;
+        int at = total + up - n;
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; ++w) {
+            if (w < warp) at += scan[w];
+            total += scan[w];
         }
+        if (e < entries) before[e] = at;
+        __syncthreads();
     }
+    total *= heads;
+    const int per = W.split ? max(KA_MIN_TILES, (total + (int)gridDim.x - 1) / (int)gridDim.x) : total;
+    const int start = W.split ? min(total, (int)blockIdx.x * per) : 0, end = min(total, start + per);
+    if (W.split && threadIdx.x == 0) W.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (start >= end) return;
 
     struct Cursor { int e, kvh, i; Kv4Tiles k; };
+    auto load = [&](int e) {
+        const int4 v = spans[e];
+        return kv4_tiles(Kv4Span{v.x, v.y, v.z, v.w}, P.sinks);
+    };
     auto forward = [&](Cursor& c, int by) {                            // the caller stays inside the range
         c.i += by;
         while (c.i >= c.k.n) {
             c.i -= c.k.n;
-            if (++c.kvh == n_kv) {
+            if (++c.kvh == heads) {
                 c.kvh = 0;
-                c.k = entry(++c.e);
+                c.k = load(++c.e);
             }
         }
     };
     Cursor at;
-    at.e = e_first;
-    at.k = entry(e_first);
-    at.kvh = (int)((start - e_at) / at.k.n);
-    at.i = (int)((start - e_at) - (long long)at.kvh * at.k.n);
-    Cursor ahead = at;                                                 // the next tile to fetch
-    int to_fetch = (int)((end - start - warp + KA_WARPS - 1) / KA_WARPS), fetched = 0, used = 0;
-    if (to_fetch > 0 && warp > 0) forward(ahead, warp);
+    at.e = 0;
+    for (int step = KA_ENTRIES / 2; step > 0; step >>= 1)              // the last entry that begins at or before `start`
+        if (at.e + step < entries && before[at.e + step] * heads <= start) at.e += step;
+    at.k = load(at.e);
+    at.kvh = (start - before[at.e] * heads) / at.k.n;
+    at.i = (start - before[at.e] * heads) - at.kvh * at.k.n;
+    // what the warp fetches next: `run` more of its tiles from `src` on, four tiles apart; then the run that `ahead` stands at
+    Cursor ahead = at;
+    const int to_fetch = (end - start - warp + KA_WARPS - 1) / KA_WARPS;
+    int fetched = 0, used = 0, run = 0, step = warp;
+    const uint8_t* src = nullptr;
     auto fetch = [&]() {
-        if (fetched == to_fetch) return;
+        if (fetched >= to_fetch) return;
+        if (run == 0) {
+            forward(ahead, step);
+            const int left = (ahead.i < ahead.k.n_sink ? ahead.k.n_sink : ahead.k.n) - ahead.i;
+            run = (left + KA_WARPS - 1) / KA_WARPS;
+            step = run * KA_WARPS;
+            src = P.cache.tiles + (long long)((entry0 + ahead.e) / W.col_tiles) * P.cache.seq_stride +
+                  ((long long)(head0 + ahead.kvh) * P.cache.n_tiles + ahead.k.tile(ahead.i)) * TILE;
+        }
         if (lane == 0) {
             const int s = fetched % KA_STAGES;
-            const uint8_t* src = P.cache.tiles + (long long)(ahead.e / W.col_tiles) * P.cache.seq_stride +
-                                 ((long long)ahead.kvh * P.cache.n_tiles + ahead.k.tile(ahead.i)) * TILE;
             mbar_arrive_expect_tx(bar0 + 8 * s, TILE);
             bulk_g2s(smem_u32(ring + s * TILE), src, TILE, bar0 + 8 * s);
         }
-        if (++fetched < to_fetch) forward(ahead, KA_WARPS);
+        ++fetched;
+        --run;
+        src += KA_WARPS * TILE;
     };
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < KA_STAGES; ++s) fetch();
 
     bool healthy = true;
-    for (long long i = start; i < end;) {
-        const int here = (int)min((long long)(at.k.n - at.i), end - i);            // tiles of this head in this CTA
-        const int seq = at.e / W.col_tiles, col0 = (at.e - seq * W.col_tiles) * 8 * NB;
+#pragma unroll 1
+    for (int i = start; i < end;) {
+        const int here = min(at.k.n - at.i, end - i);                  // tiles of this head in this CTA
+        const int seq = (entry0 + at.e) / W.col_tiles, col0 = ((entry0 + at.e) - seq * W.col_tiles) * 8 * NB, kvh = head0 + at.kvh;
+        const Kv4Span span = {spans[at.e].x, spans[at.e].y, spans[at.e].z, spans[at.e].w};
         // ---- queries as B operands: column g of every group of eight, channels 16t .. 16t + 15 of every group of 64
         uint32_t qf[NB][G][8];
         float qs[NB][G][2], fac[NB][2];
@@ -495,23 +543,23 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int col = col0 + 8 * nb + g;
-            float x[G][16], top = 0.0f;
+            uint4 w[G][2];
+            uint32_t top = 0u;                                         // largest magnitude; a NaN stays on top
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-                uint32_t w[8] = {};
-                if (col < W.cols) {
-                    const uint16_t* src = P.q + ((long long)seq * P.T + col / P.rep) * P.ld_q + (at.kvh * P.rep + col % P.rep) * D + 64 * gr + 16 * t;
+            for (int gr = 0; gr < G; ++gr)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) w[k] = __ldg(reinterpret_cast<const uint32_t*>(src) + k);
+                for (int k = 0; k < 2; ++k) {
+                    w[gr][k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (col < W.cols)
+                        w[gr][k] = __ldg(reinterpret_cast<const uint4*>(P.q + ((long long)seq * P.T + col / P.rep) * P.ld_q + (kvh * P.rep + col % P.rep) * D +
+                                                                        64 * gr + 16 * t) + k);
+                    const uint32_t v[4] = {w[gr][k].x, w[gr][k].y, w[gr][k].z, w[gr][k].w};
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) top = max(top, max(v[d] & 0x7FFF0000u, (v[d] & 0x7FFFu) << 16));
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) { x[gr][2 * k] = __uint_as_float(w[k] << 16); x[gr][2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u); }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(fabsf(x[gr][k]))));     // a NaN stays on top
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) top = __uint_as_float(max(__float_as_uint(top), __shfl_xor_sync(0xFFFFFFFFu, __float_as_uint(top), o)));
-            const int ex = max(-112, (int)(__float_as_uint(top) >> 23) - 127);     // largest magnitude in [2^ex, 2^(ex + 1))
+            for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            const int ex = max(-112, (int)(top >> 23) - 127);          // largest magnitude in [2^ex, 2^(ex + 1))
             const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);     // exact: a power of two
             // (queries that are not finite, or beyond 2^117, give no number)
             const float my_fac = ex <= 117 ? P.scale_log2 * __uint_as_float((uint32_t)(ex + 10 + 127) << 23) : __uint_as_float(0x7FC00000u);
@@ -520,18 +568,20 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
             for (int gr = 0; gr < G; ++gr) {
                 float s = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) { x[gr][k] *= up; s += x[gr][k]; }
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t v[4] = {w[gr][j].x, w[gr][j].y, w[gr][j].z, w[gr][j].w};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {                      // channels 2h, 2h + 1 and 2h + 4, 2h + 5 of the eight
+                        const float a = __uint_as_float(v[h] << 16) * up, b = __uint_as_float(v[h] & 0xFFFF0000u) * up;
+                        const float c = __uint_as_float(v[h + 2] << 16) * up, d = __uint_as_float(v[h + 2] & 0xFFFF0000u) * up;
+                        s += (a + b) + (c + d);
+                        qf[nb][gr][4 * j + 2 * h] = pack_f16x2(a, c);
+                        qf[nb][gr][4 * j + 2 * h + 1] = pack_f16x2(b * 0.0625f, d * 0.0625f);
+                    }
+                }
 #pragma unroll
                 for (int o = 1; o < 4; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
                 my_sum[gr] = s * 0x1p-24f;
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int d = 8 * j + 2 * h;
-                        qf[nb][gr][4 * j + 2 * h] = pack_f16x2(x[gr][d], x[gr][d + 4]);
-                        qf[nb][gr][4 * j + 2 * h + 1] = pack_f16x2(x[gr][d + 1] * 0.0625f, x[gr][d + 5] * 0.0625f);
-                    }
             }
             // what the scores of columns 2t, 2t + 1 need
 #pragma unroll
@@ -543,13 +593,15 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
                 range[nb][c] = cc < W.cols ? kv4_range(P, seq, cc / P.rep) : Kv4Range{0, 0x7FFFFFFF};
             }
         }
-        float o[NB][G][4][4], zero[NB][G][4], ref[NB][2], sum[NB][2], up_v[G];      // up_v: power of two that the weights are scaled by
+        // scores are taken relative to a reference per column (base: its negative); one above `room` moves it.  up_v: power of two that the
+        // weights of a group are scaled by
+        float o[NB][G][4][4], zero[NB][G][4], base[NB][2], room[NB][2], sum[NB][2], up_v[G];
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) up_v[gr] = 0x1p126f;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) { ref[nb][c] = -INFINITY; sum[nb][c] = 0.0f; }
+            for (int c = 0; c < 2; ++c) { base[nb][c] = 0.0f; room[nb][c] = -INFINITY; sum[nb][c] = 0.0f; }
 #pragma unroll
             for (int gr = 0; gr < G; ++gr)
 #pragma unroll
@@ -560,185 +612,191 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
                 }
         }
 
-        for (int k = (warp - (int)(i - start)) & (KA_WARPS - 1); k < here && healthy; k += KA_WARPS) {
+#pragma unroll 1
+        for (int k = (warp - (i - start)) & (KA_WARPS - 1); k < here; k += KA_WARPS) {
             const int s = used % KA_STAGES;
-            healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE));
-            if (!healthy) break;
+            if (__builtin_expect(!__all_sync(0xFFFFFFFFu, mbar_try_wait(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u)), 0)) {
+                healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE));
+                if (!healthy) break;
+            }
             ++used;
             const uint8_t* tile = ring + s * TILE;
             const int j0 = at.k.tile(at.i + k) * KV4_TILE;
-            const bool whole = j0 + KV4_TILE - 1 <= at.k.hi_min && (j0 >= at.k.lo_max || j0 + KV4_TILE <= P.sinks);
-
-            // ---- scores of slots 16 b + g (and + 8), columns 2t, 2t + 1
-            float x[NB][2][4];
+            const bool whole = j0 + KV4_TILE - 1 <= span.hi_min && (j0 >= span.lo_max || j0 + KV4_TILE <= P.sinks);
+            auto nobody = [&](int j) { return j > span.hi_max || (j < span.lo_min && j >= P.sinks); };      // such a slot may hold anything
+            // ---- a value scale of this tile that is too large for the weights' range moves the power of two that they are scaled by
+            {
+                float sv[G];
+                kv4_halves<G>(tile + kv4_v_scale(G, 0, lane), sv);
+                bool grow = false;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+                for (int gr = 0; gr < G; ++gr) grow |= sv[gr] * up_v[gr] >= 128.0f;
+                if (__builtin_expect(__any_sync(0xFFFFFFFFu, grow), 0)) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+                    for (int gr = 0; gr < G; ++gr) {
+                        const float top = nobody(j0 + lane) ? 0.0f : fmaxf(sv[gr], 0.0f);          // a NaN stays out
+                        const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
+                        const int ex = max(-120, (int)(bits >> 23) - 127);
+                        const float up = fminf(up_v[gr], __uint_as_float((uint32_t)(6 - ex + 127) << 23));
+                        const float down = up * __uint_as_float((254u - (__float_as_uint(up_v[gr]) >> 23)) << 23);
+                        up_v[gr] = up;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[nb][b][r] = 0.0f;
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                zero[nb][gr][r] *= down;
+#pragma unroll
+                                for (int m = 0; m < 4; ++m) o[nb][gr][m][r] *= down;
+                            }
+                    }
+                }
+            }
+            // sixteen slots at a time: the loop's code stays small, four warps per scheduler cover its latencies
+            auto sixteen = [&](auto masked, int b) {
+                constexpr bool MASKED = decltype(masked)::value;
+                // ---- scores of slots g and g + 8, columns 2t, 2t + 1, relative to the reference; value scales of the same slots, times up_v
+                float x[NB][4], vs[G][2], acc[NB][G][4];
+                const uint8_t* keys = tile + 512 * b + 32 * g + 8 * t;
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
-                    float acc[NB][4];
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[nb][r] = 0.0f;
-                    const uint2 ka = *reinterpret_cast<const uint2*>(tile + kv4_k_row(G, gr, 16 * b + g) + 8 * t);
-                    const uint2 kb = *reinterpret_cast<const uint2*>(tile + kv4_k_row(G, gr, 16 * b + g + 8) + 8 * t);
+                    const uint2 ka = *reinterpret_cast<const uint2*>(keys + kv4_k_row(G, gr, 0));
+                    const uint2 kb = *reinterpret_cast<const uint2*>(keys + kv4_k_row(G, gr, 8));
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const uint32_t wa = (j ? ka.y : ka.x) >> (8 * h), wb = (j ? kb.y : kb.x) >> (8 * h);
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb)
-                                mma_f16(acc[nb], wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, qf[nb][gr][4 * j + 2 * h],
-                                        qf[nb][gr][4 * j + 2 * h + 1]);
+                            for (int nb = 0; nb < NB; ++nb) {
+                                const uint32_t* q = &qf[nb][gr][4 * j + 2 * h];
+                                if (j + h == 0)
+                                    mma_f16_first(acc[nb][gr], wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, q[0], q[1]);
+                                else
+                                    mma_f16(acc[nb][gr], wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, q[0], q[1]);
+                            }
+                        }
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    uint32_t m[G];
+                    float sv[G];
+                    kv4_words<G>(tile + kv4_k_meta(G, 0, 16 * b + g + 8 * r), m);
+                    kv4_halves<G>(tile + kv4_v_scale(G, 0, 16 * b + g + 8 * r), sv);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float v = 0.0f;
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) {
+                                const float in = fmaf(-f16_to_float(m[gr] & 0xFFFFu), qs[nb][gr][c], acc[nb][gr][2 * r + c]);
+                                v = gr == 0 ? __uint_as_float(m[gr] & 0xFFFF0000u) * in : fmaf(__uint_as_float(m[gr] & 0xFFFF0000u), in, v);
+                            }
+                            x[nb][2 * r + c] = fmaf(v, fac[nb][c], base[nb][c]);
                         }
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const uint32_t m = *reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, gr, 16 * b + g + 8 * r));
-                        const float sc = __uint_as_float(m & 0xFFFF0000u), z = f16_to_float(m & 0xFFFFu);
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                            for (int c = 0; c < 2; ++c) x[nb][b][2 * r + c] = fmaf(sc, fmaf(-z, qs[nb][gr][c], acc[nb][2 * r + c]), x[nb][b][2 * r + c]);
-                    }
-                }
-            }
-            // ---- value scales of the same slots, times what brings the largest seen below 2^7
-            float vs[G][2][2];
-            bool move = false;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr)
-                        vs[gr][b][r] = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, gr, 16 * b + g + 8 * r)) << 16);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[nb][b][r] *= fac[nb][r & 1];
-            if (!whole) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+                    for (int gr = 0; gr < G; ++gr) vs[gr][r] = sv[gr] * up_v[gr];
+                    if (MASKED) {
                         const int j = j0 + 16 * b + g + 8 * r;
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                             for (int c = 0; c < 2; ++c)
-                                if (j > range[nb][c].hi || (j < range[nb][c].lo && j >= P.sinks)) x[nb][b][2 * r + c] = -INFINITY;
-                        if (j > at.k.hi_max || (j < at.k.lo_min && j >= P.sinks))                  // nobody sees it: it may hold anything
+                                if (j > range[nb][c].hi || (j < range[nb][c].lo && j >= P.sinks)) x[nb][2 * r + c] = -INFINITY;
 #pragma unroll
-                            for (int gr = 0; gr < G; ++gr) vs[gr][b][r] = 0.0f;
+                        for (int gr = 0; gr < G; ++gr)
+                            if (nobody(j)) vs[gr][r] = 0.0f;
                     }
-            }
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    move |= fmaxf(fmaxf(x[nb][0][c], x[nb][0][c + 2]), fmaxf(x[nb][1][c], x[nb][1][c + 2])) > ref[nb][c] + 8.0f;
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) move |= fmaxf(fmaxf(vs[gr][0][0], vs[gr][0][1]), fmaxf(vs[gr][1][0], vs[gr][1][1])) * up_v[gr] >= 128.0f;
-            if (__any_sync(0xFFFFFFFFu, move)) {                       // new references
-                float down_v[G];
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) {
-                    float top = 0.0f;
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) top = fmaxf(top, vs[gr][b][r]);                // a NaN stays out
-                    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
-                    const int ex = max(-120, (int)(bits >> 23) - 127);
-                    const float up = fminf(up_v[gr], __uint_as_float((uint32_t)(6 - ex + 127) << 23));
-                    down_v[gr] = up_v[gr] == up ? 1.0f : up * __uint_as_float((uint32_t)(254 - (__float_as_uint(up_v[gr]) >> 23)) << 23);
-                    up_v[gr] = up;
                 }
+                bool move = false;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    float f[2];
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float top = fmaxf(fmaxf(x[nb][0][c], x[nb][0][c + 2]), fmaxf(x[nb][1][c], x[nb][1][c + 2]));
+                    for (int c = 0; c < 2; ++c) move |= fmaxf(x[nb][c], x[nb][c + 2]) > room[nb][c];
+                if (__builtin_expect(__any_sync(0xFFFFFFFFu, move), 0)) {                  // new references
 #pragma unroll
-                        for (int s2 = 4; s2 < 32; s2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s2));
-                        top = fmaxf(top, ref[nb][c]);
-                        f[c] = ref[nb][c] == top ? 1.0f : ex2(ref[nb][c] - top);
-                        ref[nb][c] = top;
-                        sum[nb][c] *= f[c];
-                    }
+                    for (int nb = 0; nb < NB; ++nb) {
+                        float f[2];
 #pragma unroll
-                    for (int gr = 0; gr < G; ++gr)
+                        for (int c = 0; c < 2; ++c) {
+                            float top = fmaxf(x[nb][c], x[nb][c + 2]);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            zero[nb][gr][r] *= f[r & 1] * down_v[gr];
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) o[nb][gr][m][r] *= f[r & 1] * down_v[gr];
+                            for (int s2 = 4; s2 < 32; s2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s2));
+                            const bool first = room[nb][c] == -INFINITY;   // (no number so far: nothing to rescale)
+                            if (!first) top = fmaxf(top, 0.0f);
+                            const bool set = top != -INFINITY;
+                            f[c] = first ? 1.0f : ex2(-top);
+                            if (set) {
+                                base[nb][c] -= top;
+                                room[nb][c] = 8.0f;
+                                x[nb][c] -= top;
+                                x[nb][c + 2] -= top;
+                            }
+                            sum[nb][c] *= f[c];
                         }
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                zero[nb][gr][r] *= f[r & 1];
+#pragma unroll
+                                for (int m = 0; m < 4; ++m) o[nb][gr][m][r] *= f[r & 1];
+                            }
+                    }
                 }
-            }
-            // ---- weights, and weights times scales as B operands (columns by slots: the transpose of how the scores lie)
-            uint32_t pf[NB][G][4];
+                // ---- weights, and weights times scales as B operands (columns by slots: the transpose of how the scores lie)
+                uint32_t pf[NB][G][2];
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) vs[gr][b][r] *= up_v[gr];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float base0 = ref[nb][0] == -INFINITY ? 0.0f : ref[nb][0], base1 = ref[nb][1] == -INFINITY ? 0.0f : ref[nb][1];
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float p0 = ex2(x[nb][b][2 * r] - base0), p1 = ex2(x[nb][b][2 * r + 1] - base1);
-                        const bool h0 = !whole && x[nb][b][2 * r] == -INFINITY, h1 = !whole && x[nb][b][2 * r + 1] == -INFINITY;
+                        const float p0 = ex2(x[nb][2 * r]), p1 = ex2(x[nb][2 * r + 1]);
                         sum[nb][0] += p0;
                         sum[nb][1] += p1;
 #pragma unroll
-                        for (int gr = 0; gr < G; ++gr)
-                            pf[nb][gr][2 * b + r] = transpose_8x8(pack_f16x2(h0 ? 0.0f : p0 * vs[gr][b][r], h1 ? 0.0f : p1 * vs[gr][b][r]));
+                        for (int gr = 0; gr < G; ++gr) {
+                            uint32_t w = pack_f16x2(p0 * vs[gr][r], p1 * vs[gr][r]);
+                            if (MASKED)                                // a slot that only some columns see: no NaN of its scale for the others
+                                w &= (x[nb][2 * r] == -INFINITY ? 0u : 0xFFFFu) | (x[nb][2 * r + 1] == -INFINITY ? 0u : 0xFFFF0000u);
+                            pf[nb][gr][r] = transpose_8x8(w);
+                        }
                     }
-            }
-            // ---- values: slots 2t, 2t + 1 of every eight, channels 8g .. 8g + 7 of every group
+                // ---- values: slots 2t, 2t + 1 of each eight, channels 8g .. 8g + 7 of every group
+                const uint8_t* vals = tile + kv4_v_chunk(G, 0, 2 * t, g) + 512 * b;
+                const uint8_t* zeros = tile + kv4_v_zero(G, 0, 16 * b + 2 * t);
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t w[2][2];                                  // [eight slots][channels 0..3, 4..7] of the even (low half) and odd slot
-                    uint32_t z[2];
+                for (int gr = 0; gr < G; ++gr) {
+                    uint32_t w[2][2], z[2];                            // [eight slots][channels 0..3, 4..7] of the even (low half) and odd slot
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const int slot = 16 * b + 8 * r + 2 * t;
-                        const uint2 v = *reinterpret_cast<const uint2*>(tile + kv4_v_chunk(G, gr, slot, g));
+                        const uint2 v = *reinterpret_cast<const uint2*>(vals + 1024 * gr + 256 * r);
                         w[r][0] = __byte_perm(v.x, v.y, 0x5410);
                         w[r][1] = __byte_perm(v.x, v.y, 0x7632);
-                        z[r] = *reinterpret_cast<const uint32_t*>(tile + kv4_v_zero(G, gr, slot));
-                        if (!whole) {
-                            const int j = j0 + slot;
-                            if (j > at.k.hi_max || (j < at.k.lo_min && j >= P.sinks)) z[r] &= 0xFFFF0000u;
-                            if (j + 1 > at.k.hi_max || (j + 1 < at.k.lo_min && j + 1 >= P.sinks)) z[r] &= 0x0000FFFFu;
+                        z[r] = *reinterpret_cast<const uint32_t*>(zeros + 64 * gr + 16 * r);
+                        if (MASKED) {
+                            const int j = j0 + 16 * b + 8 * r + 2 * t;
+                            if (nobody(j)) z[r] &= 0xFFFF0000u;
+                            if (nobody(j + 1)) z[r] &= 0x0000FFFFu;
                         }
                     }
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        mma_f16(zero[nb][gr], z[0], z[0], z[1], z[1], pf[nb][gr][2 * b], pf[nb][gr][2 * b + 1]);
+                        mma_f16(zero[nb][gr], z[0], z[0], z[1], z[1], pf[nb][gr][0], pf[nb][gr][1]);
 #pragma unroll
                         for (int m = 0; m < 4; ++m) {
                             const uint32_t wa = w[0][m >> 1] >> (8 * (m & 1)), wb = w[1][m >> 1] >> (8 * (m & 1));
-                            mma_f16(o[nb][gr][m], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu, wb & 0x00F000F0u, pf[nb][gr][2 * b],
-                                    pf[nb][gr][2 * b + 1]);
+                            mma_f16(o[nb][gr][m], wa & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x000F000Fu, wb & 0x00F000F0u, pf[nb][gr][0], pf[nb][gr][1]);
                         }
                     }
                 }
+            };
+            if (__builtin_expect(whole, 1)) {
+#pragma unroll 1
+                for (int b = 0; b < 2; ++b) sixteen(std::false_type{}, b);
+            } else {
+#pragma unroll 1
+                for (int b = 0; b < 2; ++b) sixteen(std::true_type{}, b);
+            }
             __syncwarp();
             fetch();
         }
@@ -754,7 +812,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
 #pragma unroll
                 for (int s2 = 4; s2 < 32; s2 <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, s2);
                 st[nb].sum[c] = v;
-                st[nb].ref[c] = ref[nb][c];
+                st[nb].ref[c] = room[nb][c] == -INFINITY ? -INFINITY : -base[nb][c];
             }
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
@@ -766,36 +824,27 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
                         st[nb].o[16 * gr + 4 * m + r] = fmaf(o[nb][gr][m][r], r < 2 ? 0x1p24f : 0x1p20f, -zero[nb][gr][r & 1]) * down;
             }
         }
-        healthy = __syncthreads_and(healthy);
-        if (healthy) {
-            if (warp >= 2)
+        if (!__syncthreads_and(healthy)) break;
+        // in two rounds (rolled: the code of one): warps 2, 3 into 0, 1, then warp 1 into 0
+#pragma unroll 1
+        for (int half = KA_WARPS / 2; half > 0; half >>= 1) {
+            if (warp >= half && warp < 2 * half)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) st[nb].store(region + ((warp - 2) * NB + nb) * (16 * G + 4) * 32, lane);
+                for (int nb = 0; nb < NB; ++nb) st[nb].store(region + ((warp - half) * NB + nb) * STATE, lane);
             __syncthreads();
-            if (warp < 2)
+            if (warp < half)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) st[nb].join(region + (warp * NB + nb) * (16 * G + 4) * 32, lane);
+                for (int nb = 0; nb < NB; ++nb) st[nb].join(region + (warp * NB + nb) * STATE, lane);
             __syncthreads();
-            if (warp == 1)
+        }
+        if (warp == 0) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) st[nb].store(region + nb * (16 * G + 4) * 32, lane);
-            __syncthreads();
-            if (warp == 0) {
-                float* to = W.partial + (blockIdx.x * 2ll + (i > start ? 1 : 0)) * ka_state_floats(G, NB) * 32;
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    st[nb].join(region + nb * (16 * G + 4) * 32, lane);
-                    if (complete) kv4_write_out<G>(P, st[nb], seq, at.kvh, col0 + 8 * nb, W.cols, D, 0, lane);
-                    else st[nb].store(to + nb * (16 * G + 4) * 32, lane);
-                }
-                if (at.i == 0 && here < at.k.n && lane == 0) {               // it begins here and goes on
-                    const long long rest = at.k.n - at.i - here;
-                    W.joins[blockIdx.x] = make_int4(at.e, at.kvh, i > start ? 1 : 0, (int)((rest + per - 1) / per));
-                }
+            for (int nb = 0; nb < NB; ++nb) {
+                if (complete) kv4_write_out<G>(P, st[nb], seq, kvh, col0 + 8 * nb, W.cols, D, 0, lane);
+                else st[nb].store(W.partial + ((blockIdx.x * 2ll + (i > start ? 1 : 0)) * NB + nb) * STATE, lane);
             }
-            __syncthreads();
-        } else {
-            break;
+            if (at.i == 0 && here < at.k.n && lane == 0)               // it begins here and goes on
+                W.joins[blockIdx.x] = make_int4(at.e, kvh, i > start ? 1 : 0, (at.k.n - here + per - 1) / per);
         }
         i += here;
         if (i < end) forward(at, here);

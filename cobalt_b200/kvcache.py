@@ -64,7 +64,7 @@ class KVCache4:
         self._lib = _lib.load()
 
     # ------------------------------------------------------------------ arguments
-    def _check(self, name: str, t: torch.Tensor, width: int, lead=None) -> torch.Tensor:
+    def _check(self, name: str, t: torch.Tensor, width: int, lead=None, align: int = 4) -> torch.Tensor:
         """``t [n, T, width]`` (or ``[T, width]``: one sequence) as rows the kernels take."""
         if not t.is_cuda or not self.tiles.is_cuda:
             raise RuntimeError("KVCache4 needs CUDA tensors; there is no CPU path")
@@ -77,7 +77,7 @@ class KVCache4:
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient: KVCache4 has no backward pass (use torch.no_grad())")
         rows = t if t.dim() == 2 else t.reshape(-1, width)
-        if rows.stride(1) != 1 or rows.stride(0) % 2 or rows.stride(0) < width or rows.data_ptr() % 4:
+        if rows.stride(1) != 1 or rows.stride(0) * 2 % align or rows.stride(0) < width or rows.data_ptr() % align:
             rows = rows.clone(memory_format=torch.contiguous_format)
         return rows
 
@@ -171,7 +171,7 @@ class KVCache4:
         heads = q.shape[-1] // D
         if heads < 1 or heads % self.n_kv_heads:
             raise ValueError(f"q must hold a multiple of {self.n_kv_heads} heads of {D}, got {list(q.shape)}")
-        qr = self._check("q", q, heads * D)
+        qr = self._check("q", q, heads * D, align=16)
         n, T = self._lead(q)
         window, sinks = int(window), int(sinks)
         if window < 0 or sinks < 0 or window >= 1 << 31 or sinks >= 1 << 31:

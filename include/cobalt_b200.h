@@ -354,7 +354,7 @@ int cobalt_attn_prompt(const void* q, const void* k_cache, const void* v_cache, 
  *                       the per-head norm of cobalt_rope_kv() if k_norm_w is given and its rotation if inv_freq is; so does q (may be NULL) with
  *                       q_norm_w, into q_out (may be q).  v is stored as it is.
  *   cobalt_kv4_read   : the slots at the positions, as bf16 [rows][n_kv_heads][head_dim]; a position outside [0, n_slots) reads as zeros.
- *   cobalt_kv4_attend : grouped-query attention of the tokens (q [rows] x ld_q, rotated) over the cache, out [rows][n_heads * head_dim]
+ *   cobalt_kv4_attend : grouped-query attention of the tokens (q [rows] x ld_q, rotated; 16-byte aligned, ld_q % 8 == 0) over the cache, out [rows][n_heads * head_dim]
  *                       (16-byte aligned).  A token at position p sees slot j < n_slots if j <= p and (window == 0 or j > p - window or
  *                       j < sinks); one that sees none (p < 0: padding) gets zeros.  Scores, softmax and sums in fp32, one rounding
  *                       at the end.  scratch: cobalt_kv4_attend_scratch_bytes() (0: none needed), 256-byte aligned, contents irrelevant;

@@ -58,7 +58,7 @@ def test_append_refuses(lib, kw):
     assert _append(lib, **kw) == -1
 
 
-@pytest.mark.parametrize("kw", [dict(q=None), dict(q=4098), dict(ld_q=127), dict(ld_q=64), dict(out=None), dict(out=4104), dict(nh=0), dict(nh=3, nkv=2, ld_q=512),
+@pytest.mark.parametrize("kw", [dict(q=None), dict(q=4104), dict(ld_q=132), dict(ld_q=64), dict(out=None), dict(out=4104), dict(nh=0), dict(nh=3, nkv=2, ld_q=512),
                                 dict(w=-1), dict(s=-1)])
 def test_attend_refuses(lib, kw):
     assert _attend(lib, **kw) == -1
