@@ -1,4 +1,6 @@
 // C ABI of the 4-bit KV cache: argument validation and launches.  See include/cobalt_b200.h.
+#include <math.h>
+
 #include "kv4_kernels.cuh"
 
 using namespace cb;
@@ -66,7 +68,7 @@ int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, i
     c->col_tiles = (eights + c->nb - 1) / c->nb;
     const double all = (double)n_seq * c->col_tiles * n_kv, tiles = all * ((n_slots + KV4_TILE - 1) / KV4_TILE);
     c->split = (int64_t)n_seq * c->col_tiles <= KA_ENTRIES && tiles < 1e9;
-    const double most = (double)sms * ka_ctas_per_sm(G, c->nb), need = tiles / KA_MIN_TILES;
+    const double most = fmin((double)sms * ka_ctas_per_sm(G, c->nb), KC_MAX_STATES), need = tiles / KA_MIN_TILES;
     if (!c->split && all > 2e9) return COBALT_ETOOBIG;
     c->grid = (int)(!c->split ? all : need < 1 ? 1 : need < most ? need + 0.999 : most);
     c->joins_off = (size_t)c->grid * 2 * ka_state_floats(G, c->nb) * 128;
@@ -91,13 +93,14 @@ int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c
     cfg.blockDim = dim3(KA_THREADS);
     cfg.dynamicSmemBytes = ka_smem_bytes(G, NB);
     cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    // (an early start of this kernel under its predecessor left SMs with a carve-out too small for all CTAs: 99 -> 126 us for 440 MB)
     if (cudaLaunchKernelEx(&cfg, kv4_attend_kernel<G, NB>, P, W) != cudaSuccess) return COBALT_ELAUNCH;
     if (!c.split) return COBALT_OK;
     cfg.gridDim = dim3((unsigned)c.grid, NB, G);
-    cfg.blockDim = dim3(32 * KC_WARPS);
+    cfg.blockDim = dim3(KC_THREADS);
     cfg.dynamicSmemBytes = 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<G, NB>, P, W) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
 }
 

@@ -384,8 +384,7 @@ struct Kv4State {
 #pragma unroll
         for (int i = 0; i < 16 * G; ++i) p[(4 + i) * 32 + lane] = o[i];
     }
-    // p: references and sums, po: values (of G groups out of those in memory)
-    __device__ __forceinline__ void join(const float* p, const float* po, int lane) {
+    __device__ __forceinline__ void join(const float* p, int lane) {
         float mine[2], other[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -396,9 +395,8 @@ struct Kv4State {
             sum[c] = sum[c] * mine[c] + p[(2 + c) * 32 + lane] * other[c];
         }
 #pragma unroll
-        for (int i = 0; i < 16 * G; ++i) o[i] = o[i] * mine[i & 1] + po[i * 32 + lane] * other[i & 1];
+        for (int i = 0; i < 16 * G; ++i) o[i] = o[i] * mine[i & 1] + p[(4 + i) * 32 + lane] * other[i & 1];
     }
-    __device__ __forceinline__ void join(const float* p, int lane) { join(p, p + 4 * 32, lane); }
 };
 template <int G>
 __device__ __forceinline__ void kv4_write_out(const Kv4AttendParams& P, const Kv4State<G>& st, int seq, int kvh, int col0, int cols, int D, int first_group, int lane) {
@@ -854,31 +852,62 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
 }
 
 // Heads that lie in several CTAs of kv4_attend_kernel: block (b, y, z) joins eight columns and a group of channels of the head that begins in
-// CTA b.  Its states are slot 1 (or 0: the CTA began with it) of CTA b and slot 0 of the CTAs behind.
-constexpr int KC_WARPS = 8;
+// CTA b.  Its states are slot 1 (or 0: the CTA began with it) of CTA b and slot 0 of the CTAs behind.  First the weight of every state
+// (one load round for all of them), then the weighted sums: four warps share the states, a lane has four values of each, four states
+// in flight.  State by state with rescaling, one chain of loads per warp, 71 states of a head of 256 took 51 us.
+constexpr int KC_THREADS = 512, KC_SHARE = 4;                          // KC_SHARE warps of the same four values
+constexpr int KC_MAX_STATES = 1024;                                    // of one head: the CTAs that a launch has at most
 template <int G, int NB>
-__global__ void __launch_bounds__(32 * KC_WARPS) kv4_combine_kernel(const Kv4AttendParams P, const Kv4Work W) {
-    __shared__ float region[KC_WARPS][20][32];
+__global__ void __launch_bounds__(KC_THREADS) kv4_combine_kernel(const Kv4AttendParams P, const Kv4Work W) {
+    constexpr int STATE = (16 * G + 4) * 32;
+    __shared__ float weight[8][KC_MAX_STATES + 1];
+    __shared__ float total[8];
+    __shared__ float part[KC_SHARE][16][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 j = W.joins[blockIdx.x];
     if (j.x < 0) return;
-    const int nb = blockIdx.y, gr = blockIdx.z, seq = j.x / W.col_tiles, col0 = (j.x - seq * W.col_tiles) * 8 * NB + 8 * nb;
-    Kv4State<1> st;
+    const int n = j.w + 1, nb = blockIdx.y, gr = blockIdx.z, seq = j.x / W.col_tiles, col0 = (j.x - seq * W.col_tiles) * 8 * NB + 8 * nb;
+    auto state = [&](int k) { return W.partial + (((long long)(blockIdx.x + k) * 2 + (k == 0 ? j.z : 0)) * NB + nb) * STATE; };
+    // references and sums of the eight columns: lane t of a state's first four has columns 2t, 2t + 1
+    const int c = warp & 7, at = (c & 1) * 32 + (c >> 1);
+    float top = -INFINITY;
+    if (warp < 8)
+        for (int k = lane; k < n; k += 32) top = fmaxf(top, weight[c][k] = state(k)[at]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) st.o[i] = 0.0f;
-    st.ref[0] = st.ref[1] = -INFINITY;
-    st.sum[0] = st.sum[1] = 0.0f;
-#pragma unroll 2
-    for (int k = warp; k <= j.w; k += KC_WARPS) {
-        const float* p = W.partial + ((long long)(blockIdx.x + k) * 2 + (k == 0 ? j.z : 0)) * ka_state_floats(G, NB) * 32 + nb * (16 * G + 4) * 32;
-        st.join(p, p + (4 + 16 * gr) * 32, lane);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (top == -INFINITY) top = 0.0f;
+    if (warp < 8) {
+        float sum = 0.0f;
+        for (int k = lane; k < n; k += 32) {
+            const float w = ex2(weight[c][k] - top);
+            weight[c][k] = w;
+            sum = fmaf(w, state(k)[at + 64], sum);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (lane == 0) total[c] = sum;
     }
-    st.store(&region[warp][0][0], lane);
+    __syncthreads();
+    const int quad = warp & 3, share = warp >> 2, t = lane & 3;
+    float acc[4] = {};
+    const float *w0 = weight[2 * t], *w1 = weight[2 * t + 1];
+#pragma unroll 4
+    for (int k = share; k < n; k += KC_SHARE) {
+        const float* p = state(k) + (4 + 16 * gr + 4 * quad) * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(p[32 * i], i & 1 ? w1[k] : w0[k], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[share][4 * quad + i][lane] = acc[i];
     __syncthreads();
     if (warp == 0) {
-        for (int w = 1; w < min(KC_WARPS, j.w + 1); ++w) st.join(&region[w][0][0], lane);
+        Kv4State<1> st;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[i] = (part[0][i][lane] + part[1][i][lane]) + (part[2][i][lane] + part[3][i][lane]);
+        st.sum[0] = total[2 * t];
+        st.sum[1] = total[2 * t + 1];
         kv4_write_out<1>(P, st, seq, j.y, col0, W.cols, 64 * G, gr, lane);
     }
 }
