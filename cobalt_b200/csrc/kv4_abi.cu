@@ -1,7 +1,7 @@
 // C ABI of the 4-bit KV cache: argument validation and launches.  See include/cobalt_b200.h.
-#include <math.h>
+#include <algorithm>
 
-#include "kv4_kernels.cuh"
+#include "kv4_attend.cuh"
 
 using namespace cb;
 
@@ -51,13 +51,16 @@ int make_cache(Kv4Cache* c, const void* tiles, int64_t seq_stride, const int64_t
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 3) && !(ld & 1) && ld >= width; }
 
 struct AttendCfg {
-    int cols, nb, col_tiles, grid;
-    bool split;
+    int cols, nb, col_tiles;
+    bool list;
+    int grid, share;                   // CTAs; heads: CTAs of a head's cluster
     size_t joins_off, scratch;
 };
-// Columns are spread evenly over the fewest tiles of 8 * nb that a warp's registers hold.  CTAs fill the GPU once, each with a tile of slots
-// per warp at least; or a CTA per head, where there are that many.
-int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, int sms, AttendCfg* c) {
+// Columns are spread evenly over the fewest tiles of 8 * nb that a warp's registers hold.  How the work is shared:
+//   a cluster per head, as large as fills the GPU once, while that leaves a warp few tiles, or where there are heads enough for several
+//   CTAs per SM, or more entries than a list takes;
+//   else the list.
+int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, int window, int sinks, int sms, AttendCfg* c) {
     const int G = D / KV4_GROUP;
     const int64_t cols = (int64_t)(n_heads / n_kv) * T;
     if (cols > 0x3FFFFFFFll) return COBALT_ETOOBIG;
@@ -66,13 +69,19 @@ int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, i
     c->col_tiles = (eights + ka_max_nb(G) - 1) / ka_max_nb(G);
     c->nb = (eights + c->col_tiles - 1) / c->col_tiles;
     c->col_tiles = (eights + c->nb - 1) / c->nb;
-    const double all = (double)n_seq * c->col_tiles * n_kv, tiles = all * ((n_slots + KV4_TILE - 1) / KV4_TILE);
-    c->split = (int64_t)n_seq * c->col_tiles <= KA_ENTRIES && tiles < 1e9;
-    const double most = fmin((double)sms * ka_ctas_per_sm(G, c->nb), KC_MAX_STATES), need = tiles / KA_MIN_TILES;
-    if (!c->split && all > 2e9) return COBALT_ETOOBIG;
-    c->grid = (int)(!c->split ? all : need < 1 ? 1 : need < most ? need + 0.999 : most);
+    const int64_t entries = (int64_t)n_seq * c->col_tiles, heads = entries * n_kv;
+    if (heads > 0x3FFFFFFFll) return COBALT_ETOOBIG;
+    const int ctas = std::min(sms * ka_ctas_per_sm(G, c->nb), KC_MAX_STATES);
+    // tiles of a head at most, if its tokens follow one another
+    int64_t tiles = (n_slots + KV4_TILE - 1) / KV4_TILE;
+    if (window > 0) tiles = std::min(tiles, ((int64_t)window + T) / KV4_TILE + 2 + ((int64_t)sinks + KV4_TILE - 1) / KV4_TILE);
+    c->share = 1;
+    while (c->share < KA_MAX_CLUSTER && c->share * 2 * heads <= ctas && c->share * KA_MIN_TILES < tiles) c->share *= 2;
+    c->list = entries <= KA_ENTRIES && heads * tiles < 1000000000ll && heads < 4ll * ctas && tiles > (int64_t)c->share * KA_WARPS * KA_LIST_TILES;
+    c->grid = c->list ? (int)std::min<int64_t>(ctas, (heads * tiles + KA_MIN_TILES - 1) / KA_MIN_TILES) : (int)heads * c->share;
+    if (!c->list && heads * c->share > 0x7FFFFFFFll) return COBALT_ETOOBIG;
     c->joins_off = (size_t)c->grid * 2 * ka_state_floats(G, c->nb) * 128;
-    c->scratch = c->split ? c->joins_off + (size_t)c->grid * sizeof(int4) : 0;
+    c->scratch = c->list ? c->joins_off + (size_t)c->grid * sizeof(int4) : 0;
     return COBALT_OK;
 }
 template <int G, int NB>
@@ -81,25 +90,34 @@ int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(kv4_attend_kernel<G, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_smem_bytes(G, NB)) != cudaSuccess)
+        if (cudaFuncSetAttribute(kv4_attend_list_kernel<G, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_list_smem(G, NB)) != cudaSuccess ||
+            cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_heads_smem(G, NB)) != cudaSuccess ||
+            cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return COBALT_ELAUNCH;
         configured[dev] = true;
     }
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)c.grid);
     cfg.blockDim = dim3(KA_THREADS);
-    cfg.dynamicSmemBytes = ka_smem_bytes(G, NB);
     cfg.stream = st;
+    cfg.attrs = attr;
+    if (!c.list) {
+        cfg.dynamicSmemBytes = ka_heads_smem(G, NB);
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)c.share;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = c.share > 1 ? 1 : 0;
+        return cudaLaunchKernelEx(&cfg, kv4_attend_heads_kernel<G, NB>, P, c.share) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+    }
+    cfg.dynamicSmemBytes = ka_list_smem(G, NB);
     // (an early start of this kernel under its predecessor left SMs with a carve-out too small for all CTAs: 99 -> 126 us for 440 MB)
-    if (cudaLaunchKernelEx(&cfg, kv4_attend_kernel<G, NB>, P, W) != cudaSuccess) return COBALT_ELAUNCH;
-    if (!c.split) return COBALT_OK;
+    if (cudaLaunchKernelEx(&cfg, kv4_attend_list_kernel<G, NB>, P, W) != cudaSuccess) return COBALT_ELAUNCH;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)c.grid, NB, G);
     cfg.blockDim = dim3(KC_THREADS);
     cfg.dynamicSmemBytes = 0;
-    cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<G, NB>, P, W) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
 }
@@ -162,11 +180,12 @@ int cobalt_kv4_read(const void* tiles, int64_t tiles_seq_stride, const int64_t* 
     return launched();
 }
 
-size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots) {
+size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks) {
     int sms = 0;
-    if (n_seq <= 0 || T <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_slots <= 0 || !dim_ok(head_dim) || sm_count(&sms)) return 0;
+    if (n_seq <= 0 || T <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_slots <= 0 || window < 0 || sinks < 0 ||
+        !dim_ok(head_dim) || sm_count(&sms)) return 0;
     AttendCfg c;
-    return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms, &c) ? 0 : c.scratch;
+    return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c) ? 0 : c.scratch;
 }
 
 int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
@@ -180,8 +199,8 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
     AttendCfg c;
-    if ((rc = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, sms, &c))) return rc;
-    if (c.split && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < c.scratch)) return COBALT_ESCRATCH;
+    if ((rc = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c))) return rc;
+    if (c.list && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < c.scratch)) return COBALT_ESCRATCH;
     P.q = (const uint16_t*)q; P.ld_q = ld_q;
     P.positions = (const long long*)positions;
     P.pos_stride = pos_seq_stride;
@@ -189,10 +208,9 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     P.n_seq = n_seq; P.T = T; P.n_heads = n_heads; P.rep = n_heads / n_kv_heads;
     P.window = window; P.sinks = sinks;
     P.scale_log2 = scale * 1.44269504f;
+    P.cols = c.cols; P.col_tiles = c.col_tiles;
+    P.by_rep = kv4_div(P.rep); P.by_tiles = kv4_div(c.col_tiles); P.by_kv = kv4_div(n_kv_heads);
     Kv4Work W;
-    W.cols = c.cols;
-    W.col_tiles = c.col_tiles;
-    W.split = c.split;
     W.partial = (float*)scratch;
     W.joins = (int4*)((uint8_t*)scratch + c.joins_off);
     switch (head_dim / KV4_GROUP * 10 + c.nb) {

@@ -182,7 +182,7 @@ class KVCache4:
             raise ValueError("out must be a contiguous tensor like q on a 16-byte boundary")
         pos, stride, tiles = self._place(positions, n, T, seq)
         if n * T:
-            need = self._lib.cobalt_kv4_attend_scratch_bytes(n, T, heads, self.n_kv_heads, D, self.slots)
+            need = self._lib.cobalt_kv4_attend_scratch_bytes(n, T, heads, self.n_kv_heads, D, self.slots, window, sinks)
             # a buffer per call, from the stream's own pool: calls on other streams and captured graphs never share one
             scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
             self._call("cobalt_kv4_attend", qr.data_ptr(), qr.stride(0), tiles, self.tiles.stride(0), pos.data_ptr(), stride, out.data_ptr(), n, T,

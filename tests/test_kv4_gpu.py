@@ -207,6 +207,14 @@ CASES = [  # n, T, heads, n_kv, D, slots, positions of the last token per sequen
     (1, 64, 4, 2, 256, 200, [199], 0, 0, 1.0),
     (1, 200, 4, 4, 192, 200, [199], 50, 1, 1.0),
     (1, 40, 130, 1, 64, 60, [59], 0, 0, 1.0),                  # more heads to one than a tile has rows
+    (3, 1, 8, 2, 64, 40000, [39999, 5, 20001], 0, 0, 1.0),     # few and long heads: their tiles in equal ranges
+    (2, 1, 4, 1, 128, 30000, [29999, 28000], 27001, 40, 4.0),
+    (5, 2, 12, 1, 64, 24000, [23999, 1, 12000, 31, 32], 0, 0, 1.0),
+    (3, 1, 3, 1, 192, 20000, [19999, 19000, 100], 0, 0, 1.0),
+    (2, 1, 2, 1, 256, 20000, [17777, 19999], 0, 0, 1.0),
+    (4, 3, 5, 1, 128, 21000, [20999, 20000, 2, 640], 20500, 3, 1.0),
+    (100, 1, 16, 16, 64, 100, list(range(100)), 0, 0, 1.0),    # heads enough for several CTAs per SM
+    (300, 1, 2, 1, 64, 260, [(7 * i) % 260 for i in range(300)], 0, 0, 1.0),   # more sequences than a list takes
 ]
 
 
