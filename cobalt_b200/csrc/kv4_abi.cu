@@ -56,10 +56,12 @@ struct AttendCfg {
     int grid, share;                   // CTAs; heads: CTAs of a head's cluster
     size_t joins_off, scratch;
 };
-// Columns are spread evenly over the fewest tiles of 8 * nb that a warp's registers hold.  How the work is shared:
-//   a cluster per head, as large as fills the GPU once, while that leaves a warp few tiles, or where there are heads enough for several
-//   CTAs per SM, or more entries than a list takes;
-//   else the list.
+// Columns are spread evenly over the fewest tiles of 8 * nb that a warp's registers hold.  The work goes by heads, a cluster as large as fills
+// the GPU once for each, or by the list, which costs its look-ups and a second kernel but leaves no SM idle and no warp with more
+// than its share.  Measured with one token, 32 / 8 heads of 128 (heads / list, us): one sequence of 8192 slots 14.4 / 16.4, 16384 22.1 / 21.7,
+// 32768 38.1 / 24.6; 4 sequences of 16384 26.1 / 29.1, 32768 45.8 / 45.7; 16 sequences of 16384 68.7 / 75.9, of 9830 to 32768
+// 94.3 / 92.3; 8 / 1 heads of 256, one sequence of 2048 9.9 / 10.7, 4096 12.5 / 11.3.  They meet at 6 tiles per warp plus 64 times the
+// share of the GPU that the clusters fill.  A CTA per head where there are heads for several CTAs per SM.
 int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, int window, int sinks, int sms, AttendCfg* c) {
     const int G = D / KV4_GROUP;
     const int64_t cols = (int64_t)(n_heads / n_kv) * T;
@@ -77,7 +79,8 @@ int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, i
     if (window > 0) tiles = std::min(tiles, ((int64_t)window + T) / KV4_TILE + 2 + ((int64_t)sinks + KV4_TILE - 1) / KV4_TILE);
     c->share = 1;
     while (c->share < KA_MAX_CLUSTER && c->share * 2 * heads <= ctas && c->share * KA_MIN_TILES < tiles) c->share *= 2;
-    c->list = entries <= KA_ENTRIES && heads * tiles < 1000000000ll && heads < 4ll * ctas && tiles > (int64_t)c->share * KA_WARPS * KA_LIST_TILES;
+    c->list = entries <= KA_ENTRIES && heads * tiles < 1000000000ll && heads < 4ll * ctas && 
+              tiles * ctas > c->share * KA_WARPS * (6ll * ctas + 64 * heads * c->share);
     c->grid = c->list ? (int)std::min<int64_t>(ctas, (heads * tiles + KA_MIN_TILES - 1) / KA_MIN_TILES) : (int)heads * c->share;
     if (!c->list && heads * c->share > 0x7FFFFFFFll) return COBALT_ETOOBIG;
     c->joins_off = (size_t)c->grid * 2 * ka_state_floats(G, c->nb) * 128;

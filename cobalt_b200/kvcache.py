@@ -9,6 +9,7 @@ There is no backward pass (codes have no gradient) and no torch fallback: on a n
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -21,8 +22,10 @@ TILE = 32
 HEAD_DIMS = (64, 128, 192, 256)
 
 
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+@functools.lru_cache(maxsize=4096)
+def _attend_scratch(device: int, *sizes: int) -> int:
+    with torch.cuda.device(device):
+        return _lib.load().cobalt_kv4_attend_scratch_bytes(*sizes)
 
 
 class KVCache4:
@@ -45,66 +48,76 @@ class KVCache4:
         """A cache over existing tiles ``[n_seq, n_kv_heads, n_tiles, 36 * head_dim]`` (shared, not copied); the sequences may lie apart."""
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
-        if tiles.dtype is not torch.uint8 or tiles.dim() != 4 or tiles.shape[3] != 36 * head_dim or 0 in tiles.shape:
-            raise ValueError(f"tiles must be uint8 [n_seq, n_kv_heads, n_tiles, {36 * head_dim}], got {tiles.dtype} {list(tiles.shape)}")
-        if not tiles[0].is_contiguous() or tiles.stride(0) % 16 or tiles.data_ptr() % 16 or (
-                tiles.shape[0] > 1 and tiles.stride(0) < tiles[0].numel()):
+        row, shape = 36 * head_dim, tiles.shape
+        if tiles.dtype is not torch.uint8 or len(shape) != 4 or shape[3] != row or 0 in shape:
+            raise ValueError(f"tiles must be uint8 [n_seq, n_kv_heads, n_tiles, {row}], got {tiles.dtype} {list(shape)}")
+        _, heads, n, _ = shape
+        apart, *inner = tiles.stride()
+        if inner != [n * row, row, 1] or apart % 16 or tiles.data_ptr() % 16 or (shape[0] > 1 and apart < heads * n * row):
             raise ValueError("the tiles of a sequence must be contiguous, and sequences must begin on 16-byte boundaries without overlap")
-        n = tiles.shape[2]
-        if slots is not None and not (n - 1) * TILE < slots <= n * TILE:
+        if slots is None:
+            slots = n * TILE
+        elif not (n - 1) * TILE < slots <= n * TILE:
             raise ValueError(f"{n} tiles hold {n * TILE} slots, not {slots}")
         obj = cls.__new__(cls)
-        obj._install(tiles, head_dim, n * TILE if slots is None else slots)
+        obj._install(tiles, head_dim, slots)
         return obj
 
     def _install(self, tiles, head_dim, slots):
         self.tiles, self.head_dim, self.slots = tiles, int(head_dim), int(slots)
         self.n_seq, self.n_kv_heads = tiles.shape[0], tiles.shape[1]
-        self.device = tiles.device
+        self._index = tiles.get_device()                     # -1: not on a GPU
+        self._apart = tiles.stride(0) if self.n_seq > 1 else 0
         self._lib = _lib.load()
 
+    @property
+    def device(self) -> torch.device:
+        return self.tiles.device
+
     # ------------------------------------------------------------------ arguments
-    def _check(self, name: str, t: torch.Tensor, width: int, lead=None, align: int = 4) -> torch.Tensor:
-        """``t [n, T, width]`` (or ``[T, width]``: one sequence) as rows the kernels take."""
-        if not t.is_cuda or not self.tiles.is_cuda:
+    def _rows(self, name: str, t: torch.Tensor, width: int, lead, align: int):
+        """(address, row stride, owner of the memory) of ``t [n, T, width]`` (or ``[T, width]``: one sequence) as rows the kernels take."""
+        if self._index < 0 or not t.is_cuda:
             raise RuntimeError("KVCache4 needs CUDA tensors; there is no CPU path")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         if t.dtype is not torch.bfloat16:
             raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
-        if t.dim() not in (2, 3) or t.shape[-1] != width or (lead is not None and t.shape[:-1] != lead):
-            raise ValueError(f"{name} must be [n, T, {width}]{'' if lead is None else ' with [n, T] = ' + str(list(lead))}, got {list(t.shape)}")
+        shape = t.shape
+        if not 2 <= len(shape) <= 3 or shape[-1] != width or (lead is not None and shape[:-1] != lead):
+            raise ValueError(f"{name} must be [n, T, {width}]{'' if lead is None else ' with [n, T] = ' + str(list(lead))}, got {list(shape)}")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient: KVCache4 has no backward pass (use torch.no_grad())")
-        rows = t if t.dim() == 2 else t.reshape(-1, width)
+        p = t.data_ptr()
+        if p % align == 0 and t.is_contiguous():
+            return p, width, t
+        rows = t if len(shape) == 2 else t.reshape(-1, width)
         if rows.stride(1) != 1 or rows.stride(0) * 2 % align or rows.stride(0) < width or rows.data_ptr() % align:
             rows = rows.clone(memory_format=torch.contiguous_format)
-        return rows
+        return rows.data_ptr(), rows.stride(0), rows
 
     def _place(self, positions: torch.Tensor, n: int, T: int, seq: int):
-        """(positions, their stride from sequence to sequence, address of the first sequence's tiles)"""
-        if positions.dtype is not torch.int64 or positions.device != self.device:
+        """(address of the positions, their stride from sequence to sequence, address of the first sequence's tiles, owner of the positions)"""
+        if positions.dtype is not torch.int64 or positions.get_device() != self._index:
             raise TypeError(f"positions must be int64 on {self.device}, got {positions.dtype} on {positions.device}")
-        if positions.shape != (n, T) and positions.shape != (T,):
-            raise ValueError(f"positions must be [{n}, {T}] or [{T}], got {list(positions.shape)}")
+        shape = positions.shape
+        if shape != (n, T) and shape != (T,):
+            raise ValueError(f"positions must be [{n}, {T}] or [{T}], got {list(shape)}")
         if seq < 0 or seq + n > self.n_seq:
             raise ValueError(f"sequences {seq} .. {seq + n - 1} of a cache of {self.n_seq}")
-        if positions.stride(-1) != 1 and T > 1:
+        stride = positions.stride()
+        if stride[-1] != 1 and T > 1:
             positions = positions.contiguous()
-        stride = positions.stride(0) if positions.dim() == 2 and n > 1 else 0
-        return positions, stride, self.tiles.data_ptr() + seq * self.tiles.stride(0)
-
-    @staticmethod
-    def _lead(t: torch.Tensor):
-        return (1, t.shape[0]) if t.dim() == 2 else tuple(t.shape[:2])
+            stride = positions.stride()
+        return positions.data_ptr(), stride[0] if n > 1 and len(shape) == 2 else 0, self.tiles.data_ptr() + seq * self._apart, positions
 
     def _call(self, name: str, *args):
-        index = self.device.index
-        if index != torch._C._cuda_getDevice():
+        index = self._index
+        if index == torch._C._cuda_getDevice():
+            rc = getattr(self._lib, name)(*args, _raw_stream(index))
+        else:
             with torch.cuda.device(index):
                 rc = getattr(self._lib, name)(*args, _raw_stream(index))
-        else:
-            rc = getattr(self._lib, name)(*args, _raw_stream(index))
         if rc:
             _lib.check(name, rc)
 
@@ -117,14 +130,15 @@ class KVCache4:
         ``cobalt_rope_kv`` does, and with ``k_norm`` (bf16 ``[head_dim]``) normalised per head before that; the same is done to
         ``q [n, T, n_heads * head_dim]`` (``q_norm``), which is returned - in ``q_out`` if given (may be ``q`` itself)."""
         D, width = self.head_dim, self.n_kv_heads * self.head_dim
-        kr, vr = self._check("k", k, width), self._check("v", v, width, k.shape[:-1])
-        n, T = self._lead(k)
-        for name, w, dtype, size in (("inv_freq", inv_freq, torch.float32, D // 2), ("q_norm", q_norm, torch.bfloat16, D),
-                                     ("k_norm", k_norm, torch.bfloat16, D)):
-            if w is not None and (w.dtype is not dtype or w.shape != (size,) or w.device != self.device or not w.is_contiguous()
-                                  or w.data_ptr() % 4):
-                raise ValueError(f"{name} must be a contiguous {dtype} [{size}] on {self.device}")
-        qr, heads = None, 0
+        kp, ld_k, k_own = self._rows("k", k, width, None, 4)
+        lead = k.shape[:-1]
+        vp, ld_v, v_own = self._rows("v", v, width, lead, 4)
+        n, T = lead if len(lead) == 2 else (1, lead[0])
+        if inv_freq is not None:
+            self._weight("inv_freq", inv_freq, torch.float32, D // 2)
+        if k_norm is not None:
+            self._weight("k_norm", k_norm, torch.bfloat16, D)
+        qp, ld_q, op, heads = None, 0, None, 0
         if q is None:
             if q_norm is not None or q_out is not None:
                 raise ValueError("q_norm and q_out belong to a q")
@@ -132,34 +146,41 @@ class KVCache4:
             heads = q.shape[-1] // D
             if heads < 1:
                 raise ValueError(f"q must be [n, T, n_heads * {D}], got {list(q.shape)}")
-            qr = self._check("q", q, heads * D, k.shape[:-1])
+            qp, ld_q, q_own = self._rows("q", q, heads * D, lead, 4)
+            if q_norm is not None:
+                self._weight("q_norm", q_norm, torch.bfloat16, D)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.device != q.device or not q_out.is_contiguous() or q_out.data_ptr() % 4:
                 raise ValueError("q_out must be a contiguous tensor like q")
-        pos, stride, tiles = self._place(positions, n, T, seq)
+            op = q_out.data_ptr()
+        pos, stride, tiles, p_own = self._place(positions, n, T, seq)
         if n * T:
-            self._call("cobalt_kv4_append", kr.data_ptr(), kr.stride(0), vr.data_ptr(), vr.stride(0), _ptr(qr), 0 if qr is None else qr.stride(0),
-                       _ptr(q_out), heads * D, pos.data_ptr(), stride, tiles, self.tiles.stride(0), n, T, heads, self.n_kv_heads, D, self.slots,
-                       _ptr(inv_freq), _ptr(q_norm), _ptr(k_norm), float(eps))
+            self._call("cobalt_kv4_append", kp, ld_k, vp, ld_v, qp, ld_q, op, heads * D, pos, stride, tiles, self._apart, n, T, heads, self.n_kv_heads, D,
+                       self.slots, None if inv_freq is None else inv_freq.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
+                       None if k_norm is None else k_norm.data_ptr(), eps)
         return q_out
+
+    def _weight(self, name: str, w: torch.Tensor, dtype, size: int):
+        if w.dtype is not dtype or w.shape != (size,) or w.get_device() != self._index or not w.is_contiguous() or w.data_ptr() % 4:
+            raise ValueError(f"{name} must be a contiguous {dtype} [{size}] on {self.device}")
 
     def read(self, positions: torch.Tensor, seq: int = 0, n: Optional[int] = None):
         """``(k, v)`` bf16 ``[n, T, n_kv_heads, head_dim]`` of the slots at ``positions`` (outside ``[0, slots)``: zeros).  ``n`` says how many
         sequences a ``positions [T]`` is for (all from ``seq`` on by default)."""
-        if not self.tiles.is_cuda:
+        if self._index < 0:
             raise RuntimeError("KVCache4 needs CUDA tensors; there is no CPU path")
-        if positions.dim() not in (1, 2):
-            raise ValueError(f"positions must be [n, T] or [T], got {list(positions.shape)}")
+        shape = positions.shape
+        if not 1 <= len(shape) <= 2:
+            raise ValueError(f"positions must be [n, T] or [T], got {list(shape)}")
         if n is None:
-            n = positions.shape[0] if positions.dim() == 2 else self.n_seq - seq
-        T = positions.shape[-1]
-        pos, stride, tiles = self._place(positions, n, T, seq)
-        k = torch.empty(n, T, self.n_kv_heads, self.head_dim, dtype=torch.bfloat16, device=self.device)
+            n = shape[0] if len(shape) == 2 else self.n_seq - seq
+        T = shape[-1]
+        pos, stride, tiles, p_own = self._place(positions, n, T, seq)
+        k = self.tiles.new_empty((n, T, self.n_kv_heads, self.head_dim), dtype=torch.bfloat16)
         v = torch.empty_like(k)
         if n * T:
-            self._call("cobalt_kv4_read", tiles, self.tiles.stride(0), pos.data_ptr(), stride, k.data_ptr(), v.data_ptr(), n, T, self.n_kv_heads,
-                       self.head_dim, self.slots)
+            self._call("cobalt_kv4_read", tiles, self._apart, pos, stride, k.data_ptr(), v.data_ptr(), n, T, self.n_kv_heads, self.head_dim, self.slots)
         return k, v
 
     def attend(self, q: torch.Tensor, positions: torch.Tensor, window: int = 0, sinks: int = 0, scale: Optional[float] = None, seq: int = 0,
@@ -167,26 +188,26 @@ class KVCache4:
         """Attention of ``q [n, T, n_heads * head_dim]`` (rotated) over the cache; query head ``h`` reads KV head ``h * n_kv_heads // n_heads``.
         A token at position ``p`` sees the slots ``j <= p`` - with ``window > 0`` only the last ``window`` of them and the first ``sinks``
         slots.  One that sees none (``p < 0``: padding) gets zeros.  ``scale``: of the scores, ``head_dim ** -0.5`` by default."""
-        D = self.head_dim
-        heads = q.shape[-1] // D
-        if heads < 1 or heads % self.n_kv_heads:
-            raise ValueError(f"q must hold a multiple of {self.n_kv_heads} heads of {D}, got {list(q.shape)}")
-        qr = self._check("q", q, heads * D, align=16)
-        n, T = self._lead(q)
-        window, sinks = int(window), int(sinks)
-        if window < 0 or sinks < 0 or window >= 1 << 31 or sinks >= 1 << 31:
+        D, n_kv = self.head_dim, self.n_kv_heads
+        shape = q.shape
+        heads = shape[-1] // D
+        if heads < 1 or heads % n_kv:
+            raise ValueError(f"q must hold a multiple of {n_kv} heads of {D}, got {list(shape)}")
+        qp, ld_q, q_own = self._rows("q", q, heads * D, None, 16)
+        n, T = shape[:2] if len(shape) == 3 else (1, shape[0])
+        if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError("window and sinks must be between 0 and 2^31 - 1")
+        pos, stride, tiles, p_own = self._place(positions, n, T, seq)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != shape or out.dtype is not q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be a contiguous tensor like q on a 16-byte boundary")
-        pos, stride, tiles = self._place(positions, n, T, seq)
         if n * T:
-            need = self._lib.cobalt_kv4_attend_scratch_bytes(n, T, heads, self.n_kv_heads, D, self.slots, window, sinks)
+            need = _attend_scratch(self._index, n, T, heads, n_kv, D, self.slots, window, sinks)
             # a buffer per call, from the stream's own pool: calls on other streams and captured graphs never share one
-            scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            self._call("cobalt_kv4_attend", qr.data_ptr(), qr.stride(0), tiles, self.tiles.stride(0), pos.data_ptr(), stride, out.data_ptr(), n, T,
-                       heads, self.n_kv_heads, D, self.slots, window, sinks, D ** -0.5 if scale is None else float(scale), _ptr(scratch), need)
+            scratch = q.new_empty(need, dtype=torch.uint8) if need else None
+            self._call("cobalt_kv4_attend", qp, ld_q, tiles, self._apart, pos, stride, out.data_ptr(), n, T, heads, n_kv, D, self.slots, window, sinks,
+                       D ** -0.5 if scale is None else scale, None if scratch is None else scratch.data_ptr(), need)
         return out
 
     def device_status(self) -> int:
@@ -194,7 +215,7 @@ class KVCache4:
         question (its rows are then not written).  Waits for the current stream."""
         word = ctypes.c_uint32(0)
         with torch.cuda.device(self.device):
-            rc = self._lib.cobalt_kv4_status(_raw_stream(self.device.index), ctypes.byref(word))
+            rc = self._lib.cobalt_kv4_status(_raw_stream(self._index), ctypes.byref(word))
         if rc not in (0, _lib.ETIMEOUT):
             _lib.check("cobalt_kv4_status", rc)
         return int(word.value)
