@@ -47,8 +47,8 @@ int make_cache(Kv4Cache* c, const void* tiles, int64_t seq_stride, const int64_t
     c->seq_stride = seq_stride;
     return COBALT_OK;
 }
-// rows of bf16 that are read four bytes at a time
-bool rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 3) && !(ld & 1) && ld >= width; }
+// rows of bf16 that are read 16 bytes at a time
+bool rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
 
 struct AttendCfg {
     int cols, nb, col_tiles;
@@ -157,14 +157,15 @@ int cobalt_kv4_append(const void* k, int64_t ld_k, const void* v, int64_t ld_v, 
     P.positions = (const long long*)positions;
     P.pos_stride = pos_seq_stride;
     P.T = T; P.n_heads = q ? n_heads : 0;
+    P.by_T = kv4_div(T);
     P.inv_freq = inv_freq;
     P.q_norm = (const uint16_t*)q_norm_w; P.k_norm = (const uint16_t*)k_norm_w;
     P.eps = eps;
-    const int rows = n_seq * T, items = 2 * n_kv_heads + P.n_heads, warps = KV4_THREADS / 32;
+    const int rows = n_seq * T, at_once = 32 / (head_dim / 8), warps = KV4_THREADS / 32;
+    const int items = 2 * ((n_kv_heads + at_once - 1) / at_once) + (P.n_heads + at_once - 1) / at_once;
     // few rows: the heads of a row are spread over blocks until the GPU has about two blocks per SM
     const int most = (items + warps - 1) / warps, want = (2 * sms + rows - 1) / rows;
-    const dim3 grid((unsigned)rows, (unsigned)(want < most ? want : most));
-    KV4_DISPATCH(head_dim, (kv4_append_kernel<G><<<grid, KV4_THREADS, 0, (cudaStream_t)stream>>>(P)));
+    KV4_DISPATCH(head_dim, (kv4_append_kernel<G><<<dim3((unsigned)rows, (unsigned)std::min(want, most)), KV4_THREADS, 0, (cudaStream_t)stream>>>(P)));
     return launched();
 }
 
@@ -173,13 +174,14 @@ int cobalt_kv4_read(const void* tiles, int64_t tiles_seq_stride, const int64_t* 
     Kv4Cache C;
     int rc = make_cache(&C, tiles, tiles_seq_stride, positions, pos_seq_stride, n_seq, T, n_kv_heads, head_dim, n_slots);
     if (rc) return rc;
-    if (!k || !v || (((uintptr_t)k | (uintptr_t)v) & 3)) return COBALT_EINVAL;
+    if (!k || !v || (((uintptr_t)k | (uintptr_t)v) & 15)) return COBALT_EINVAL;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
-    const long long items = (long long)n_seq * T * n_kv_heads, blocks = (items + KV4_THREADS / 32 - 1) / (KV4_THREADS / 32);
+    const int at_once = 32 / (head_dim / 8), per_row = (n_kv_heads + at_once - 1) / at_once;
+    const long long items = (long long)n_seq * T * per_row, blocks = (items + KV4_THREADS / 32 - 1) / (KV4_THREADS / 32);
     if (blocks > 0x7FFFFFFFll) return COBALT_ETOOBIG;
     KV4_DISPATCH(head_dim, (kv4_read_kernel<G><<<(unsigned)blocks, KV4_THREADS, 0, (cudaStream_t)stream>>>(
-                               C, (const long long*)positions, pos_seq_stride, T, items, (uint16_t*)k, (uint16_t*)v)));
+                               C, (const long long*)positions, pos_seq_stride, T, items, per_row, (uint16_t*)k, (uint16_t*)v)));
     return launched();
 }
 
@@ -198,7 +200,7 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     int rc = make_cache(&P.cache, tiles, tiles_seq_stride, positions, pos_seq_stride, n_seq, T, n_kv_heads, head_dim, n_slots);
     if (rc) return rc;
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || window < 0 || sinks < 0) return COBALT_EINVAL;
-    if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || ((uintptr_t)q & 15) || (ld_q & 7) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
+    if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
     AttendCfg c;

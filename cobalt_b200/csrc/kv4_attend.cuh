@@ -25,18 +25,6 @@
 
 namespace cb {
 
-// x / d for 0 <= x < 2^31 (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994)
-struct Kv4Div {
-    uint32_t mul, shift;
-    __device__ __forceinline__ int operator()(int x) const { return (int)((__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift); }
-};
-inline Kv4Div kv4_div(int d) {
-    Kv4Div v = {0, 0};
-    while ((1ll << v.shift) < d) ++v.shift;
-    v.mul = (uint32_t)((((1ull << v.shift) - (uint64_t)d) << 32) / (uint64_t)d + 1);
-    return v;
-}
-
 struct Kv4AttendParams {
     const uint16_t* q;                                                 // [n_seq * T] rows of n_heads * D
     long long ld_q;

@@ -30,6 +30,7 @@ import torch.nn.functional as F
 
 from .compress import SparseQuantConfig, compress_weight
 from . import _lib
+from .kvcache import KVCache4
 from .linear import CobaltSparseLinear, FusedProjections, called_plainly, status_word
 
 PROJ = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj",
@@ -126,11 +127,16 @@ class CobaltDecoder:
     the token limit of the decode GEMV).  ``linears[(layer, proj)]`` are ``CobaltSparseLinear`` modules; ``dense`` holds
     embedding / norms / lm_head.  ``head`` (optional) is the head as a compressed module - group-128 RTN without a mask,
     the reference's recipe for the tied embedding / head (src/cobaltkernel/pack_cobalt.py:375-386, 538-558); with tensor
-    parallelism it holds this rank's slice of the vocabulary and the logits are gathered over the ranks."""
+    parallelism it holds this rank's slice of the vocabulary and the logits are gathered over the ranks.  ``kv_bits = 4`` keeps keys and
+    values in 4 bits (``kvcache.KVCache4``, one per layer): 9/32 of the memory, attention in fp32 without the spec's roundings of scores and
+    probabilities, and sums whose order may depend on how many sequences run together.  ``attention_sinks`` (4-bit caches only): in
+    sliding-window layers that many first slots stay visible."""
+
+    kv4, sinks = None, 0
 
     def __init__(self, cfg: dict, linears: Dict[tuple, CobaltSparseLinear], dense: Dict[str, torch.Tensor],
                  max_ctx: int, device, tp_world: int = 1, reducer=None, group=None, batch: int = 1,
-                 head: Optional[CobaltSparseLinear] = None, fuse_steps: bool = True):
+                 head: Optional[CobaltSparseLinear] = None, fuse_steps: bool = True, kv_bits: int = 16, attention_sinks: int = 0):
         self.cfg, self.lin, self.P, self.max_ctx, self.dev = cfg, linears, dense, max_ctx, device
         self.world, self.reducer, self.group = tp_world, reducer, group
         self.head, self.B = head, int(batch)
@@ -141,8 +147,16 @@ class CobaltDecoder:
             raise ValueError("heads must split evenly over the tensor-parallel ranks")
         self.nh, self.nkv = cfg["num_attention_heads"] // tp_world, cfg["num_key_value_heads"] // tp_world   # local heads
         L, nkv, D = cfg["num_hidden_layers"], self.nkv, cfg["head_dim"]
-        self.k_cache = torch.zeros(L, self.B, nkv, max_ctx, D, dtype=torch.bfloat16, device=device)     # [layer][sequence][kv head][slot][D]
-        self.v_cache = torch.zeros(L, self.B, nkv, max_ctx, D, dtype=torch.bfloat16, device=device)
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, got {kv_bits}")
+        if attention_sinks < 0 or (attention_sinks and kv_bits != 4):
+            raise ValueError("attention_sinks must not be negative, and needs kv_bits = 4")
+        self.sinks = int(attention_sinks)
+        self.kv4 = [KVCache4(self.B, nkv, max_ctx, D, device) for _ in range(L)] if kv_bits == 4 else None
+        self.k_cache = self.v_cache = None
+        if self.kv4 is None:
+            self.k_cache = torch.zeros(L, self.B, nkv, max_ctx, D, dtype=torch.bfloat16, device=device)     # [layer][sequence][kv head][slot][D]
+            self.v_cache = torch.zeros(L, self.B, nkv, max_ctx, D, dtype=torch.bfloat16, device=device)
         self.seq_stride = nkv * max_ctx * D                                    # elements of one sequence's cache in a layer
         self.gemma = is_gemma(cfg)
         self.types = layer_types(cfg)
@@ -152,10 +166,10 @@ class CobaltDecoder:
             self.embed_scale = torch.tensor(float(cfg["hidden_size"]) ** 0.5, dtype=torch.bfloat16, device=device)
         self.kv_pos = torch.arange(max_ctx, device=device)
         need = _lib.load().cobalt_attn_decode_scratch_bytes(self.nh, D, max_ctx) * self.B
-        self.att_scratch = torch.empty(need, dtype=torch.uint8, device=device) if self.nh // self.nkv <= 8 and D % 64 == 0 and D <= 256 \
-            and max_ctx <= 65536 else None
+        self.att_scratch = torch.empty(need, dtype=torch.uint8, device=device) if self.kv4 is None and self.nh // self.nkv <= 8 and D % 64 == 0 \
+            and D <= 256 and max_ctx <= 65536 else None
         # Prompts take the library's tcgen05 attention (128 / 64 wide heads), other head widths batched matmuls
-        self.prompt_kernel = D in (64, 128) and self.nh // self.nkv <= 128 and max_ctx <= 1 << 24
+        self.prompt_kernel = self.kv4 is not None or (D in (64, 128) and self.nh // self.nkv <= 128 and max_ctx <= 1 << 24)
         # Rows (tokens of all prompts) that go through the layers together when several sequences are prefilled: the activations of
         # 8192 are a GB or more at the widest MLPs.  The caller may lower it; 0 = one prompt at a time.
         self.prompt_rows = 8192
@@ -203,6 +217,9 @@ class CobaltDecoder:
     def _rope_kv(self, q, k, v, positions, layer, seq: Optional[int]):
         """``seq`` = the sequence the T tokens belong to, or None: token t belongs to sequence t (batched decode)."""
         cfg = self.cfg
+        if self.kv4 is not None:
+            self._append4(q, k, v, positions, layer, 0 if seq is None else seq, q.shape[0] if seq is None else 1)
+            return
         kc = self.k_cache[layer] if seq is None else self.k_cache[layer][seq]
         vc = self.v_cache[layer] if seq is None else self.v_cache[layer][seq]
         qn = kn = None
@@ -216,10 +233,28 @@ class CobaltDecoder:
                                       self.seq_stride if seq is None else 0, torch.cuda.current_stream(self.dev).cuda_stream)
         _lib.check("cobalt_rope_kv", rc)
 
+    def _append4(self, q, k, v, positions, layer, seq: int, n: int):
+        """Rotation of q (in place) and k, and the append, into the 4-bit cache: rows of ``n`` sequences from ``seq`` on; ``positions`` of every row,
+        or ``[T]`` for all sequences."""
+        norm = (lambda name: self.P[f"model.layers.{layer}.self_attn.{name}.weight"]) if self.gemma else (lambda name: None)
+        T = q.shape[0] // n
+        q3 = q.view(n, T, -1)
+        self.kv4[layer].append(k.view(n, T, -1), v.view(n, T, -1), positions if positions.shape[0] == T else positions.view(n, T), q=q3,
+                               inv_freq=self.inv_freq[self.types[layer]], q_norm=norm("q_norm"), k_norm=norm("k_norm"),
+                               eps=float(self.cfg["rms_norm_eps"]), seq=seq, q_out=q3)
+
+    def _attend4(self, q, positions, layer, seq: int, n: int):
+        window = int(self.cfg.get("sliding_window") or 0) if self.types[layer] == "sliding_attention" else 0
+        T = q.shape[0] // n
+        return self.kv4[layer].attend(q.view(n, T, -1), positions if positions.shape[0] == T else positions.view(n, T), window=window,
+                                      sinks=self.sinks if window else 0, scale=self.scale, seq=seq).view(q.shape)
+
     def _attn_one(self, q, positions, layer, seq: Optional[int]):
         """Attention of one new token per sequence over cache slots 0..positions[b] (three small launches, lengths read on
         the device).  ``seq`` = a single sequence (q [1, nh*D]) or None = all ``batch`` sequences (q [B, nh*D])."""
         cfg = self.cfg
+        if self.kv4 is not None:
+            return self._attend4(q, positions, layer, 0 if seq is None else seq, q.shape[0] if seq is None else 1)
         ctx = torch.empty_like(q)
         window = int(cfg.get("sliding_window") or 0) if self.types[layer] == "sliding_attention" else 0
         kc = self.k_cache[layer] if seq is None else self.k_cache[layer][seq]
@@ -248,6 +283,8 @@ class CobaltDecoder:
 
     def _attn_prompt(self, q, positions, layer, seq: int, n_slots: int, n_seq: int = 1):
         """Attention of the prompts of ``n_seq`` sequences from ``seq`` on (``q [n_seq * T, nh*D]``) over cache slots [0, n_slots), one kernel."""
+        if self.kv4 is not None:
+            return self._attend4(q, positions, layer, seq, n_seq)
         ctx = torch.empty_like(q)
         window = int(self.cfg.get("sliding_window") or 0) if self.types[layer] == "sliding_attention" else 0
         rc = self._lib.cobalt_attn_prompt(q.data_ptr(), self.k_cache[layer][seq].data_ptr(), self.v_cache[layer][seq].data_ptr(),
@@ -352,7 +389,7 @@ class CobaltDecoder:
         T, rep, S = ids.shape[0], nh // nkv, attend_len
         h = self._embed(ids)                                                           # [T, H]
         blocked, allowed_of = {}, {}
-        if seq is not None and (self.fused_prompt_attention or not self.prompt_kernel) and (T > 1 or self.att_scratch is None):
+        if self.kv4 is None and seq is not None and (self.fused_prompt_attention or not self.prompt_kernel) and (T > 1 or self.att_scratch is None):
             causal = self.kv_pos[None, :S] <= positions[:, None]                       # [T, S]
             for lt in set(self.types):
                 allowed = causal
@@ -366,10 +403,10 @@ class CobaltDecoder:
             p = f"model.layers.{i}."
             h, (q, k, v) = self._norm_then(self.qkv[i], h, delta, P[p + "input_layernorm.weight"], delta_w)   # one launch for up to 8 tokens
             self._rope_kv(q, k, v, positions, i, seq)                                  # q in place, k/v into the caches
-            if seq is not None:
+            if seq is not None and self.kv4 is None:
                 Kc, Vc = self.k_cache[i][seq][:, :S], self.v_cache[i][seq][:, :S]      # [nkv, S, D]
             if seq is None:                                                            # one new token per sequence
-                if self.att_scratch is None:
+                if self.att_scratch is None and self.kv4 is None:
                     raise NotImplementedError("batched decode needs the library's decode attention (head_dim % 64 == 0, <= 8 q heads per kv head)")
                 ctx = self._attn_one(q, positions, i, None)
             elif T == 1 and self.att_scratch is not None:
@@ -445,6 +482,8 @@ class CobaltDecoder:
             words += [self.head.device_status(), self.head_f.device_status()]
         if self.reducer is not None:
             words.append(self.reducer.device_status())
+        if getattr(self, "kv4", None) is not None:
+            words.append(self.kv4[0].device_status())
         return max(words)
 
     def _check_prompt_attention(self):
@@ -453,6 +492,9 @@ class CobaltDecoder:
         if word:
             self.prompt_status.zero_()
             raise _lib.CobaltError("cobalt_attn_prompt", word, "a bounded wait gave up: the attention of a prompt is incomplete")
+        word = self.kv4[0].device_status() if self.kv4 is not None else 0
+        if word:
+            raise _lib.CobaltError("cobalt_kv4_attend", word, "a bounded wait gave up: an attention over the cache is incomplete")
 
     @torch.no_grad()
     def time_head_ms(self, reps: int = 20) -> float:
@@ -504,9 +546,12 @@ class CobaltDecoder:
             p = f"model.layers.{i}."
             h, x = self._add_rmsnorm(h, delta, P[p + "input_layernorm.weight"], delta_w if delta is not None else None)
             q, k, v = self.qkv[i](x, T)
-            for b in range(n):
-                r = slice(b * T, (b + 1) * T)
-                self._rope_kv(q[r], k[r], v[r], positions, i, first + b)
+            if self.kv4 is not None:
+                self._append4(q, k, v, positions, i, first, n)
+            else:
+                for b in range(n):
+                    r = slice(b * T, (b + 1) * T)
+                    self._rope_kv(q[r], k[r], v[r], positions, i, first + b)
             (o,) = self.o_f[i](self._attn_prompt(q, positions, i, first, T, n), T)
             if self.gemma:
                 h, x = self._add_rmsnorm(h, o, P[p + "pre_feedforward_layernorm.weight"], P[p + "post_attention_layernorm.weight"])
@@ -627,14 +672,14 @@ def compress_head(dense: Dict[str, torch.Tensor], cfg: dict, bits: int, tp_rank:
 
 def build_random_decoder(cfg: dict, qcfg: SparseQuantConfig, max_ctx: int, device, keep_raw: bool = False,
                          tp_rank: int = 0, tp_world: int = 1, reducer=None, group=None, clone_first_layer: bool = False,
-                         batch: int = 1, head_bits: int = 0, fuse_steps: bool = True):
+                         batch: int = 1, head_bits: int = 0, fuse_steps: bool = True, kv_bits: int = 16, attention_sinks: int = 0):
     """Random-init model of the given shape with every projection compressed.  Returns the decoder
     and, when ``keep_raw``, the RAW tensors per (layer, proj) for an oracle to dequantise.  With
     ``tp_world > 1`` every matrix is compressed whole (same seeds on every rank) and this rank keeps its shard.
     ``clone_first_layer`` compresses only layer 0 and gives every other layer its own copy of those packed bytes
     (for timing very large shapes: the bytes streamed per token are the same, the compression time is not).
     ``batch`` sequences decode together; ``head_bits`` (2..4) compresses the head with group-128 RTN and, with
-    tensor parallelism, splits its vocabulary over the ranks."""
+    tensor parallelism, splits its vocabulary over the ranks; ``kv_bits`` and ``attention_sinks`` as for ``CobaltDecoder``."""
     from .format import TileImage
     from .tp import kind_of, shard_raw
     lin, raws = {}, {}
@@ -656,5 +701,5 @@ def build_random_decoder(cfg: dict, qcfg: SparseQuantConfig, max_ctx: int, devic
     dense = random_dense_params(cfg, device)
     head = compress_head(dense, cfg, head_bits, tp_rank, tp_world) if head_bits else None
     dec = CobaltDecoder(cfg, lin, dense, max_ctx, device, tp_world=tp_world, reducer=reducer, group=group, batch=batch, head=head,
-                        fuse_steps=fuse_steps)
+                        fuse_steps=fuse_steps, kv_bits=kv_bits, attention_sinks=attention_sinks)
     return (dec, raws) if keep_raw else dec

@@ -75,7 +75,7 @@ class KVCache4:
         return self.tiles.device
 
     # ------------------------------------------------------------------ arguments
-    def _rows(self, name: str, t: torch.Tensor, width: int, lead, align: int):
+    def _rows(self, name: str, t: torch.Tensor, width: int, lead):
         """(address, row stride, owner of the memory) of ``t [n, T, width]`` (or ``[T, width]``: one sequence) as rows the kernels take."""
         if self._index < 0 or not t.is_cuda:
             raise RuntimeError("KVCache4 needs CUDA tensors; there is no CPU path")
@@ -89,10 +89,10 @@ class KVCache4:
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient: KVCache4 has no backward pass (use torch.no_grad())")
         p = t.data_ptr()
-        if p % align == 0 and t.is_contiguous():
+        if p % 16 == 0 and t.is_contiguous():
             return p, width, t
         rows = t if len(shape) == 2 else t.reshape(-1, width)
-        if rows.stride(1) != 1 or rows.stride(0) * 2 % align or rows.stride(0) < width or rows.data_ptr() % align:
+        if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.stride(0) < width or rows.data_ptr() % 16:
             rows = rows.clone(memory_format=torch.contiguous_format)
         return rows.data_ptr(), rows.stride(0), rows
 
@@ -130,9 +130,9 @@ class KVCache4:
         ``cobalt_rope_kv`` does, and with ``k_norm`` (bf16 ``[head_dim]``) normalised per head before that; the same is done to
         ``q [n, T, n_heads * head_dim]`` (``q_norm``), which is returned - in ``q_out`` if given (may be ``q`` itself)."""
         D, width = self.head_dim, self.n_kv_heads * self.head_dim
-        kp, ld_k, k_own = self._rows("k", k, width, None, 4)
+        kp, ld_k, k_own = self._rows("k", k, width, None)
         lead = k.shape[:-1]
-        vp, ld_v, v_own = self._rows("v", v, width, lead, 4)
+        vp, ld_v, v_own = self._rows("v", v, width, lead)
         n, T = lead if len(lead) == 2 else (1, lead[0])
         if inv_freq is not None:
             self._weight("inv_freq", inv_freq, torch.float32, D // 2)
@@ -146,13 +146,13 @@ class KVCache4:
             heads = q.shape[-1] // D
             if heads < 1:
                 raise ValueError(f"q must be [n, T, n_heads * {D}], got {list(q.shape)}")
-            qp, ld_q, q_own = self._rows("q", q, heads * D, lead, 4)
+            qp, ld_q, q_own = self._rows("q", q, heads * D, lead)
             if q_norm is not None:
                 self._weight("q_norm", q_norm, torch.bfloat16, D)
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.device != q.device or not q_out.is_contiguous() or q_out.data_ptr() % 4:
-                raise ValueError("q_out must be a contiguous tensor like q")
+            elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.device != q.device or not q_out.is_contiguous() or q_out.data_ptr() % 16:
+                raise ValueError("q_out must be a contiguous tensor like q on a 16-byte boundary")
             op = q_out.data_ptr()
         pos, stride, tiles, p_own = self._place(positions, n, T, seq)
         if n * T:
@@ -193,7 +193,7 @@ class KVCache4:
         heads = shape[-1] // D
         if heads < 1 or heads % n_kv:
             raise ValueError(f"q must hold a multiple of {n_kv} heads of {D}, got {list(shape)}")
-        qp, ld_q, q_own = self._rows("q", q, heads * D, None, 16)
+        qp, ld_q, q_own = self._rows("q", q, heads * D, None)
         n, T = shape[:2] if len(shape) == 3 else (1, shape[0])
         if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError("window and sinks must be between 0 and 2^31 - 1")

@@ -349,12 +349,12 @@ int cobalt_attn_prompt(const void* q, const void* k_cache, const void* v_cache, 
  *
  * All calls: n_seq sequences of T tokens, row seq * T + t; positions[seq * pos_seq_stride + t] (pos_seq_stride 0: the same for every
  * sequence) is read on the device.
- *   cobalt_kv4_append : k and v [rows] x ld (elements, even; 4-byte aligned), n_kv_heads * head_dim values each, into the slots at
+ *   cobalt_kv4_append : k and v [rows] x ld (elements, a multiple of 8; rows of all calls 16-byte aligned), n_kv_heads * head_dim values each, into the slots at
  *                       their positions (outside [0, n_slots): not stored; the positions of one sequence must differ).  k first gets
  *                       the per-head norm of cobalt_rope_kv() if k_norm_w is given and its rotation if inv_freq is; so does q (may be NULL) with
  *                       q_norm_w, into q_out (may be q).  v is stored as it is.
  *   cobalt_kv4_read   : the slots at the positions, as bf16 [rows][n_kv_heads][head_dim]; a position outside [0, n_slots) reads as zeros.
- *   cobalt_kv4_attend : grouped-query attention of the tokens (q [rows] x ld_q, rotated; 16-byte aligned, ld_q % 8 == 0) over the cache, out [rows][n_heads * head_dim]
+ *   cobalt_kv4_attend : grouped-query attention of the tokens (q [rows] x ld_q, rotated) over the cache, out [rows][n_heads * head_dim]
  *                       (16-byte aligned).  A token at position p sees slot j < n_slots if j <= p and (window == 0 or j > p - window or
  *                       j < sinks); one that sees none (p < 0: padding) gets zeros.  Scores, softmax and sums in fp32, one rounding
  *                       at the end.  scratch: cobalt_kv4_attend_scratch_bytes() (0: none needed), 256-byte aligned, contents irrelevant;

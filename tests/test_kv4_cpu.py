@@ -51,8 +51,8 @@ def test_sizes_beyond_the_kernels_counts_are_refused(lib, kw):
     assert _read(lib, **kw) == -6 and _attend(lib, **kw) == -6
 
 
-@pytest.mark.parametrize("kw", [dict(k=None), dict(v=None), dict(k=4098), dict(ld_k=127), dict(ld_v=126), dict(q=4096, nh=0, qo=4096),
-                                dict(q=4096, nh=1, ld_q=128, qo=None, ld_qo=128), dict(q=4096, nh=1, ld_q=64, qo=4096, ld_qo=128), dict(qn=4096),
+@pytest.mark.parametrize("kw", [dict(k=None), dict(v=None), dict(k=4104), dict(ld_k=132), dict(ld_v=126), dict(q=4096, nh=0, qo=4096),
+                                dict(q=4096, nh=1, ld_q=128, qo=None, ld_qo=128), dict(q=4096, nh=1, ld_q=64, qo=4096, ld_qo=128), dict(q=4096, nh=1, ld_q=128, qo=4104, ld_qo=128), dict(qn=4096),
                                 dict(f=4097), dict(kn=4098)])
 def test_append_refuses(lib, kw):
     assert _append(lib, **kw) == -1
@@ -65,7 +65,7 @@ def test_attend_refuses(lib, kw):
 
 
 def test_read_refuses(lib):
-    assert _read(lib, k=None) == -1 and _read(lib, v=4097) == -1
+    assert _read(lib, k=None) == -1 and _read(lib, v=4104) == -1
 
 
 def test_class_refuses():
