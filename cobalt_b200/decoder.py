@@ -492,7 +492,8 @@ class CobaltDecoder:
         if word:
             self.prompt_status.zero_()
             raise _lib.CobaltError("cobalt_attn_prompt", word, "a bounded wait gave up: the attention of a prompt is incomplete")
-        word = self.kv4[0].device_status() if self.kv4 is not None else 0
+        caches = getattr(self, "kv4", None)
+        word = caches[0].device_status() if caches else 0
         if word:
             raise _lib.CobaltError("cobalt_kv4_attend", word, "a bounded wait gave up: an attention over the cache is incomplete")
 
