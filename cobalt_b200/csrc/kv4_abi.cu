@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "kv4_attend.cuh"
+#include "kv4_prompt.cuh"
 
 using namespace cb;
 
@@ -125,6 +126,27 @@ int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c
     return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<G, NB>, P, W) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
 }
 
+// Rows (columns of the other kernels) of a KV head from which a prompt's kernel takes them.
+constexpr int KP_MIN_ROWS = 64;
+bool prompt_takes(int n_seq, int rep, int T, int D) {
+    return (D == 64 || D == 128) && n_seq <= 65535 && rep <= KP_ROWS && (int64_t)rep * T >= KP_MIN_ROWS;
+}
+template <int G>
+int launch_prompt(const Kv4AttendParams& P, cudaStream_t st) {
+    static bool configured[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(kv4_prompt_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kp_smem_bytes(G)) != cudaSuccess) return COBALT_ELAUNCH;
+        configured[dev] = true;
+    }
+    const int tok_per_cta = KP_ROWS / P.rep;
+    const int64_t blocks = ((int64_t)P.T + tok_per_cta - 1) / tok_per_cta * P.cache.n_kv;
+    if (blocks > 0x3FFFFFFFll) return COBALT_ETOOBIG;
+    kv4_prompt_kernel<G><<<dim3((unsigned)blocks, (unsigned)P.n_seq), KP_THREADS, kp_smem_bytes(G), st>>>(P, tok_per_cta);
+    return cudaGetLastError() == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+}
+
 }  // namespace
 
 #define KV4_DISPATCH(D, CALL)                    \
@@ -189,6 +211,7 @@ size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_h
     int sms = 0;
     if (n_seq <= 0 || T <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_slots <= 0 || window < 0 || sinks < 0 ||
         !dim_ok(head_dim) || sm_count(&sms)) return 0;
+    if (prompt_takes(n_seq, n_heads / n_kv_heads, T, head_dim)) return 0;
     AttendCfg c;
     return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c) ? 0 : c.scratch;
 }
@@ -203,8 +226,9 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
-    AttendCfg c;
-    if ((rc = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c))) return rc;
+    const bool prompt = prompt_takes(n_seq, n_heads / n_kv_heads, T, head_dim);
+    AttendCfg c = {};
+    if (!prompt && (rc = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c))) return rc;
     if (c.list && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < c.scratch)) return COBALT_ESCRATCH;
     P.q = (const uint16_t*)q; P.ld_q = ld_q;
     P.positions = (const long long*)positions;
@@ -214,7 +238,9 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     P.window = window; P.sinks = sinks;
     P.scale_log2 = scale * 1.44269504f;
     P.cols = c.cols; P.col_tiles = c.col_tiles;
-    P.by_rep = kv4_div(P.rep); P.by_tiles = kv4_div(c.col_tiles); P.by_kv = kv4_div(n_kv_heads);
+    P.by_rep = kv4_div(P.rep); P.by_kv = kv4_div(n_kv_heads);
+    if (prompt) return head_dim == 64 ? launch_prompt<1>(P, (cudaStream_t)stream) : launch_prompt<2>(P, (cudaStream_t)stream);
+    P.by_tiles = kv4_div(c.col_tiles);
     Kv4Work W;
     W.partial = (float*)scratch;
     W.joins = (int4*)((uint8_t*)scratch + c.joins_off);

@@ -1,0 +1,362 @@
+// Attention of many rows per KV head (prompts) over the 4-bit cache, tcgen05.mma for both contractions; heads of 64 or 128.  The format is in
+// kv4_kernels.cuh.
+//
+// One CTA = 128 query rows of one KV head: (token, head) pairs, 128 / rep tokens of the rep query heads that share it.  One pass over the
+// keys, 128 at a time, with running maxima and sums:
+//   warps 0-7   softmax: warp w owns TMEM lanes 32*(w%4).. (a thread = a row) and key columns 64*(w/4).. of every tile.  The two halves of a
+//               row's keys keep a maximum, a sum and a context of their own - nothing is exchanged between threads until the end,
+//               where the two are joined.  A maximum moves only when a score exceeds it by 2^8 (the probabilities are bf16, which have
+//               the room); then the warp rescales its part of the context in tensor memory, after the product before it.
+//   warps 8-11  keys: expand 32 slots of every tile each, codes to bf16 in a K-major, 128-byte-swizzled operand
+//   warps 12-15 values: the same
+//   warp 16     MMA: scores into one of two TMEM buffers, the two contexts into two others; the scores of tile j+1 are issued before
+//               the context of tile j
+// Key tiles that no row of the CTA sees are skipped (between the first slots and the window, too); only tiles on a border are masked.
+// Keys, values and probabilities are rounded to bf16 once (the operands' type); scores, maxima, sums and contexts are fp32.
+//
+// A slot that only some rows see has to stay out of the others' products even where its values are not numbers: such groups are
+// expanded to zeros and marked, and marked CTAs look through the scales of their rows' slots once at the end.
+// MEASURED_PROMPT
+#pragma once
+#include "kv4_attend.cuh"
+#include "tcgen05.cuh"
+
+namespace cb {
+
+constexpr int KP_ROWS = 128, KP_KEYS = 128;
+constexpr int KP_SOFTMAX = 256, KP_THREADS = KP_SOFTMAX + 256 + 32;
+constexpr uint32_t KP_SUB = 128 * 128;                                 // bytes of 128 rows x 64 bf16: one swizzled sub-tile
+constexpr uint32_t kp_smem_bytes(int G) { return KP_SUB * (uint32_t)(5 * G + 4) + 256 + 1024; }      // Q, 2 K, 2 V, 2 P of two halves; barriers
+static_assert(kp_smem_bytes(2) <= 227 * 1024, "the 128-wide head fills the shared memory of one SM");
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+          "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+          "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+          "r"(v[31]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Eight codes of a word as bf16 values c * s + b, b = -z * s: a code in the low bits of a bf16 pattern is 128 + c exactly, so the product is
+// taken of that and the constant carries the rest, in fp32 (135 s at most, so 2^-17 of a step), and rounded once.
+__device__ __forceinline__ uint4 kv4_expand(uint32_t w, float s, float z) {
+    const float b128 = -(128.0f + z) * s;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t p = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+        x[i] = fmaf(__uint_as_float(p << 16), s, b128);
+        x[i + 4] = fmaf(__uint_as_float(p & 0xFFFF0000u), s, b128);
+    }
+    if (__builtin_expect(s > 0x1p110f, 0)) {                           // 135 s may leave the range of fp32 where (c - z) s does not
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = ((float)(w >> (4 * i) & 15u) - z) * s;
+    }
+    return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+}
+
+// The same with tiles of 128 slots
+__device__ __forceinline__ Kv4Tiles kv4_key_tiles(const Kv4Span& s, int sinks) {
+    Kv4Tiles e;
+    const int tiles = (s.hi_max + KP_KEYS) / KP_KEYS;
+    e.n_sink = (min(sinks, s.hi_max + 1) + KP_KEYS - 1) / KP_KEYS;
+    e.first = min(tiles, s.lo_min / KP_KEYS);
+    if (e.first <= e.n_sink) e.first = e.n_sink = 0;
+    e.n = e.n_sink + tiles - e.first;
+    if (e.n == 0) { e.n = 1; e.first = 0; }
+    return e;
+}
+
+template <int G>
+__global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4AttendParams P, const int tok_per_cta) {
+    constexpr int D = 64 * G, TILE = kv4_tile_bytes(G);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint32_t no_number;                                     // a group of values that is not a number was seen
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full_mask = 0xFFFFFFFFu;
+    const uint32_t s_raw = smem_u32(smem), s0 = (s_raw + 1023u) & ~1023u;
+    const uint32_t q_base = s0, k_base = q_base + G * KP_SUB, v_base = k_base + 2 * G * KP_SUB, p_base = v_base + 2 * G * KP_SUB;
+    const uint32_t bars = p_base + 4 * KP_SUB, tmem_slot = bars + 8u * 20u;
+    auto bar_kfull = [&](int s) { return bars + 8u * s; };
+    auto bar_kempty = [&](int s) { return bars + 16u + 8u * s; };
+    auto bar_vfull = [&](int s) { return bars + 32u + 8u * s; };
+    auto bar_vempty = [&](int s) { return bars + 48u + 8u * s; };
+    auto bar_sfull = [&](int s) { return bars + 64u + 8u * s; };
+    auto bar_sempty = [&](int s) { return bars + 80u + 8u * s; };
+    auto bar_pfull = [&](int h, int s) { return bars + 96u + 16u * h + 8u * s; };
+    auto bar_pempty = [&](int h, int s) { return bars + 128u + 16u * h + 8u * s; };
+    float* stat = reinterpret_cast<float*>(smem + (p_base - s_raw));   // (at the end) [half][row] maximum, then [half][row] sum
+    uint32_t* status = &g_kv4_status;
+
+    // the longest rows (last tokens of the prompt) first, so that the short ones fill the end of the grid
+    const int n_kv = P.cache.n_kv, order = (int)(gridDim.x - 1 - blockIdx.x);
+    const int block = P.by_kv(order), kvh = order - block * n_kv, seq = blockIdx.y, tok0 = block * tok_per_cta;
+    Kv4Span span = {-1, 0x7FFFFFFF, 0x7FFFFFFF, 0};
+    for (int i = lane; i < tok_per_cta && tok0 + i < P.T; i += 32) {
+        const Kv4Range r = kv4_range(P, seq, tok0 + i);
+        span.hi_max = max(span.hi_max, r.hi);
+        span.hi_min = min(span.hi_min, r.hi);
+        span.lo_max = max(span.lo_max, r.lo);
+        if (r.lo <= r.hi) span.lo_min = min(span.lo_min, r.lo);
+    }
+    span.hi_max = __reduce_max_sync(full_mask, span.hi_max);
+    span.hi_min = __reduce_min_sync(full_mask, span.hi_min);
+    span.lo_max = __reduce_max_sync(full_mask, span.lo_max);
+    span.lo_min = __reduce_min_sync(full_mask, span.lo_min);
+    const Kv4Tiles tiles = kv4_key_tiles(span, P.sinks);
+    const int n = tiles.n;
+    auto nobody = [&](int j) { return j > span.hi_max || (j < span.lo_min && j >= P.sinks); };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(bar_kfull(s), 128); mbar_init(bar_kempty(s), 1);
+            mbar_init(bar_vfull(s), 128); mbar_init(bar_vempty(s), 1);
+            mbar_init(bar_sfull(s), 1); mbar_init(bar_sempty(s), KP_SOFTMAX);
+            for (int h = 0; h < 2; ++h) { mbar_init(bar_pfull(h, s), 128); mbar_init(bar_pempty(h, s), 1); }
+        }
+        mbar_fence_init();
+        no_number = 0u;
+    }
+    // queries: rows that are none are zero
+    for (int i = threadIdx.x; i < KP_ROWS * D / 8; i += KP_THREADS) {
+        const int r = i / (D / 8), c = i % (D / 8), tok = P.by_rep(r), row_tok = tok0 + tok;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (tok < tok_per_cta && row_tok < P.T)
+            v = __ldg(reinterpret_cast<const uint4*>(P.q + ((long long)seq * P.T + row_tok) * P.ld_q + (kvh * P.rep + r - tok * P.rep) * D) + c);
+        sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), v.x, v.y, v.z, v.w);
+    }
+    fence_proxy_async();
+    if (warp == 16) { tmem_alloc<false>(tmem_slot, 512); tmem_relinquish<false>(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = lds32(tmem_slot), tmem_o = tmem + 2 * KP_KEYS;              // scores 2 x 128 columns, contexts 2 x D
+
+    if (warp < 8) {
+        // =========================================================== softmax, epilogue
+        const int half = warp >> 2, r = threadIdx.x & 127;
+        const int sub = P.by_rep(r), tok = tok0 + sub, head = r - sub * P.rep;
+        const bool valid = sub < tok_per_cta && tok < P.T;
+        const Kv4Range range = valid ? kv4_range(P, seq, tok) : Kv4Range{0, -1};
+        const uint32_t my_lanes = (uint32_t)((warp & 3) * 32) << 16, my_o = tmem_o + my_lanes + (uint32_t)(half * D);
+        bool healthy = true;
+        float m = -INFINITY, l = 0.0f;                                  // reference and sum of this row's half, scores times log2(e)
+        for (int j = 0; j < n; ++j) {
+            healthy = __all_sync(full_mask, mbar_wait_bounded(bar_sfull(j & 1), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_ACC));
+            if (!healthy) break;
+            tc_fence_after();
+            uint32_t v[2][32];
+            tmem_ld32(tmem + my_lanes + (uint32_t)((j & 1) * KP_KEYS + half * 64), v[0]);
+            tmem_ld32(tmem + my_lanes + (uint32_t)((j & 1) * KP_KEYS + half * 64 + 32), v[1]);
+            tmem_ld_wait();
+            tc_fence_before();
+            mbar_arrive(bar_sempty(j & 1));
+            float x[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(v[i >> 5][i & 31]) * P.scale_log2;
+            const int k0 = tiles.tile(j) * KP_KEYS;
+            if (k0 + KP_KEYS - 1 > span.hi_min || (k0 < span.lo_max && k0 + KP_KEYS > P.sinks)) {                      // a border crosses this tile
+                const int hi = range.hi - k0 - half * 64, lo = range.lo - k0 - half * 64, sinks = P.sinks - k0 - half * 64;
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (i > hi || (i < lo && i >= sinks)) x[i] = -INFINITY;
+            }
+            float t[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int i = 4; i < 64; ++i) t[i & 3] = fmaxf(t[i & 3], x[i]);
+            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            const bool move = top > m + 8.0f;
+            if (__any_sync(full_mask, move)) {
+                // (a row without a reference has a context of zeros: nothing to rescale)
+                const float f = move && m != -INFINITY ? ex2(m - top) : 1.0f;
+                if (move) { m = top; l *= f; }
+                if (j > 0 && __any_sync(full_mask, f != 1.0f)) {
+                    healthy = __all_sync(full_mask, mbar_wait_bounded(bar_pempty(half, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u, status, DEV_TIMEOUT_EMPTY));
+                    if (!healthy) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(my_o + (uint32_t)c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st32(my_o + (uint32_t)c, o);
+                        tmem_st_wait();
+                    }
+                    tc_fence_before();
+                }
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t p[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float a = ex2(x[2 * i] - base), b = ex2(x[2 * i + 1] - base);
+                p[i] = pack_bf16x2(a, b);
+                s[i & 3] += a + b;
+            }
+            l += (s[0] + s[1]) + (s[2] + s[3]);
+            healthy = __all_sync(full_mask, mbar_wait_bounded(bar_pempty(half, j & 1), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY));
+            if (!healthy) break;
+            const uint32_t row = p_base + (uint32_t)(j & 1) * 2u * KP_SUB + (uint32_t)half * KP_SUB + (uint32_t)r * 128u;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                sts128(row + (((uint32_t)c ^ (uint32_t)(r & 7)) << 4), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+            fence_proxy_async();
+            mbar_arrive(bar_pfull(half, j & 1));
+        }
+        if (healthy)                                                   // the last products of both halves
+            for (int h = 0; h < 2; ++h)
+                healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_pempty(h, (n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u, status, DEV_TIMEOUT_ACC));
+        tc_fence_after();
+        stat[half * KP_ROWS + r] = m;
+        stat[(2 + half) * KP_ROWS + r] = l;
+        asm volatile("bar.sync 1, 384;" ::: "memory");                  // the softmax warps; those of the values have arrived (no_number)
+        const float om = stat[(half ^ 1) * KP_ROWS + r], ol = stat[(2 + (half ^ 1)) * KP_ROWS + r];
+        const float gm = fmaxf(m, om), base = gm == -INFINITY ? 0.0f : gm;
+        const float mine = ex2(m - base), other = ex2(om - base), inv = 1.0f / (l * mine + ol * other);
+        const float w0 = (half ? other : mine) * inv, w1 = (half ? mine : other) * inv;        // of the contexts of halves 0 and 1
+        if (healthy) {
+            const bool any = range.hi >= 0 && (range.lo <= range.hi || P.sinks > 0);
+            bool nan = false;
+            if (no_number && any) {                                    // a marked group: does this row see one?
+                const int g = half * (D / 2) / 64;
+                for (int j = 0; j <= range.hi; ++j) {
+                    if (j < range.lo && j >= P.sinks) { j = range.lo - 1; continue; }
+                    const uint8_t* tile = P.cache.tile(seq, kvh, j, G);
+                    const uint32_t sc = *reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, j % KV4_TILE));
+                    nan |= (sc & 0x7F80u) == 0x7F80u;
+                }
+            }
+#pragma unroll 1
+            for (int c0 = 0; c0 < D / 2; c0 += 32) {
+                uint32_t a[32], b[32];
+                const uint32_t col = (uint32_t)(half * (D / 2) + c0);
+                tmem_ld32(tmem_o + my_lanes + col, a);
+                tmem_ld32(tmem_o + my_lanes + (uint32_t)D + col, b);
+                tmem_ld_wait();
+                if (valid) {
+                    uint4* dst = reinterpret_cast<uint4*>(P.out + (((long long)seq * P.T + tok) * P.n_heads + kvh * P.rep + head) * D + col);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 8 * c + 2 * e;
+                            o[e] = pack_bf16x2(fmaf(__uint_as_float(a[i]), w0, __uint_as_float(b[i]) * w1),
+                                               fmaf(__uint_as_float(a[i + 1]), w0, __uint_as_float(b[i + 1]) * w1));
+                            o[e] = !any ? 0u : nan ? 0x7FC07FC0u : o[e];
+                        }
+                        dst[c] = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                }
+            }
+        }
+        tc_fence_before();
+    } else if (warp < 16) {
+        // =========================================================== keys, values: slots 32 w .. of every tile; 8 lanes a slot and group
+        const bool keys = warp < 12;
+        const int w = warp & 3, chunk = lane & 7, quarter = lane >> 3;
+        const uint8_t* base = P.cache.tiles + (long long)seq * P.cache.seq_stride + (long long)kvh * P.cache.n_tiles * TILE;
+        uint32_t codes[G][8], meta[G][8];                              // of the next tile: codes, { zero, scale }
+        auto request = [&](int j) {
+            const int at = tiles.tile(j) * (KP_KEYS / KV4_TILE) + w;
+            const bool held = at < P.cache.n_tiles;                    // (the last tile may reach beyond the cache)
+            const uint8_t* tile = base + (long long)(held ? at : 0) * TILE;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int slot = 4 * i + quarter;
+                    if (keys) {
+                        codes[g][i] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_row(G, g, slot) + 4 * chunk));
+                        meta[g][i] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, slot)));
+                    } else {
+                        codes[g][i] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_v_chunk(G, g, slot, chunk)));
+                        meta[g][i] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, slot))) << 16 |
+                                     __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_zero(G, g, slot)));
+                    }
+                    if (!held || nobody(KV4_TILE * at + slot)) meta[g][i] = 0u;        // zeros: nobody sees it, it may hold anything
+                }
+        };
+        request(0);
+        for (int j = 0; j < n; ++j) {
+            const int s = j & 1;
+            if (!__all_sync(full_mask, mbar_wait_bounded(keys ? bar_kempty(s) : bar_vempty(s), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY))) break;
+            const uint32_t dst = (keys ? k_base : v_base) + (uint32_t)s * G * KP_SUB + (uint32_t)(32 * w) * 128u;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t row = (uint32_t)(4 * i + quarter);
+                    uint32_t mt = meta[g][i];
+                    if (!keys && (mt & 0x7F800000u) == 0x7F800000u) { mt = 0u; no_number = 1u; }
+                    const float sc = __uint_as_float(mt & 0xFFFF0000u), z = f16_to_float(mt & 0xFFFFu);
+                    const uint4 x = kv4_expand(codes[g][i], sc, z);
+                    sts128(dst + (uint32_t)g * KP_SUB + row * 128u + ((((uint32_t)chunk) ^ (row & 7u)) << 4), x.x, x.y, x.z, x.w);
+                }
+            if (j + 1 < n) request(j + 1);
+            fence_proxy_async();
+            mbar_arrive(keys ? bar_kfull(s) : bar_vfull(s));
+        }
+        if (!keys) asm volatile("bar.arrive 1, 384;" ::: "memory");
+    } else {
+        // =========================================================== MMA
+        const uint32_t idesc_s = umma_idesc(KP_KEYS);
+        const uint32_t idesc_o = umma_idesc(D) | (1u << 16);            // B (= V) is N-major
+        const uint64_t qd = umma_smem_desc(q_base);
+        bool healthy = true;
+        auto issue_scores = [&](int j) {
+            const int s = j & 1;
+            healthy = healthy && mbar_wait_bounded(bar_kfull(s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_STAGE);
+            healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_sempty(s), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY));
+            if (!healthy) return;
+            tc_fence_after();
+            const uint64_t kd = umma_smem_desc(k_base + (uint32_t)s * G * KP_SUB);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t off = (uint64_t)((k / 4) * (KP_SUB >> 4) + (k % 4) * 2);
+                    umma_bf16<false>(tmem + (uint32_t)(s * KP_KEYS), qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
+                }
+                umma_commit<false>(bar_kempty(s));
+                umma_commit<false>(bar_sfull(s));
+            }
+            __syncwarp();
+        };
+        auto issue_context = [&](int j) {
+            const int s = j & 1;
+            healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_vfull(s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_STAGE));
+            for (int h = 0; h < 2; ++h) {
+                healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_pfull(h, s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_FULL));
+                if (!healthy) return;
+                tc_fence_after();
+                const uint64_t pd = umma_smem_desc(p_base + (uint32_t)(2 * s + h) * KP_SUB);
+                const uint64_t vd = umma_smem_desc_mn(v_base + (uint32_t)s * G * KP_SUB, KP_SUB);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_bf16<false>(tmem_o + (uint32_t)(h * D), pd + (uint64_t)(k * 2), vd + (uint64_t)((4 * h + k) * (2048 >> 4)), idesc_o,
+                                         (j > 0 || k > 0) ? 1u : 0u);
+                    umma_commit<false>(bar_pempty(h, s));
+                    if (h == 1) umma_commit<false>(bar_vempty(s));
+                }
+                __syncwarp();
+            }
+        };
+        issue_scores(0);
+        for (int j = 0; j < n && healthy; ++j) {
+            if (j + 1 < n) issue_scores(j + 1);
+            issue_context(j);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 16) { tc_fence_after(); tmem_dealloc<false>(tmem, 512); }
+}
+
+}  // namespace cb

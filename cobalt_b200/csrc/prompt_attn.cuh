@@ -59,17 +59,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-// N-major operand (value tile: 64 context columns per 128-byte row, one row per key), 128-byte swizzle: 8-key groups are
-// 1024 bytes apart, 64-column blocks `block_bytes`
-__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t smem_addr, uint32_t block_bytes) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(block_bytes >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
 // a / b with inv = 1.0f / b, which every probability of a row shares: the quotient by the reciprocal, put right by its remainder
 // (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  Equal to the division
 // for the sums met here (1 <= b < 2^25).
