@@ -7,9 +7,9 @@
 //               row's keys keep a maximum, a sum and a context of their own - nothing is exchanged between threads until the end,
 //               where the two are joined.  A maximum moves only when a score exceeds it by 2^8 (the probabilities are bf16, which have
 //               the room); then the warp rescales its part of the context in tensor memory, after the product before it.
-//   warps 8-11  keys: expand 32 slots of every tile each, codes to bf16 in a K-major, 128-byte-swizzled operand
-//   warps 12-15 values: the same
-//   warp 16     MMA: scores into one of two TMEM buffers, the two contexts into two others; the scores of tile j+1 are issued before
+//   warps 8-14  expand: a unit is 32 slots of a group of keys, or of values; codes to bf16 in K-major (values: N-major), 128-byte-swizzled
+//               operands.  Units go round the seven warps, each with its next unit requested ahead
+//   warp 15     MMA: scores into one of two TMEM buffers, the two contexts into two others; the scores of tile j+1 are issued before
 //               the context of tile j
 // Key tiles that no row of the CTA sees are skipped (between the first slots and the window, too); only tiles on a border are masked.
 // Keys, values and probabilities are rounded to bf16 once (the operands' type); scores, maxima, sums and contexts are fp32.
@@ -24,7 +24,7 @@
 namespace cb {
 
 constexpr int KP_ROWS = 128, KP_KEYS = 128;
-constexpr int KP_SOFTMAX = 256, KP_THREADS = KP_SOFTMAX + 256 + 32;
+constexpr int KP_SOFTMAX = 256, KP_EXPAND = 7, KP_THREADS = KP_SOFTMAX + 32 * KP_EXPAND + 32;
 constexpr uint32_t KP_SUB = 128 * 128;                                 // bytes of 128 rows x 64 bf16: one swizzled sub-tile
 constexpr uint32_t kp_smem_bytes(int G) { return KP_SUB * (uint32_t)(5 * G + 4) + 256 + 1024; }      // Q, 2 K, 2 V, 2 P of two halves; barriers
 static_assert(kp_smem_bytes(2) <= 227 * 1024, "the 128-wide head fills the shared memory of one SM");
@@ -40,23 +40,31 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight codes of a word as bf16 values c * s + b, b = -z * s: a code in the low bits of a bf16 pattern is 128 + c exactly, so the product is
-// taken of that and the constant carries the rest, in fp32 (135 s at most, so 2^-17 of a step), and rounded once.
-__device__ __forceinline__ uint4 kv4_expand(uint32_t w, float s, float z) {
-    const float b128 = -(128.0f + z) * s;
+// Eight codes of a word as bf16 values (c - z) * s.  A code anywhere in the mantissa of an fp32 number is that power of two plus c; at bits 8, 12
+// and 16 (2^15, 2^11, 2^7) the constant -(2^k + z) * s is still good to 2^-8 of a step, less than the rounding to bf16 that follows, and
+// one "and-or" per code makes the number: ten operations a word, where masks in pairs and halves took fifteen.
+__device__ __noinline__ uint4 kv4_expand_large(uint32_t w, float s, float z) {        // 2^15 s would leave the range of fp32
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t p = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-        x[i] = fmaf(__uint_as_float(p << 16), s, b128);
-        x[i + 4] = fmaf(__uint_as_float(p & 0xFFFF0000u), s, b128);
-    }
-    if (__builtin_expect(s > 0x1p110f, 0)) {                           // 135 s may leave the range of fp32 where (c - z) s does not
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = ((float)(w >> (4 * i) & 15u) - z) * s;
-    }
+    for (int i = 0; i < 8; ++i) x[i] = ((float)(w >> (4 * i) & 15u) - z) * s;
     return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
+struct Kv4Step {
+    float s, z, b[3];
+    __device__ __forceinline__ Kv4Step(float scale, float zero) : s(scale), z(zero) {
+        b[0] = -(32768.0f + z) * s; b[1] = -(2048.0f + z) * s; b[2] = -(128.0f + z) * s;
+    }
+    template <int K>                                                   // of the code at bits 8 + 4 K of w
+    __device__ __forceinline__ float value(uint32_t w) const {
+        return fmaf(__uint_as_float((w & (0xF00u << (4 * K))) | ((uint32_t)(127 + 15 - 4 * K) << 23)), s, b[K]);
+    }
+    __device__ __forceinline__ uint4 values(uint32_t w) const {
+        if (__builtin_expect(s > 0x1p110f, 0)) return kv4_expand_large(w, s, z);
+        const uint32_t up = w << 12, down = w >> 12;
+        return make_uint4(pack_bf16x2(value<1>(up), value<2>(up)), pack_bf16x2(value<0>(w), value<1>(w)), pack_bf16x2(value<2>(w), value<0>(down)),
+                          pack_bf16x2(value<1>(down), value<2>(down)));
+    }
+};
 
 // The same with tiles of 128 slots
 __device__ __forceinline__ Kv4Tiles kv4_key_tiles(const Kv4Span& s, int sinks) {
@@ -72,7 +80,7 @@ __device__ __forceinline__ Kv4Tiles kv4_key_tiles(const Kv4Span& s, int sinks) {
 
 template <int G>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4AttendParams P, const int tok_per_cta) {
-    constexpr int D = 64 * G, TILE = kv4_tile_bytes(G);
+    constexpr int D = 64 * G, TILE = kv4_tile_bytes(G), SUBTILES = KP_KEYS / KV4_TILE;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t no_number;                                     // a group of values that is not a number was seen
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -112,24 +120,28 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
-            mbar_init(bar_kfull(s), 128); mbar_init(bar_kempty(s), 1);
-            mbar_init(bar_vfull(s), 128); mbar_init(bar_vempty(s), 1);
+            mbar_init(bar_kfull(s), SUBTILES * G); mbar_init(bar_kempty(s), 1);
+            mbar_init(bar_vfull(s), SUBTILES * G); mbar_init(bar_vempty(s), 1);
             mbar_init(bar_sfull(s), 1); mbar_init(bar_sempty(s), KP_SOFTMAX);
             for (int h = 0; h < 2; ++h) { mbar_init(bar_pfull(h, s), 128); mbar_init(bar_pempty(h, s), 1); }
         }
         mbar_fence_init();
         no_number = 0u;
     }
-    // queries: rows that are none are zero
+    // queries: rows that are none are zero.  The scale is made positive (its sign goes to the queries; none at all: queries of zero), so that
+    // maxima can be taken of raw scores
+    const float scale = P.scale_log2 == 0.0f ? 1.0f : fabsf(P.scale_log2);
+    const uint32_t q_and = P.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu, q_xor = P.scale_log2 < 0.0f ? 0x80008000u : 0u;
     for (int i = threadIdx.x; i < KP_ROWS * D / 8; i += KP_THREADS) {
         const int r = i / (D / 8), c = i % (D / 8), tok = P.by_rep(r), row_tok = tok0 + tok;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (tok < tok_per_cta && row_tok < P.T)
             v = __ldg(reinterpret_cast<const uint4*>(P.q + ((long long)seq * P.T + row_tok) * P.ld_q + (kvh * P.rep + r - tok * P.rep) * D) + c);
-        sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), v.x, v.y, v.z, v.w);
+        sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), (v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor,
+               (v.w & q_and) ^ q_xor);
     }
     fence_proxy_async();
-    if (warp == 16) { tmem_alloc<false>(tmem_slot, 512); tmem_relinquish<false>(); }
+    if (warp == KP_THREADS / 32 - 1) { tmem_alloc<false>(tmem_slot, 512); tmem_relinquish<false>(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -156,7 +168,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             mbar_arrive(bar_sempty(j & 1));
             float x[64];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(v[i >> 5][i & 31]) * P.scale_log2;
+            for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(v[i >> 5][i & 31]);
             const int k0 = tiles.tile(j) * KP_KEYS;
             if (k0 + KP_KEYS - 1 > span.hi_min || (k0 < span.lo_max && k0 + KP_KEYS > P.sinks)) {                      // a border crosses this tile
                 const int hi = range.hi - k0 - half * 64, lo = range.lo - k0 - half * 64, sinks = P.sinks - k0 - half * 64;
@@ -166,8 +178,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             }
             float t[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int i = 4; i < 64; ++i) t[i & 3] = fmaxf(t[i & 3], x[i]);
-            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            for (int i = 4; i < 60; i += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), x[i + 4 + k]);
+            const float top = scale * fmaxf(fmaxf(fmaxf(t[0], x[60]), fmaxf(t[1], x[61])), fmaxf(fmaxf(t[2], x[62]), fmaxf(t[3], x[63])));
             const bool move = top > m + 8.0f;
             if (__any_sync(full_mask, move)) {
                 // (a row without a reference has a context of zeros: nothing to rescale)
@@ -190,12 +204,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
                     tc_fence_before();
                 }
             }
-            const float base = m == -INFINITY ? 0.0f : m;
+            const float base = m == -INFINITY ? 0.0f : -m;
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             uint32_t p[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                const float a = ex2(x[2 * i] - base), b = ex2(x[2 * i + 1] - base);
+                const float a = ex2(fmaf(x[2 * i], scale, base)), b = ex2(fmaf(x[2 * i + 1], scale, base));
                 p[i] = pack_bf16x2(a, b);
                 s[i & 3] += a + b;
             }
@@ -215,7 +229,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         tc_fence_after();
         stat[half * KP_ROWS + r] = m;
         stat[(2 + half) * KP_ROWS + r] = l;
-        asm volatile("bar.sync 1, 384;" ::: "memory");                  // the softmax warps; those of the values have arrived (no_number)
+        asm volatile("bar.sync 1, 480;" ::: "memory");                  // the softmax warps; those that expand have arrived (no_number)
         const float om = stat[(half ^ 1) * KP_ROWS + r], ol = stat[(2 + (half ^ 1)) * KP_ROWS + r];
         const float gm = fmaxf(m, om), base = gm == -INFINITY ? 0.0f : gm;
         const float mine = ex2(m - base), other = ex2(om - base), inv = 1.0f / (l * mine + ol * other);
@@ -257,53 +271,73 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             }
         }
         tc_fence_before();
-    } else if (warp < 16) {
-        // =========================================================== keys, values: slots 32 w .. of every tile; 8 lanes a slot and group
-        const bool keys = warp < 12;
-        const int w = warp & 3, chunk = lane & 7, quarter = lane >> 3;
+    } else if (warp < 8 + KP_EXPAND) {
+        // =========================================================== expansion: units (tile, keys or values, group, 32 slots) in this order
         const uint8_t* base = P.cache.tiles + (long long)seq * P.cache.seq_stride + (long long)kvh * P.cache.n_tiles * TILE;
-        uint32_t codes[G][8], meta[G][8];                              // of the next tile: codes, { zero, scale }
-        auto request = [&](int j) {
-            const int at = tiles.tile(j) * (KP_KEYS / KV4_TILE) + w;
-            const bool held = at < P.cache.n_tiles;                    // (the last tile may reach beyond the cache)
+        const int units = n * 2 * G * SUBTILES;
+        // Keys: a lane has a slot, all 64 channels.  Values: a lane has half the chunks of a pair of slots; every other two pairs swap neighbouring
+        // chunks, so that eight lanes store to eight places of a row
+        const int pair = lane >> 1, swap = (pair >> 1) & 1;
+        uint4 raw[2];
+        uint32_t meta[2];                                              // keys: { zero, scale }; values: both scales, both zeros
+        auto request = [&](int u) {
+            const int sub = u % SUBTILES, g = u / SUBTILES % G, at = tiles.tile(u / (2 * G * SUBTILES)) * SUBTILES + sub;
+            const bool keys = u / (G * SUBTILES) % 2 == 0, held = at < P.cache.n_tiles;              // (the last tile may reach beyond the cache)
             const uint8_t* tile = base + (long long)(held ? at : 0) * TILE;
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int slot = 4 * i + quarter;
-                    if (keys) {
-                        codes[g][i] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_row(G, g, slot) + 4 * chunk));
-                        meta[g][i] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, slot)));
-                    } else {
-                        codes[g][i] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_v_chunk(G, g, slot, chunk)));
-                        meta[g][i] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, slot))) << 16 |
-                                     __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_zero(G, g, slot)));
-                    }
-                    if (!held || nobody(KV4_TILE * at + slot)) meta[g][i] = 0u;        // zeros: nobody sees it, it may hold anything
-                }
+            const uint4* p = reinterpret_cast<const uint4*>(tile + (keys ? 0 : 1024 * G) + 1024 * g + 32 * lane);       // 32 slots, or 16 pairs of 2 halves
+            raw[0] = __ldg(p);
+            raw[1] = __ldg(p + 1);
+            const int j = KV4_TILE * at;
+            if (keys) {
+                meta[0] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, lane)));
+                if (!held || nobody(j + lane)) meta[0] = 0u;           // zeros: nobody sees it, it may hold anything
+            } else {
+                meta[0] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair))) |
+                          (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair + 1))) << 16;
+                meta[1] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_v_zero(G, g, 2 * pair)));
+                if (!held || nobody(j + 2 * pair)) { meta[0] &= 0xFFFF0000u; meta[1] &= 0xFFFF0000u; }
+                if (!held || nobody(j + 2 * pair + 1)) { meta[0] &= 0x0000FFFFu; meta[1] &= 0x0000FFFFu; }
+            }
         };
-        request(0);
-        for (int j = 0; j < n; ++j) {
-            const int s = j & 1;
+        int u = warp - 8;
+        if (u < units) request(u);
+#pragma unroll 1
+        for (; u < units; u += KP_EXPAND) {
+            const int sub = u % SUBTILES, g = u / SUBTILES % G, j = u / (2 * G * SUBTILES), s = j & 1;
+            const bool keys = u / (G * SUBTILES) % 2 == 0;
             if (!__all_sync(full_mask, mbar_wait_bounded(keys ? bar_kempty(s) : bar_vempty(s), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY))) break;
-            const uint32_t dst = (keys ? k_base : v_base) + (uint32_t)s * G * KP_SUB + (uint32_t)(32 * w) * 128u;
+            const uint32_t dst = (keys ? k_base : v_base) + (uint32_t)(s * G + g) * KP_SUB + (uint32_t)(32 * sub) * 128u;
+            const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+            if (keys) {
+                const Kv4Step st(__uint_as_float(meta[0] & 0xFFFF0000u), f16_to_float(meta[0] & 0xFFFFu));
+                if (u + KP_EXPAND < units) request(u + KP_EXPAND);
 #pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t row = (uint32_t)(4 * i + quarter);
-                    uint32_t mt = meta[g][i];
-                    if (!keys && (mt & 0x7F800000u) == 0x7F800000u) { mt = 0u; no_number = 1u; }
-                    const float sc = __uint_as_float(mt & 0xFFFF0000u), z = f16_to_float(mt & 0xFFFFu);
-                    const uint4 x = kv4_expand(codes[g][i], sc, z);
-                    sts128(dst + (uint32_t)g * KP_SUB + row * 128u + ((((uint32_t)chunk) ^ (row & 7u)) << 4), x.x, x.y, x.z, x.w);
+                for (int c = 0; c < 8; ++c) {
+                    const uint4 x = st.values(w[c]);
+                    sts128(dst + (uint32_t)lane * 128u + (((uint32_t)c ^ ((uint32_t)lane & 7u)) << 4), x.x, x.y, x.z, x.w);
                 }
-            if (j + 1 < n) request(j + 1);
+            } else {
+                uint32_t sc = meta[0], ze = meta[1];
+                if ((sc & 0x7F80u) == 0x7F80u) { sc &= 0xFFFF0000u; ze &= 0xFFFF0000u; no_number = 1u; }
+                if ((sc & 0x7F800000u) == 0x7F800000u) { sc &= 0x0000FFFFu; ze &= 0x0000FFFFu; no_number = 1u; }
+                const Kv4Step even(__uint_as_float(sc << 16), f16_to_float(ze & 0xFFFFu)), odd(__uint_as_float(sc & 0xFFFF0000u), f16_to_float(ze >> 16));
+                if (u + KP_EXPAND < units) request(u + KP_EXPAND);
+                const uint32_t row = 2u * (uint32_t)pair;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {                          // words 2k, 2k + 1: place 4 h + k of both slots
+                    const int k1 = i ^ 1;
+                    const uint32_t we = swap ? w[2 * k1] : w[2 * i], wo = swap ? w[2 * k1 + 1] : w[2 * i + 1];
+                    const uint32_t place = 4u * ((uint32_t)lane & 1u) + (uint32_t)(swap ? k1 : i), chunk = place ^ (((uint32_t)pair & 2u) << 1);
+                    const uint4 x = even.values(we), y = odd.values(wo);
+                    sts128(dst + row * 128u + ((chunk ^ (row & 7u)) << 4), x.x, x.y, x.z, x.w);
+                    sts128(dst + (row + 1u) * 128u + ((chunk ^ ((row + 1u) & 7u)) << 4), y.x, y.y, y.z, y.w);
+                }
+            }
             fence_proxy_async();
-            mbar_arrive(keys ? bar_kfull(s) : bar_vfull(s));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(keys ? bar_kfull(s) : bar_vfull(s));
         }
-        if (!keys) asm volatile("bar.arrive 1, 384;" ::: "memory");
+        asm volatile("bar.arrive 1, 480;" ::: "memory");
     } else {
         // =========================================================== MMA
         const uint32_t idesc_s = umma_idesc(KP_KEYS);
@@ -356,7 +390,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) { tc_fence_after(); tmem_dealloc<false>(tmem, 512); }
+    if (warp == KP_THREADS / 32 - 1) { tc_fence_after(); tmem_dealloc<false>(tmem, 512); }
 }
 
 }  // namespace cb

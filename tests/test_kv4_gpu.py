@@ -364,7 +364,7 @@ def test_a_value_group_that_is_no_number_reaches_who_sees_it(T, D):
 
 
 @pytest.mark.parametrize("T", [1, 2, 70])
-@pytest.mark.parametrize("k_gain,v_gain,q_gain", [(1e-6, 1e-5, 1.0), (1e4, 1e6, 1e-4), (1e-20, 1e30, 1e20), (1.0, 1e-30, 1.0), (1e15, 1.0, 1e-15)])
+@pytest.mark.parametrize("k_gain,v_gain,q_gain", [(1e-6, 1e-5, 1.0), (1e4, 1e6, 1e-4), (1e-20, 1e30, 1e20), (1.0, 1e-30, 1.0), (1e15, 1.0, 1e-15), (1e33, 1e33, 1e-33)])
 def test_ranges_of_keys_values_and_queries(T, k_gain, v_gain, q_gain):
     """bf16 inputs of any size whose scores are ordinary; scales that differ from slot to slot by many powers of two."""
     heads, n_kv, D, slots = 4, 2, 128, 300
