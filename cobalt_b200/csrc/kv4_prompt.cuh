@@ -59,7 +59,6 @@ struct Kv4Step {
         return fmaf(__uint_as_float((w & (0xF00u << (4 * K))) | ((uint32_t)(127 + 15 - 4 * K) << 23)), s, b[K]);
     }
     __device__ __forceinline__ uint4 values(uint32_t w) const {
-        if (__builtin_expect(s > 0x1p110f, 0)) return kv4_expand_large(w, s, z);
         const uint32_t up = w << 12, down = w >> 12;
         return make_uint4(pack_bf16x2(value<1>(up), value<2>(up)), pack_bf16x2(value<0>(w), value<1>(w)), pack_bf16x2(value<2>(w), value<0>(down)),
                           pack_bf16x2(value<1>(down), value<2>(down)));
@@ -279,7 +278,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         // chunks, so that eight lanes store to eight places of a row
         const int pair = lane >> 1, swap = (pair >> 1) & 1;
         uint4 raw[2];
-        uint32_t meta[2];                                              // keys: { zero, scale }; values: both scales, both zeros
+        uint32_t meta[3];                                              // keys: { zero, scale }; values: the scales, both zeros.  Nothing is done
+        bool hidden[2];                                                // with them before they are used: the request would wait for its loads
         auto request = [&](int u) {
             const int sub = u % SUBTILES, g = u / SUBTILES % G, at = tiles.tile(u / (2 * G * SUBTILES)) * SUBTILES + sub;
             const bool keys = u / (G * SUBTILES) % 2 == 0, held = at < P.cache.n_tiles;              // (the last tile may reach beyond the cache)
@@ -287,16 +287,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             const uint4* p = reinterpret_cast<const uint4*>(tile + (keys ? 0 : 1024 * G) + 1024 * g + 32 * lane);       // 32 slots, or 16 pairs of 2 halves
             raw[0] = __ldg(p);
             raw[1] = __ldg(p + 1);
-            const int j = KV4_TILE * at;
+            const int j = KV4_TILE * at + (keys ? lane : 2 * pair);
+            hidden[0] = !held || nobody(j);                            // zeros: nobody sees the slot, it may hold anything
+            hidden[1] = !held || nobody(j + 1);
             if (keys) {
                 meta[0] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, lane)));
-                if (!held || nobody(j + lane)) meta[0] = 0u;           // zeros: nobody sees it, it may hold anything
             } else {
-                meta[0] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair))) |
-                          (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair + 1))) << 16;
-                meta[1] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_v_zero(G, g, 2 * pair)));
-                if (!held || nobody(j + 2 * pair)) { meta[0] &= 0xFFFF0000u; meta[1] &= 0xFFFF0000u; }
-                if (!held || nobody(j + 2 * pair + 1)) { meta[0] &= 0x0000FFFFu; meta[1] &= 0x0000FFFFu; }
+                meta[0] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair)));
+                meta[1] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair + 1)));
+                meta[2] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_v_zero(G, g, 2 * pair)));
             }
         };
         int u = warp - 8;
@@ -309,28 +308,45 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             const uint32_t dst = (keys ? k_base : v_base) + (uint32_t)(s * G + g) * KP_SUB + (uint32_t)(32 * sub) * 128u;
             const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
             if (keys) {
-                const Kv4Step st(__uint_as_float(meta[0] & 0xFFFF0000u), f16_to_float(meta[0] & 0xFFFFu));
+                const uint32_t m = hidden[0] ? 0u : meta[0];
+                const Kv4Step st(__uint_as_float(m & 0xFFFF0000u), f16_to_float(m & 0xFFFFu));
                 if (u + KP_EXPAND < units) request(u + KP_EXPAND);
+                auto store = [&](int c, const uint4 x) { sts128(dst + (uint32_t)lane * 128u + (((uint32_t)c ^ ((uint32_t)lane & 7u)) << 4), x.x, x.y, x.z, x.w); };
+                if (__builtin_expect(__any_sync(full_mask, st.s > 0x1p110f), 0)) {
+                    for (int c = 0; c < 8; ++c) store(c, kv4_expand_large(w[c], st.s, st.z));
+                } else {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const uint4 x = st.values(w[c]);
-                    sts128(dst + (uint32_t)lane * 128u + (((uint32_t)c ^ ((uint32_t)lane & 7u)) << 4), x.x, x.y, x.z, x.w);
+                    for (int c = 0; c < 8; ++c) store(c, st.values(w[c]));
                 }
             } else {
-                uint32_t sc = meta[0], ze = meta[1];
-                if ((sc & 0x7F80u) == 0x7F80u) { sc &= 0xFFFF0000u; ze &= 0xFFFF0000u; no_number = 1u; }
-                if ((sc & 0x7F800000u) == 0x7F800000u) { sc &= 0x0000FFFFu; ze &= 0x0000FFFFu; no_number = 1u; }
-                const Kv4Step even(__uint_as_float(sc << 16), f16_to_float(ze & 0xFFFFu)), odd(__uint_as_float(sc & 0xFFFF0000u), f16_to_float(ze >> 16));
+                uint32_t s0v = hidden[0] ? 0u : meta[0], s1v = hidden[1] ? 0u : meta[1];
+                uint32_t z0 = hidden[0] ? 0u : meta[2] & 0xFFFFu, z1 = hidden[1] ? 0u : meta[2] >> 16;
+                if ((s0v & 0x7F80u) == 0x7F80u) { s0v = z0 = 0u; no_number = 1u; }
+                if ((s1v & 0x7F80u) == 0x7F80u) { s1v = z1 = 0u; no_number = 1u; }
+                const Kv4Step even(__uint_as_float(s0v << 16), f16_to_float(z0)), odd(__uint_as_float(s1v << 16), f16_to_float(z1));
                 if (u + KP_EXPAND < units) request(u + KP_EXPAND);
                 const uint32_t row = 2u * (uint32_t)pair;
+                uint32_t we[4], wo[4], at[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {                          // words 2k, 2k + 1: place 4 h + k of both slots
                     const int k1 = i ^ 1;
-                    const uint32_t we = swap ? w[2 * k1] : w[2 * i], wo = swap ? w[2 * k1 + 1] : w[2 * i + 1];
-                    const uint32_t place = 4u * ((uint32_t)lane & 1u) + (uint32_t)(swap ? k1 : i), chunk = place ^ (((uint32_t)pair & 2u) << 1);
-                    const uint4 x = even.values(we), y = odd.values(wo);
-                    sts128(dst + row * 128u + ((chunk ^ (row & 7u)) << 4), x.x, x.y, x.z, x.w);
-                    sts128(dst + (row + 1u) * 128u + ((chunk ^ ((row + 1u) & 7u)) << 4), y.x, y.y, y.z, y.w);
+                    we[i] = swap ? w[2 * k1] : w[2 * i];
+                    wo[i] = swap ? w[2 * k1 + 1] : w[2 * i + 1];
+                    const uint32_t place = 4u * ((uint32_t)lane & 1u) + (uint32_t)(swap ? k1 : i);
+                    at[i] = place ^ (((uint32_t)pair & 2u) << 1);      // its chunk
+                }
+                auto store = [&](uint32_t r, uint32_t chunk, const uint4 x) { sts128(dst + r * 128u + ((chunk ^ (r & 7u)) << 4), x.x, x.y, x.z, x.w); };
+                if (__builtin_expect(__any_sync(full_mask, fmaxf(even.s, odd.s) > 0x1p110f), 0)) {
+                    for (int i = 0; i < 4; ++i) {
+                        store(row, at[i], kv4_expand_large(we[i], even.s, even.z));
+                        store(row + 1u, at[i], kv4_expand_large(wo[i], odd.s, odd.z));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        store(row, at[i], even.values(we[i]));
+                        store(row + 1u, at[i], odd.values(wo[i]));
+                    }
                 }
             }
             fence_proxy_async();
