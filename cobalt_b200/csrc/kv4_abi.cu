@@ -1,5 +1,6 @@
 // C ABI of the 4-bit KV cache: argument validation and launches.  See include/cobalt_b200.h.
 #include <algorithm>
+#include <cmath>
 
 #include "kv4_attend.cuh"
 #include "kv4_prompt.cuh"
@@ -75,12 +76,13 @@ int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, i
     const int64_t entries = (int64_t)n_seq * c->col_tiles, heads = entries * n_kv;
     if (heads > 0x3FFFFFFFll) return COBALT_ETOOBIG;
     const int ctas = std::min(sms * ka_ctas_per_sm(G, c->nb), KC_MAX_STATES);
-    // tiles of a head at most, if its tokens follow one another
-    int64_t tiles = (n_slots + KV4_TILE - 1) / KV4_TILE;
+    // tiles of a head at most, if its tokens follow one another (and if not: the counts of the list are 32-bit)
+    const int64_t whole = (n_slots + KV4_TILE - 1) / KV4_TILE;
+    int64_t tiles = whole;
     if (window > 0) tiles = std::min(tiles, ((int64_t)window + T) / KV4_TILE + 2 + ((int64_t)sinks + KV4_TILE - 1) / KV4_TILE);
     c->share = 1;
     while (c->share < KA_MAX_CLUSTER && c->share * 2 * heads <= ctas && c->share * KA_MIN_TILES < tiles) c->share *= 2;
-    c->list = entries <= KA_ENTRIES && heads * tiles < 1000000000ll && heads < 4ll * ctas && 
+    c->list = entries <= KA_ENTRIES && heads * whole < 1000000000ll && heads < 4ll * ctas && 
               tiles * ctas > c->share * KA_WARPS * (6ll * ctas + 64 * heads * c->share);
     c->grid = c->list ? (int)std::min<int64_t>(ctas, (heads * tiles + KA_MIN_TILES - 1) / KA_MIN_TILES) : (int)heads * c->share;
     if (!c->list && heads * c->share > 0x7FFFFFFFll) return COBALT_ETOOBIG;
@@ -126,10 +128,21 @@ int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c
     return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<G, NB>, P, W) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
 }
 
-// Rows (columns of the other kernels) of a KV head from which a prompt's kernel takes them.
+// Whether the prompts' kernel takes a call: at 64 rows per KV head and more, where it is expected to be faster.  Its CTAs walk all keys of their
+// rows, a tile of 128 every 2.3 us (128 channels; 1.5 us: 64), so few of them over a long cache are slow; the kernel of few rows splits
+// the keys, too, and takes 1.33 ns per tile of 32 slots and tile of columns (16 at 128 channels, 32 at 64), over the whole GPU.  Measured
+// (prompt / few, us), 16 / 2 heads of 128, one sequence: 64 tokens over 600 slots 20 / 12, 512 over 600 20 / 21, 512 over 4096 83 / 101,
+// 512 over 32768 602 / 697, 128 over 32768 594 / 188; 32 / 8 heads, 4 sequences, 64 tokens over 4096 83 / 107, 32768 658 / 704.
 constexpr int KP_MIN_ROWS = 64;
-bool prompt_takes(int n_seq, int rep, int T, int D) {
-    return (D == 64 || D == 128) && n_seq <= 65535 && rep <= KP_ROWS && (int64_t)rep * T >= KP_MIN_ROWS;
+bool prompt_takes(int n_seq, int n_kv, int rep, int T, int D, int n_slots, int window, int sinks, int sms) {
+    if ((D != 64 && D != 128) || n_seq > 65535 || rep > KP_ROWS || (int64_t)rep * T < KP_MIN_ROWS) return false;
+    double slots = n_slots;
+    if (window > 0) slots = std::min(slots, (double)window + sinks + std::min(T, KP_ROWS) + 2 * KP_KEYS);
+    const int tok = KP_ROWS / rep;
+    const double ctas = (double)((T + tok - 1) / tok) * n_kv * n_seq, eights = ((double)rep * T + 7) / 8;
+    const double prompt = std::ceil(ctas / sms) * std::ceil(slots / KP_KEYS) * (D == 128 ? 2.3 : 1.5) + 6.0;
+    const double few = std::ceil(eights / ka_max_nb(D / KV4_GROUP)) * n_kv * n_seq * std::ceil(slots / KV4_TILE) * 1.33e-3 + 7.0;
+    return prompt < few;
 }
 template <int G>
 int launch_prompt(const Kv4AttendParams& P, cudaStream_t st) {
@@ -211,7 +224,7 @@ size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_h
     int sms = 0;
     if (n_seq <= 0 || T <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_slots <= 0 || window < 0 || sinks < 0 ||
         !dim_ok(head_dim) || sm_count(&sms)) return 0;
-    if (prompt_takes(n_seq, n_heads / n_kv_heads, T, head_dim)) return 0;
+    if (prompt_takes(n_seq, n_kv_heads, n_heads / n_kv_heads, T, head_dim, n_slots, window, sinks, sms)) return 0;
     AttendCfg c;
     return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c) ? 0 : c.scratch;
 }
@@ -226,7 +239,7 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
-    const bool prompt = prompt_takes(n_seq, n_heads / n_kv_heads, T, head_dim);
+    const bool prompt = prompt_takes(n_seq, n_kv_heads, n_heads / n_kv_heads, T, head_dim, n_slots, window, sinks, sms);
     AttendCfg c = {};
     if (!prompt && (rc = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c))) return rc;
     if (c.list && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < c.scratch)) return COBALT_ESCRATCH;

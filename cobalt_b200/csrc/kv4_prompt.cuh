@@ -5,18 +5,27 @@
 // keys, 128 at a time, with running maxima and sums:
 //   warps 0-7   softmax: warp w owns TMEM lanes 32*(w%4).. (a thread = a row) and key columns 64*(w/4).. of every tile.  The two halves of a
 //               row's keys keep a maximum, a sum and a context of their own - nothing is exchanged between threads until the end,
-//               where the two are joined.  A maximum moves only when a score exceeds it by 2^8 (the probabilities are bf16, which have
-//               the room); then the warp rescales its part of the context in tensor memory, after the product before it.
-//   warps 8-14  expand: a unit is 32 slots of a group of keys, or of values; codes to bf16 in K-major (values: N-major), 128-byte-swizzled
+//               where the two are joined.  A maximum moves only when a score exceeds it by 2^8 (the probabilities are fp16, times 2^6,
+//               which have the room); then the warp rescales its part of the context in tensor memory, after the product before it.
+//   warps 8-14  expand: a unit is 32 slots of a group of keys, or of values; codes to fp16 in K-major (values: N-major), 128-byte-swizzled
 //               operands.  Units go round the seven warps, each with its next unit requested ahead
 //   warp 15     MMA: scores into one of two TMEM buffers, the two contexts into two others; the scores of tile j+1 are issued before
 //               the context of tile j
 // Key tiles that no row of the CTA sees are skipped (between the first slots and the window, too); only tiles on a border are masked.
-// Keys, values and probabilities are rounded to bf16 once (the operands' type); scores, maxima, sums and contexts are fp32.
+// Operands are fp16 (2^-11): in bf16 the roundings of keys, values and probabilities doubled the result's error (3.3e-3 against 1.7e-3, which
+// is that of its own rounding).  So that any bf16 range fits, queries are scaled by a power of two per row, keys and values by one each
+// per CTA, from the largest magnitude that the scales and zeros of its visible slots allow (looked through once at the start: 4 G + 4 G
+// bytes a slot); scores, maxima, sums and contexts are fp32.
 //
 // A slot that only some rows see has to stay out of the others' products even where its values are not numbers: such groups are
 // expanded to zeros and marked, and marked CTAs look through the scales of their rows' slots once at the end.
-// MEASURED_PROMPT
+//
+// Bound: the latency of instructions at 16 warps an SM (1.7 a clock; no pipe above 40 %).  A unit of expansion takes 1440 clocks, so the 16 units
+// of a tile of 128 channels 3300 on seven warps; softmax takes 2000 a tile beside it, the tensor pipe 1000.  2048 tokens, 32 / 8 heads of 128:
+// 102 us; 2 x 500 tokens with a window of 1024 over 6000 slots, 32 / 16 heads: 71 us (the kernel of few rows: 248 and 138 us).
+// Steps: a lane per eight channels with scale, zero and visibility for each word 166 us; whole rows per lane, ten operations a word, maxima of raw
+// scores 113 us; no branch per word, so that words overlap 97 us; fp16 operands 102 us.  Eleven expanding warps at 72 registers (softmax
+// 128) slowed the softmax by 30 % and gained nothing.
 #pragma once
 #include "kv4_attend.cuh"
 #include "tcgen05.cuh"
@@ -25,7 +34,7 @@ namespace cb {
 
 constexpr int KP_ROWS = 128, KP_KEYS = 128;
 constexpr int KP_SOFTMAX = 256, KP_EXPAND = 7, KP_THREADS = KP_SOFTMAX + 32 * KP_EXPAND + 32;
-constexpr uint32_t KP_SUB = 128 * 128;                                 // bytes of 128 rows x 64 bf16: one swizzled sub-tile
+constexpr uint32_t KP_SUB = 128 * 128;                                 // bytes of 128 rows x 64 fp16: one swizzled sub-tile
 constexpr uint32_t kp_smem_bytes(int G) { return KP_SUB * (uint32_t)(5 * G + 4) + 256 + 1024; }      // Q, 2 K, 2 V, 2 P of two halves; barriers
 static_assert(kp_smem_bytes(2) <= 227 * 1024, "the 128-wide head fills the shared memory of one SM");
 
@@ -40,18 +49,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight codes of a word as bf16 values (c - z) * s.  A code anywhere in the mantissa of an fp32 number is that power of two plus c; at bits 8, 12
-// and 16 (2^15, 2^11, 2^7) the constant -(2^k + z) * s is still good to 2^-8 of a step, less than the rounding to bf16 that follows, and
-// one "and-or" per code makes the number: ten operations a word, where masks in pairs and halves took fifteen.
-__device__ __noinline__ uint4 kv4_expand_large(uint32_t w, float s, float z) {        // 2^15 s would leave the range of fp32
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ((float)(w >> (4 * i) & 15u) - z) * s;
-    return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-}
+// Eight codes of a word as fp16 values (c - z) * s.  A code anywhere in the mantissa of an fp32 number is that power of two plus c; at bits 8, 12
+// and 16 (2^15, 2^11, 2^7) the constant -(2^k + z) * s is still good to 2^-8 of a step, and one "and-or" per code makes the number: ten
+// operations a word, where masks in pairs and halves took fifteen.
 struct Kv4Step {
-    float s, z, b[3];
-    __device__ __forceinline__ Kv4Step(float scale, float zero) : s(scale), z(zero) {
+    float s, b[3];
+    __device__ __forceinline__ Kv4Step(float scale, float z) : s(scale) {
         b[0] = -(32768.0f + z) * s; b[1] = -(2048.0f + z) * s; b[2] = -(128.0f + z) * s;
     }
     template <int K>                                                   // of the code at bits 8 + 4 K of w
@@ -60,10 +63,15 @@ struct Kv4Step {
     }
     __device__ __forceinline__ uint4 values(uint32_t w) const {
         const uint32_t up = w << 12, down = w >> 12;
-        return make_uint4(pack_bf16x2(value<1>(up), value<2>(up)), pack_bf16x2(value<0>(w), value<1>(w)), pack_bf16x2(value<2>(w), value<0>(down)),
-                          pack_bf16x2(value<1>(down), value<2>(down)));
+        return make_uint4(pack_f16x2(value<1>(up), value<2>(up)), pack_f16x2(value<0>(w), value<1>(w)), pack_f16x2(value<2>(w), value<0>(down)),
+                          pack_f16x2(value<1>(down), value<2>(down)));
     }
 };
+// largest magnitude that a group can hold; 0 for one that is no number
+__device__ __forceinline__ float kv4_largest(uint32_t scale, uint32_t zero) {
+    const float s = __uint_as_float(scale << 16), z = f16_to_float(zero), m = s * fmaxf(fabsf(z), fabsf(15.0f - z));
+    return m < INFINITY ? m : 0.0f;
+}
 
 // The same with tiles of 128 slots
 __device__ __forceinline__ Kv4Tiles kv4_key_tiles(const Kv4Span& s, int sinks) {
@@ -82,6 +90,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     constexpr int D = 64 * G, TILE = kv4_tile_bytes(G), SUBTILES = KP_KEYS / KV4_TILE;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t no_number;                                     // a group of values that is not a number was seen
+    __shared__ uint32_t largest[2];                                    // magnitude (bits) among the visible keys, values
+    __shared__ float q_fac[KP_ROWS];                                   // what the queries of a row were divided by
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full_mask = 0xFFFFFFFFu;
     const uint32_t s_raw = smem_u32(smem), s0 = (s_raw + 1023u) & ~1023u;
@@ -125,25 +135,57 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             for (int h = 0; h < 2; ++h) { mbar_init(bar_pfull(h, s), 128); mbar_init(bar_pempty(h, s), 1); }
         }
         mbar_fence_init();
-        no_number = 0u;
+        no_number = largest[0] = largest[1] = 0u;
+    }
+    __syncthreads();
+    const uint8_t* base = P.cache.tiles + (long long)seq * P.cache.seq_stride + (long long)kvh * P.cache.n_tiles * TILE;
+    {                                                                  // the largest key and value that some row sees
+        float top_k = 0.0f, top_v = 0.0f;
+        const int slots = n * KP_KEYS;
+        for (int i = threadIdx.x; i < slots; i += KP_THREADS) {
+            const int j = tiles.tile(i / KP_KEYS) * KP_KEYS + i % KP_KEYS, slot = j % KV4_TILE;
+            if (nobody(j)) continue;                                   // (slots beyond the cache among them)
+            const uint8_t* tile = base + (long long)(j / KV4_TILE) * TILE;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint32_t m = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, slot)));
+                top_k = fmaxf(top_k, kv4_largest(m >> 16, m & 0xFFFFu));
+                top_v = fmaxf(top_v, kv4_largest(__ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, slot))),
+                                                 __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_zero(G, g, slot)))));
+            }
+        }
+        const uint32_t bk = __reduce_max_sync(full_mask, __float_as_uint(top_k)), bv = __reduce_max_sync(full_mask, __float_as_uint(top_v));
+        if (lane == 0) { atomicMax(&largest[0], bk); atomicMax(&largest[1], bv); }
     }
     // queries: rows that are none are zero.  The scale is made positive (its sign goes to the queries; none at all: queries of zero), so that
     // maxima can be taken of raw scores
-    const float scale = P.scale_log2 == 0.0f ? 1.0f : fabsf(P.scale_log2);
     const uint32_t q_and = P.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu, q_xor = P.scale_log2 < 0.0f ? 0x80008000u : 0u;
     for (int i = threadIdx.x; i < KP_ROWS * D / 8; i += KP_THREADS) {
         const int r = i / (D / 8), c = i % (D / 8), tok = P.by_rep(r), row_tok = tok0 + tok;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (tok < tok_per_cta && row_tok < P.T)
             v = __ldg(reinterpret_cast<const uint4*>(P.q + ((long long)seq * P.T + row_tok) * P.ld_q + (kvh * P.rep + r - tok * P.rep) * D) + c);
-        sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), (v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor,
-               (v.w & q_and) ^ q_xor);
+        const uint32_t w[4] = {(v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor, (v.w & q_and) ^ q_xor};
+        uint32_t top = 0u, o[4];                                       // largest magnitude of the row; a NaN stays on top
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFF0000u, (w[k] & 0x7FFFu) << 16));
+#pragma unroll
+        for (int x = 1; x < D / 8; x <<= 1) top = max(top, __shfl_xor_sync(full_mask, top, x));
+        const int ex = max(-112, (int)(top >> 23) - 127);              // in [2^ex, 2^(ex + 1)), to [2^14, 2^15)
+        const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = pack_f16x2(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xFFFF0000u) * up);
+        if (c == 0) q_fac[r] = ex < 128 ? __uint_as_float((uint32_t)max(1, ex - 14 + 127) << 23) : __uint_as_float(0x7FC00000u);
+        sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), o[0], o[1], o[2], o[3]);
     }
     fence_proxy_async();
     if (warp == KP_THREADS / 32 - 1) { tmem_alloc<false>(tmem_slot, 512); tmem_relinquish<false>(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // keys and values times a power of two that brings the largest into [2^14, 2^15)
+    const int ex_k = max(-110, (int)(largest[0] >> 23) - 127), ex_v = max(-110, (int)(largest[1] >> 23) - 127);
+    const float up_k = __uint_as_float((uint32_t)(14 - ex_k + 127) << 23), up_v = __uint_as_float((uint32_t)(14 - ex_v + 127) << 23);
     const uint32_t tmem = lds32(tmem_slot), tmem_o = tmem + 2 * KP_KEYS;              // scores 2 x 128 columns, contexts 2 x D
 
     if (warp < 8) {
@@ -154,6 +196,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         const Kv4Range range = valid ? kv4_range(P, seq, tok) : Kv4Range{0, -1};
         const uint32_t my_lanes = (uint32_t)((warp & 3) * 32) << 16, my_o = tmem_o + my_lanes + (uint32_t)(half * D);
         bool healthy = true;
+        const float scale = q_fac[r] * __uint_as_float((uint32_t)(ex_k - 14 + 127) << 23) * (P.scale_log2 == 0.0f ? 1.0f : fabsf(P.scale_log2));
         float m = -INFINITY, l = 0.0f;                                  // reference and sum of this row's half, scores times log2(e)
         for (int j = 0; j < n; ++j) {
             healthy = __all_sync(full_mask, mbar_wait_bounded(bar_sfull(j & 1), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_ACC));
@@ -203,13 +246,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
                     tc_fence_before();
                 }
             }
-            const float base = m == -INFINITY ? 0.0f : -m;
+            const float base = m == -INFINITY ? 0.0f : 6.0f - m;           // probabilities times 2^6
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             uint32_t p[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
                 const float a = ex2(fmaf(x[2 * i], scale, base)), b = ex2(fmaf(x[2 * i + 1], scale, base));
-                p[i] = pack_bf16x2(a, b);
+                p[i] = pack_f16x2(a, b);
                 s[i & 3] += a + b;
             }
             l += (s[0] + s[1]) + (s[2] + s[3]);
@@ -231,7 +274,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         asm volatile("bar.sync 1, 480;" ::: "memory");                  // the softmax warps; those that expand have arrived (no_number)
         const float om = stat[(half ^ 1) * KP_ROWS + r], ol = stat[(2 + (half ^ 1)) * KP_ROWS + r];
         const float gm = fmaxf(m, om), base = gm == -INFINITY ? 0.0f : gm;
-        const float mine = ex2(m - base), other = ex2(om - base), inv = 1.0f / (l * mine + ol * other);
+        const float mine = ex2(m - base), other = ex2(om - base);
+        const float inv = __uint_as_float((uint32_t)(ex_v - 14 + 127) << 23) / (l * mine + ol * other);
         const float w0 = (half ? other : mine) * inv, w1 = (half ? mine : other) * inv;        // of the contexts of halves 0 and 1
         if (healthy) {
             const bool any = range.hi >= 0 && (range.lo <= range.hi || P.sinks > 0);
@@ -272,7 +316,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         tc_fence_before();
     } else if (warp < 8 + KP_EXPAND) {
         // =========================================================== expansion: units (tile, keys or values, group, 32 slots) in this order
-        const uint8_t* base = P.cache.tiles + (long long)seq * P.cache.seq_stride + (long long)kvh * P.cache.n_tiles * TILE;
+        // (seven warps: after keys of a tile a warp comes to keys of the same or the next one or to values of the same, so that what it last waited
+        // for puts every slot at most one turn of its barrier behind; with a step of more than a tile's units it could pass a turn unseen)
+        static_assert(KP_EXPAND < 2 * SUBTILES, "units of a tile of the narrowest head");
         const int units = n * 2 * G * SUBTILES;
         // Keys: a lane has a slot, all 64 channels.  Values: a lane has half the chunks of a pair of slots; every other two pairs swap neighbouring
         // chunks, so that eight lanes store to eight places of a row
@@ -309,21 +355,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
             if (keys) {
                 const uint32_t m = hidden[0] ? 0u : meta[0];
-                const Kv4Step st(__uint_as_float(m & 0xFFFF0000u), f16_to_float(m & 0xFFFFu));
+                const Kv4Step st(__uint_as_float(m & 0xFFFF0000u) * up_k, f16_to_float(m & 0xFFFFu));
                 if (u + KP_EXPAND < units) request(u + KP_EXPAND);
                 auto store = [&](int c, const uint4 x) { sts128(dst + (uint32_t)lane * 128u + (((uint32_t)c ^ ((uint32_t)lane & 7u)) << 4), x.x, x.y, x.z, x.w); };
-                if (__builtin_expect(__any_sync(full_mask, st.s > 0x1p110f), 0)) {
-                    for (int c = 0; c < 8; ++c) store(c, kv4_expand_large(w[c], st.s, st.z));
-                } else {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) store(c, st.values(w[c]));
-                }
+                for (int c = 0; c < 8; ++c) store(c, st.values(w[c]));
             } else {
                 uint32_t s0v = hidden[0] ? 0u : meta[0], s1v = hidden[1] ? 0u : meta[1];
                 uint32_t z0 = hidden[0] ? 0u : meta[2] & 0xFFFFu, z1 = hidden[1] ? 0u : meta[2] >> 16;
                 if ((s0v & 0x7F80u) == 0x7F80u) { s0v = z0 = 0u; no_number = 1u; }
                 if ((s1v & 0x7F80u) == 0x7F80u) { s1v = z1 = 0u; no_number = 1u; }
-                const Kv4Step even(__uint_as_float(s0v << 16), f16_to_float(z0)), odd(__uint_as_float(s1v << 16), f16_to_float(z1));
+                const Kv4Step even(__uint_as_float(s0v << 16) * up_v, f16_to_float(z0)), odd(__uint_as_float(s1v << 16) * up_v, f16_to_float(z1));
                 if (u + KP_EXPAND < units) request(u + KP_EXPAND);
                 const uint32_t row = 2u * (uint32_t)pair;
                 uint32_t we[4], wo[4], at[4];
@@ -336,17 +378,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
                     at[i] = place ^ (((uint32_t)pair & 2u) << 1);      // its chunk
                 }
                 auto store = [&](uint32_t r, uint32_t chunk, const uint4 x) { sts128(dst + r * 128u + ((chunk ^ (r & 7u)) << 4), x.x, x.y, x.z, x.w); };
-                if (__builtin_expect(__any_sync(full_mask, fmaxf(even.s, odd.s) > 0x1p110f), 0)) {
-                    for (int i = 0; i < 4; ++i) {
-                        store(row, at[i], kv4_expand_large(we[i], even.s, even.z));
-                        store(row + 1u, at[i], kv4_expand_large(wo[i], odd.s, odd.z));
-                    }
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        store(row, at[i], even.values(we[i]));
-                        store(row + 1u, at[i], odd.values(wo[i]));
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    store(row, at[i], even.values(we[i]));
+                    store(row + 1u, at[i], odd.values(wo[i]));
                 }
             }
             fence_proxy_async();
@@ -356,8 +391,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         asm volatile("bar.arrive 1, 480;" ::: "memory");
     } else {
         // =========================================================== MMA
-        const uint32_t idesc_s = umma_idesc(KP_KEYS);
-        const uint32_t idesc_o = umma_idesc(D) | (1u << 16);            // B (= V) is N-major
+        constexpr uint32_t BF16 = (1u << 7) | (1u << 10);               // (both operands fp16 instead)
+        const uint32_t idesc_s = umma_idesc(KP_KEYS) & ~BF16;
+        const uint32_t idesc_o = (umma_idesc(D) & ~BF16) | (1u << 16);            // B (= V) is N-major
         const uint64_t qd = umma_smem_desc(q_base);
         bool healthy = true;
         auto issue_scores = [&](int j) {

@@ -74,14 +74,14 @@ def visible(positions, slots, window, sinks):
 
 def attend(q, k, v, positions, slots, n_heads, scale, window=0, sinks=0):
     """fp64 ``[n, T, n_heads * D]``, per element the largest visible |value| of its channel's head, and per element what bounds of
-    roundings need: sum p |v|, sum p^2 v^2, sum p^2, and the largest visible scale * |q k| (2-norm of the products) of the row."""
+    roundings need: sum p |v|, and the largest visible scale * |q k| (2-norm of the products) of the row."""
     n, T, _ = q.shape
     D, n_kv = k.shape[-1], k.shape[1]
     rep = n_heads // n_kv
     see = visible(positions, slots, window, sinks)                                     # [n, T, slots]
     out = torch.zeros(n, T, n_heads, D, dtype=torch.float64, device=q.device)
     top = torch.zeros(n, T, n_heads, 1, dtype=torch.float64, device=q.device)
-    more = torch.zeros(4, n, T, n_heads, D, dtype=torch.float64, device=q.device)
+    more = torch.zeros(2, n, T, n_heads, D, dtype=torch.float64, device=q.device)
     qh = q.double().view(n, T, n_heads, D)
     for h in range(n_heads):
         kh, vh = k[:, h // rep, :slots], v[:, h // rep, :slots]
@@ -89,9 +89,7 @@ def attend(q, k, v, positions, slots, n_heads, scale, window=0, sinks=0):
         p = torch.nan_to_num(torch.softmax(s, -1))                                      # a row without slots: zeros
         out[:, :, h] = p @ torch.nan_to_num(vh)
         more[0, :, :, h] = p @ torch.nan_to_num(vh).abs()
-        more[1, :, :, h] = (p * p) @ torch.nan_to_num(vh).square()
-        more[2, :, :, h] = (p * p).sum(-1, keepdim=True)
         qk = (qh[:, :, h].square() @ torch.nan_to_num(kh).square().transpose(1, 2)).sqrt() * abs(scale)
-        more[3, :, :, h] = torch.where(see, qk, 0.0).amax(-1, keepdim=True)
+        more[1, :, :, h] = torch.where(see, qk, 0.0).amax(-1, keepdim=True)
         top[:, :, h] = torch.where(see[..., None], torch.nan_to_num(vh).abs().amax(-1)[:, None, :, None], 0.0).amax(2)
-    return out.view(n, T, -1), top.expand(-1, -1, -1, D).reshape(n, T, -1), more.view(4, n, T, -1)
+    return out.view(n, T, -1), top.expand(-1, -1, -1, D).reshape(n, T, -1), more.view(2, n, T, -1)

@@ -4,12 +4,11 @@ Writing and reading are compared bit for bit with fp32 operations on the CPU.  A
 value) of sums whose weights may be rounded to 16-bit floats on the way (2^-11 each, so at most 2^-11 of the largest visible value), with
 everything else in fp32 (below that again): |got - want| <= 2^-8 |want| + 2^-10 max|v|.
 
-Prompts (64 rows per KV head and more, heads of 64 and 128) have bf16 operands: probabilities, values and keys are rounded, 2^-8 relative at
-most each.  The first two add up to 2 * 2^-8 sum p|v|.  A score moves by d = scale * sum q k e with |e| <= 2^-8 independent roundings: by
-more than 7 * 2^-8 * scale * |q k| (2-norm of the products) with a probability below 2 exp(-49/2) (Hoeffding) each, and the context by
-2 d sum p|v| at most.  So |got - want| <= 2^-8 |want| + (2 * 2^-8 + 2 d) sum p|v|.  That bound is for single elements; the 2-norm of
-all errors has the roundings' spread, 2^-8 / sqrt(3) of each term: the variance is (2^-16 / 3) times
-want^2 + 2 sum p^2 v^2 + (scale |q k|)^2 sum p^2 (v - want)^2, with (v - want)^2 <= 2 v^2 + 2 want^2; its root may be exceeded by 1.5."""
+Prompts (64 rows per KV head and more, heads of 64 and 128) have fp16 operands: probabilities, values and keys are rounded, 2^-11 relative at
+most each.  The first two add up to 2 * 2^-11 sum p|v|.  A score moves by d = scale * sum q k e with |e| <= 2^-11 independent roundings: by
+more than 7 * 2^-11 * scale * |q k| (2-norm of the products) with a probability below 2 exp(-49/2) (Hoeffding) each, and the context by
+2 d sum p|v| at most.  Values far below the largest visible one are held to 2^-25 of it, as probabilities are (2^-24, times 2^6): 2^-22 max|v|.
+So |got - want| <= 2^-8 |want| + (2 * 2^-11 + 2 d) sum p|v| + 2^-22 max|v|."""
 import pytest
 import torch
 
@@ -32,13 +31,12 @@ def filled(n_seq, n_kv, slots, D, seed=0, gain=1.0):
 
 
 def assert_near(got, ref, cache, heads):
-    want, top, (pv, p2v2, p2, qk) = ref
+    want, top, (pv, qk) = ref
     off = (got.double() - want).abs()
     rep = heads // cache.n_kv_heads
     if cache.head_dim in (64, 128) and rep <= 128 and rep * got.shape[1] >= 64:
-        tol = 2.0 ** -8 * want.abs() + (2 * 2.0 ** -8 + 2 * 7 * 2.0 ** -8 * qk) * pv
-        var = want.square() + 2 * p2v2 + qk.square() * 2 * (p2v2 + want.square() * p2)
-        assert float(off.norm()) <= 1.5 * 2.0 ** -8 / 3 ** 0.5 * float(var.sum().sqrt()), (float(off.norm()), float(var.sum().sqrt()))
+        # (such calls go to either kernel, whichever is expected to be faster)
+        tol = 2.0 ** -8 * want.abs() + torch.maximum((2 * 2.0 ** -11 + 2 * 7 * 2.0 ** -11 * qk) * pv + 2.0 ** -22 * top, 2.0 ** -10 * top)
     else:
         tol = 2.0 ** -8 * want.abs() + 2.0 ** -10 * top
     far = off - tol
