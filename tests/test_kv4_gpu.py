@@ -406,6 +406,26 @@ def test_scale_and_equal_heads():
     assert_near(alone, R.attend(q, k, v, pos, slots, heads, 0.3), c, heads)
 
 
+@pytest.mark.parametrize("T", [1, 6, 300])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30])
+def test_scales_of_any_sign(T, scale):
+    """A negative scale turns the scores round, none at all makes every visible slot equal."""
+    heads, n_kv, D, slots = 8, 2, 128, 500
+    c, k, v = filled(1, n_kv, slots, D)
+    q = randn(1, 1, T, heads * D)
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    assert_near(c.attend(q, pos, window=200, sinks=2, scale=scale), R.attend(q, k, v, pos, slots, heads, scale, 200, 2), c, heads)
+
+
+@pytest.mark.parametrize("n,T,heads,n_kv,D,slots", [(1, 1, 8, 2, 128, 2000), (2, 1, 8, 1, 64, 30000), (1, 400, 8, 2, 128, 400), (40, 3, 16, 16, 64, 90)])
+def test_the_result_may_take_the_place_of_the_queries(n, T, heads, n_kv, D, slots):
+    c, _, _ = filled(n, n_kv, slots, D)
+    q = randn(1, n, T, heads * D)
+    pos = (slots - T + torch.arange(T, device="cuda")).expand(n, T)
+    want = c.attend(q, pos)
+    assert c.attend(q, pos, out=q) is q and torch.equal(q, want)
+
+
 @pytest.mark.parametrize("T", [1, 100])
 def test_captured_and_replayed_with_other_positions(T):
     """Append and attend in one graph; positions, keys and queries change between replays; a second graph of the same cache is alive and an
