@@ -22,11 +22,10 @@
 //
 // Bound: the latency of instructions at 16 warps an SM (1.7 a clock; no pipe above 40 %).  A unit of expansion takes 1440 clocks, so the 16 units
 // of a tile of 128 channels 3300 on seven warps; softmax takes 2000 a tile beside it, the tensor pipe 1000.  2048 tokens, 32 / 8 heads of 128:
-// 101 us; 2 x 500 tokens with a window of 1024 over 6000 slots, 32 / 16 heads: 70 us (the kernel of few rows: 248 and 138 us).
+// 100 us; 2 x 500 tokens with a window of 1024 over 6000 slots, 32 / 16 heads: 69 us (the kernel of few rows: 248 and 138 us).
 // Steps: a lane per eight channels with scale, zero and visibility for each word 166 us; whole rows per lane, ten operations a word, maxima of raw
-// scores 113 us; no branch per word, so that words overlap 97 us; fp16 operands 102 us, two codes
-// per fused multiply-add 101 us.  Eleven expanding warps at 72 registers (softmax
-// 128) slowed the softmax by 30 % and gained nothing.
+// scores 113 us; no branch per word, so that words overlap 97 us; fp16 operands 102 us, two codes per fused multiply-add 101 us, loads of the start together 100 us.  Eleven
+// expanding warps at 72 registers (softmax 128) slowed the softmax by 30 % and gained nothing.
 #pragma once
 #include "kv4_attend.cuh"
 #include "tcgen05.cuh"
@@ -123,6 +122,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     // the longest rows (last tokens of the prompt) first, so that the short ones fill the end of the grid
     const int n_kv = P.cache.n_kv, order = (int)(gridDim.x - 1 - blockIdx.x);
     const int block = P.by_kv(order), kvh = order - block * n_kv, seq = blockIdx.y, tok0 = block * tok_per_cta;
+    // queries (rows that are none are zero): requested at once, worked on below
+    constexpr int CHUNKS = KP_ROWS * D / 8 / KP_THREADS;
+    static_assert(CHUNKS * KP_THREADS * 8 == KP_ROWS * D, "whole rounds");
+    uint4 queries[CHUNKS];
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+        const int i = threadIdx.x + k * KP_THREADS, r = i / (D / 8), c = i % (D / 8), tok = P.by_rep(r), row_tok = tok0 + tok;
+        queries[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (tok < tok_per_cta && row_tok < P.T)
+            queries[k] = __ldg(reinterpret_cast<const uint4*>(P.q + ((long long)seq * P.T + row_tok) * P.ld_q + (kvh * P.rep + r - tok * P.rep) * D) + c);
+    }
     Kv4Span span = {-1, 0x7FFFFFFF, 0x7FFFFFFF, 0};
     for (int i = lane; i < tok_per_cta && tok0 + i < P.T; i += 32) {
         const Kv4Range r = kv4_range(P, seq, tok0 + i);
@@ -154,39 +164,48 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     {                                                                  // the largest key and value that some row sees
         float top_k = 0.0f, top_v = 0.0f;
         const int slots = n * KP_KEYS;
-        for (int i = threadIdx.x; i < slots; i += KP_THREADS) {
-            const int j = tiles.tile(i / KP_KEYS) * KP_KEYS + i % KP_KEYS, slot = j % KV4_TILE;
-            if (nobody(j)) continue;                                   // (slots beyond the cache among them)
-            const uint8_t* tile = base + (long long)(j / KV4_TILE) * TILE;
+#pragma unroll 1
+        for (int i0 = threadIdx.x; i0 < slots; i0 += 4 * KP_THREADS) {
+            uint32_t mk[4][G], vs[4][G], vz[4][G];                     // four slots in flight
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const uint32_t m = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, slot)));
-                top_k = fmaxf(top_k, kv4_largest(m >> 16, m & 0xFFFFu));
-                top_v = fmaxf(top_v, kv4_largest(__ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, slot))),
-                                                 __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_zero(G, g, slot)))));
+            for (int k = 0; k < 4; ++k) {
+                const int i = min(i0 + k * KP_THREADS, slots - 1), j = tiles.tile(i / KP_KEYS) * KP_KEYS + i % KP_KEYS, slot = j % KV4_TILE;
+                const bool seen = !nobody(j);                          // (slots beyond the cache are not)
+                const uint8_t* tile = base + (long long)(j / KV4_TILE) * TILE;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    mk[k][g] = seen ? __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, slot))) : 0u;
+                    vs[k][g] = seen ? __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, slot))) : 0u;
+                    vz[k][g] = seen ? __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_zero(G, g, slot))) : 0u;
+                }
             }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    top_k = fmaxf(top_k, kv4_largest(mk[k][g] >> 16, mk[k][g] & 0xFFFFu));
+                    top_v = fmaxf(top_v, kv4_largest(vs[k][g], vz[k][g]));
+                }
         }
         const uint32_t bk = __reduce_max_sync(full_mask, __float_as_uint(top_k)), bv = __reduce_max_sync(full_mask, __float_as_uint(top_v));
         if (lane == 0) { atomicMax(&largest[0], bk); atomicMax(&largest[1], bv); }
     }
-    // queries: rows that are none are zero.  The scale is made positive (its sign goes to the queries; none at all: queries of zero), so that
-    // maxima can be taken of raw scores
+    // The scale is made positive (its sign goes to the queries; none at all: queries of zero), so that maxima can be taken of raw scores
     const uint32_t q_and = P.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu, q_xor = P.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    for (int i = threadIdx.x; i < KP_ROWS * D / 8; i += KP_THREADS) {
-        const int r = i / (D / 8), c = i % (D / 8), tok = P.by_rep(r), row_tok = tok0 + tok;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (tok < tok_per_cta && row_tok < P.T)
-            v = __ldg(reinterpret_cast<const uint4*>(P.q + ((long long)seq * P.T + row_tok) * P.ld_q + (kvh * P.rep + r - tok * P.rep) * D) + c);
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+        const int i = threadIdx.x + k * KP_THREADS, r = i / (D / 8), c = i % (D / 8);
+        const uint4 v = queries[k];
         const uint32_t w[4] = {(v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor, (v.w & q_and) ^ q_xor};
         uint32_t top = 0u, o[4];                                       // largest magnitude of the row; a NaN stays on top
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFF0000u, (w[k] & 0x7FFFu) << 16));
+        for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7FFF0000u, (w[e] & 0x7FFFu) << 16));
 #pragma unroll
         for (int x = 1; x < D / 8; x <<= 1) top = max(top, __shfl_xor_sync(full_mask, top, x));
         const int ex = max(-112, (int)(top >> 23) - 127);              // in [2^ex, 2^(ex + 1)), to [2^14, 2^15)
         const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = pack_f16x2(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xFFFF0000u) * up);
+        for (int e = 0; e < 4; ++e) o[e] = pack_f16x2(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xFFFF0000u) * up);
         if (c == 0) q_fac[r] = ex < 128 ? __uint_as_float((uint32_t)max(1, ex - 14 + 127) << 23) : __uint_as_float(0x7FC00000u);
         sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), o[0], o[1], o[2], o[3]);
     }
