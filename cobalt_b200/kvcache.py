@@ -212,7 +212,7 @@ class KVCache4:
 
     def device_status(self) -> int:
         """0, or the code of the first bounded wait of an attention over such caches on this device that gave up since the last
-        question (its rows are then not written).  Waits for the current stream."""
+        question (the results of such a call are not to be used).  Waits for the current stream."""
         word = ctypes.c_uint32(0)
         with torch.cuda.device(self.device):
             rc = self._lib.cobalt_kv4_status(_raw_stream(self._index), ctypes.byref(word))

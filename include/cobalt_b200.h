@@ -360,7 +360,7 @@ int cobalt_attn_prompt(const void* q, const void* k_cache, const void* v_cache, 
  *                       at the end.  scratch: cobalt_kv4_attend_scratch_bytes() (0: none needed), 256-byte aligned, contents irrelevant;
  *                       calls that may overlap on the GPU need buffers of their own.
  *   cobalt_kv4_status : 0, or the code of the first bounded wait of an attend call on the current device that gave up since the
- *                       last question (its rows are then not written).  Synchronises `stream`; not during capture.
+ *                       last question (the results of such a call are not to be used).  Synchronises `stream`; not during capture.
  * The reference holds its cache in bf16 and has no counterpart. */
 size_t cobalt_kv4_tile_bytes(int head_dim);
 int cobalt_kv4_append(const void* k, int64_t ld_k, const void* v, int64_t ld_v, const void* q, int64_t ld_q, void* q_out, int64_t ld_q_out,
