@@ -493,6 +493,25 @@ def test_offsets_beyond_32_bits():
     assert all(torch.equal(a, b) for a, b in zip(c.read(pos), plain.read(pos)))
 
 
+@pytest.mark.parametrize("T,D,slots", [(1, 128, 30_000_000), (70, 128, 30_000_000), (70, 64, 60_000_000), (1, 256, 15_000_000)])
+def test_slots_beyond_4_gb_of_one_head(T, D, slots):
+    """The last slots of a head whose tiles take more than 2^32 bytes, against the same slots at the beginning of a small cache."""
+    heads, used = 8, 192
+    far, near = KVCache4(1, 1, slots, D), KVCache4(1, 1, used, D)
+    assert far.nbytes() > 1 << 32
+    q, k, v = randn(1, 1, T, heads * D), randn(2, 1, used, D), randn(3, 1, used, D)
+    at = torch.arange(used, device="cuda")[None]
+    first = (slots - used) // 32 * 32
+    near.append(k, v, at)
+    far.append(k, v, at + first)
+    assert all(torch.equal(a, b) for a, b in zip(near.read(at), far.read(at + first)))
+    kd, vd = R.cache_values(near.tiles, D)
+    pos = (used - T + torch.arange(T, device="cuda"))[None]
+    ref = R.attend(q, kd, vd, pos, used, heads, D ** -0.5, 90)
+    assert_near(near.attend(q, pos, window=90), ref, near, heads)
+    assert_near(far.attend(q, pos + first, window=90), ref, far, heads)
+
+
 def test_refusals_of_gpu_tensors():
     c = KVCache4(2, 2, 40, 64)
     x, pos = torch.zeros(2, 3, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 3, dtype=torch.long, device="cuda")
