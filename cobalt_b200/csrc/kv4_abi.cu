@@ -63,7 +63,12 @@ struct AttendCfg {
 // than its share.  Measured with one token, 32 / 8 heads of 128 (heads / list, us): one sequence of 8192 slots 14.4 / 16.4, 16384 22.1 / 21.7,
 // 32768 38.1 / 24.6; 4 sequences of 16384 26.1 / 29.1, 32768 45.8 / 45.7; 16 sequences of 16384 68.7 / 75.9, of 9830 to 32768
 // 94.3 / 92.3; 8 / 1 heads of 256, one sequence of 2048 9.9 / 10.7, 4096 12.5 / 11.3.  They meet at 6 tiles per warp plus 64 times the
-// share of the GPU that the clusters fill.  A CTA per head where there are heads for several CTAs per SM.
+// share of the GPU that the clusters fill.  Up to eight heads take clusters of sixteen where eight would leave a warp more than four tiles
+// (eight / sixteen / list, us: 32 / 8 heads of 128, one sequence of 9000 slots 15.2 / 13.5 / 20.3, 16384 22.2 / 17.6 / 21.5, 32768
+// 38.0 / 27.1 / 24.4; 8 / 1 heads of 256, one sequence of 16384 26.8 / 18.4 / 15.2, four of 9000 18.5 / 14.8 / 20.0, of 32768
+// 46.1 / 28.3 / 24.0).  Those give way to the list at 6 tiles per warp plus 22 times the share: within 10 % of the better side at most
+// lengths, at worst 22 % behind it (8 / 1 heads of 128, four of 3600 to 24000: sixteen 18.7, list, which is taken, 22.9).
+// A CTA per head where there are heads for several CTAs per SM.
 int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, int window, int sinks, int sms, AttendCfg* c) {
     const int G = D / KV4_GROUP;
     const int64_t cols = (int64_t)(n_heads / n_kv) * T;
@@ -80,10 +85,11 @@ int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, i
     const int64_t whole = (n_slots + KV4_TILE - 1) / KV4_TILE;
     int64_t tiles = whole;
     if (window > 0) tiles = std::min(tiles, ((int64_t)window + T) / KV4_TILE + 2 + ((int64_t)sinks + KV4_TILE - 1) / KV4_TILE);
+    const int most = heads <= KA_WIDE_HEADS && tiles > KA_MAX_CLUSTER * KA_WARPS * 4 ? 2 * KA_MAX_CLUSTER : KA_MAX_CLUSTER;
     c->share = 1;
-    while (c->share < KA_MAX_CLUSTER && c->share * 2 * heads <= ctas && c->share * KA_MIN_TILES < tiles) c->share *= 2;
+    while (c->share < most && c->share * 2 * heads <= ctas && c->share * KA_MIN_TILES < tiles) c->share *= 2;
     c->list = entries <= KA_ENTRIES && heads * whole < 1000000000ll && heads < 4ll * ctas && 
-              tiles * ctas > c->share * KA_WARPS * (6ll * ctas + 64 * heads * c->share);
+              tiles * ctas > c->share * KA_WARPS * (6ll * ctas + (c->share > KA_MAX_CLUSTER ? 22 : 64) * heads * c->share);
     c->grid = c->list ? (int)std::min<int64_t>(ctas, (heads * tiles + KA_MIN_TILES - 1) / KA_MIN_TILES) : (int)heads * c->share;
     if (!c->list && heads * c->share > 0x7FFFFFFFll) return COBALT_ETOOBIG;
     c->joins_off = (size_t)c->grid * 2 * ka_state_floats(G, c->nb) * 128;

@@ -136,7 +136,8 @@ constexpr int KA_WARPS = 4, KA_THREADS = 32 * KA_WARPS;
 constexpr int KA_STAGES = 2;
 constexpr int KA_MIN_TILES = 4;                                        // per CTA: one per warp
 constexpr int KA_ENTRIES = 256;                                        // (sequence, tile of columns) pairs of a list
-constexpr int KA_MAX_CLUSTER = 8;                                      // (sixteen is not portable, and took 8 us longer to start: 20.1 us against 12.0)
+constexpr int KA_MAX_CLUSTER = 8;                                      // (sixteen are slow to place: 32 heads of 128 tiles took 20.1 us against 12.0)
+constexpr int KA_WIDE_HEADS = 8;                                       // of so few heads, with more than four tiles a warp, sixteen all the same
 constexpr int ka_max_nb(int G) { return G == 1 ? 4 : G == 2 ? 2 : 1; } // groups of eight columns a warp holds
 constexpr int ka_ctas_per_sm(int G, int NB) { return NB == 1 ? (G <= 2 ? 4 : G == 3 ? 3 : 2) : G * NB <= 2 ? 3 : 2; }
 constexpr int ka_state_floats(int G, int NB) { return NB * (16 * G + 4); }      // per lane: O, reference and sum of two columns

@@ -247,6 +247,20 @@ def test_attention_matches_fp64(n, T, heads, n_kv, D, slots, last, window, sinks
     assert torch.equal(got, c.attend(q, pos, window=window, sinks=sinks)) and c.device_status() == 0
 
 
+# at most eight heads, long enough for the widest clusters: even and ragged lengths, sequences that leave most CTAs of a cluster without
+# a key, a window with first slots, every width, several columns a tile
+@pytest.mark.parametrize("n,T,heads,n_kv,D,slots,last,window,sinks,gain", [
+    (1, 1, 32, 8, 128, 9000, [8999], 0, 0, 1.0),
+    (4, 1, 8, 1, 256, 9001, [9000, 0, 31, 4500], 0, 0, 1.0),
+    (2, 3, 14, 2, 64, 6000, [5999, 2], 0, 0, 4.0),
+    (2, 1, 3, 3, 192, 6017, [6016, 100], 0, 0, 1.0),
+    (1, 2, 8, 4, 128, 12000, [11999], 9000, 5, 1.0),
+    (8, 1, 8, 1, 128, 16000, [15999, 1, 64, 8000, 15000, 0, 12345, 33], 0, 0, 1.0),
+])
+def test_few_long_heads_match_fp64(n, T, heads, n_kv, D, slots, last, window, sinks, gain):
+    test_attention_matches_fp64(n, T, heads, n_kv, D, slots, last, window, sinks, gain)
+
+
 @pytest.mark.parametrize("T", [1, 4, 80])
 def test_what_is_hidden_is_not_seen(T):
     """Slots behind a token, before its window, or left by an earlier sequence (here: bytes that read as NaN and infinities) do not reach it."""
