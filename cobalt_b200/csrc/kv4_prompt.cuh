@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t no_number;                                     // a group of values that is not a number was seen
     __shared__ uint32_t largest[2];                                    // magnitude (bits) among the visible keys, values
-    __shared__ float q_fac[KP_ROWS];                                   // what the queries of a row were divided by
+    __shared__ int q_exp[KP_ROWS];                                     // queries of a row were divided by 2^(this - 14); 128: one is not finite
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full_mask = 0xFFFFFFFFu;
     const uint32_t s_raw = smem_u32(smem), s0 = (s_raw + 1023u) & ~1023u;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = pack_f16x2(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xFFFF0000u) * up);
-        if (c == 0) q_fac[r] = ex < 128 ? __uint_as_float((uint32_t)max(1, ex - 14 + 127) << 23) : __uint_as_float(0x7FC00000u);
+        if (c == 0) q_exp[r] = ex;
         sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), o[0], o[1], o[2], o[3]);
     }
     fence_proxy_async();
@@ -227,7 +227,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         const Kv4Range range = valid ? kv4_range(P, seq, tok) : Kv4Range{0, -1};
         const uint32_t my_lanes = (uint32_t)((warp & 3) * 32) << 16, my_o = tmem_o + my_lanes + (uint32_t)(half * D);
         bool healthy = true;
-        const float scale = q_fac[r] * __uint_as_float((uint32_t)(ex_k - 14 + 127) << 23) * (P.scale_log2 == 0.0f ? 1.0f : fabsf(P.scale_log2));
+        // What a raw score is times.  Positive: a masked score is -inf before it, and must stay so.  Raw scores are below 2^38, so those that are held to
+        // the smallest normal number here are nothing (below 2^-88) either way; the exponents are added as whole numbers, as a
+        // product of two of the three factors may leave fp32 where that of all three does not
+        float scale = q_exp[r] < 128 ? ldexpf(P.scale_log2 == 0.0f ? 1.0f : fabsf(P.scale_log2), q_exp[r] + ex_k - 28) : __uint_as_float(0x7FC00000u);
+        if (scale < 0x1p-126f) scale = 0x1p-126f;
         float m = -INFINITY, l = 0.0f;                                  // reference and sum of this row's half, scores times log2(e)
         for (int j = 0; j < n; ++j) {
             healthy = __all_sync(full_mask, mbar_wait_bounded(bar_sfull(j & 1), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_ACC));

@@ -93,3 +93,28 @@ def attend(q, k, v, positions, slots, n_heads, scale, window=0, sinks=0):
         more[1, :, :, h] = torch.where(see, qk, 0.0).amax(-1, keepdim=True)
         top[:, :, h] = torch.where(see[..., None], torch.nan_to_num(vh).abs().amax(-1)[:, None, :, None], 0.0).amax(2)
     return out.view(n, T, -1), top.expand(-1, -1, -1, D).reshape(n, T, -1), more.view(2, n, T, -1)
+
+
+def spread(q, k, v, positions, slots, n_heads, scale, window=0, sinks=0):
+    """fp64 ``[n, T, n_heads * D]``: root of sum p^2 v^2, what independent errors of weights or values add up to per unit of error."""
+    n, T, _ = q.shape
+    D, rep = k.shape[-1], n_heads // k.shape[1]
+    see = visible(positions, slots, window, sinks)
+    out = torch.zeros(n, T, n_heads, D, dtype=torch.float64, device=q.device)
+    qh = q.double().view(n, T, n_heads, D)
+    for h in range(n_heads):
+        kh, vh = torch.nan_to_num(k[:, h // rep, :slots]), torch.nan_to_num(v[:, h // rep, :slots])
+        s = (qh[:, :, h] @ kh.transpose(1, 2) * scale).masked_fill(~see, float("-inf"))
+        out[:, :, h] = (torch.nan_to_num(torch.softmax(s, -1)).square() @ vh.square()).sqrt()
+    return out.view(n, T, -1)
+
+
+def kernels(call):
+    """Names of the attention kernels of the 4-bit cache that a call launches, and what it returns."""
+    import re
+    from torch.profiler import ProfilerActivity, profile
+    with profile(activities=[ProfilerActivity.CUDA]) as prof:
+        out = call()
+        torch.cuda.synchronize()
+    names = " ".join(e.key for e in prof.key_averages())
+    return set(re.findall(r"kv4_(attend_heads|attend_list|combine|prompt)_kernel", names)), out
