@@ -24,7 +24,8 @@
 // of a tile of 128 channels 3300 on seven warps; softmax takes 2000 a tile beside it, the tensor pipe 1000.  2048 tokens, 32 / 8 heads of 128:
 // 100 us; 2 x 500 tokens with a window of 1024 over 6000 slots, 32 / 16 heads: 69 us (the kernel of few rows: 248 and 138 us).
 // Steps: a lane per eight channels with scale, zero and visibility for each word 166 us; whole rows per lane, ten operations a word, maxima of raw
-// scores 113 us; no branch per word, so that words overlap 97 us; fp16 operands 102 us, two codes per fused multiply-add 101 us, loads of the start together 100 us.  Eleven
+// scores 113 us; no branch per word, so that words overlap 97 us; fp16 operands 102 us, two codes per fused multiply-add 101 us, loads of the start together 100 us; codes at bits that keep a constant's
+// rounding below 2^-12 of a step, two shifts a word more, 100.6 us.  Eleven
 // expanding warps at 72 registers (softmax 128) slowed the softmax by 30 % and gained nothing.
 #pragma once
 #include "kv4_attend.cuh"
@@ -49,34 +50,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight codes of a word as fp16 values (c - z) * s.  A code anywhere in the mantissa of an fp32 number is that power of two plus c; at bits 8, 12
-// and 16 (2^15, 2^11, 2^7) the constant -(2^k + z) * s is still good to 2^-8 of a step, and one "and-or" per code makes the number: ten
-// operations a word, where masks in pairs and halves took fifteen.
+// Eight codes of a word as fp16 values (c - z) * s.  A code anywhere in the mantissa of an fp32 number is that power of two plus c; at bits 12 and
+// 16 (2^11, 2^7) one "and-or" per code makes the number, and the constant -(2^k + z) * s is good to 2^-12 of a step.  (At bit 8, which would save
+// two shifts of twelve operations a word, the constant of 2^15 is off by up to 2^-8 of a step: as much as fp16 rounds the largest values of a group,
+// but of every value, those next to zero among them.)
 struct Kv4Step {
-    uint64_t s2, b12, b01, b20;                                        // pairs: fma.rn.f32x2 takes two codes at a time
+    uint64_t s2, b2;                                                   // pairs: fma.rn.f32x2 takes two codes at a time
     __device__ __forceinline__ static uint64_t two(float lo, float hi) {
         uint64_t d;
         asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
         return d;
     }
-    __device__ __forceinline__ Kv4Step(float s, float z) {
-        const float b0 = -(32768.0f + z) * s, b1 = -(2048.0f + z) * s, b2 = -(128.0f + z) * s;
-        s2 = two(s, s); b12 = two(b1, b2); b01 = two(b0, b1); b20 = two(b2, b0);
-    }
-    template <int K>                                                   // 2^(15 - 4 K) + the code at bits 8 + 4 K of w
-    __device__ __forceinline__ static float code(uint32_t w) {
-        return __uint_as_float((w & (0xF00u << (4 * K))) | ((uint32_t)(127 + 15 - 4 * K) << 23));
-    }
-    __device__ __forceinline__ uint32_t pair(float lo, float hi, uint64_t b) const {
+    __device__ __forceinline__ Kv4Step(float s, float z) : s2(two(s, s)), b2(two(-(2048.0f + z) * s, -(128.0f + z) * s)) {}
+    __device__ __forceinline__ uint32_t pair(uint32_t w) const {       // the codes at bits 12 and 16
+        const uint64_t x = two(__uint_as_float((w & 0xF000u) | 0x45000000u), __uint_as_float((w & 0xF0000u) | 0x43000000u));
         uint32_t d;
-        asm("{\n\t.reg .b64 x;\n\t.reg .f32 l, h;\n\tfma.rn.f32x2 x, %1, %2, %3;\n\tmov.b64 {l, h}, x;\n\tcvt.rn.f16x2.f32 %0, h, l;\n\t}" : "=r"(d) : "l"(two(lo, hi)), "l"(s2), "l"(b));
+        asm("{\n\t.reg .b64 x;\n\t.reg .f32 l, h;\n\tfma.rn.f32x2 x, %1, %2, %3;\n\tmov.b64 {l, h}, x;\n\tcvt.rn.f16x2.f32 %0, h, l;\n\t}" : "=r"(d) : "l"(x), "l"(s2), "l"(b2));
         return d;
     }
-    __device__ __forceinline__ uint4 values(uint32_t w) const {
-        const uint32_t up = w << 12, down = w >> 12;
-        return make_uint4(pair(code<1>(up), code<2>(up), b12), pair(code<0>(w), code<1>(w), b01), pair(code<2>(w), code<0>(down), b20),
-                          pair(code<1>(down), code<2>(down), b12));
-    }
+    __device__ __forceinline__ uint4 values(uint32_t w) const { return make_uint4(pair(w << 12), pair(w << 4), pair(w >> 4), pair(w >> 12)); }
 };
 // largest magnitude that a group can hold; 0 for one that is no number
 __device__ __forceinline__ float kv4_largest(uint32_t scale, uint32_t zero) {

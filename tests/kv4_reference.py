@@ -96,17 +96,20 @@ def attend(q, k, v, positions, slots, n_heads, scale, window=0, sinks=0):
 
 
 def spread(q, k, v, positions, slots, n_heads, scale, window=0, sinks=0):
-    """fp64 ``[n, T, n_heads * D]``: root of sum p^2 v^2, what independent errors of weights or values add up to per unit of error."""
+    """fp64 ``[n, T, n_heads * D]``: roots of sum p^2 v^2 and of sum p^2, what independent errors of weights or values, or of the same size in
+    every slot, add up to per unit of error."""
     n, T, _ = q.shape
     D, rep = k.shape[-1], n_heads // k.shape[1]
     see = visible(positions, slots, window, sinks)
-    out = torch.zeros(n, T, n_heads, D, dtype=torch.float64, device=q.device)
+    out, even = (torch.zeros(n, T, n_heads, D, dtype=torch.float64, device=q.device) for _ in range(2))
     qh = q.double().view(n, T, n_heads, D)
     for h in range(n_heads):
         kh, vh = torch.nan_to_num(k[:, h // rep, :slots]), torch.nan_to_num(v[:, h // rep, :slots])
         s = (qh[:, :, h] @ kh.transpose(1, 2) * scale).masked_fill(~see, float("-inf"))
-        out[:, :, h] = (torch.nan_to_num(torch.softmax(s, -1)).square() @ vh.square()).sqrt()
-    return out.view(n, T, -1)
+        p2 = torch.nan_to_num(torch.softmax(s, -1)).square()
+        out[:, :, h] = (p2 @ vh.square()).sqrt()
+        even[:, :, h] = p2.sum(-1, keepdim=True).sqrt()
+    return out.view(n, T, -1), even.view(n, T, -1)
 
 
 def kernels(call):
