@@ -126,3 +126,178 @@ def test_attention_matches_fp64(n, T, heads, n_kv, D, slots, last, window, sinks
     got = attend_prompt(c, q, pos, window=window, sinks=sinks)
     assert_near(got, q, k, v, pos, slots, heads, D ** -0.5, window, sinks)
     assert torch.equal(got, c.attend(q, pos, window=window, sinks=sinks)) and c.device_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_positions_in_any_order(D):
+    """Tokens of a prompt need not follow one another: padding among them, repeated and shuffled positions, some behind the cache."""
+    (T, heads, n_kv), slots = size(D), 500
+    c, k, v = filled(2, n_kv, slots, D)
+    q = randn(8, 2, T, heads * D)
+    pos = torch.randint(-60, slots, (2, T), generator=torch.Generator().manual_seed(D)).cuda()
+    pos[1, :128] = -1                                                                  # whole CTAs without a slot
+    pos[0, 7], pos[0, 8], pos[0, 9] = slots + 30, 1 << 40, -(1 << 63)
+    for window, sinks in ((0, 0), (90, 0), (90, 7)):
+        out = torch.full((3, T, heads * D), 5.0, dtype=torch.bfloat16, device="cuda")
+        got = attend_prompt(c, q, pos, window=window, sinks=sinks, out=out[:2])
+        assert_near(got, q, k, v, pos, slots, heads, D ** -0.5, window, sinks)
+        assert not bool(got[pos < 0].any()) and bool((out[2] == 5.0).all())
+        assert window == 0 or sinks or not bool(got[0, 8].any())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 0.5])
+def test_scales_of_any_sign(D, scale):
+    (T, heads, n_kv), slots = size(D), 500
+    c, k, v = filled(1, n_kv, slots, D)
+    q = randn(1, 1, T, heads * D)
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    assert_near(attend_prompt(c, q, pos, window=200, sinks=2, scale=scale), q, k, v, pos, slots, heads, scale, 200, 2)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("k_gain,v_gain,q_gain", [(1e-6, 1e-5, 1.0), (1e4, 1e6, 1e-4), (1e-20, 1e30, 1e20), (1e33, 1e33, 1e-33)])
+def test_ranges_of_keys_values_and_queries(D, k_gain, v_gain, q_gain):
+    """bf16 inputs of any size whose scores are ordinary; value scales that differ from slot to slot by up to 2^16."""
+    (T, heads, n_kv), slots = size(D), 450
+    c = KVCache4(1, n_kv, slots, D)
+    apart = torch.exp2(torch.randint(-8, 9, (1, slots, 1), generator=torch.Generator().manual_seed(1)).float()).cuda()
+    c.append(randn(1, 1, slots, n_kv * D, gain=k_gain), (randn(2, 1, slots, n_kv * D).float() * v_gain * apart).bfloat16(), torch.arange(slots, device="cuda"))
+    q = randn(3, 1, T, heads * D, gain=q_gain)
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    assert_near(attend_prompt(c, q, pos), q, *R.cache_values(c.tiles, D), pos, slots, heads, D ** -0.5)
+
+
+# ----------------------------------------------------------------------------- what is hidden, what is no number
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("byte", [0xFF, 0x7F, 0x00])
+def test_what_is_hidden_is_not_seen(D, byte):
+    """Slots that no token sees hold other bytes (which read as NaN, as huge values, as zeros): the same bits."""
+    (T, heads, n_kv), slots = size(D), 700
+    c, _, _ = filled(2, n_kv, slots, D)
+    pos = torch.stack([torch.arange(p - T + 1, p + 1) for p in (520, 660)]).cuda()
+    q = randn(3, 2, T, heads * D)
+    want = attend_prompt(c, q, pos, window=90, sinks=3)
+    other = KVCache4(2, n_kv, slots, D)
+    other.tiles.fill_(byte)
+    see = R.visible(pos, slots, 90, 3).any(1)
+    for b in range(2):
+        copy_slots(c.tiles[b:b + 1], other.tiles[b:b + 1], see[b].nonzero().flatten().tolist(), D)
+    assert torch.equal(attend_prompt(other, q, pos, window=90, sinks=3), want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_groups_that_are_not_finite_reach_who_sees_them(D):
+    """A value group that is no number: NaN in its channels for the rows that see its slot; a key: the whole row; a query: its own row.  The slot
+    lies inside the rows and key tiles of one CTA, before and behind whole ones."""
+    (T, heads, n_kv), slots, bad, rep = size(D), 450, 230, 4
+    g = D // 64 - 1                                                                   # the last group of KV head 1
+    k, v = randn(1, 1, slots, n_kv * D), randn(2, 1, slots, n_kv * D)
+    kbad, vbad = k.clone(), v.clone()
+    kbad[0, bad, D + 1], vbad[0, bad, D + 64 * g + 5] = float("nan"), float("inf")
+    q = randn(3, 1, T, heads * D)
+    pos = (10 + torch.arange(T, device="cuda"))[None]
+    for keys, values in ((k, vbad), (kbad, v)):
+        c = KVCache4(1, n_kv, slots, D)
+        c.append(keys, values, torch.arange(slots, device="cuda"))
+        kd, vd = R.cache_values(c.tiles, D)
+        for window, sinks in ((0, 0), (9, 0), (9, 300)):
+            got = attend_prompt(c, q, pos, window=window, sinks=sinks)
+            nan = torch.isnan(got.float()).view(T, heads, D)
+            see = R.visible(pos, slots, window, sinks)[0, :, bad]
+            want = torch.zeros(T, heads, D, dtype=torch.bool, device="cuda")
+            if values is vbad:
+                want[:, rep:2 * rep, 64 * g:64 * g + 64] = see[:, None, None]
+            else:
+                want[:, rep:2 * rep] = see[:, None, None]
+            assert torch.equal(nan, want)
+            assert_near(got, q, kd, vd, pos, slots, heads, D ** -0.5, window, sinks, rows=~see[None])
+    c = KVCache4(1, n_kv, slots, D)
+    c.append(k, v, torch.arange(slots, device="cuda"))
+    q[0, 37, 5], q[0, 300, 3 * D] = float("inf"), float("nan")
+    nan = torch.isnan(attend_prompt(c, q, pos).float()).view(T, heads, D)
+    assert bool(nan[37, 0].all()) and bool(nan[300, 3].all()) and int(nan.sum()) == 2 * D
+
+
+# ----------------------------------------------------------------------------- memory
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_result_may_take_the_place_of_the_queries(D):
+    (T, heads, n_kv), slots = size(D), 450
+    c, _, _ = filled(1, n_kv, slots, D)
+    q = randn(1, 1, T, heads * D)
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    want = attend_prompt(c, q, pos)
+    assert attend_prompt(c, q, pos, out=q) is q and torch.equal(q, want)
+    fused = randn(2, 1, T, heads * D + 24)                                             # rows with a stride of their own
+    assert torch.equal(attend_prompt(c, fused[..., 8:-16], pos), c.attend(fused[..., 8:-16].contiguous(), pos))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_captured_and_replayed_with_other_positions(D):
+    (T, heads, n_kv), slots = size(D), 900
+    c, other = KVCache4(2, n_kv, slots, D), KVCache4(2, n_kv, slots, D)
+    fill = randn(1, 2, slots, n_kv * D), randn(2, 2, slots, n_kv * D)
+    for x in (c, other):
+        x.append(*fill, torch.arange(slots, device="cuda"))
+    inv = 1.0 / (1e4 ** (torch.arange(0, D, 2, dtype=torch.float32, device="cuda") / D))
+    q, k, v = randn(3, 2, T, heads * D), randn(4, 2, T, n_kv * D), randn(5, 2, T, n_kv * D)
+    pos = torch.stack([torch.arange(T), 200 + torch.arange(T)]).cuda()
+
+    def once(cache):
+        return cache.attend(cache.append(k, v, pos, q=q, inv_freq=inv), pos, window=200, sinks=4)
+
+    assert R.kernels(lambda: once(c))[0] == {"prompt"}
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(once(c))
+        graphs.append(g)
+    once(other)
+    for step in range(4):
+        pos += 60
+        q.copy_(randn(10 + step, *q.shape)); k.copy_(randn(20 + step, *k.shape)); v.copy_(randn(30 + step, *v.shape))
+        graphs[step % 2].replay()
+        got = outs[step % 2].clone()
+        assert torch.equal(got, once(other)) and torch.equal(c.tiles, other.tiles)
+
+
+@pytest.mark.parametrize("T,D,slots", [(256, 128, 30_000_000), (384, 64, 60_000_000)])
+def test_slots_beyond_4_gb_of_one_head(T, D, slots):
+    """The last slots of a head whose tiles take more than 2^32 bytes, against the same slots at the beginning of a small cache."""
+    heads, used = 64, 500
+    far, near = KVCache4(1, 1, slots, D), KVCache4(1, 1, used, D)
+    assert far.nbytes() > 1 << 32
+    q, k, v = randn(1, 1, T, heads * D), randn(2, 1, used, D), randn(3, 1, used, D)
+    at = torch.arange(used, device="cuda")[None]
+    first = (slots - used) // 128 * 128
+    near.append(k, v, at)
+    far.append(k, v, at + first)
+    pos = (used - T + torch.arange(T, device="cuda"))[None]
+    want = attend_prompt(near, q, pos, window=90)
+    assert_near(want, q, *R.cache_values(near.tiles, D), pos, used, heads, D ** -0.5, 90)
+    assert torch.equal(attend_prompt(far, q, pos + first, window=90), want)
+
+
+def test_prompts_of_a_decoder():
+    """The prompt of a decoder with a 4-bit cache goes through this kernel, and every layer's attention is that of 64 bits."""
+    from cobalt_b200 import SparseQuantConfig
+    from cobalt_b200.decoder import CobaltDecoder, build_random_decoder
+    from oracle import model_oracle as MO
+    cfg = MO.llama_config(hidden=512, layers=2, heads=32, kv_heads=8, head_dim=128, inter=1024, vocab=1008)
+    dec = build_random_decoder(cfg, SparseQuantConfig(4, 0.5, 0.5), 400, torch.device("cuda"), batch=2, kv_bits=4)
+    checked = []
+
+    class Checked(CobaltDecoder):
+        def _attend4(self, q, positions, layer, seq, n):
+            got = super()._attend4(q, positions, layer, seq, n)
+            c, T = self.kv4[layer], q.shape[0] // n
+            k, v = R.cache_values(c.tiles[seq:seq + n], c.head_dim)
+            assert_near(got.view(n, T, -1), q.view(n, T, -1), k, v, positions.expand(n, T), c.slots, self.nh, self.scale)
+            checked.append(layer)
+            return got
+
+    chk = Checked(cfg, dec.lin, dec.P, 400, dec.dev, batch=2, kv_bits=4)
+    ids = torch.randint(0, 1000, (2, 330), generator=torch.Generator().manual_seed(1))
+    took, want = R.kernels(lambda: dec.prefill(ids))
+    assert took == {"prompt"} and torch.equal(chk.prefill(ids), want) and checked == [0, 1]
