@@ -209,264 +209,277 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     // keys and values times a power of two that brings the largest into [2^14, 2^15)
     const int ex_k = max(-110, (int)(largest[0] >> 23) - 127), ex_v = max(-110, (int)(largest[1] >> 23) - 127);
     const float up_k = __uint_as_float((uint32_t)(14 - ex_k + 127) << 23), up_v = __uint_as_float((uint32_t)(14 - ex_v + 127) << 23);
+    // Scores that may pass 2^24 (times log2(e)) are rounded before the maximum is taken off: it was rounded, too, and what an exact product would leave
+    // of the two is no longer small
+    int ex_q = -1000;
+#pragma unroll
+    for (int r = lane; r < KP_ROWS; r += 32) ex_q = max(ex_q, q_exp[r] < 128 ? q_exp[r] : -1000);
+    ex_q = __reduce_max_sync(full_mask, ex_q);
+    const bool big = ldexpf(fabsf(P.scale_log2), ex_q + ex_k + 2 + 7) > 0x1p24f;
     const uint32_t tmem = lds32(tmem_slot), tmem_o = tmem + 2 * KP_KEYS;              // scores 2 x 128 columns, contexts 2 x D
 
-    if (warp < 8) {
-        // =========================================================== softmax, epilogue
-        const int half = warp >> 2, r = threadIdx.x & 127;
-        const int sub = P.by_rep(r), tok = tok0 + sub, head = r - sub * P.rep;
-        const bool valid = sub < tok_per_cta && tok < P.T;
-        const Kv4Range range = valid ? kv4_range(P, seq, tok) : Kv4Range{0, -1};
-        const uint32_t my_lanes = (uint32_t)((warp & 3) * 32) << 16, my_o = tmem_o + my_lanes + (uint32_t)(half * D);
-        bool healthy = true;
-        // What a raw score is times.  Positive: a masked score is -inf before it, and must stay so.  Raw scores are below 2^38, so those that are held to
-        // the smallest normal number here are nothing (below 2^-88) either way; the exponents are added as whole numbers, as a
-        // product of two of the three factors may leave fp32 where that of all three does not
-        float scale = q_exp[r] < 128 ? ldexpf(P.scale_log2 == 0.0f ? 1.0f : fabsf(P.scale_log2), q_exp[r] + ex_k - 28) : __uint_as_float(0x7FC00000u);
-        if (scale < 0x1p-126f) scale = 0x1p-126f;
-        float m = -INFINITY, l = 0.0f;                                  // reference and sum of this row's half, scores times log2(e)
-        for (int j = 0; j < n; ++j) {
-            healthy = __all_sync(full_mask, mbar_wait_bounded(bar_sfull(j & 1), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_ACC));
-            if (!healthy) break;
-            tc_fence_after();
-            uint32_t v[2][32];
-            tmem_ld32(tmem + my_lanes + (uint32_t)((j & 1) * KP_KEYS + half * 64), v[0]);
-            tmem_ld32(tmem + my_lanes + (uint32_t)((j & 1) * KP_KEYS + half * 64 + 32), v[1]);
-            tmem_ld_wait();
-            tc_fence_before();
-            mbar_arrive(bar_sempty(j & 1));
-            float x[64];
-#pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(v[i >> 5][i & 31]);
-            const int k0 = tiles.tile(j) * KP_KEYS;
-            if (k0 + KP_KEYS - 1 > span.hi_min || (k0 < span.lo_max && k0 + KP_KEYS > P.sinks)) {                      // a border crosses this tile
-                const int hi = range.hi - k0 - half * 64, lo = range.lo - k0 - half * 64, sinks = P.sinks - k0 - half * 64;
-#pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (i > hi || (i < lo && i >= sinks)) x[i] = -INFINITY;
-            }
-            float t[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-            for (int i = 4; i < 60; i += 8)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), x[i + 4 + k]);
-            const float top = scale * fmaxf(fmaxf(fmaxf(t[0], x[60]), fmaxf(t[1], x[61])), fmaxf(fmaxf(t[2], x[62]), fmaxf(t[3], x[63])));
-            const bool move = top > m + 8.0f;
-            if (__any_sync(full_mask, move)) {
-                // (a row without a reference has a context of zeros: nothing to rescale)
-                const float f = move && m != -INFINITY ? ex2(m - top) : 1.0f;
-                if (move) { m = top; l *= f; }
-                if (j > 0 && __any_sync(full_mask, f != 1.0f)) {
-                    healthy = __all_sync(full_mask, mbar_wait_bounded(bar_pempty(half, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u, status, DEV_TIMEOUT_EMPTY));
-                    if (!healthy) break;
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(my_o + (uint32_t)c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(my_o + (uint32_t)c, o);
-                        tmem_st_wait();
-                    }
-                    tc_fence_before();
-                }
-            }
-            const float base = m == -INFINITY ? 0.0f : 6.0f - m;           // probabilities times 2^6
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            uint32_t p[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float a = ex2(fmaf(x[2 * i], scale, base)), b = ex2(fmaf(x[2 * i + 1], scale, base));
-                p[i] = pack_f16x2(a, b);
-                s[i & 3] += a + b;
-            }
-            l += (s[0] + s[1]) + (s[2] + s[3]);
-            healthy = __all_sync(full_mask, mbar_wait_bounded(bar_pempty(half, j & 1), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY));
-            if (!healthy) break;
-            const uint32_t row = p_base + (uint32_t)(j & 1) * 2u * KP_SUB + (uint32_t)half * KP_SUB + (uint32_t)r * 128u;
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-                sts128(row + (((uint32_t)c ^ (uint32_t)(r & 7)) << 4), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
-            fence_proxy_async();
-            mbar_arrive(bar_pfull(half, j & 1));
-        }
-        if (healthy)                                                   // the last products of both halves
-            for (int h = 0; h < 2; ++h)
-                healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_pempty(h, (n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u, status, DEV_TIMEOUT_ACC));
-        tc_fence_after();
-        stat[half * KP_ROWS + r] = m;
-        stat[(2 + half) * KP_ROWS + r] = l;
-        asm volatile("bar.sync 1, 480;" ::: "memory");                  // the softmax warps; those that expand have arrived (no_number)
-        const float om = stat[(half ^ 1) * KP_ROWS + r], ol = stat[(2 + (half ^ 1)) * KP_ROWS + r];
-        const float gm = fmaxf(m, om), base = gm == -INFINITY ? 0.0f : gm;
-        const float mine = ex2(m - base), other = ex2(om - base);
-        const float inv = __uint_as_float((uint32_t)(ex_v - 14 + 127) << 23) / (l * mine + ol * other);
-        const float w0 = (half ? other : mine) * inv, w1 = (half ? mine : other) * inv;        // of the contexts of halves 0 and 1
-        if (healthy) {
-            const bool any = range.hi >= 0 && (range.lo <= range.hi || P.sinks > 0);
-            bool nan = false;
-            if (no_number && any) {                                    // a marked group: does this row see one?
-                const int g = half * (D / 2) / 64;
-                for (int j = 0; j <= range.hi; ++j) {
-                    if (j < range.lo && j >= P.sinks) { j = range.lo - 1; continue; }
-                    const uint8_t* tile = P.cache.tile(seq, kvh, j, G);
-                    const uint32_t sc = *reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, j % KV4_TILE));
-                    nan |= (sc & 0x7F80u) == 0x7F80u;
-                }
-            }
-#pragma unroll 1
-            for (int c0 = 0; c0 < D / 2; c0 += 32) {
-                uint32_t a[32], b[32];
-                const uint32_t col = (uint32_t)(half * (D / 2) + c0);
-                tmem_ld32(tmem_o + my_lanes + col, a);
-                tmem_ld32(tmem_o + my_lanes + (uint32_t)D + col, b);
+    auto roles = [&](auto plain) {
+        constexpr bool PLAIN = decltype(plain)::value;
+        if (warp < 8) {
+            // =========================================================== softmax, epilogue
+            const int half = warp >> 2, r = threadIdx.x & 127;
+            const int sub = P.by_rep(r), tok = tok0 + sub, head = r - sub * P.rep;
+            const bool valid = sub < tok_per_cta && tok < P.T;
+            const Kv4Range range = valid ? kv4_range(P, seq, tok) : Kv4Range{0, -1};
+            const uint32_t my_lanes = (uint32_t)((warp & 3) * 32) << 16, my_o = tmem_o + my_lanes + (uint32_t)(half * D);
+            bool healthy = true;
+            // What a raw score is times.  Positive: a masked score is -inf before it, and must stay so.  Raw scores are below 2^38, so those that are held to
+            // the smallest normal number here are nothing (below 2^-88) either way; the exponents are added as whole numbers, as a
+            // product of two of the three factors may leave fp32 where that of all three does not
+            float scale = q_exp[r] < 128 ? ldexpf(P.scale_log2 == 0.0f ? 1.0f : fabsf(P.scale_log2), q_exp[r] + ex_k - 28) : __uint_as_float(0x7FC00000u);
+            if (scale < 0x1p-126f) scale = 0x1p-126f;
+            float m = -INFINITY, l = 0.0f;                                  // reference and sum of this row's half, scores times log2(e)
+            for (int j = 0; j < n; ++j) {
+                healthy = __all_sync(full_mask, mbar_wait_bounded(bar_sfull(j & 1), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_ACC));
+                if (!healthy) break;
+                tc_fence_after();
+                uint32_t v[2][32];
+                tmem_ld32(tmem + my_lanes + (uint32_t)((j & 1) * KP_KEYS + half * 64), v[0]);
+                tmem_ld32(tmem + my_lanes + (uint32_t)((j & 1) * KP_KEYS + half * 64 + 32), v[1]);
                 tmem_ld_wait();
-                if (valid) {
-                    uint4* dst = reinterpret_cast<uint4*>(P.out + (((long long)seq * P.T + tok) * P.n_heads + kvh * P.rep + head) * D + col);
+                tc_fence_before();
+                mbar_arrive(bar_sempty(j & 1));
+                float x[64];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[4];
+                for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(v[i >> 5][i & 31]);
+                const int k0 = tiles.tile(j) * KP_KEYS;
+                if (k0 + KP_KEYS - 1 > span.hi_min || (k0 < span.lo_max && k0 + KP_KEYS > P.sinks)) {                      // a border crosses this tile
+                    const int hi = range.hi - k0 - half * 64, lo = range.lo - k0 - half * 64, sinks = P.sinks - k0 - half * 64;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = 8 * c + 2 * e;
-                            o[e] = pack_bf16x2(fmaf(__uint_as_float(a[i]), w0, __uint_as_float(b[i]) * w1),
-                                               fmaf(__uint_as_float(a[i + 1]), w0, __uint_as_float(b[i + 1]) * w1));
-                            o[e] = !any ? 0u : nan ? 0x7FC07FC0u : o[e];
+                    for (int i = 0; i < 64; ++i)
+                        if (i > hi || (i < lo && i >= sinks)) x[i] = -INFINITY;
+                }
+                float t[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int i = 4; i < 60; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), x[i + 4 + k]);
+                const float top = scale * fmaxf(fmaxf(fmaxf(t[0], x[60]), fmaxf(t[1], x[61])), fmaxf(fmaxf(t[2], x[62]), fmaxf(t[3], x[63])));
+                const bool move = top > m + 8.0f;
+                if (__any_sync(full_mask, move)) {
+                    // (a row without a reference has a context of zeros: nothing to rescale)
+                    const float f = move && m != -INFINITY ? ex2(m - top) : 1.0f;
+                    if (move) { m = top; l *= f; }
+                    if (j > 0 && __any_sync(full_mask, f != 1.0f)) {
+                        healthy = __all_sync(full_mask, mbar_wait_bounded(bar_pempty(half, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u, status, DEV_TIMEOUT_EMPTY));
+                        if (!healthy) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(my_o + (uint32_t)c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(my_o + (uint32_t)c, o);
+                            tmem_st_wait();
                         }
-                        dst[c] = make_uint4(o[0], o[1], o[2], o[3]);
+                        tc_fence_before();
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.0f : m, base = m == -INFINITY ? 0.0f : 6.0f - m;            // probabilities times 2^6
+                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float a = ex2(PLAIN ? fmaf(x[2 * i], scale, base) : __fmul_rn(x[2 * i], scale) - ref + 6.0f);
+                    const float b = ex2(PLAIN ? fmaf(x[2 * i + 1], scale, base) : __fmul_rn(x[2 * i + 1], scale) - ref + 6.0f);
+                    p[i] = pack_f16x2(a, b);
+                    s[i & 3] += a + b;
+                }
+                l += (s[0] + s[1]) + (s[2] + s[3]);
+                healthy = __all_sync(full_mask, mbar_wait_bounded(bar_pempty(half, j & 1), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY));
+                if (!healthy) break;
+                const uint32_t row = p_base + (uint32_t)(j & 1) * 2u * KP_SUB + (uint32_t)half * KP_SUB + (uint32_t)r * 128u;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    sts128(row + (((uint32_t)c ^ (uint32_t)(r & 7)) << 4), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+                fence_proxy_async();
+                mbar_arrive(bar_pfull(half, j & 1));
+            }
+            if (healthy)                                                   // the last products of both halves
+                for (int h = 0; h < 2; ++h)
+                    healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_pempty(h, (n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u, status, DEV_TIMEOUT_ACC));
+            tc_fence_after();
+            stat[half * KP_ROWS + r] = m;
+            stat[(2 + half) * KP_ROWS + r] = l;
+            asm volatile("bar.sync 1, 480;" ::: "memory");                  // the softmax warps; those that expand have arrived (no_number)
+            const float om = stat[(half ^ 1) * KP_ROWS + r], ol = stat[(2 + (half ^ 1)) * KP_ROWS + r];
+            const float gm = fmaxf(m, om), base = gm == -INFINITY ? 0.0f : gm;
+            const float mine = ex2(m - base), other = ex2(om - base);
+            const float inv = __uint_as_float((uint32_t)(ex_v - 14 + 127) << 23) / (l * mine + ol * other);
+            const float w0 = (half ? other : mine) * inv, w1 = (half ? mine : other) * inv;        // of the contexts of halves 0 and 1
+            if (healthy) {
+                const bool any = range.hi >= 0 && (range.lo <= range.hi || P.sinks > 0);
+                bool nan = false;
+                if (no_number && any) {                                    // a marked group: does this row see one?
+                    const int g = half * (D / 2) / 64;
+                    for (int j = 0; j <= range.hi; ++j) {
+                        if (j < range.lo && j >= P.sinks) { j = range.lo - 1; continue; }
+                        const uint8_t* tile = P.cache.tile(seq, kvh, j, G);
+                        const uint32_t sc = *reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, j % KV4_TILE));
+                        nan |= (sc & 0x7F80u) == 0x7F80u;
+                    }
+                }
+#pragma unroll 1
+                for (int c0 = 0; c0 < D / 2; c0 += 32) {
+                    uint32_t a[32], b[32];
+                    const uint32_t col = (uint32_t)(half * (D / 2) + c0);
+                    tmem_ld32(tmem_o + my_lanes + col, a);
+                    tmem_ld32(tmem_o + my_lanes + (uint32_t)D + col, b);
+                    tmem_ld_wait();
+                    if (valid) {
+                        uint4* dst = reinterpret_cast<uint4*>(P.out + (((long long)seq * P.T + tok) * P.n_heads + kvh * P.rep + head) * D + col);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int i = 8 * c + 2 * e;
+                                o[e] = pack_bf16x2(fmaf(__uint_as_float(a[i]), w0, __uint_as_float(b[i]) * w1),
+                                                   fmaf(__uint_as_float(a[i + 1]), w0, __uint_as_float(b[i + 1]) * w1));
+                                o[e] = !any ? 0u : nan ? 0x7FC07FC0u : o[e];
+                            }
+                            dst[c] = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
                     }
                 }
             }
-        }
-        tc_fence_before();
-    } else if (warp < 8 + KP_EXPAND) {
-        // =========================================================== expansion: units (tile, keys or values, group, 32 slots) in this order
-        // (seven warps: after keys of a tile a warp comes to keys of the same or the next one or to values of the same, so that what it last waited
-        // for puts every slot at most one turn of its barrier behind; with a step of more than a tile's units it could pass a turn unseen)
-        static_assert(KP_EXPAND < 2 * SUBTILES, "units of a tile of the narrowest head");
-        const int units = n * 2 * G * SUBTILES;
-        // Keys: a lane has a slot, all 64 channels.  Values: a lane has half the chunks of a pair of slots; every other two pairs swap neighbouring
-        // chunks, so that eight lanes store to eight places of a row
-        const int pair = lane >> 1, swap = (pair >> 1) & 1;
-        uint4 raw[2];
-        uint32_t meta[3];                                              // keys: { zero, scale }; values: the scales, both zeros.  Nothing is done
-        bool hidden[2];                                                // with them before they are used: the request would wait for its loads
-        auto request = [&](int u) {
-            const int sub = u % SUBTILES, g = u / SUBTILES % G, at = tiles.tile(u / (2 * G * SUBTILES)) * SUBTILES + sub;
-            const bool keys = u / (G * SUBTILES) % 2 == 0, held = at < P.cache.n_tiles;              // (the last tile may reach beyond the cache)
-            const uint8_t* tile = base + (long long)(held ? at : 0) * TILE;
-            const uint4* p = reinterpret_cast<const uint4*>(tile + (keys ? 0 : 1024 * G) + 1024 * g + 32 * lane);       // 32 slots, or 16 pairs of 2 halves
-            raw[0] = __ldg(p);
-            raw[1] = __ldg(p + 1);
-            const int j = KV4_TILE * at + (keys ? lane : 2 * pair);
-            hidden[0] = !held || nobody(j);                            // zeros: nobody sees the slot, it may hold anything
-            hidden[1] = !held || nobody(j + 1);
-            if (keys) {
-                meta[0] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, lane)));
-            } else {
-                meta[0] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair)));
-                meta[1] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair + 1)));
-                meta[2] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_v_zero(G, g, 2 * pair)));
-            }
-        };
-        int u = warp - 8;
-        if (u < units) request(u);
+            tc_fence_before();
+        } else if (warp < 8 + KP_EXPAND) {
+            // =========================================================== expansion: units (tile, keys or values, group, 32 slots) in this order
+            // (seven warps: after keys of a tile a warp comes to keys of the same or the next one or to values of the same, so that what it last waited
+            // for puts every slot at most one turn of its barrier behind; with a step of more than a tile's units it could pass a turn unseen)
+            static_assert(KP_EXPAND < 2 * SUBTILES, "units of a tile of the narrowest head");
+            const int units = n * 2 * G * SUBTILES;
+            // Keys: a lane has a slot, all 64 channels.  Values: a lane has half the chunks of a pair of slots; every other two pairs swap neighbouring
+            // chunks, so that eight lanes store to eight places of a row
+            const int pair = lane >> 1, swap = (pair >> 1) & 1;
+            uint4 raw[2];
+            uint32_t meta[3];                                              // keys: { zero, scale }; values: the scales, both zeros.  Nothing is done
+            bool hidden[2];                                                // with them before they are used: the request would wait for its loads
+            auto request = [&](int u) {
+                const int sub = u % SUBTILES, g = u / SUBTILES % G, at = tiles.tile(u / (2 * G * SUBTILES)) * SUBTILES + sub;
+                const bool keys = u / (G * SUBTILES) % 2 == 0, held = at < P.cache.n_tiles;              // (the last tile may reach beyond the cache)
+                const uint8_t* tile = base + (long long)(held ? at : 0) * TILE;
+                const uint4* p = reinterpret_cast<const uint4*>(tile + (keys ? 0 : 1024 * G) + 1024 * g + 32 * lane);       // 32 slots, or 16 pairs of 2 halves
+                raw[0] = __ldg(p);
+                raw[1] = __ldg(p + 1);
+                const int j = KV4_TILE * at + (keys ? lane : 2 * pair);
+                hidden[0] = !held || nobody(j);                            // zeros: nobody sees the slot, it may hold anything
+                hidden[1] = !held || nobody(j + 1);
+                if (keys) {
+                    meta[0] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_k_meta(G, g, lane)));
+                } else {
+                    meta[0] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair)));
+                    meta[1] = __ldg(reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, 2 * pair + 1)));
+                    meta[2] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_v_zero(G, g, 2 * pair)));
+                }
+            };
+            int u = warp - 8;
+            if (u < units) request(u);
 #pragma unroll 1
-        for (; u < units; u += KP_EXPAND) {
-            const int sub = u % SUBTILES, g = u / SUBTILES % G, j = u / (2 * G * SUBTILES), s = j & 1;
-            const bool keys = u / (G * SUBTILES) % 2 == 0;
-            if (!__all_sync(full_mask, mbar_wait_bounded(keys ? bar_kempty(s) : bar_vempty(s), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY))) break;
-            const uint32_t dst = (keys ? k_base : v_base) + (uint32_t)(s * G + g) * KP_SUB + (uint32_t)(32 * sub) * 128u;
-            const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-            if (keys) {
-                const uint32_t m = hidden[0] ? 0u : meta[0];
-                const Kv4Step st(__uint_as_float(m & 0xFFFF0000u) * up_k, f16_to_float(m & 0xFFFFu));
-                if (u + KP_EXPAND < units) request(u + KP_EXPAND);
-                auto store = [&](int c, const uint4 x) { sts128(dst + (uint32_t)lane * 128u + (((uint32_t)c ^ ((uint32_t)lane & 7u)) << 4), x.x, x.y, x.z, x.w); };
+            for (; u < units; u += KP_EXPAND) {
+                const int sub = u % SUBTILES, g = u / SUBTILES % G, j = u / (2 * G * SUBTILES), s = j & 1;
+                const bool keys = u / (G * SUBTILES) % 2 == 0;
+                if (!__all_sync(full_mask, mbar_wait_bounded(keys ? bar_kempty(s) : bar_vempty(s), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY))) break;
+                const uint32_t dst = (keys ? k_base : v_base) + (uint32_t)(s * G + g) * KP_SUB + (uint32_t)(32 * sub) * 128u;
+                const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+                if (keys) {
+                    const uint32_t m = hidden[0] ? 0u : meta[0];
+                    const Kv4Step st(__uint_as_float(m & 0xFFFF0000u) * up_k, f16_to_float(m & 0xFFFFu));
+                    if (u + KP_EXPAND < units) request(u + KP_EXPAND);
+                    auto store = [&](int c, const uint4 x) { sts128(dst + (uint32_t)lane * 128u + (((uint32_t)c ^ ((uint32_t)lane & 7u)) << 4), x.x, x.y, x.z, x.w); };
 #pragma unroll
-                for (int c = 0; c < 8; ++c) store(c, st.values(w[c]));
-            } else {
-                uint32_t s0v = hidden[0] ? 0u : meta[0], s1v = hidden[1] ? 0u : meta[1];
-                uint32_t z0 = hidden[0] ? 0u : meta[2] & 0xFFFFu, z1 = hidden[1] ? 0u : meta[2] >> 16;
-                if ((s0v & 0x7F80u) == 0x7F80u) { s0v = z0 = 0u; no_number = 1u; }
-                if ((s1v & 0x7F80u) == 0x7F80u) { s1v = z1 = 0u; no_number = 1u; }
-                const Kv4Step even(__uint_as_float(s0v << 16) * up_v, f16_to_float(z0)), odd(__uint_as_float(s1v << 16) * up_v, f16_to_float(z1));
-                if (u + KP_EXPAND < units) request(u + KP_EXPAND);
-                const uint32_t row = 2u * (uint32_t)pair;
-                uint32_t we[4], wo[4], at[4];
+                    for (int c = 0; c < 8; ++c) store(c, st.values(w[c]));
+                } else {
+                    uint32_t s0v = hidden[0] ? 0u : meta[0], s1v = hidden[1] ? 0u : meta[1];
+                    uint32_t z0 = hidden[0] ? 0u : meta[2] & 0xFFFFu, z1 = hidden[1] ? 0u : meta[2] >> 16;
+                    if ((s0v & 0x7F80u) == 0x7F80u) { s0v = z0 = 0u; no_number = 1u; }
+                    if ((s1v & 0x7F80u) == 0x7F80u) { s1v = z1 = 0u; no_number = 1u; }
+                    const Kv4Step even(__uint_as_float(s0v << 16) * up_v, f16_to_float(z0)), odd(__uint_as_float(s1v << 16) * up_v, f16_to_float(z1));
+                    if (u + KP_EXPAND < units) request(u + KP_EXPAND);
+                    const uint32_t row = 2u * (uint32_t)pair;
+                    uint32_t we[4], wo[4], at[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {                          // words 2k, 2k + 1: place 4 h + k of both slots
-                    const int k1 = i ^ 1;
-                    we[i] = swap ? w[2 * k1] : w[2 * i];
-                    wo[i] = swap ? w[2 * k1 + 1] : w[2 * i + 1];
-                    const uint32_t place = 4u * ((uint32_t)lane & 1u) + (uint32_t)(swap ? k1 : i);
-                    at[i] = place ^ (((uint32_t)pair & 2u) << 1);      // its chunk
+                    for (int i = 0; i < 4; ++i) {                          // words 2k, 2k + 1: place 4 h + k of both slots
+                        const int k1 = i ^ 1;
+                        we[i] = swap ? w[2 * k1] : w[2 * i];
+                        wo[i] = swap ? w[2 * k1 + 1] : w[2 * i + 1];
+                        const uint32_t place = 4u * ((uint32_t)lane & 1u) + (uint32_t)(swap ? k1 : i);
+                        at[i] = place ^ (((uint32_t)pair & 2u) << 1);      // its chunk
+                    }
+                    auto store = [&](uint32_t r, uint32_t chunk, const uint4 x) { sts128(dst + r * 128u + ((chunk ^ (r & 7u)) << 4), x.x, x.y, x.z, x.w); };
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        store(row, at[i], even.values(we[i]));
+                        store(row + 1u, at[i], odd.values(wo[i]));
+                    }
                 }
-                auto store = [&](uint32_t r, uint32_t chunk, const uint4 x) { sts128(dst + r * 128u + ((chunk ^ (r & 7u)) << 4), x.x, x.y, x.z, x.w); };
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    store(row, at[i], even.values(we[i]));
-                    store(row + 1u, at[i], odd.values(wo[i]));
-                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(keys ? bar_kfull(s) : bar_vfull(s));
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(keys ? bar_kfull(s) : bar_vfull(s));
-        }
-        asm volatile("bar.arrive 1, 480;" ::: "memory");
-    } else {
-        // =========================================================== MMA
-        constexpr uint32_t BF16 = (1u << 7) | (1u << 10);               // (both operands fp16 instead)
-        const uint32_t idesc_s = umma_idesc(KP_KEYS) & ~BF16;
-        const uint32_t idesc_o = (umma_idesc(D) & ~BF16) | (1u << 16);            // B (= V) is N-major
-        const uint64_t qd = umma_smem_desc(q_base);
-        bool healthy = true;
-        auto issue_scores = [&](int j) {
-            const int s = j & 1;
-            healthy = healthy && mbar_wait_bounded(bar_kfull(s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_STAGE);
-            healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_sempty(s), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY));
-            if (!healthy) return;
-            tc_fence_after();
-            const uint64_t kd = umma_smem_desc(k_base + (uint32_t)s * G * KP_SUB);
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t off = (uint64_t)((k / 4) * (KP_SUB >> 4) + (k % 4) * 2);
-                    umma_bf16<false>(tmem + (uint32_t)(s * KP_KEYS), qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
-                }
-                umma_commit<false>(bar_kempty(s));
-                umma_commit<false>(bar_sfull(s));
-            }
-            __syncwarp();
-        };
-        auto issue_context = [&](int j) {
-            const int s = j & 1;
-            healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_vfull(s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_STAGE));
-            for (int h = 0; h < 2; ++h) {
-                healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_pfull(h, s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_FULL));
+            asm volatile("bar.arrive 1, 480;" ::: "memory");
+        } else {
+            // =========================================================== MMA
+            constexpr uint32_t BF16 = (1u << 7) | (1u << 10);               // (both operands fp16 instead)
+            const uint32_t idesc_s = umma_idesc(KP_KEYS) & ~BF16;
+            const uint32_t idesc_o = (umma_idesc(D) & ~BF16) | (1u << 16);            // B (= V) is N-major
+            const uint64_t qd = umma_smem_desc(q_base);
+            bool healthy = true;
+            auto issue_scores = [&](int j) {
+                const int s = j & 1;
+                healthy = healthy && mbar_wait_bounded(bar_kfull(s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_STAGE);
+                healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_sempty(s), ((uint32_t)(j >> 1) & 1u) ^ 1u, status, DEV_TIMEOUT_EMPTY));
                 if (!healthy) return;
                 tc_fence_after();
-                const uint64_t pd = umma_smem_desc(p_base + (uint32_t)(2 * s + h) * KP_SUB);
-                const uint64_t vd = umma_smem_desc_mn(v_base + (uint32_t)s * G * KP_SUB, KP_SUB);
+                const uint64_t kd = umma_smem_desc(k_base + (uint32_t)s * G * KP_SUB);
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_bf16<false>(tmem_o + (uint32_t)(h * D), pd + (uint64_t)(k * 2), vd + (uint64_t)((4 * h + k) * (2048 >> 4)), idesc_o,
-                                         (j > 0 || k > 0) ? 1u : 0u);
-                    umma_commit<false>(bar_pempty(h, s));
-                    if (h == 1) umma_commit<false>(bar_vempty(s));
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint64_t off = (uint64_t)((k / 4) * (KP_SUB >> 4) + (k % 4) * 2);
+                        umma_bf16<false>(tmem + (uint32_t)(s * KP_KEYS), qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
+                    }
+                    umma_commit<false>(bar_kempty(s));
+                    umma_commit<false>(bar_sfull(s));
                 }
                 __syncwarp();
+            };
+            auto issue_context = [&](int j) {
+                const int s = j & 1;
+                healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_vfull(s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_STAGE));
+                for (int h = 0; h < 2; ++h) {
+                    healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_pfull(h, s), (uint32_t)(j >> 1) & 1u, status, DEV_TIMEOUT_FULL));
+                    if (!healthy) return;
+                    tc_fence_after();
+                    const uint64_t pd = umma_smem_desc(p_base + (uint32_t)(2 * s + h) * KP_SUB);
+                    const uint64_t vd = umma_smem_desc_mn(v_base + (uint32_t)s * G * KP_SUB, KP_SUB);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_bf16<false>(tmem_o + (uint32_t)(h * D), pd + (uint64_t)(k * 2), vd + (uint64_t)((4 * h + k) * (2048 >> 4)), idesc_o,
+                                             (j > 0 || k > 0) ? 1u : 0u);
+                        umma_commit<false>(bar_pempty(h, s));
+                        if (h == 1) umma_commit<false>(bar_vempty(s));
+                    }
+                    __syncwarp();
+                }
+            };
+            issue_scores(0);
+            for (int j = 0; j < n && healthy; ++j) {
+                if (j + 1 < n) issue_scores(j + 1);
+                issue_context(j);
             }
-        };
-        issue_scores(0);
-        for (int j = 0; j < n && healthy; ++j) {
-            if (j + 1 < n) issue_scores(j + 1);
-            issue_context(j);
         }
-    }
+    };
+    if (__builtin_expect(big, 0)) roles(std::false_type());
+    else roles(std::true_type());
     tc_fence_before();
     __syncthreads();
     if (warp == KP_THREADS / 32 - 1) { tc_fence_after(); tmem_dealloc<false>(tmem, 512); }

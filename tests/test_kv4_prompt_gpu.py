@@ -78,6 +78,35 @@ def test_a_fresh_cache(D):
     assert not bool(attend_prompt(c, torch.zeros(1, T, heads * D, dtype=torch.bfloat16, device="cuda"), pos).any())
 
 
+# ----------------------------------------------------------------------------- large scores
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q_gain,k_gain,scale", [(1e3, 1e3, None), (3e4, 1e4, None), (1e8, 1e6, None), (1e18, 1e18, -0.1), (1.0, 1.0, 1e30)])
+def test_large_scores(D, q_gain, k_gain, scale):
+    """Scores so far apart that one slot has all the weight: its value, where no other score comes near it (nearer than operands' roundings tell apart:
+    2 * 9 e |q k| and 2^-8 of the scores, which is more than fp32 takes), and finite everywhere."""
+    (T, heads, n_kv), slots = size(D), 450
+    c = KVCache4(1, n_kv, slots, D)
+    c.append(randn(1, 1, slots, n_kv * D, gain=k_gain), randn(2, 1, slots, n_kv * D), torch.arange(slots, device="cuda"))
+    kd, vd = R.cache_values(c.tiles, D)
+    q = randn(3, 1, T, heads * D, gain=q_gain)
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    scale = D ** -0.5 if scale is None else scale
+    got = attend_prompt(c, q, pos, scale=scale)
+    assert bool(torch.isfinite(got.float()).all())
+    see, clear = R.visible(pos, slots, 0, 0)[0], 0
+    for h in range(heads):
+        s = (q.view(T, heads, D)[:, h].double() @ kd[0, h // 4, :slots].T * scale).masked_fill(~see, float("-inf"))
+        (first, second), j = s.topk(2, 1)[0].T, s.argmax(1)
+        qk = (q.view(T, heads, D)[:, h].double().square() @ kd[0, h // 4, :slots].square().T).sqrt().amax(1) * abs(scale)
+        sure = first - second > 2 * 9 * FP16 * qk + 2.0 ** -8 * s.masked_fill(~see, 0.0).abs().amax(1) + 30
+        want = vd[0, h // 4, :slots][j]
+        off = (got.view(T, heads, D)[:, h].double() - want).abs()
+        tol = 2.0 ** -8 * want.abs() + 2 * FP16 * want.abs() + 2.0 ** -14 * vd.abs().amax()
+        assert bool((off <= tol)[sure].all())
+        clear += int(sure.sum())
+    assert clear > T * heads // 2
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_rows_of_zeros(D):
     T, heads, n_kv = size(D)
