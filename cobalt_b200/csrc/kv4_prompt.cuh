@@ -15,7 +15,9 @@
 // Operands are fp16 (2^-11): in bf16 the roundings of keys, values and probabilities doubled the result's error (3.3e-3 against 1.7e-3, which
 // is that of its own rounding).  So that any bf16 range fits, queries are scaled by a power of two per row, keys and values by one each
 // per CTA, from the largest magnitude that the scales and zeros of its visible slots allow (looked through once at the start: 4 G + 4 G
-// bytes a slot); scores, maxima, sums and contexts are fp32.
+// bytes a slot); scores, maxima, sums and contexts are fp32.  fp16 holds 2^-39 of that largest magnitude, so groups down to 2^-20 of it keep
+// 2^-19 of their own.  Where groups lie further apart, a slot that only some rows see would cost the others their bits: such a CTA's
+// queries and keys, or probabilities and values, are bf16, which holds any of them to 2^-8.
 //
 // A slot that only some rows see has to stay out of the others' products even where its values are not numbers: such groups are
 // expanded to zeros and marked, and marked CTAs look through the scales of their rows' slots once at the end.
@@ -50,7 +52,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight codes of a word as fp16 values (c - z) * s.  A code anywhere in the mantissa of an fp32 number is that power of two plus c; at bits 12 and
+// Eight codes of a word as fp16 or bf16 values (c - z) * s.  A code anywhere in the mantissa of an fp32 number is that power of two plus c; at bits 12 and
 // 16 (2^11, 2^7) one "and-or" per code makes the number, and the constant -(2^k + z) * s is good to 2^-12 of a step.  (At bit 8, which would save
 // two shifts of twelve operations a word, the constant of 2^15 is off by up to 2^-8 of a step: as much as fp16 rounds the largest values of a group,
 // but of every value, those next to zero among them.)
@@ -62,18 +64,21 @@ struct Kv4Step {
         return d;
     }
     __device__ __forceinline__ Kv4Step(float s, float z) : s2(two(s, s)), b2(two(-(2048.0f + z) * s, -(128.0f + z) * s)) {}
-    __device__ __forceinline__ uint32_t pair(uint32_t w) const {       // the codes at bits 12 and 16
+    // the codes at bits 12 and 16
+    __device__ __forceinline__ uint32_t pair(uint32_t w, bool bf16) const {
         const uint64_t x = two(__uint_as_float((w & 0xF000u) | 0x45000000u), __uint_as_float((w & 0xF0000u) | 0x43000000u));
-        uint32_t d;
-        asm("{\n\t.reg .b64 x;\n\t.reg .f32 l, h;\n\tfma.rn.f32x2 x, %1, %2, %3;\n\tmov.b64 {l, h}, x;\n\tcvt.rn.f16x2.f32 %0, h, l;\n\t}" : "=r"(d) : "l"(x), "l"(s2), "l"(b2));
-        return d;
+        float lo, hi;
+        asm("{\n\t.reg .b64 x;\n\tfma.rn.f32x2 x, %2, %3, %4;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(lo), "=f"(hi) : "l"(x), "l"(s2), "l"(b2));
+        return bf16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
     }
-    __device__ __forceinline__ uint4 values(uint32_t w) const { return make_uint4(pair(w << 12), pair(w << 4), pair(w >> 4), pair(w >> 12)); }
+    __device__ __forceinline__ uint4 values(uint32_t w, bool bf16) const {
+        return make_uint4(pair(w << 12, bf16), pair(w << 4, bf16), pair(w >> 4, bf16), pair(w >> 12, bf16));
+    }
 };
-// largest magnitude that a group can hold; 0 for one that is no number
+// largest magnitude that a group's codes could stand for (a constant group near the end of fp32 would leave it); 0 for one that is no number
 __device__ __forceinline__ float kv4_largest(uint32_t scale, uint32_t zero) {
     const float s = __uint_as_float(scale << 16), z = f16_to_float(zero), m = s * fmaxf(fabsf(z), fabsf(15.0f - z));
-    return m < INFINITY ? m : 0.0f;
+    return (scale & 0x7F80u) == 0x7F80u ? 0.0f : fminf(m, 0x1.fffffep127f);
 }
 
 // The same with tiles of 128 slots
@@ -93,7 +98,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     constexpr int D = 64 * G, TILE = kv4_tile_bytes(G), SUBTILES = KP_KEYS / KV4_TILE;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t no_number;                                     // a group of values that is not a number was seen
-    __shared__ uint32_t largest[2];                                    // magnitude (bits) among the visible keys, values
+    __shared__ uint32_t largest[2], smallest[2];                       // magnitude (bits) of a group among the visible keys, values; but for groups of zeros
     __shared__ int q_exp[KP_ROWS];                                     // queries of a row were divided by 2^(this - 14); 128: one is not finite
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full_mask = 0xFFFFFFFFu;
@@ -150,11 +155,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
         }
         mbar_fence_init();
         no_number = largest[0] = largest[1] = 0u;
+        smallest[0] = smallest[1] = 0x7F800000u;
     }
     __syncthreads();
     const uint8_t* base = P.cache.tiles + (long long)seq * P.cache.seq_stride + (long long)kvh * P.cache.n_tiles * TILE;
-    {                                                                  // the largest key and value that some row sees
-        float top_k = 0.0f, top_v = 0.0f;
+    {                                                                  // the largest and smallest groups of keys and values that some row sees
+        float top_k = 0.0f, top_v = 0.0f, low_k = INFINITY, low_v = INFINITY;
         const int slots = n * KP_KEYS;
 #pragma unroll 1
         for (int i0 = threadIdx.x; i0 < slots; i0 += 4 * KP_THREADS) {
@@ -175,33 +181,43 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    top_k = fmaxf(top_k, kv4_largest(mk[k][g] >> 16, mk[k][g] & 0xFFFFu));
-                    top_v = fmaxf(top_v, kv4_largest(vs[k][g], vz[k][g]));
+                    const float key = kv4_largest(mk[k][g] >> 16, mk[k][g] & 0xFFFFu), value = kv4_largest(vs[k][g], vz[k][g]);
+                    top_k = fmaxf(top_k, key);
+                    top_v = fmaxf(top_v, value);
+                    if (key > 0.0f) low_k = fminf(low_k, key);
+                    if (value > 0.0f) low_v = fminf(low_v, value);
                 }
         }
         const uint32_t bk = __reduce_max_sync(full_mask, __float_as_uint(top_k)), bv = __reduce_max_sync(full_mask, __float_as_uint(top_v));
-        if (lane == 0) { atomicMax(&largest[0], bk); atomicMax(&largest[1], bv); }
+        const uint32_t ck = __reduce_min_sync(full_mask, __float_as_uint(low_k)), cv = __reduce_min_sync(full_mask, __float_as_uint(low_v));
+        if (lane == 0) { atomicMax(&largest[0], bk); atomicMax(&largest[1], bv); atomicMin(&smallest[0], ck); atomicMin(&smallest[1], cv); }
     }
     // The scale is made positive (its sign goes to the queries; none at all: queries of zero), so that maxima can be taken of raw scores
     const uint32_t q_and = P.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu, q_xor = P.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    auto store_queries = [&](bool bf16) {
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-        const int i = threadIdx.x + k * KP_THREADS, r = i / (D / 8), c = i % (D / 8);
-        const uint4 v = queries[k];
-        const uint32_t w[4] = {(v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor, (v.w & q_and) ^ q_xor};
-        uint32_t top = 0u, o[4];                                       // largest magnitude of the row; a NaN stays on top
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int i = threadIdx.x + k * KP_THREADS, r = i / (D / 8), c = i % (D / 8);
+            const uint4 v = queries[k];
+            const uint32_t w[4] = {(v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor, (v.w & q_and) ^ q_xor};
+            uint32_t top = 0u, o[4];                                   // largest magnitude of the row; a NaN stays on top
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7FFF0000u, (w[e] & 0x7FFFu) << 16));
+            for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7FFF0000u, (w[e] & 0x7FFFu) << 16));
 #pragma unroll
-        for (int x = 1; x < D / 8; x <<= 1) top = max(top, __shfl_xor_sync(full_mask, top, x));
-        const int ex = max(-112, (int)(top >> 23) - 127);              // in [2^ex, 2^(ex + 1)), to [2^14, 2^15)
-        const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+            for (int x = 1; x < D / 8; x <<= 1) top = max(top, __shfl_xor_sync(full_mask, top, x));
+            const int ex = max(-112, (int)(top >> 23) - 127);          // in [2^ex, 2^(ex + 1)), to [2^14, 2^15)
+            const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = pack_f16x2(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xFFFF0000u) * up);
-        if (c == 0) q_exp[r] = ex;
-        sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), o[0], o[1], o[2], o[3]);
-    }
-    fence_proxy_async();
+            for (int e = 0; e < 4; ++e) {
+                const float lo = __uint_as_float(w[e] << 16) * up, hi = __uint_as_float(w[e] & 0xFFFF0000u) * up;
+                o[e] = bf16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+            }
+            if (c == 0) q_exp[r] = ex;
+            sts128(q_base + (uint32_t)(c >> 3) * KP_SUB + (uint32_t)r * 128u + ((((uint32_t)c & 7u) ^ ((uint32_t)r & 7u)) << 4), o[0], o[1], o[2], o[3]);
+        }
+        fence_proxy_async();
+    };
+    store_queries(false);
     if (warp == KP_THREADS / 32 - 1) { tmem_alloc<false>(tmem_slot, 512); tmem_relinquish<false>(); }
     tc_fence_before();
     __syncthreads();
@@ -209,6 +225,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     // keys and values times a power of two that brings the largest into [2^14, 2^15)
     const int ex_k = max(-110, (int)(largest[0] >> 23) - 127), ex_v = max(-110, (int)(largest[1] >> 23) - 127);
     const float up_k = __uint_as_float((uint32_t)(14 - ex_k + 127) << 23), up_v = __uint_as_float((uint32_t)(14 - ex_v + 127) << 23);
+    auto apart = [&](int i) { return __uint_as_float(smallest[i]) * 0x1p20f < __uint_as_float(largest[i]); };
+    const bool wide_k = apart(0), wide_v = apart(1);                   // bf16 operands
+    if (wide_k) {
+        store_queries(true);
+        __syncthreads();
+    }
     // Scores that may pass 2^24 (times log2(e)) are rounded before the maximum is taken off: it was rounded, too, and what an exact product would leave
     // of the two is no longer small
     int ex_q = -1000;
@@ -218,6 +240,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     const bool big = ldexpf(fabsf(P.scale_log2), ex_q + ex_k + 2 + 7) > 0x1p24f;
     const uint32_t tmem = lds32(tmem_slot), tmem_o = tmem + 2 * KP_KEYS;              // scores 2 x 128 columns, contexts 2 x D
 
+    // (PLAIN: fp16 operands, scores below 2^24.  The rest, which asks at every step, has a copy of its own: asked in one, 100.6 -> 106.6 us)
     auto roles = [&](auto plain) {
         constexpr bool PLAIN = decltype(plain)::value;
         if (warp < 8) {
@@ -289,7 +312,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
                 for (int i = 0; i < 32; ++i) {
                     const float a = ex2(PLAIN ? fmaf(x[2 * i], scale, base) : __fmul_rn(x[2 * i], scale) - ref + 6.0f);
                     const float b = ex2(PLAIN ? fmaf(x[2 * i + 1], scale, base) : __fmul_rn(x[2 * i + 1], scale) - ref + 6.0f);
-                    p[i] = pack_f16x2(a, b);
+                    p[i] = !PLAIN && wide_v ? pack_bf16x2(a, b) : pack_f16x2(a, b);
                     s[i & 3] += a + b;
                 }
                 l += (s[0] + s[1]) + (s[2] + s[3]);
@@ -396,7 +419,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
                     if (u + KP_EXPAND < units) request(u + KP_EXPAND);
                     auto store = [&](int c, const uint4 x) { sts128(dst + (uint32_t)lane * 128u + (((uint32_t)c ^ ((uint32_t)lane & 7u)) << 4), x.x, x.y, x.z, x.w); };
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) store(c, st.values(w[c]));
+                    for (int c = 0; c < 8; ++c) store(c, st.values(w[c], !PLAIN && wide_k));
                 } else {
                     uint32_t s0v = hidden[0] ? 0u : meta[0], s1v = hidden[1] ? 0u : meta[1];
                     uint32_t z0 = hidden[0] ? 0u : meta[2] & 0xFFFFu, z1 = hidden[1] ? 0u : meta[2] >> 16;
@@ -417,8 +440,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
                     auto store = [&](uint32_t r, uint32_t chunk, const uint4 x) { sts128(dst + r * 128u + ((chunk ^ (r & 7u)) << 4), x.x, x.y, x.z, x.w); };
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        store(row, at[i], even.values(we[i]));
-                        store(row + 1u, at[i], odd.values(wo[i]));
+                        store(row, at[i], even.values(we[i], !PLAIN && wide_v));
+                        store(row + 1u, at[i], odd.values(wo[i], !PLAIN && wide_v));
                     }
                 }
                 fence_proxy_async();
@@ -428,9 +451,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             asm volatile("bar.arrive 1, 480;" ::: "memory");
         } else {
             // =========================================================== MMA
-            constexpr uint32_t BF16 = (1u << 7) | (1u << 10);               // (both operands fp16 instead)
-            const uint32_t idesc_s = umma_idesc(KP_KEYS) & ~BF16;
-            const uint32_t idesc_o = (umma_idesc(D) & ~BF16) | (1u << 16);            // B (= V) is N-major
+            constexpr uint32_t BF16 = (1u << 7) | (1u << 10);           // (both operands fp16 without)
+            const uint32_t idesc_s = umma_idesc(KP_KEYS) & ~(!PLAIN && wide_k ? 0u : BF16);
+            const uint32_t idesc_o = (umma_idesc(D) & ~(!PLAIN && wide_v ? 0u : BF16)) | (1u << 16);        // B (= V) is N-major
             const uint64_t qd = umma_smem_desc(q_base);
             bool healthy = true;
             auto issue_scores = [&](int j) {
@@ -478,7 +501,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             }
         }
     };
-    if (__builtin_expect(big, 0)) roles(std::false_type());
+    if (__builtin_expect(big || wide_k || wide_v, 0)) roles(std::false_type());
     else roles(std::true_type());
     tc_fence_before();
     __syncthreads();

@@ -14,7 +14,8 @@ The result is rounded once, by 2^-8 of the value:
     |got - want| <= 2^-8 |want| + (2 e + 2 * 9 e |q k|) sum p|v| + (2^-14 + 2^-22) max|v|.
 Over a whole result the roundings are independent, with a standard deviation of at most e each, so its 2-norm is held to
     ||got - want|| <= 2^-8 ||want|| + 2 e || (2 + |q k|) sqrt(sum p^2 v^2) || + 2^-14 || max|v| sqrt(sum p^2) || + 2^-22 ||max|v|||
-(twice the expectation of what does not come from the last rounding)."""
+(twice the expectation of what does not come from the last rounding).  Where groups of the slots that 128 rows see lie more than 2^20 apart, the
+operands are bf16: e = 2^-8."""
 import pytest
 import torch
 
@@ -24,7 +25,7 @@ from test_kv4_gpu import copy_slots, filled, randn
 
 pytestmark = pytest.mark.gpu
 
-FP16 = 2.0 ** -11
+FP16, BF16 = 2.0 ** -11, 2.0 ** -8
 
 
 def attend_prompt(c, q, pos, **kw):
@@ -330,3 +331,66 @@ def test_prompts_of_a_decoder():
     ids = torch.randint(0, 1000, (2, 330), generator=torch.Generator().manual_seed(1))
     took, want = R.kernels(lambda: dec.prefill(ids))
     assert took == {"prompt"} and torch.equal(chk.prefill(ids), want) and checked == [0, 1]
+
+
+# ----------------------------------------------------------------------------- magnitudes far apart
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("what", ["key", "value", "value in the last group", "both"])
+@pytest.mark.parametrize("size_of", [1e8, 1e13, 1e30])
+def test_a_huge_slot_does_not_reach_rows_that_do_not_see_it(D, what, size_of):
+    """A finite key or value far above all others, in the slot of a token in the middle of a CTA's rows: the rows before it, and (window) those
+    that have left it behind, are what they are without it, to within the operands' rounding."""
+    (T, heads, n_kv), slots = size(D), 450
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    at = int(pos[0, T // 2 + 9])
+    k, v = randn(1, 1, slots, n_kv * D), randn(2, 1, slots, n_kv * D)
+    channels = torch.arange(n_kv, device="cuda") * D + (D - 1 if "last" in what else 3)
+    if what in ("key", "both"):
+        k[0, at, channels] = size_of
+    if what != "key":
+        v[0, at, channels] = -size_of
+    c = KVCache4(1, n_kv, slots, D)
+    c.append(k, v, torch.arange(slots, device="cuda"))
+    kd, vd = R.cache_values(c.tiles, D)
+    q = randn(3, 1, T, heads * D)
+    for window, sinks in ((0, 0), (20, 0), (20, 2)):
+        got = attend_prompt(c, q, pos, window=window, sinks=sinks)
+        see = R.visible(pos, slots, window, sinks)[0, :, at]
+        assert bool(torch.isfinite(got.float()).all())
+        assert_near(got, q, kd, vd, pos, slots, heads, D ** -0.5, window, sinks, e=BF16, rows=~see[None])
+        if what in ("value", "value in the last group"):
+            assert_near(got, q, kd, vd, pos, slots, heads, D ** -0.5, window, sinks, e=BF16, rows=see[None])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_magnitudes_that_fall_and_rise_by_many_powers_of_two(D):
+    """Keys and values of 2^-60 to 2^60 from slot to slot, queries to match: every row against what it sees itself."""
+    (T, heads, n_kv), slots = size(D), 450
+    at = torch.arange(slots, device="cuda")
+    c = KVCache4(1, n_kv, slots, D)
+    rise = torch.exp2(60 * torch.sin(at.float() / 40))[None, :, None]
+    c.append(randn(1, 1, slots, n_kv * D, gain=2.0 ** -8), (randn(2, 1, slots, n_kv * D).float() * rise).bfloat16(), at)
+    q = randn(3, 1, T, heads * D)
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    for window, sinks in ((0, 0), (9, 0), (1, 0)):
+        got = attend_prompt(c, q, pos, window=window, sinks=sinks)
+        assert_near(got, q, *R.cache_values(c.tiles, D), pos, slots, heads, D ** -0.5, window, sinks, e=BF16)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_constant_group_near_the_end_of_fp32(D):
+    """256 s is such a group's value, 271 s would be beyond fp32; the rows before it do not see it, those behind have it in its channels only."""
+    (T, heads, n_kv), slots = size(D), 450
+    pos = (slots - T + torch.arange(T, device="cuda"))[None]
+    at = int(pos[0, T // 2 + 9])
+    k, v = randn(1, 1, slots, n_kv * D), randn(2, 1, slots, n_kv * D)
+    v[0, at, :64] = -3.3e38
+    c = KVCache4(1, n_kv, slots, D)
+    c.append(k, v, torch.arange(slots, device="cuda"))
+    kd, vd = R.cache_values(c.tiles, D)
+    q = randn(3, 1, T, heads * D)
+    got = attend_prompt(c, q, pos)
+    see = R.visible(pos, slots, 0, 0)[0, :, at]
+    assert bool(torch.isfinite(got.float()).all())
+    for rows in (see, ~see):
+        assert_near(got, q, kd, vd, pos, slots, heads, D ** -0.5, e=BF16, rows=rows[None])
