@@ -96,15 +96,15 @@ int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, i
     c->scratch = c->list ? c->joins_off + (size_t)c->grid * sizeof(int4) : 0;
     return COBALT_OK;
 }
-template <int G, int NB>
-int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c, cudaStream_t st) {
+template <int G, int NB, bool MANY>
+int launch_attend_as(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c, cudaStream_t st) {
     static bool configured[MAX_DEVICES];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(kv4_attend_list_kernel<G, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_list_smem(G, NB)) != cudaSuccess ||
-            cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_heads_smem(G, NB)) != cudaSuccess ||
-            cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        if (cudaFuncSetAttribute(kv4_attend_list_kernel<G, NB, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_list_smem(G, NB)) != cudaSuccess ||
+            cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_heads_smem(G, NB)) != cudaSuccess ||
+            cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB, MANY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return COBALT_ELAUNCH;
         configured[dev] = true;
     }
@@ -120,11 +120,11 @@ int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c
         attr[0].val.clusterDim.x = (unsigned)c.share;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.numAttrs = c.share > 1 ? 1 : 0;
-        return cudaLaunchKernelEx(&cfg, kv4_attend_heads_kernel<G, NB>, P, c.share) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+        return cudaLaunchKernelEx(&cfg, kv4_attend_heads_kernel<G, NB, MANY>, P, c.share) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
     }
     cfg.dynamicSmemBytes = ka_list_smem(G, NB);
     // (an early start of this kernel under its predecessor left SMs with a carve-out too small for all CTAs: 99 -> 126 us for 440 MB)
-    if (cudaLaunchKernelEx(&cfg, kv4_attend_list_kernel<G, NB>, P, W) != cudaSuccess) return COBALT_ELAUNCH;
+    if (cudaLaunchKernelEx(&cfg, kv4_attend_list_kernel<G, NB, MANY>, P, W) != cudaSuccess) return COBALT_ELAUNCH;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)c.grid, NB, G);
@@ -132,6 +132,10 @@ int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<G, NB>, P, W) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+}
+template <int G, int NB>
+int launch_attend(const Kv4AttendParams& P, const Kv4Work& W, const AttendCfg& c, cudaStream_t st) {
+    return P.T > 1 ? launch_attend_as<G, NB, true>(P, W, c, st) : launch_attend_as<G, NB, false>(P, W, c, st);
 }
 
 // Whether the prompts' kernel takes a call: at 64 rows per KV head and more, where it is expected to be faster.  Its CTAs walk all keys of their

@@ -11,7 +11,9 @@
 // the last sum through the tensor core too (z is an fp16 operand), so that both sums carry the same rounded weights: with many
 // slots of nearly equal weight they cancel down to the mean, and a rounding of one alone would show.
 // Queries are scaled by a power of two into the upper range of fp16, which holds every bf16 significand; so are the weights P s, by
-// the largest scale seen so far: fp16 weights (2^-11), everything else fp32.  A running maximum per column, moved only when a score
+// the largest scale seen so far: fp16 weights (2^-11), everything else fp32.  With several tokens (MANY) every column has a power of its own per
+// group, as a slot that one token sees and another does not would else cost the other its bits (five tokens, 16 / 4 heads of 64, 8 sequences of
+// 700 to 6000 slots 14.1 -> 14.5 us; 40 tokens, 4 of 300 to 2000 18.0 -> 19.4 us).  A running maximum per column, moved only when a score
 // exceeds it by 2^8 (fp16 weights have that room), keeps the rescaling of O out of the loop.
 //
 // A warp owns a ring of tiles, one bulk copy each, and walks every 4th tile of its CTA's share alone; the states of a head are joined
@@ -149,14 +151,16 @@ static_assert(ka_list_smem(4, 1) * 2 <= 226 * 1024 && ka_heads_smem(4, 1) * 2 <=
 // ----------------------------------------------------------------------------- one warp, one head, one tile of columns
 // Lane (g, t) = (lane / 4, lane % 4): query column g of every eight; scores of slots g and g + 8 of every sixteen, columns 2t and 2t + 1;
 // results of columns 2t, 2t + 1, channels 8g .. 8g + 7 of every group of 64.
-template <int G, int NB>
+template <int G, int NB, bool MANY>
 struct Kv4Columns {
+    static constexpr int UPS = MANY ? 2 * NB : 1;
     uint32_t qf[NB][G][8];                                             // queries as B operands
     float qs[NB][G][2], fac[NB][2];                                    // their sums per group, what makes a score of a sum
     Kv4Range range[NB][2];
     // scores are taken relative to a reference per column (base: its negative); one above `room` moves it.  up_v: power of two that the
-    // weights of a group are scaled by
-    float o[NB][G][4][4], zero[NB][G][4], base[NB][2], room[NB][2], sum[NB][2], up_v[G];
+    // weights of a group are scaled by (MANY: of columns nb, c at 2 nb + c; 0 for a column that sees nothing); up_top: the largest
+    float o[NB][G][4][4], zero[NB][G][4], base[NB][2], room[NB][2], sum[NB][2], up_v[UPS][G], up_top[G];
+    __device__ __forceinline__ float up(int nb, int c, int gr) const { return up_v[MANY ? 2 * nb + c : 0][gr]; }
 
     __device__ __forceinline__ static void load_queries(const Kv4AttendParams& P, int seq, int kvh, int col0, int lane, uint4 (&raw)[NB][G][2]) {
 #pragma unroll
@@ -215,13 +219,18 @@ struct Kv4Columns {
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) qs[nb][gr][c] = __shfl_sync(0xFFFFFFFFu, my_sum[gr], 4 * (2 * t + c));
                 const int cc = col0 + 8 * nb + 2 * t + c;
-                range[nb][c] = cc < P.cols ? kv4_range(P, seq, P.by_rep(cc)) : Kv4Range{0, 0x7FFFFFFF};
+                range[nb][c] = cc < P.cols ? kv4_range(P, seq, P.by_rep(cc)) : Kv4Range{0, MANY ? -1 : 0x7FFFFFFF};
+                if (MANY)
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr)
+                        up_v[(2 * nb + c) % UPS][gr] = range[nb][c].hi >= 0 && (range[nb][c].lo <= range[nb][c].hi || P.sinks > 0) ? 0x1p126f : 0.0f;
                 base[nb][c] = sum[nb][c] = 0.0f;
                 room[nb][c] = -INFINITY;
             }
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                up_v[gr] = 0x1p126f;
+                up_top[gr] = 0x1p126f;
+                if (!MANY) up_v[0][gr] = 0x1p126f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     zero[nb][gr][r] = 0.0f;
@@ -237,7 +246,7 @@ struct Kv4Columns {
     __device__ __forceinline__ void sixteen(const uint8_t* tile, int j0, int b, const Kv4Span& span, int sinks, int lane) {
         const int g = lane >> 2, t = lane & 3;
         auto nobody = [&](int j) { return j > span.hi_max || (j < span.lo_min && j >= sinks); };           // such a slot may hold anything
-        // ---- scores of slots g and g + 8, columns 2t, 2t + 1, relative to the reference; value scales of the same slots, times up_v
+        // ---- scores of slots g and g + 8, columns 2t, 2t + 1, relative to the reference; value scales of the same slots, times up_v (MANY: not yet)
         float x[NB][4], vs[G][2], acc[NB][G][4];
         const uint8_t* keys = tile + 512 * b + 32 * g + 8 * t;
 #pragma unroll
@@ -278,7 +287,7 @@ struct Kv4Columns {
                     x[nb][2 * r + c] = fmaf(v, fac[nb][c], base[nb][c]);
                 }
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) vs[gr][r] = sv[gr] * up_v[gr];
+            for (int gr = 0; gr < G; ++gr) vs[gr][r] = MANY ? sv[gr] : sv[gr] * up_v[0][gr];
             if (MASKED) {
                 const int j = j0 + 16 * b + g + 8 * r;
 #pragma unroll
@@ -338,7 +347,7 @@ struct Kv4Columns {
                 sum[nb][1] += p1;
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
-                    uint32_t w = pack_f16x2(p0 * vs[gr][r], p1 * vs[gr][r]);
+                    uint32_t w = MANY ? pack_f16x2(p0 * (vs[gr][r] * up(nb, 0, gr)), p1 * (vs[gr][r] * up(nb, 1, gr))) : pack_f16x2(p0 * vs[gr][r], p1 * vs[gr][r]);
                     if (MASKED)                                        // a slot that only some columns see: no NaN of its scale for the others
                         w &= (x[nb][2 * r] == -INFINITY ? 0u : 0xFFFFu) | (x[nb][2 * r + 1] == -INFINITY ? 0u : 0xFFFF0000u);
                     pf[nb][gr][r] = transpose_8x8(w);
@@ -374,6 +383,47 @@ struct Kv4Columns {
         }
     }
 
+    // The power of two that a scale (its bits) leaves; returns what makes values scaled by `up` so before ones scaled so now
+    __device__ __forceinline__ static float lower(float& up, uint32_t scale) {
+        const int ex = max(-120, (int)(scale >> 23) - 127);
+        const float was = up;
+        up = fminf(was, __uint_as_float((uint32_t)(6 - ex + 127) << 23));
+        return up * __uint_as_float((254u - (__float_as_uint(was) >> 23)) << 23);
+    }
+    // The same for every column, by the scales of the slots that it sees itself (here a lane has slots g, g + 8, g + 16, g + 24).  A column whose first
+    // visible slot is still to come keeps `up_top` high, and every tile until then comes here
+    __device__ __forceinline__ void rescale_columns(const uint8_t* tile, int j0, int sinks, int lane) {
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float sv[4], most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                sv[k] = fmaxf(__uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, gr, (lane >> 2) + 8 * k)) << 16), 0.0f);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int j = j0 + (lane >> 2) + 8 * k;
+                        if (j <= range[nb][c].hi && (j >= range[nb][c].lo || j < sinks)) top = fmaxf(top, sv[k]);
+                    }
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                    float& mine = up_v[(2 * nb + c) % UPS][gr];
+                    const float down = lower(mine, __float_as_uint(top));
+                    most = fmaxf(most, mine);
+                    zero[nb][gr][c] *= down;
+                    zero[nb][gr][c + 2] *= down;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) { o[nb][gr][m][c] *= down; o[nb][gr][m][c + 2] *= down; }
+                }
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            up_top[gr] = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+        }
+    }
+
     // the 32 slots from j0 on
     __device__ __forceinline__ void tile(const uint8_t* tile, int j0, const Kv4Span& span, int sinks, int lane) {
         // a value scale that is too large for the weights' range moves the power of two that they are scaled by
@@ -381,30 +431,35 @@ struct Kv4Columns {
         kv4_halves<G>(tile + kv4_v_scale(G, 0, lane), sv);
         bool grow = false;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) grow |= sv[gr] * up_v[gr] >= 128.0f;
+        for (int gr = 0; gr < G; ++gr) grow |= sv[gr] * (MANY ? up_top[gr] : up_v[0][gr]) >= 128.0f;
+        const bool whole = j0 + KV4_TILE - 1 <= span.hi_min && (j0 >= span.lo_max || j0 + KV4_TILE <= sinks);
         if (__builtin_expect(__any_sync(0xFFFFFFFFu, grow), 0)) {
-            const int j = j0 + lane;
-            const bool nobody = j > span.hi_max || (j < span.lo_min && j >= sinks);
+            if (MANY && !whole) {
+                rescale_columns(tile, j0, sinks, lane);
+            } else {                                                   // every column sees the same slots
+                const int j = j0 + lane;
+                const bool nobody = j > span.hi_max || (j < span.lo_min && j >= sinks);
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-                const float top = nobody ? 0.0f : fmaxf(sv[gr], 0.0f);                             // a NaN stays out
-                const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
-                const int ex = max(-120, (int)(bits >> 23) - 127);
-                const float up = fminf(up_v[gr], __uint_as_float((uint32_t)(6 - ex + 127) << 23));
-                const float down = up * __uint_as_float((254u - (__float_as_uint(up_v[gr]) >> 23)) << 23);
-                up_v[gr] = up;
+                for (int gr = 0; gr < G; ++gr) {
+                    const float top = nobody ? 0.0f : fmaxf(sv[gr], 0.0f);                         // a NaN stays out
+                    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
+                    if (MANY) lower(up_top[gr], bits);
+                    float down[UPS];
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+                    for (int i = 0; i < UPS; ++i) down[i] = lower(up_v[i][gr], bits);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        zero[nb][gr][r] *= down;
+                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) o[nb][gr][m][r] *= down;
-                    }
+                        for (int r = 0; r < 4; ++r) {
+                            const float d = down[MANY ? 2 * nb + (r & 1) : 0];
+                            zero[nb][gr][r] *= d;
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) o[nb][gr][m][r] *= d;
+                        }
+                }
             }
         }
         // sixteen slots at a time: unrolled to 32 the loop's code no longer fits where four warps per scheduler fetch it from
-        const bool whole = j0 + KV4_TILE - 1 <= span.hi_min && (j0 >= span.lo_max || j0 + KV4_TILE <= sinks);
         if (__builtin_expect(whole, 1)) {
 #pragma unroll 1
             for (int b = 0; b < 2; ++b) sixteen<false>(tile, j0, b, span, sinks, lane);
@@ -420,8 +475,8 @@ struct Kv4Columns {
 template <int G>
 struct Kv4State {
     float o[16 * G], ref[2], sum[2];
-    template <int NB>
-    __device__ __forceinline__ void take(const Kv4Columns<G, NB>& C, int nb) {
+    template <int NB, bool MANY>
+    __device__ __forceinline__ void take(const Kv4Columns<G, NB, MANY>& C, int nb) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             float v = C.sum[nb][c];
@@ -432,12 +487,14 @@ struct Kv4State {
         }
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-            const float down = __uint_as_float((254u - (__float_as_uint(C.up_v[gr]) >> 23)) << 23);
+            float down[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) down[c] = __uint_as_float((254u - (__float_as_uint(C.up(nb, c, gr)) >> 23)) << 23);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    o[16 * gr + 4 * m + r] = fmaf(C.o[nb][gr][m][r], r < 2 ? 0x1p24f : 0x1p20f, -C.zero[nb][gr][r & 1]) * down;
+                    o[16 * gr + 4 * m + r] = fmaf(C.o[nb][gr][m][r], r < 2 ? 0x1p24f : 0x1p20f, -C.zero[nb][gr][r & 1]) * down[r & 1];
         }
     }
     __device__ __forceinline__ void store(float* p, int lane) const {
@@ -518,7 +575,7 @@ struct Kv4Quad {
 };
 
 // grid: heads x `share` CTAs (a cluster).  Nothing is looked up: queries and positions are requested at once, then the tiles.
-template <int G, int NB>
+template <int G, int NB, bool MANY>
 __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_heads_kernel(const Kv4AttendParams P, const int share) {
     constexpr int D = 64 * G, TILE = kv4_tile_bytes(G), STATE = (16 * G + 4) * 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -533,7 +590,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
     const int rank = share > 1 ? (int)cluster_rank() : 0, head = (share > 1 ? (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)share) : (int)(gridDim.x - 1 - blockIdx.x));
     const int entry = P.by_kv(head), kvh = head - entry * P.cache.n_kv, seq = P.by_tiles(entry), col0 = (entry - seq * P.col_tiles) * 8 * NB;
     uint4 raw[NB][G][2];
-    Kv4Columns<G, NB>::load_queries(P, seq, kvh, col0, lane, raw);
+    Kv4Columns<G, NB, MANY>::load_queries(P, seq, kvh, col0, lane, raw);
     const Kv4Span span = kv4_span(P, seq, P.by_rep(col0), P.by_rep(min(col0 + 8 * NB, P.cols) - 1));
     if (lane == 0) {
         for (int s = 0; s < KA_STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
@@ -558,7 +615,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
     int i = next;
 #pragma unroll 1
     for (int s = 0; s < KA_STAGES; ++s) fetch();
-    Kv4Columns<G, NB> C;
+    Kv4Columns<G, NB, MANY> C;
     C.begin(P, seq, col0, lane, raw);
     bool healthy = true;
 #pragma unroll 1
@@ -642,7 +699,7 @@ struct Kv4Work {
     int4* joins;                                                       // [CTA]: head that begins in this CTA and ends in a later one
 };
 
-template <int G, int NB>
+template <int G, int NB, bool MANY>
 __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_list_kernel(const Kv4AttendParams P, const Kv4Work W) {
     constexpr int D = 64 * G, TILE = kv4_tile_bytes(G), STATE = (16 * G + 4) * 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -753,10 +810,10 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
         const int here = min(at.k.n - at.i, end - i);                  // tiles of this head in this CTA
         const int seq = P.by_tiles(at.e), col0 = (at.e - seq * P.col_tiles) * 8 * NB;
         const Kv4Span span = {spans[at.e].x, spans[at.e].y, spans[at.e].z, spans[at.e].w};
-        Kv4Columns<G, NB> C;
+        Kv4Columns<G, NB, MANY> C;
         {
             uint4 raw[NB][G][2];
-            Kv4Columns<G, NB>::load_queries(P, seq, at.kvh, col0, lane, raw);
+            Kv4Columns<G, NB, MANY>::load_queries(P, seq, at.kvh, col0, lane, raw);
             C.begin(P, seq, col0, lane, raw);
         }
 #pragma unroll 1
