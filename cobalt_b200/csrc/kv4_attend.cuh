@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
             C.begin(P, seq, col0, lane, raw);
         }
 #pragma unroll 1
-        for (int k = (warp - (i - start)) & (KA_WARPS - 1); k < here; k += KA_WARPS) {
+        for (int k = (warp - (i - start)) & (KA_WARPS - 1); k < here && healthy; k += KA_WARPS) {
             const int s = used % KA_STAGES;
             if (__builtin_expect(!__all_sync(0xFFFFFFFFu, mbar_try_wait(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u)), 0)) {
                 healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE));
@@ -833,7 +833,10 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
         Kv4State<G> st[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) st[nb].take(C, nb);
-        if (!__syncthreads_and(healthy)) break;
+        healthy = __syncthreads_and(healthy);                          // (after a wait that gave up: no number, to the end of the range)
+        if (!healthy)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) st[nb].sum[0] = st[nb].sum[1] = __uint_as_float(0x7FC00000u);
         // in two rounds (rolled: the code of one): warps 2, 3 into 0, 1, then warp 1 into 0
 #pragma unroll 1
         for (int half = KA_WARPS / 2; half > 0; half >>= 1) {

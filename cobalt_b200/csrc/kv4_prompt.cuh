@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     const uint32_t full_mask = 0xFFFFFFFFu;
     const uint32_t s_raw = smem_u32(smem), s0 = (s_raw + 1023u) & ~1023u;
     const uint32_t q_base = s0, k_base = q_base + G * KP_SUB, v_base = k_base + 2 * G * KP_SUB, p_base = v_base + 2 * G * KP_SUB;
-    const uint32_t bars = p_base + 4 * KP_SUB, tmem_slot = bars + 8u * 20u;
+    const uint32_t bars = p_base + 4 * KP_SUB, tmem_slot = bars + 8u * 20u, bar_end = bars + 8u * 21u;
     auto bar_kfull = [&](int s) { return bars + 8u * s; };
     auto bar_kempty = [&](int s) { return bars + 16u + 8u * s; };
     auto bar_vfull = [&](int s) { return bars + 32u + 8u * s; };
@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             mbar_init(bar_sfull(s), 1); mbar_init(bar_sempty(s), KP_SOFTMAX);
             for (int h = 0; h < 2; ++h) { mbar_init(bar_pfull(h, s), 128); mbar_init(bar_pempty(h, s), 1); }
         }
+        mbar_init(bar_end, 1);
         mbar_fence_init();
         no_number = largest[0] = largest[1] = 0u;
         smallest[0] = smallest[1] = 0x7F800000u;
@@ -330,6 +331,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
                     healthy = __all_sync(full_mask, healthy && mbar_wait_bounded(bar_pempty(h, (n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u, status, DEV_TIMEOUT_ACC));
             tc_fence_after();
             stat[half * KP_ROWS + r] = m;
+            if (!healthy) l = __uint_as_float(0x7FC00000u);            // (a wait gave up: no number, in the channels of both halves)
             stat[(2 + half) * KP_ROWS + r] = l;
             asm volatile("bar.sync 1, 480;" ::: "memory");                  // the softmax warps; those that expand have arrived (no_number)
             const float om = stat[(half ^ 1) * KP_ROWS + r], ol = stat[(2 + (half ^ 1)) * KP_ROWS + r];
@@ -337,39 +339,37 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             const float mine = ex2(m - base), other = ex2(om - base);
             const float inv = __uint_as_float((uint32_t)(ex_v - 14 + 127) << 23) / (l * mine + ol * other);
             const float w0 = (half ? other : mine) * inv, w1 = (half ? mine : other) * inv;        // of the contexts of halves 0 and 1
-            if (healthy) {
-                const bool any = range.hi >= 0 && (range.lo <= range.hi || P.sinks > 0);
-                bool nan = false;
-                if (no_number && any) {                                    // a marked group: does this row see one?
-                    const int g = half * (D / 2) / 64;
-                    for (int j = 0; j <= range.hi; ++j) {
-                        if (j < range.lo && j >= P.sinks) { j = range.lo - 1; continue; }
-                        const uint8_t* tile = P.cache.tile(seq, kvh, j, G);
-                        const uint32_t sc = *reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, j % KV4_TILE));
-                        nan |= (sc & 0x7F80u) == 0x7F80u;
-                    }
+            const bool any = range.hi >= 0 && (range.lo <= range.hi || P.sinks > 0);
+            bool nan = !healthy;
+            if (no_number && any && healthy) {                         // a marked group: does this row see one?
+                const int g = half * (D / 2) / 64;
+                for (int j = 0; j <= range.hi; ++j) {
+                    if (j < range.lo && j >= P.sinks) { j = range.lo - 1; continue; }
+                    const uint8_t* tile = P.cache.tile(seq, kvh, j, G);
+                    const uint32_t sc = *reinterpret_cast<const uint16_t*>(tile + kv4_v_scale(G, g, j % KV4_TILE));
+                    nan |= (sc & 0x7F80u) == 0x7F80u;
                 }
+            }
 #pragma unroll 1
-                for (int c0 = 0; c0 < D / 2; c0 += 32) {
-                    uint32_t a[32], b[32];
-                    const uint32_t col = (uint32_t)(half * (D / 2) + c0);
-                    tmem_ld32(tmem_o + my_lanes + col, a);
-                    tmem_ld32(tmem_o + my_lanes + (uint32_t)D + col, b);
-                    tmem_ld_wait();
-                    if (valid) {
-                        uint4* dst = reinterpret_cast<uint4*>(P.out + (((long long)seq * P.T + tok) * P.n_heads + kvh * P.rep + head) * D + col);
+            for (int c0 = 0; c0 < D / 2; c0 += 32) {
+                uint32_t a[32], b[32];
+                const uint32_t col = (uint32_t)(half * (D / 2) + c0);
+                tmem_ld32(tmem_o + my_lanes + col, a);
+                tmem_ld32(tmem_o + my_lanes + (uint32_t)D + col, b);
+                tmem_ld_wait();
+                if (valid) {
+                    uint4* dst = reinterpret_cast<uint4*>(P.out + (((long long)seq * P.T + tok) * P.n_heads + kvh * P.rep + head) * D + col);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t o[4];
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int i = 8 * c + 2 * e;
-                                o[e] = pack_bf16x2(fmaf(__uint_as_float(a[i]), w0, __uint_as_float(b[i]) * w1),
-                                                   fmaf(__uint_as_float(a[i + 1]), w0, __uint_as_float(b[i + 1]) * w1));
-                                o[e] = !any ? 0u : nan ? 0x7FC07FC0u : o[e];
-                            }
-                            dst[c] = make_uint4(o[0], o[1], o[2], o[3]);
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 8 * c + 2 * e;
+                            o[e] = pack_bf16x2(fmaf(__uint_as_float(a[i]), w0, __uint_as_float(b[i]) * w1),
+                                               fmaf(__uint_as_float(a[i + 1]), w0, __uint_as_float(b[i + 1]) * w1));
+                            o[e] = !any ? 0u : nan ? 0x7FC07FC0u : o[e];
                         }
+                        dst[c] = make_uint4(o[0], o[1], o[2], o[3]);
                     }
                 }
             }
@@ -498,6 +498,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
             for (int j = 0; j < n && healthy; ++j) {
                 if (j + 1 < n) issue_scores(j + 1);
                 issue_context(j);
+            }
+            if (!healthy) {                                            // nothing issued may run behind the CTA's end
+                if (elect_one()) umma_commit<false>(bar_end);
+                __syncwarp();
+                mbar_wait_bounded(bar_end, 0u, status, DEV_TIMEOUT_ACC);
             }
         }
     };
