@@ -116,6 +116,8 @@ EXPORTS = {
     "cobalt_kv4_attend_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "cobalt_kv4_attend": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                   c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    "cobalt_kv4_attend_watched": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                          c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cobalt_kv4_status": (c_int, [c_void_p, POINTER(c_uint32)]),
     "cobalt_allreduce_peer": (c_int, [c_void_p, c_int, c_int, c_size_t, c_size_t, c_size_t, c_void_p, c_int, c_void_p,
                                       c_void_p]),

@@ -26,10 +26,13 @@ int sm_count(int* n) {
     *n = sms[dev];
     return COBALT_OK;
 }
-// the status word of the current device (part of the library's image: nothing is allocated)
+// the status word of the current device, for calls without one (part of the library's image: nothing is allocated)
 uint32_t* status_word() {
-    void* p = nullptr;
-    return cudaGetSymbolAddress(&p, g_kv4_status) == cudaSuccess ? (uint32_t*)p : nullptr;
+    static void* words[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return nullptr;
+    if (!words[dev] && cudaGetSymbolAddress(&words[dev], g_kv4_status) != cudaSuccess) return nullptr;
+    return (uint32_t*)words[dev];
 }
 int launched() { return cudaGetLastError() == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH; }
 bool dim_ok(int D) { return D > 0 && D % KV4_GROUP == 0 && D <= KV4_GROUP * KV4_MAX_GROUPS; }
@@ -242,11 +245,18 @@ size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_h
 int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
                       void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks, float scale,
                       void* scratch, size_t scratch_bytes, void* stream) {
+    return cobalt_kv4_attend_watched(q, ld_q, tiles, tiles_seq_stride, positions, pos_seq_stride, out, n_seq, T, n_heads, n_kv_heads, head_dim, n_slots,
+                                     window, sinks, scale, scratch, scratch_bytes, nullptr, stream);
+}
+
+int cobalt_kv4_attend_watched(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions,
+                              int64_t pos_seq_stride, void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window,
+                              int sinks, float scale, void* scratch, size_t scratch_bytes, void* status, void* stream) {
     Kv4AttendParams P = {};
     int rc = make_cache(&P.cache, tiles, tiles_seq_stride, positions, pos_seq_stride, n_seq, T, n_kv_heads, head_dim, n_slots);
     if (rc) return rc;
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || window < 0 || sinks < 0) return COBALT_EINVAL;
-    if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15)) return COBALT_EINVAL;
+    if (!rows_ok(q, ld_q, (int64_t)n_heads * head_dim) || !out || ((uintptr_t)out & 15) || ((uintptr_t)status & 3)) return COBALT_EINVAL;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
     const bool prompt = prompt_takes(n_seq, n_kv_heads, n_heads / n_kv_heads, T, head_dim, n_slots, window, sinks, sms);
@@ -261,6 +271,8 @@ int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t ti
     P.window = window; P.sinks = sinks;
     P.scale_log2 = scale * 1.44269504f;
     P.cols = c.cols; P.col_tiles = c.col_tiles;
+    P.status = status ? (uint32_t*)status : status_word();
+    if (!P.status) return COBALT_ELAUNCH;
     P.by_rep = kv4_div(P.rep); P.by_kv = kv4_div(n_kv_heads);
     if (prompt) return head_dim == 64 ? launch_prompt<1>(P, (cudaStream_t)stream) : launch_prompt<2>(P, (cudaStream_t)stream);
     P.by_tiles = kv4_div(c.col_tiles);
@@ -287,9 +299,11 @@ int cobalt_kv4_status(void* stream, uint32_t* status_out) {
     uint32_t* word = status_word();
     if (!word) return COBALT_ELAUNCH;
     if (cudaMemcpyAsync(status_out, word, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
-    if (cudaMemsetAsync(word, 0, 4, (cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
     if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
-    return *status_out == 0 ? COBALT_OK : COBALT_ETIMEOUT;
+    if (*status_out == 0) return COBALT_OK;
+    // cleared only once it was read as set: kernels write it while it is 0 alone, so a failure on another stream meanwhile is not erased unread
+    if (cudaMemsetAsync(word, 0, 4, (cudaStream_t)stream) != cudaSuccess || cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
+    return COBALT_ETIMEOUT;
 }
 
 }  // extern "C"

@@ -39,6 +39,7 @@ struct Kv4AttendParams {
     float scale_log2;                                                  // scale * log2(e)
     int cols, col_tiles;                                               // rep * T columns per KV head, in tiles of 8 * NB
     Kv4Div by_rep, by_tiles, by_kv;
+    uint32_t* status;                                                  // first bounded wait that gave up
 };
 
 // The slots that a token sees: j <= hi and (j >= lo or j < sinks); hi = -1: none.
@@ -622,7 +623,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
     for (; i < end; i += KA_WARPS) {
         const int s = used % KA_STAGES;
         if (__builtin_expect(!__all_sync(0xFFFFFFFFu, mbar_try_wait(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u)), 0)) {
-            healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE));
+            healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, P.status, DEV_TIMEOUT_TILE));
             if (!healthy) break;
         }
         ++used;
@@ -631,7 +632,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
         fetch();
     }
     for (; used < fetched; ++used)                                     // (after a wait that gave up) no copy may land behind the CTA's end
-        mbar_wait_bounded(bar0 + 8 * (used % KA_STAGES), (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE);
+        mbar_wait_bounded(bar0 + 8 * (used % KA_STAGES), (uint32_t)(used / KA_STAGES) & 1u, P.status, DEV_TIMEOUT_TILE);
     // ---- join: the warps' states over shared memory, warp w the channel pair w of every group; then the CTAs' over the cluster
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -820,7 +821,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
         for (int k = (warp - (i - start)) & (KA_WARPS - 1); k < here && healthy; k += KA_WARPS) {
             const int s = used % KA_STAGES;
             if (__builtin_expect(!__all_sync(0xFFFFFFFFu, mbar_try_wait(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u)), 0)) {
-                healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE));
+                healthy = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar0 + 8 * s, (uint32_t)(used / KA_STAGES) & 1u, P.status, DEV_TIMEOUT_TILE));
                 if (!healthy) break;
             }
             ++used;
@@ -862,7 +863,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_ctas_per_sm(G, NB)) kv4_attend_
         if (i < end) forward(at, here);
     }
     for (; used < fetched; ++used)                                     // (after a wait that gave up) no copy may land behind the CTA's end
-        mbar_wait_bounded(bar0 + 8 * (used % KA_STAGES), (uint32_t)(used / KA_STAGES) & 1u, &g_kv4_status, DEV_TIMEOUT_TILE);
+        mbar_wait_bounded(bar0 + 8 * (used % KA_STAGES), (uint32_t)(used / KA_STAGES) & 1u, P.status, DEV_TIMEOUT_TILE);
 }
 
 // Heads that lie in several CTAs of kv4_attend_list_kernel: block (b, y, z) joins eight columns and a group of channels of the head that begins in

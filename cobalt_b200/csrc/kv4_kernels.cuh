@@ -35,7 +35,7 @@ __device__ __forceinline__ int kv4_k_meta(int G, int g, int slot) { return 2048 
 __device__ __forceinline__ int kv4_v_scale(int G, int g, int slot) { return 2176 * G + (slot * G + g) * 2; }
 __device__ __forceinline__ int kv4_v_zero(int G, int g, int slot) { return 2240 * G + (g * KV4_TILE + slot) * 2; }
 
-__device__ uint32_t g_kv4_status;                                      // first bounded wait that gave up, on this device
+__device__ uint32_t g_kv4_status;                                      // first bounded wait that gave up, on this device, of calls without a word of their own
 
 struct Kv4Cache {
     uint8_t* tiles;

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const Kv4Atte
     auto bar_pfull = [&](int h, int s) { return bars + 96u + 16u * h + 8u * s; };
     auto bar_pempty = [&](int h, int s) { return bars + 128u + 16u * h + 8u * s; };
     float* stat = reinterpret_cast<float*>(smem + (p_base - s_raw));   // (at the end) [half][row] maximum, then [half][row] sum
-    uint32_t* status = &g_kv4_status;
+    uint32_t* status = P.status;
 
     // the longest rows (last tokens of the prompt) first, so that the short ones fill the end of the grid
     const int n_kv = P.cache.n_kv, order = (int)(gridDim.x - 1 - blockIdx.x);

@@ -152,7 +152,8 @@ class CobaltDecoder:
         if attention_sinks < 0 or (attention_sinks and kv_bits != 4):
             raise ValueError("attention_sinks must not be negative, and needs kv_bits = 4")
         self.sinks = int(attention_sinks)
-        self.kv4 = [KVCache4(self.B, nkv, max_ctx, D, device) for _ in range(L)] if kv_bits == 4 else None
+        self.prompt_status = torch.zeros(1, dtype=torch.int32, device=device)          # non-zero: a bounded wait of a prompt's attention (4-bit cache: of any) gave up
+        self.kv4 = [KVCache4(self.B, nkv, max_ctx, D, device, status=self.prompt_status) for _ in range(L)] if kv_bits == 4 else None
         self.k_cache = self.v_cache = None
         if self.kv4 is None:
             self.k_cache = torch.zeros(L, self.B, nkv, max_ctx, D, dtype=torch.bfloat16, device=device)     # [layer][sequence][kv head][slot][D]
@@ -173,7 +174,6 @@ class CobaltDecoder:
         # Rows (tokens of all prompts) that go through the layers together when several sequences are prefilled: the activations of
         # 8192 are a GB or more at the widest MLPs.  The caller may lower it; 0 = one prompt at a time.
         self.prompt_rows = 8192
-        self.prompt_status = torch.zeros(1, dtype=torch.int32, device=device)          # non-zero: a bounded wait gave up
         # One-kernel attention (cooperative launch; its scratch starts zeroed; only while its whole grid fits on the GPU).
         # Off by default: bit-identical to the three kernels but slower inside the decode graph (4-layer 7B-shaped step
         # 0.574 ms against 0.524 ms) - a cooperative launch does not overlap its neighbours.  Set the flag before the
@@ -482,8 +482,6 @@ class CobaltDecoder:
             words += [self.head.device_status(), self.head_f.device_status()]
         if self.reducer is not None:
             words.append(self.reducer.device_status())
-        if getattr(self, "kv4", None) is not None:
-            words.append(self.kv4[0].device_status())
         return max(words)
 
     def _check_prompt_attention(self):
@@ -491,11 +489,8 @@ class CobaltDecoder:
         word = int(self.prompt_status.item())
         if word:
             self.prompt_status.zero_()
-            raise _lib.CobaltError("cobalt_attn_prompt", word, "a bounded wait gave up: the attention of a prompt is incomplete")
-        caches = getattr(self, "kv4", None)
-        word = caches[0].device_status() if caches else 0
-        if word:
-            raise _lib.CobaltError("cobalt_kv4_attend", word, "a bounded wait gave up: an attention over the cache is incomplete")
+            name, what = ("cobalt_attn_prompt", "the attention of a prompt") if getattr(self, "kv4", None) is None else ("cobalt_kv4_attend_watched", "an attention over the cache")
+            raise _lib.CobaltError(name, word, f"a bounded wait gave up: {what} is incomplete")
 
     @torch.no_grad()
     def time_head_ms(self, reps: int = 20) -> float:

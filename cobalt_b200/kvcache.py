@@ -30,22 +30,25 @@ def _attend_scratch(device: int, *sizes: int) -> int:
 
 class KVCache4:
     """Keys and values of ``n_seq`` sequences, ``slots`` positions each, ``n_kv_heads`` heads of ``head_dim`` (64, 128, 192 or 256).
-    ``tiles [n_seq, n_kv_heads, ceil(slots / 32), 36 * head_dim]`` (uint8) is the whole state.
+    ``tiles [n_seq, n_kv_heads, ceil(slots / 32), 36 * head_dim]`` (uint8) is the whole state.  ``status`` (int32 ``[1]``, zero): where
+    ``device_status()`` finds waits that gave up; caches may share one, each has its own by default.
 
     Every method takes ``n`` sequences of ``T`` tokens each, the first of them being sequence ``seq`` of the cache, and int64
     ``positions`` - ``[n, T]``, or ``[T]`` for the same in every sequence - read on the device: a captured graph follows them.  Calls run on
     the current stream of the cache's device."""
 
-    def __init__(self, n_seq: int, n_kv_heads: int, slots: int, head_dim: int, device="cuda"):
+    def __init__(self, n_seq: int, n_kv_heads: int, slots: int, head_dim: int, device="cuda", status: Optional[torch.Tensor] = None):
         if min(n_seq, n_kv_heads, slots) < 1:
             raise ValueError("a cache needs at least one sequence, one KV head and one slot")
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
-        self._install(torch.zeros(n_seq, n_kv_heads, -(-slots // TILE), 36 * head_dim, dtype=torch.uint8, device=device), head_dim, slots)
+        tiles = torch.zeros(n_seq, n_kv_heads, -(-slots // TILE), 36 * head_dim, dtype=torch.uint8, device=device)
+        self._install(tiles, head_dim, slots, torch.zeros(1, dtype=torch.int32, device=device) if status is None else status)
 
     @classmethod
-    def wrap(cls, tiles: torch.Tensor, head_dim: int, slots: Optional[int] = None) -> "KVCache4":
-        """A cache over existing tiles ``[n_seq, n_kv_heads, n_tiles, 36 * head_dim]`` (shared, not copied); the sequences may lie apart."""
+    def wrap(cls, tiles: torch.Tensor, head_dim: int, slots: Optional[int] = None, status: Optional[torch.Tensor] = None) -> "KVCache4":
+        """A cache over existing tiles ``[n_seq, n_kv_heads, n_tiles, 36 * head_dim]`` (shared, not copied); the sequences may lie apart.  Without
+        a ``status`` word it reports to the one of its device, which all such caches share."""
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
         row, shape = 36 * head_dim, tiles.shape
@@ -60,14 +63,18 @@ class KVCache4:
         elif not (n - 1) * TILE < slots <= n * TILE:
             raise ValueError(f"{n} tiles hold {n * TILE} slots, not {slots}")
         obj = cls.__new__(cls)
-        obj._install(tiles, head_dim, slots)
+        obj._install(tiles, head_dim, slots, status)
         return obj
 
-    def _install(self, tiles, head_dim, slots):
+    def _install(self, tiles, head_dim, slots, status):
         self.tiles, self.head_dim, self.slots = tiles, int(head_dim), int(slots)
         self.n_seq, self.n_kv_heads = tiles.shape[0], tiles.shape[1]
         self._index = tiles.get_device()                     # -1: not on a GPU
         self._apart = tiles.stride(0) if self.n_seq > 1 else 0
+        if status is not None and (status.dtype is not torch.int32 or status.shape != (1,) or status.device != tiles.device):
+            raise ValueError(f"status must be int32 [1] on {tiles.device}, got {status.dtype} {list(status.shape)} on {status.device}")
+        self._status = status
+        self._word = None if status is None else status.data_ptr()
         self._lib = _lib.load()
 
     @property
@@ -206,13 +213,18 @@ class KVCache4:
             need = _attend_scratch(self._index, n, T, heads, n_kv, D, self.slots, window, sinks)
             # a buffer per call, from the stream's own pool: calls on other streams and captured graphs never share one
             scratch = q.new_empty(need, dtype=torch.uint8) if need else None
-            self._call("cobalt_kv4_attend", qp, ld_q, tiles, self._apart, pos, stride, out.data_ptr(), n, T, heads, n_kv, D, self.slots, window, sinks,
-                       D ** -0.5 if scale is None else scale, None if scratch is None else scratch.data_ptr(), need)
+            self._call("cobalt_kv4_attend_watched", qp, ld_q, tiles, self._apart, pos, stride, out.data_ptr(), n, T, heads, n_kv, D, self.slots, window, sinks,
+                       D ** -0.5 if scale is None else scale, None if scratch is None else scratch.data_ptr(), need, self._word)
         return out
 
     def device_status(self) -> int:
-        """0, or the code of the first bounded wait of an attention over such caches on this device that gave up since the last
-        question (the results of such a call are not to be used).  Waits for the current stream."""
+        """0, or the code of the first bounded wait of an attention over this cache (and those that share its word) that gave up since the
+        last question; rows that it concerns are NaN.  Waits for the current stream."""
+        if self._status is not None:
+            code = int(self._status.item())
+            if code:                                         # (never cleared unread: kernels write it while it is 0 alone)
+                self._status.zero_()
+            return code
         word = ctypes.c_uint32(0)
         with torch.cuda.device(self.device):
             rc = self._lib.cobalt_kv4_status(_raw_stream(self._index), ctypes.byref(word))

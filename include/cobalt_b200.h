@@ -359,8 +359,10 @@ int cobalt_attn_prompt(const void* q, const void* k_cache, const void* v_cache, 
  *                       j < sinks); one that sees none (p < 0: padding) gets zeros.  Scores, softmax and sums in fp32, one rounding
  *                       at the end.  scratch: cobalt_kv4_attend_scratch_bytes() (0: none needed), 256-byte aligned, contents irrelevant;
  *                       calls that may overlap on the GPU need buffers of their own.
- *   cobalt_kv4_status : 0, or the code of the first bounded wait of an attend call on the current device that gave up since the
- *                       last question (the results of such a call are not to be used).  Synchronises `stream`; not during capture.
+ *   cobalt_kv4_attend_watched : the same with a status word of the caller's (device memory, 4-byte aligned, zeroed by the caller): a bounded wait of the
+ *                       call that gives up leaves its code there while it is 0, and NaN in the rows that it concerns.  NULL: the device's word.
+ *   cobalt_kv4_status : 0, or the code of the first bounded wait that gave up since the last question, of the attend calls on the current
+ *                       device without a word of their own - whosever they are.  Synchronises `stream`; not during capture.
  * The reference holds its cache in bf16 and has no counterpart. */
 size_t cobalt_kv4_tile_bytes(int head_dim);
 int cobalt_kv4_append(const void* k, int64_t ld_k, const void* v, int64_t ld_v, const void* q, int64_t ld_q, void* q_out, int64_t ld_q_out,
@@ -373,6 +375,9 @@ size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_h
 int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
                       void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks, float scale,
                       void* scratch, size_t scratch_bytes, void* stream);
+int cobalt_kv4_attend_watched(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions,
+                              int64_t pos_seq_stride, void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window,
+                              int sinks, float scale, void* scratch, size_t scratch_bytes, void* status, void* stream);
 int cobalt_kv4_status(void* stream, uint32_t* status_out);
 
 /* All-reduce (sum) of the fp32 partial outputs of a row-parallel layer over peer memory, for tensor-parallel decode
