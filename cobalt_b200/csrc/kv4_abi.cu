@@ -55,6 +55,49 @@ int make_cache(Kv4Cache* c, const void* tiles, int64_t seq_stride, const int64_t
 // rows of bf16 that are read 16 bytes at a time
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
 
+// Whether the device places a cluster of sixteen CTAs of a kernel at all (on one whose SMs are shared out it may not); asked once
+template <int G, int NB, bool MANY>
+bool places_sixteen() {
+    static signed char known[MAX_DEVICES];                             // 0: not asked yet
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return false;
+    if (!known[dev]) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2 * KA_MAX_CLUSTER;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * KA_MAX_CLUSTER);
+        cfg.blockDim = dim3(KA_THREADS);
+        cfg.dynamicSmemBytes = ka_heads_smem(G, NB);
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        const bool fits = cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_heads_smem(G, NB)) == cudaSuccess &&
+                          cudaFuncSetAttribute(kv4_attend_heads_kernel<G, NB, MANY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                          cudaOccupancyMaxActiveClusters(&n, kv4_attend_heads_kernel<G, NB, MANY>, &cfg) == cudaSuccess && n > 0;
+        if (!fits) cudaGetLastError();                                 // not the next launch's
+        known[dev] = fits ? 1 : -1;
+    }
+    return known[dev] > 0;
+}
+#define KV4_COLUMNS(G_, NB_, CALL)                                     \
+    switch ((G_) * 10 + (NB_)) {                                       \
+        case 11: { constexpr int G = 1, NB = 1; CALL; } break;         \
+        case 12: { constexpr int G = 1, NB = 2; CALL; } break;         \
+        case 13: { constexpr int G = 1, NB = 3; CALL; } break;         \
+        case 14: { constexpr int G = 1, NB = 4; CALL; } break;         \
+        case 21: { constexpr int G = 2, NB = 1; CALL; } break;         \
+        case 22: { constexpr int G = 2, NB = 2; CALL; } break;         \
+        case 31: { constexpr int G = 3, NB = 1; CALL; } break;         \
+        default: { constexpr int G = 4, NB = 1; CALL; } break;         \
+    }
+bool sixteen_fit(int groups, int nb, bool many) {
+    bool fit = false;
+    KV4_COLUMNS(groups, nb, fit = (many ? places_sixteen<G, NB, true>() : places_sixteen<G, NB, false>()));
+    return fit;
+}
+
 struct AttendCfg {
     int cols, nb, col_tiles;
     bool list;
@@ -88,7 +131,8 @@ int attend_config(int n_seq, int T, int n_heads, int n_kv, int D, int n_slots, i
     const int64_t whole = (n_slots + KV4_TILE - 1) / KV4_TILE;
     int64_t tiles = whole;
     if (window > 0) tiles = std::min(tiles, ((int64_t)window + T) / KV4_TILE + 2 + ((int64_t)sinks + KV4_TILE - 1) / KV4_TILE);
-    const int most = heads <= KA_WIDE_HEADS && tiles > KA_MAX_CLUSTER * KA_WARPS * 4 ? 2 * KA_MAX_CLUSTER : KA_MAX_CLUSTER;
+    const bool wide = heads <= KA_WIDE_HEADS && tiles > KA_MAX_CLUSTER * KA_WARPS * 4 && sixteen_fit(G, c->nb, T > 1);
+    const int most = wide ? 2 * KA_MAX_CLUSTER : KA_MAX_CLUSTER;
     c->share = 1;
     while (c->share < most && c->share * 2 * heads <= ctas && c->share * KA_MIN_TILES < tiles) c->share *= 2;
     c->list = entries <= KA_ENTRIES && heads * whole < 1000000000ll && heads < 4ll * ctas && 
@@ -279,16 +323,7 @@ int cobalt_kv4_attend_watched(const void* q, int64_t ld_q, const void* tiles, in
     Kv4Work W;
     W.partial = (float*)scratch;
     W.joins = (int4*)((uint8_t*)scratch + c.joins_off);
-    switch (head_dim / KV4_GROUP * 10 + c.nb) {
-        case 11: return launch_attend<1, 1>(P, W, c, (cudaStream_t)stream);
-        case 12: return launch_attend<1, 2>(P, W, c, (cudaStream_t)stream);
-        case 13: return launch_attend<1, 3>(P, W, c, (cudaStream_t)stream);
-        case 14: return launch_attend<1, 4>(P, W, c, (cudaStream_t)stream);
-        case 21: return launch_attend<2, 1>(P, W, c, (cudaStream_t)stream);
-        case 22: return launch_attend<2, 2>(P, W, c, (cudaStream_t)stream);
-        case 31: return launch_attend<3, 1>(P, W, c, (cudaStream_t)stream);
-        default: return launch_attend<4, 1>(P, W, c, (cudaStream_t)stream);
-    }
+    KV4_COLUMNS(head_dim / KV4_GROUP, c.nb, return (launch_attend<G, NB>(P, W, c, (cudaStream_t)stream)));
 }
 
 int cobalt_kv4_status(void* stream, uint32_t* status_out) {
