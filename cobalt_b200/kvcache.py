@@ -93,8 +93,7 @@ class KVCache4:
         shape = t.shape
         if not 2 <= len(shape) <= 3 or shape[-1] != width or (lead is not None and shape[:-1] != lead):
             raise ValueError(f"{name} must be [n, T, {width}]{'' if lead is None else ' with [n, T] = ' + str(list(lead))}, got {list(shape)}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} requires a gradient: KVCache4 has no backward pass (use torch.no_grad())")
+        self._no_grad(name, t)
         p = t.data_ptr()
         if p % 16 == 0 and t.is_contiguous():
             return p, width, t
@@ -158,8 +157,8 @@ class KVCache4:
                 self._weight("q_norm", q_norm, torch.bfloat16, D)
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.device != q.device or not q_out.is_contiguous() or q_out.data_ptr() % 16:
-                raise ValueError("q_out must be a contiguous tensor like q on a 16-byte boundary")
+            else:
+                self._result("q_out", q_out, q)
             op = q_out.data_ptr()
         pos, stride, tiles, p_own = self._place(positions, n, T, seq)
         if n * T:
@@ -168,7 +167,18 @@ class KVCache4:
                        None if k_norm is None else k_norm.data_ptr(), eps)
         return q_out
 
+    @staticmethod
+    def _no_grad(name: str, t: torch.Tensor):
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires a gradient: KVCache4 has no backward pass (use torch.no_grad())")
+
+    def _result(self, name: str, t: torch.Tensor, like: torch.Tensor):
+        if t.shape != like.shape or t.dtype is not like.dtype or t.device != like.device or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be a contiguous tensor like q on a 16-byte boundary")
+        self._no_grad(name, t)
+
     def _weight(self, name: str, w: torch.Tensor, dtype, size: int):
+        self._no_grad(name, w)
         if w.dtype is not dtype or w.shape != (size,) or w.get_device() != self._index or not w.is_contiguous() or w.data_ptr() % 4:
             raise ValueError(f"{name} must be a contiguous {dtype} [{size}] on {self.device}")
 
@@ -207,8 +217,8 @@ class KVCache4:
         pos, stride, tiles, p_own = self._place(positions, n, T, seq)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != shape or out.dtype is not q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError("out must be a contiguous tensor like q on a 16-byte boundary")
+        else:
+            self._result("out", out, q)
         if n * T:
             need = _attend_scratch(self._index, n, T, heads, n_kv, D, self.slots, window, sinks)
             # a buffer per call, from the stream's own pool: calls on other streams and captured graphs never share one

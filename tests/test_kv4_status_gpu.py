@@ -38,3 +38,18 @@ def test_healthy_calls_leave_words_alone():
             got = [x.attend(q, pos) for x in (c, watched, device)]
             assert all(torch.equal(got[0], g) for g in got[1:]) and word.tolist() == [value] * 3
         assert watched.device_status() == 7 and word.tolist() == [7, 0, 7] and c.device_status() == 0 and device.device_status() == 0
+
+
+def test_arguments_that_require_a_gradient_are_refused():
+    """Norm weights as parameters of a module, frequencies and results too, not q, k and v alone; under no_grad() they are taken."""
+    c = KVCache4(1, 1, 40, 64)
+    x, pos = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, dtype=torch.long, device="cuda")
+    w, f = torch.nn.Parameter(torch.ones(64, dtype=torch.bfloat16, device="cuda")), torch.ones(32, device="cuda", requires_grad=True)
+    out = torch.zeros_like(x, requires_grad=True)
+    calls = (lambda: c.append(x, x, pos, k_norm=w), lambda: c.append(x, x, pos, q=x, q_norm=w), lambda: c.append(x, x, pos, inv_freq=f),
+             lambda: c.append(x, x, pos, q=x, q_out=out), lambda: c.attend(x, pos, out=out))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            call()
+        with torch.no_grad():
+            call()
