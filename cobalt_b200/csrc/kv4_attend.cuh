@@ -48,7 +48,7 @@ __device__ __forceinline__ Kv4Range kv4_range(const Kv4AttendParams& P, int seq,
     const long long pos = P.positions[seq * P.pos_stride + tok];
     Kv4Range r;
     r.hi = pos < 0 ? -1 : (int)min(pos, (long long)P.cache.n_slots - 1);
-    r.lo = P.window > 0 ? (int)max(0ll, min(pos - P.window + 1, (long long)P.cache.n_slots)) : 0;
+    r.lo = P.window > 0 && pos > 0 ? (int)max(0ll, min(pos - P.window + 1, (long long)P.cache.n_slots)) : 0;
     return r;
 }
 // What a range of tokens sees: the slots between the bounds of all of them, and those between the bounds that bind every one.
