@@ -49,6 +49,7 @@ class CobaltStagedInput(Structure):
 
 IN_PLAIN, IN_GLU, IN_ADDNORM = 0, 1, 2
 ETIMEOUT, EUNSUPPORTED = -5, -7
+KV4_HEADS, KV4_LIST, KV4_PROMPT = 0, 1, 2            # cobalt_kv4_attend_form()
 
 
 class CobaltError(RuntimeError):
@@ -113,6 +114,7 @@ EXPORTS = {
     "cobalt_kv4_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                   c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p]),
     "cobalt_kv4_read": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "cobalt_kv4_attend_form": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "cobalt_kv4_attend_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "cobalt_kv4_attend": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                   c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),

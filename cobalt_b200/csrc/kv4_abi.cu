@@ -286,6 +286,17 @@ size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_h
     return attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c) ? 0 : c.scratch;
 }
 
+int cobalt_kv4_attend_form(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks) {
+    if (n_seq <= 0 || T <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || n_slots <= 0 || window < 0 || sinks < 0 || !dim_ok(head_dim))
+        return COBALT_EINVAL;
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    if (prompt_takes(n_seq, n_kv_heads, n_heads / n_kv_heads, T, head_dim, n_slots, window, sinks, sms)) return COBALT_KV4_PROMPT;
+    AttendCfg c;
+    if ((rc = attend_config(n_seq, T, n_heads, n_kv_heads, head_dim, n_slots, window, sinks, sms, &c))) return rc;
+    return c.list ? COBALT_KV4_LIST : COBALT_KV4_HEADS;
+}
+
 int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
                       void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks, float scale,
                       void* scratch, size_t scratch_bytes, void* stream) {

@@ -359,6 +359,8 @@ int cobalt_attn_prompt(const void* q, const void* k_cache, const void* v_cache, 
  *                       j < sinks); one that sees none (p < 0: padding) gets zeros.  Scores, softmax and sums in fp32, one rounding
  *                       at the end.  scratch: cobalt_kv4_attend_scratch_bytes() (0: none needed), 256-byte aligned, contents irrelevant;
  *                       calls that may overlap on the GPU need buffers of their own.
+ *   cobalt_kv4_attend_form : which kernel a call of these sizes takes on the current device: COBALT_KV4_HEADS (a cluster per head), COBALT_KV4_LIST (all tiles
+ *                       in equal ranges, with scratch) or COBALT_KV4_PROMPT; negative: an error.
  *   cobalt_kv4_attend_watched : the same with a status word of the caller's (device memory, 4-byte aligned, zeroed by the caller): a bounded wait of the
  *                       call that gives up leaves its code there while it is 0, and NaN in the rows that it concerns.  NULL: the device's word.
  *   cobalt_kv4_status : 0, or the code of the first bounded wait that gave up since the last question, of the attend calls on the current
@@ -371,6 +373,10 @@ int cobalt_kv4_append(const void* k, int64_t ld_k, const void* v, int64_t ld_v, 
                       void* stream);
 int cobalt_kv4_read(const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride, void* k, void* v, int n_seq,
                     int T, int n_kv_heads, int head_dim, int n_slots, void* stream);
+#define COBALT_KV4_HEADS  0
+#define COBALT_KV4_LIST   1
+#define COBALT_KV4_PROMPT 2
+int cobalt_kv4_attend_form(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks);
 size_t cobalt_kv4_attend_scratch_bytes(int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks);
 int cobalt_kv4_attend(const void* q, int64_t ld_q, const void* tiles, int64_t tiles_seq_stride, const int64_t* positions, int64_t pos_seq_stride,
                       void* out, int n_seq, int T, int n_heads, int n_kv_heads, int head_dim, int n_slots, int window, int sinks, float scale,

@@ -112,12 +112,8 @@ def spread(q, k, v, positions, slots, n_heads, scale, window=0, sinks=0):
     return out.view(n, T, -1), even.view(n, T, -1)
 
 
-def kernels(call):
-    """Names of the attention kernels of the 4-bit cache that a call launches, and what it returns."""
-    import re
-    from torch.profiler import ProfilerActivity, profile
-    with profile(activities=[ProfilerActivity.CUDA]) as prof:
-        out = call()
-        torch.cuda.synchronize()
-    names = " ".join(e.key for e in prof.key_averages())
-    return set(re.findall(r"kv4_(attend_heads|attend_list|combine|prompt)_kernel", names)), out
+def form(cache, n, T, heads, window=0, sinks=0):
+    """Which kernel an attention call takes (``_lib.KV4_HEADS``, ``KV4_LIST`` or ``KV4_PROMPT``)."""
+    from cobalt_b200 import _lib
+    with torch.cuda.device(cache.device):
+        return _lib.load().cobalt_kv4_attend_form(n, T, heads, cache.n_kv_heads, cache.head_dim, cache.slots, window, sinks)

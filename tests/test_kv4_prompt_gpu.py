@@ -20,7 +20,7 @@ import pytest
 import torch
 
 import kv4_reference as R
-from cobalt_b200 import KVCache4
+from cobalt_b200 import KVCache4, _lib
 from test_kv4_gpu import copy_slots, filled, randn
 
 pytestmark = pytest.mark.gpu
@@ -29,9 +29,8 @@ FP16, BF16 = 2.0 ** -11, 2.0 ** -8
 
 
 def attend_prompt(c, q, pos, **kw):
-    took, got = R.kernels(lambda: c.attend(q, pos, **kw))
-    assert took == {"prompt"}
-    return got
+    assert R.form(c, *q.shape[:2], q.shape[2] // c.head_dim, kw.get("window", 0), kw.get("sinks", 0)) == _lib.KV4_PROMPT
+    return c.attend(q, pos, **kw)
 
 
 def assert_near(got, q, k, v, pos, slots, heads, scale, window=0, sinks=0, e=FP16, rows=None):
@@ -276,7 +275,8 @@ def test_captured_and_replayed_with_other_positions(D):
     def once(cache):
         return cache.attend(cache.append(k, v, pos, q=q, inv_freq=inv), pos, window=200, sinks=4)
 
-    assert R.kernels(lambda: once(c))[0] == {"prompt"}
+    assert R.form(c, 2, T, heads, 200, 4) == _lib.KV4_PROMPT
+    once(c)
     graphs, outs = [], []
     for _ in range(2):
         g = torch.cuda.CUDAGraph()
@@ -329,8 +329,8 @@ def test_prompts_of_a_decoder():
 
     chk = Checked(cfg, dec.lin, dec.P, 400, dec.dev, batch=2, kv_bits=4)
     ids = torch.randint(0, 1000, (2, 330), generator=torch.Generator().manual_seed(1))
-    took, want = R.kernels(lambda: dec.prefill(ids))
-    assert took == {"prompt"} and torch.equal(chk.prefill(ids), want) and checked == [0, 1]
+    assert R.form(dec.kv4[0], 2, 330, 32) == _lib.KV4_PROMPT                          # both prompts together
+    assert torch.equal(chk.prefill(ids), dec.prefill(ids)) and checked == [0, 1]
 
 
 # ----------------------------------------------------------------------------- magnitudes far apart

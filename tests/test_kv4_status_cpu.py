@@ -1,4 +1,4 @@
-"""Status words of the 4-bit KV cache, what needs no GPU."""
+"""Status words and forms of attention calls of the 4-bit KV cache, what needs no GPU."""
 import pytest
 import torch
 
@@ -33,3 +33,11 @@ def test_every_cache_has_a_word_of_its_own_or_the_one_it_is_given():
             KVCache4(1, 1, 40, 64, device="cpu", status=bad)
         with pytest.raises(ValueError):
             KVCache4.wrap(a.tiles, 64, 40, status=bad)
+
+
+def test_form_refuses(lib):
+    good = (1, 1, 8, 2, 128, 64, 0, 0)
+    for i, bad in ((0, 0), (1, 0), (2, 7), (3, 0), (4, 96), (5, 0), (6, -1), (7, -1)):
+        assert lib.cobalt_kv4_attend_form(*good[:i], bad, *good[i + 1:]) == -1
+    if not torch.cuda.is_available():
+        assert lib.cobalt_kv4_attend_form(*good) < 0 and lib.cobalt_kv4_attend_scratch_bytes(*good) == 0      # no device to plan for
