@@ -11,7 +11,9 @@
 // the last sum through the tensor core too (z is an fp16 operand), so that both sums carry the same rounded weights: with many
 // slots of nearly equal weight they cancel down to the mean, and a rounding of one alone would show.
 // Queries are scaled by a power of two into the upper range of fp16, which holds every bf16 significand; so are the weights P s, by
-// the largest scale seen so far: fp16 weights (2^-11), everything else fp32.  With several tokens (MANY) every column has a power of its own per
+// the largest scale seen so far: fp16 weights (2^-11).  Everything else is fp32 as the tensor core adds it, which cuts each product of a step of 16
+// at a quarter of the last place of its running sum: over 80 steps of nearly equal weight (16 sequences of 15000 to 32768 slots) the result's error
+// is 1.81e-3 where its own rounding gives 1.65e-3, over a few steps 1.65e-3 to 1.70e-3.  With several tokens (MANY) every column has a power of its own per
 // group, as a slot that one token sees and another does not would else cost the other its bits (five tokens, 16 / 4 heads of 64, 8 sequences of
 // 700 to 6000 slots 14.1 -> 14.5 us; 40 tokens, 4 of 300 to 2000 18.0 -> 19.4 us).  A running maximum per column, moved only when a score
 // exceeds it by 2^8 (fp16 weights have that room), keeps the rescaling of O out of the loop.

@@ -22,13 +22,14 @@
 // A slot that only some rows see has to stay out of the others' products even where its values are not numbers: such groups are
 // expanded to zeros and marked, and marked CTAs look through the scales of their rows' slots once at the end.
 //
-// Bound: the latency of instructions at 16 warps an SM (1.7 a clock; no pipe above 40 %).  A unit of expansion takes 1440 clocks, so the 16 units
-// of a tile of 128 channels 3300 on seven warps; softmax takes 2000 a tile beside it, the tensor pipe 1000.  2048 tokens, 32 / 8 heads of 128:
-// 100 us; 2 x 500 tokens with a window of 1024 over 6000 slots, 32 / 16 heads: 69 us (the kernel of few rows: 248 and 138 us).
+// Bound: the latency of instructions at 16 warps an SM (1.9 a clock; ALU 47 %, tensor and XU 15 to 18 %).  A unit of expansion takes 1440 clocks, so the
+// 16 units of a tile of 128 channels 3300 on seven warps; softmax takes 2000 a tile beside it, the tensor pipe 1000.  2048 tokens, 32 / 8 heads
+// of 128: 102.7 us; 2 x 500 tokens with a window of 1024 over 6000 slots, 32 / 16 heads: 70.6 us (the kernel of few rows: 248 and 138 us).
 // Steps: a lane per eight channels with scale, zero and visibility for each word 166 us; whole rows per lane, ten operations a word, maxima of raw
-// scores 113 us; no branch per word, so that words overlap 97 us; fp16 operands 102 us, two codes per fused multiply-add 101 us, loads of the start together 100 us; codes at bits that keep a constant's
-// rounding below 2^-12 of a step, two shifts a word more, 100.6 us.  Eleven
-// expanding warps at 72 registers (softmax 128) slowed the softmax by 30 % and gained nothing.
+// scores 113 us; no branch per word, so that words overlap 97 us; fp16 operands 102 us, two codes per fused multiply-add 101 us, loads of the start
+// together 100 us.  Codes at bits that keep a constant's rounding below 2^-12 of a step, two shifts a word more, 100.6 us; a second copy of the roles
+// for large scores 101.6 us, for magnitudes far apart 102.4 us.  Eleven expanding warps at 72 registers (softmax 128) slowed the softmax by
+// 30 % and gained nothing.
 #pragma once
 #include "kv4_attend.cuh"
 #include "tcgen05.cuh"

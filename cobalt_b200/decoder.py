@@ -128,8 +128,8 @@ class CobaltDecoder:
     embedding / norms / lm_head.  ``head`` (optional) is the head as a compressed module - group-128 RTN without a mask,
     the reference's recipe for the tied embedding / head (src/cobaltkernel/pack_cobalt.py:375-386, 538-558); with tensor
     parallelism it holds this rank's slice of the vocabulary and the logits are gathered over the ranks.  ``kv_bits = 4`` keeps keys and
-    values in 4 bits (``kvcache.KVCache4``, one per layer): 9/32 of the memory, attention in fp32 without the spec's roundings of scores and
-    probabilities, and sums whose order may depend on how many sequences run together.  ``attention_sinks`` (4-bit caches only): in
+    values in 4 bits (``kvcache.KVCache4``, one per layer): 9/32 of the memory, scores and softmax in fp32 without the spec's roundings (weights are
+    fp16), and sums whose order may depend on how many sequences run together.  ``attention_sinks`` (4-bit caches only): in
     sliding-window layers that many first slots stay visible."""
 
     kv4, sinks = None, 0
@@ -523,7 +523,8 @@ class CobaltDecoder:
 
     def _prompts_at_once(self, T: int) -> int:
         """How many sequences' prompts of ``T`` tokens run through the layers together: weights are expanded once for all of them.
-        Every row's sums are added as if its sequence ran alone (``sum_tokens``), so the logits do not depend on it.  Up to
+        Every row's sums are added as if its sequence ran alone (``sum_tokens``), so the logits do not depend on it (but for the order
+        of sums over a 4-bit cache).  Up to
         ``prompt_rows`` rows; prompts that the decode GEMV takes, tensor parallelism, head widths without the prompt kernel
         and modules whose call runs more than their kernel go one by one."""
         if self.world > 1 or T <= 16 or not self.prompt_kernel or self.fused_prompt_attention or self.B == 1:
@@ -583,7 +584,7 @@ class CobaltDecoder:
             try:
                 parts = [self._forward_prompts(ids2[b:b + at_once], pos, b) for b in range(0, n, at_once)]
                 logits = parts[0] if len(parts) == 1 else torch.cat(parts)
-            except torch.cuda.OutOfMemoryError:              # one at a time needs less, and writes the same bits over what is in the caches
+            except torch.cuda.OutOfMemoryError:              # one at a time needs less, and writes the same again over what is in the caches (4-bit ones: to within the order of sums)
                 parts = None
         if logits is None:
             parts = [self._forward(ids2[b], pos, T, seq=b) for b in range(n)]              # [1, T, V] each
