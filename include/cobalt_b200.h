@@ -359,6 +359,7 @@ int cobalt_attn_prompt(const void* q, const void* k_cache, const void* v_cache, 
  *                       j < sinks); one that sees none (p < 0: padding) gets zeros.  Scores, softmax and sums in fp32 (|q| below
  *                       2^118; 2^8 times the slots times the largest |v| below 2^128); weights, and a prompt's keys and values, are rounded to
  *                       fp16 on the way, or to bf16 where the groups of a prompt's visible slots lie more than 2^20 apart; the result to bf16.
+ *                       Scores beyond 2^22 (times log2(e)) that differ by less than their fp32 rounding may get any share of their weight.
  *                       What no token of the call sees may hold anything.  scratch: cobalt_kv4_attend_scratch_bytes() (0: none needed), 256-byte aligned, contents irrelevant;
  *                       calls that may overlap on the GPU need buffers of their own.
  *   cobalt_kv4_attend_form : which kernel a call of these sizes takes on the current device: COBALT_KV4_HEADS (a cluster per head), COBALT_KV4_LIST (all tiles
