@@ -121,6 +121,16 @@ EXPORTS = {
     "cobalt_kv4_attend_watched": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                           c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cobalt_kv4_status": (c_int, [c_void_p, POINTER(c_uint32)]),
+    "cobalt_embed": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_float, c_void_p, c_int64, c_void_p]),
+    "cobalt_embed_grad_scratch_bytes": (c_size_t, [c_int64, c_int]),
+    "cobalt_embed_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cobalt_head_loss_scratch_bytes": (c_size_t, [c_int, c_int, c_int64]),
+    "cobalt_head_loss": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                 c_size_t, c_void_p, c_void_p]),
+    "cobalt_head_loss_grad_scratch_bytes": (c_size_t, [c_int, c_int, c_int64, c_int]),
+    "cobalt_head_loss_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int64, c_void_p,
+                                      c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "cobalt_vocab_status": (c_int, [c_void_p, POINTER(c_uint32)]),
     "cobalt_allreduce_peer": (c_int, [c_void_p, c_int, c_int, c_size_t, c_size_t, c_size_t, c_void_p, c_int, c_void_p,
                                       c_void_p]),
     "cobalt_device_status": (c_int, [c_void_p, c_void_p, POINTER(c_uint32)]),

@@ -96,23 +96,6 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
-// arrival on a barrier of another CTA of the cluster; releases this thread's (and, after a __syncwarp, its warp's) writes to the shared
-// memory of its own CTA
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("fence.release.sync_restrict::shared::cta.cluster;\n\tmbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// 2-D tiled TMA load (no multicast): box of the tensor map at (x = column, y = token) -> this CTA's shared memory; the pair
-// form may count its bytes on a barrier of either CTA of the pair
-template <bool PAIR>
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    if (PAIR)
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
-
 // What a thread needs to expand 64 columns of its row; requested one group ahead.  The rows of a warp lie about 128 bytes
 // apart in the code stream, so every load touches 32 lines whatever its width: the up to 256 bits come in as aligned
 // 16-byte chunks (only those that hold survivors of these columns) and the words are picked out of registers.  With one

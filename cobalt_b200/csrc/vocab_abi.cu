@@ -1,0 +1,406 @@
+// C ABI of the operators at the ends of a vocabulary: embedding lookup and head loss, with their gradients.  See include/cobalt_b200.h.
+#include <algorithm>
+
+#include "embed_kernels.cuh"
+#include "head_loss.cuh"
+
+using namespace cb;
+
+namespace {
+
+constexpr int MAX_DEVICES = 64;
+
+__device__ uint32_t g_vocab_status;
+
+int sm_count(int* n) {
+    static int sms[MAX_DEVICES], major[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
+    if (dev < 0 || dev >= MAX_DEVICES) return COBALT_EINVAL;
+    if (!sms[dev]) {
+        if (cudaDeviceGetAttribute(&major[dev], cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return COBALT_ELAUNCH;
+        int count = 0;
+        if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return COBALT_ELAUNCH;
+        sms[dev] = count;
+    }
+    if (major[dev] != 10) return COBALT_EARCH;
+    *n = sms[dev];
+    return COBALT_OK;
+}
+// the status word of the current device (part of the library's image: nothing is allocated)
+uint32_t* status_word() {
+    static void* words[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return nullptr;
+    if (!words[dev] && cudaGetSymbolAddress(&words[dev], g_vocab_status) != cudaSuccess) return nullptr;
+    return (uint32_t*)words[dev];
+}
+int launched() { return cudaGetLastError() == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH; }
+template <typename A, typename B>
+auto ceil_div(A a, B b) { return (a + b - 1) / b; }
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+// bytes of a value of a type of the embedding calls, 0: no such type
+int type_bytes(int type) { return type == COBALT_FP32 ? 4 : type == COBALT_FP16 || type == COBALT_BF16 ? 2 : 0; }
+// Calls CALL with T, the type as it lies in memory, and N, the values of a 16-byte pack (1: rows do not lie on 16-byte boundaries)
+#define EMBED_DISPATCH(TYPE, PACKED, CALL)                                                   \
+    if ((TYPE) == COBALT_FP32) { using T = float; if (PACKED) { constexpr int N = 4; CALL; } else { constexpr int N = 1; CALL; } } \
+    else if ((TYPE) == COBALT_FP16) { using T = Fp16; if (PACKED) { constexpr int N = 8; CALL; } else { constexpr int N = 1; CALL; } } \
+    else { using T = Bf16; if (PACKED) { constexpr int N = 8; CALL; } else { constexpr int N = 1; CALL; } }
+
+struct EmbedGradScratch {
+    int blocks, tiles;
+    size_t block_ids, block_pos, ids, pos, part, bytes;
+};
+EmbedGradScratch embed_grad_scratch(int64_t n, int width) {
+    EmbedGradScratch s = {};
+    s.blocks = (int)ceil_div(n, EG_BLOCK);
+    s.tiles = (int)ceil_div(n, EG_TILE);
+    const size_t list = align256((size_t)s.blocks * EG_BLOCK * 4);
+    s.block_ids = 0;
+    s.block_pos = list;
+    s.ids = s.blocks > 1 ? 2 * list : s.block_ids;
+    s.pos = s.blocks > 1 ? 3 * list : s.block_pos;
+    s.part = (s.blocks > 1 ? 4 : 2) * list;
+    s.bytes = s.part + (s.tiles > 1 ? align256((size_t)s.tiles * 2 * width * 4) : 0);
+    return s;
+}
+constexpr int64_t EMBED_MAX_TOKENS = 1 << 24;
+
+// ----------------------------------------------------------------------------- head loss
+constexpr int HEAD_MAX_TOKENS = 1 << 20, HEAD_MAX_HIDDEN = 1 << 16;
+constexpr int HEAD_STATS_TOKENS = 16384;               // tokens whose tile statistics are held at once (8 bytes for 128 columns)
+constexpr size_t HEAD_PIECE_BYTES = (size_t)256 << 20;
+
+typedef CUresult (*TensorMapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                      const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// bf16 [rows][cols], row stride ld elements: boxes of 64 x 64, 128-byte swizzle, zeros outside.  Encoding is a driver call and needs the device's context
+// on this thread, which a thread that has launched nothing yet (autograd's) does not have: cudaSetDevice() of the current device sees to it.
+int make_map(CUtensorMap* map, const void* p, int64_t ld, int64_t rows, int64_t cols) {
+    static TensorMapEncodeFn encode = nullptr;
+    if (!encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return COBALT_ELAUNCH;
+        encode = (TensorMapEncodeFn)fn;
+    }
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return COBALT_ELAUNCH;
+    const cuuint64_t dim[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64, 64}, one[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? COBALT_OK : COBALT_EINVAL;
+}
+
+bool head_rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
+int head_sizes(int n, int hidden, int64_t vocab) {
+    if (n <= 0 || hidden <= 0 || hidden % 8 || vocab <= 0) return COBALT_EINVAL;
+    if (n > HEAD_MAX_TOKENS || hidden > HEAD_MAX_HIDDEN || vocab > 0x7FFFF000ll) return COBALT_ETOOBIG;
+    return COBALT_OK;
+}
+
+struct HeadScratch {
+    int piece, pieces, splits, stats_tokens;
+    size_t count, slot, target, at, row, packed, part, slab, d[2], bytes;
+};
+HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool want_x, int sms) {
+    HeadScratch s = {};
+    const size_t rows = (size_t)ceil_div(n, HL_TILE) * HL_TILE;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t p = at; at += align256(bytes); return p; };
+    s.count = take(256);
+    s.slot = take((size_t)n * 4);
+    s.target = take((size_t)n * 4);
+    s.packed = take((size_t)n * hidden * 2);
+    if (!backward) {
+        s.stats_tokens = (int)std::min<size_t>(rows, HEAD_STATS_TOKENS);
+        s.at = take((size_t)n * 4);
+        s.part = take((size_t)ceil_div(vocab, HL_TILE) * 2 * s.stats_tokens * 8);
+    } else {
+        s.row = take((size_t)n * 16);
+        // pieces of equal size, each within HEAD_PIECE_BYTES of scratch
+        const int64_t most = std::max<int64_t>(HEAD_PIECE_BYTES / 2 / rows / HL_TILE * HL_TILE, HL_TILE);
+        s.pieces = (int)ceil_div(vocab, most);
+        s.piece = (int)(ceil_div(ceil_div(vocab, s.pieces), HL_TILE) * HL_TILE);
+        s.pieces = (int)ceil_div(vocab, s.piece);
+        for (int b = 0; b < 2; ++b) s.d[b] = b < s.pieces ? take(rows * s.piece * 2) : s.d[0];
+        if (want_x) {
+            const int64_t tiles = (int64_t)(rows / HL_TILE) * ceil_div(hidden, HL_TILE);
+            s.splits = (int)std::min<int64_t>(std::max<int64_t>(sms / tiles, 1), std::max(s.piece / 512, 1));
+            s.slab = take((size_t)s.splits * n * hidden * 4);
+        }
+    }
+    s.bytes = at;
+    return s;
+}
+
+int prepare(const HlPrepareParams& in, cudaStream_t st) {
+    HlPrepareParams P = in;
+    P.per_block = std::max((int)ceil_div(P.n, 1024), 4);
+    head_prepare_kernel<<<ceil_div(P.n, P.per_block), HL_PREP_THREADS, 0, st>>>(P);
+    return launched();
+}
+int product(const HlParams& P, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& d0, const CUtensorMap& d1, int64_t tiles, int sms, cudaStream_t st) {
+    static bool configured[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(head_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)HL_SMEM) != cudaSuccess) return COBALT_ELAUNCH;
+        configured[dev] = true;
+    }
+    if (tiles > 0x3FFFFFFF) return COBALT_ETOOBIG;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
+    cfg.blockDim = dim3(HL_THREADS);
+    cfg.dynamicSmemBytes = HL_SMEM;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, head_product_kernel, P, x, w, d0, d1) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out, int64_t ld_out,
+                 void* stream) {
+    const int size = type_bytes(type);
+    if (!ids || !table || !out || !size || n <= 0 || n_rows <= 0 || width <= 0 || ld < width || ld_out < width) return COBALT_EINVAL;
+    if (((uintptr_t)ids & 7) || (((uintptr_t)table | (uintptr_t)out) & (size - 1))) return COBALT_EINVAL;
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc) return rc;
+    const bool packed = !(((uintptr_t)table | (uintptr_t)out | (uintptr_t)(ld * size) | (uintptr_t)(ld_out * size) | (uintptr_t)((int64_t)width * size)) & 15);
+    EmbedParams P;
+    P.ids = (const long long*)ids;
+    P.table = table; P.out = out;
+    P.n = n; P.ld = ld; P.ld_out = ld_out; P.n_rows = n_rows;
+    P.chunks = packed ? width * size / 16 : width;
+    P.threads_per_row = 8;
+    while (P.threads_per_row < EMB_THREADS && 4 * P.threads_per_row < P.chunks) P.threads_per_row *= 2;
+    P.scale = scale;
+    P.plain = scale == 1.0f;
+    const int64_t blocks = ceil_div(n, EMB_THREADS / P.threads_per_row);
+    if (blocks > 0x7FFFFFFFll) return COBALT_ETOOBIG;
+    EMBED_DISPATCH(type, packed, (embed_kernel<T, N><<<(unsigned)blocks, EMB_THREADS, 0, (cudaStream_t)stream>>>(P)));
+    return launched();
+}
+
+size_t cobalt_embed_grad_scratch_bytes(int64_t n, int width) {
+    return n <= 0 || n > EMBED_MAX_TOKENS || width <= 0 ? 0 : embed_grad_scratch(n, width).bytes;
+}
+
+int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out, void* scratch,
+                      size_t scratch_bytes, void* stream) {
+    const int size = type_bytes(type);
+    if (!ids || !grad || !out || !size || n <= 0 || n_rows <= 0 || width <= 0 || ld < width) return COBALT_EINVAL;
+    if (((uintptr_t)ids & 7) || ((uintptr_t)grad & (size - 1)) || ((uintptr_t)out & 15)) return COBALT_EINVAL;
+    if (n > EMBED_MAX_TOKENS || n_rows > 0x7FFFFFFFll) return COBALT_ETOOBIG;
+    const EmbedGradScratch s = embed_grad_scratch(n, width);
+    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
+    int sms = 0;
+    int rc = sm_count(&sms);
+    if (rc) return rc;
+    uint8_t* base = (uint8_t*)scratch;
+    EmbedGradParams P;
+    P.ids = (const long long*)ids;
+    P.grad = grad; P.out = out;
+    P.n = n; P.ld = ld; P.n_rows = n_rows;
+    P.width = width; P.blocks = s.blocks; P.tiles = s.tiles;
+    P.scale = scale;
+    P.block_ids = (uint32_t*)(base + s.block_ids);
+    P.block_pos = (uint32_t*)(base + s.block_pos);
+    P.ids_sorted = (uint32_t*)(base + s.ids);
+    P.pos_sorted = (uint32_t*)(base + s.pos);
+    P.part = (float*)(base + s.part);
+    cudaStream_t st = (cudaStream_t)stream;
+    const int64_t out_bytes = n_rows * width * size;
+    const int zeros = (int)std::min<int64_t>(ceil_div(out_bytes, 16 * EG_SORT_THREADS), 2 * sms);
+    embed_grad_sort_kernel<<<s.blocks + zeros, EG_SORT_THREADS, 0, st>>>(P, out_bytes);
+    if ((rc = launched())) return rc;
+    if (s.blocks > 1) {
+        embed_grad_place_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(P);
+        if ((rc = launched())) return rc;
+    }
+    const bool packed = !(((uintptr_t)grad | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)width * size)) & 15);
+    const int per_block = EG_SUM_THREADS * (packed ? 16 / size : 1);
+    if (ceil_div(width, per_block) > 65535) return COBALT_ETOOBIG;
+    EMBED_DISPATCH(type, packed, (embed_grad_sum_kernel<T, N><<<dim3((unsigned)s.tiles, (unsigned)ceil_div(width, per_block)), EG_SUM_THREADS, 0, st>>>(P)));
+    if ((rc = launched())) return rc;
+    if (s.tiles > 1) {
+        const dim3 grid((unsigned)s.tiles, (unsigned)ceil_div(width, 128));
+        if (type == COBALT_FP32) embed_grad_join_kernel<float><<<grid, 256, 0, st>>>(P);
+        else if (type == COBALT_FP16) embed_grad_join_kernel<Fp16><<<grid, 256, 0, st>>>(P);
+        else embed_grad_join_kernel<Bf16><<<grid, 256, 0, st>>>(P);
+    }
+    return launched();
+}
+
+size_t cobalt_head_loss_scratch_bytes(int n, int hidden, int64_t vocab) {
+    return head_sizes(n, hidden, vocab) ? 0 : head_scratch(n, hidden, vocab, false, false, 0).bytes;
+}
+
+int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, int n, int hidden, int64_t vocab, float* loss,
+                     float* stats, float* total, int mean, void* scratch, size_t scratch_bytes, void* status, void* stream) {
+    int rc = head_sizes(n, hidden, vocab);
+    if (rc) return rc;
+    if (!head_rows_ok(x, ldx, hidden) || !head_rows_ok(weight, ldw, hidden) || !targets || !loss) return COBALT_EINVAL;
+    if (((uintptr_t)targets & 7) || (((uintptr_t)loss | (uintptr_t)total) & 3) || ((uintptr_t)stats & 7) || ((uintptr_t)status & 3)) return COBALT_EINVAL;
+    const HeadScratch s = head_scratch(n, hidden, vocab, false, false, 0);
+    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
+    int sms = 0;
+    if ((rc = sm_count(&sms))) return rc;
+    uint8_t* base = (uint8_t*)scratch;
+    cudaStream_t st = (cudaStream_t)stream;
+    HlPrepareParams A = {};
+    A.x = (const uint16_t*)x; A.ldx = ldx;
+    A.targets = (const long long*)targets;
+    A.n = n; A.hidden = hidden; A.vocab = vocab;
+    A.count = (int*)(base + s.count);
+    A.slot = (int*)(base + s.slot);
+    A.target = (int*)(base + s.target);
+    A.packed = (uint16_t*)(base + s.packed);
+    HlParams P = {};
+    P.status = status ? (uint32_t*)status : status_word();
+    if (!P.status) return COBALT_ELAUNCH;
+    CUtensorMap xm, wm;
+    if ((rc = make_map(&xm, A.packed, hidden, n, hidden)) || (rc = make_map(&wm, weight, ldw, vocab, hidden))) return rc;
+    if ((rc = prepare(A, st))) return rc;
+    const int v_tiles = (int)ceil_div(vocab, HL_TILE);
+    P.n_jobs = 1;
+    P.job[0].kind = HL_STATS;
+    P.job[0].cols = (int)vocab;
+    P.job[0].n_tiles = v_tiles;
+    P.job[0].splits = 1;
+    P.count = A.count;
+    P.n_rows = n; P.hidden = hidden;
+    P.target = A.target;
+    P.part = (float2*)(base + s.part);
+    P.at = (float*)(base + s.at);
+    P.ld_part = s.stats_tokens;
+    HlJoinParams J = {};
+    J.part = P.part; J.at = P.at; J.slot = A.slot; J.count = A.count;
+    J.n = n; J.parts = 2 * v_tiles; J.ld_part = P.ld_part;
+    J.loss = loss; J.stats = (float2*)stats; J.mean = mean;
+    for (int tok0 = 0; tok0 < n; tok0 += s.stats_tokens) {
+        J.tok0 = P.tok0 = tok0;
+        J.tokens = std::min(n - tok0, s.stats_tokens);
+        P.tok_tiles = ceil_div(J.tokens, HL_TILE);
+        J.total = tok0 + s.stats_tokens >= n ? total : nullptr;
+        if ((rc = product(P, xm, wm, xm, xm, (int64_t)P.tok_tiles * v_tiles, sms, st))) return rc;
+        head_join_kernel<<<ceil_div(n, HL_JOIN_TOKENS), HL_JOIN_THREADS, 0, st>>>(J);
+        if ((rc = launched())) return rc;
+    }
+    return COBALT_OK;
+}
+
+size_t cobalt_head_loss_grad_scratch_bytes(int n, int hidden, int64_t vocab, int want_x) {
+    int sms = 0;
+    return head_sizes(n, hidden, vocab) || sm_count(&sms) ? 0 : head_scratch(n, hidden, vocab, true, want_x != 0, sms).bytes;
+}
+
+int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, const float* stats, const float* grad,
+                          int64_t grad_step, int mean, int n, int hidden, int64_t vocab, void* dx, int64_t ld_dx, void* dw, int64_t ld_dw, void* scratch,
+                          size_t scratch_bytes, void* status, void* stream) {
+    int rc = head_sizes(n, hidden, vocab);
+    if (rc) return rc;
+    if (!head_rows_ok(x, ldx, hidden) || !head_rows_ok(weight, ldw, hidden) || !targets || !stats || !grad || (!dx && !dw)) return COBALT_EINVAL;
+    if ((dx && !head_rows_ok(dx, ld_dx, hidden)) || (dw && !head_rows_ok(dw, ld_dw, hidden))) return COBALT_EINVAL;
+    if (((uintptr_t)targets & 7) || ((uintptr_t)stats & 7) || (((uintptr_t)grad | (uintptr_t)status) & 3) || grad_step < 0 || grad_step > 1) return COBALT_EINVAL;
+    int sms = 0;
+    if ((rc = sm_count(&sms))) return rc;
+    const HeadScratch s = head_scratch(n, hidden, vocab, true, dx != nullptr, sms);
+    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
+    uint8_t* base = (uint8_t*)scratch;
+    cudaStream_t st = (cudaStream_t)stream;
+    HlPrepareParams A = {};
+    A.x = (const uint16_t*)x; A.ldx = ldx;
+    A.targets = (const long long*)targets;
+    A.n = n; A.hidden = hidden; A.vocab = vocab;
+    A.count = (int*)(base + s.count);
+    A.slot = (int*)(base + s.slot);
+    A.target = (int*)(base + s.target);
+    A.packed = (uint16_t*)(base + s.packed);
+    A.stats = (const float2*)stats;
+    A.grad = grad; A.grad_step = (int)grad_step; A.mean = mean;
+    A.row = (float4*)(base + s.row);
+    A.factor = (float*)(base + s.count) + 2;
+    HlParams P = {};
+    P.status = status ? (uint32_t*)status : status_word();
+    if (!P.status) return COBALT_ELAUNCH;
+    const int64_t rows = (int64_t)ceil_div(n, HL_TILE) * HL_TILE;
+    CUtensorMap xm, wm, dm[2];
+    if ((rc = make_map(&xm, A.packed, hidden, n, hidden)) || (rc = make_map(&wm, weight, ldw, vocab, hidden))) return rc;
+    for (int b = 0; b < 2; ++b)
+        if ((rc = make_map(&dm[b], base + s.d[b], s.piece, rows, s.piece))) return rc;
+    if ((rc = prepare(A, st))) return rc;
+    P.count = A.count;
+    P.tok_tiles = (int)(rows / HL_TILE);
+    P.n_rows = n; P.hidden = hidden;
+    P.target = A.target;
+    P.row = A.row;
+    P.factor = A.factor;
+    P.d[0] = (uint16_t*)(base + s.d[0]); P.d[1] = (uint16_t*)(base + s.d[1]);
+    P.ld_d = s.piece;
+    P.slab = (float*)(base + s.slab);
+    P.dw = (uint16_t*)dw; P.ld_dw = ld_dw;
+    P.wide = !((uintptr_t)dw & 31) && !(ld_dw & 15);
+    // One launch per piece and one more: the products with piece i's d beside the logits of piece i + 1
+    const int h_tiles = ceil_div(hidden, HL_TILE);
+    for (int i = 0; i <= s.pieces; ++i) {
+        int64_t tiles = 0;
+        P.n_jobs = 0;
+        auto piece = [&](int kind, int k) -> HlJob& {
+            HlJob& j = P.job[P.n_jobs++];
+            j = HlJob{};
+            j.kind = kind;
+            j.v0 = k * s.piece;
+            j.cols = (int)std::min<int64_t>(s.piece, vocab - j.v0);
+            j.splits = 1;
+            j.buf = k & 1;
+            return j;
+        };
+        if (i > 0 && dx) {
+            HlJob& j = piece(HL_DX, i - 1);
+            j.n_tiles = h_tiles;
+            j.splits = s.splits;
+            j.add = i > 1;
+            tiles += (int64_t)P.tok_tiles * h_tiles * s.splits;
+        }
+        if (i > 0 && dw) {
+            HlJob& j = piece(HL_DW, i - 1);
+            j.n_tiles = h_tiles;
+            tiles += (int64_t)ceil_div(j.cols, HL_TILE) * h_tiles;
+        }
+        if (i < s.pieces) {
+            HlJob& j = piece(HL_DLOGITS, i);
+            j.n_tiles = ceil_div(j.cols, HL_TILE);
+            tiles += (int64_t)P.tok_tiles * j.n_tiles;
+        }
+        if ((rc = product(P, xm, wm, dm[0], dm[1], tiles, sms, st))) return rc;
+    }
+    if (dx) head_dx_kernel<<<n, 256, 0, st>>>(P.slab, A.slot, n, hidden, s.splits, A.factor, (uint16_t*)dx, ld_dx);
+    return launched();
+}
+
+int cobalt_vocab_status(void* stream, uint32_t* status_out) {
+    if (!status_out) return COBALT_EINVAL;
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc) return rc;
+    uint32_t* word = status_word();
+    if (!word) return COBALT_ELAUNCH;
+    if (cudaMemcpyAsync(status_out, word, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
+    if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
+    if (*status_out == 0) return COBALT_OK;
+    // cleared only once it was read as set: kernels write it while it is 0 alone
+    if (cudaMemsetAsync(word, 0, 4, (cudaStream_t)stream) != cudaSuccess || cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return COBALT_ELAUNCH;
+    return COBALT_ETIMEOUT;
+}
+
+}  // extern "C"

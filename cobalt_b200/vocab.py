@@ -1,0 +1,264 @@
+"""The two dense ends of a compressed model: embedding lookup and softmax cross entropy against the head, with their gradients.
+
+The recipe compresses the projections and leaves the embedding table and the head alone (the reference's sinq/patch_model.py:49), the largest
+tensors of a model with a large vocabulary.  ``embed`` is what a decoder begins with; ``head_loss`` scores its last hidden states without
+ever holding the logits, and both are differentiable, so the tables can be tuned after compression - a tied table through either end.
+The kernels' contract is in ``include/cobalt_b200.h``.  There is no torch fallback: on a non-CUDA tensor every function raises.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .linear import _raw_stream
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_REDUCTIONS = ("none", "sum", "mean")
+
+
+def _call(index: int, name: str, *args):
+    """A library call on device ``index`` and its current stream (the last argument)."""
+    lib = _lib.load()
+    if index == torch._C._cuda_getDevice():
+        rc = getattr(lib, name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(lib, name)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(name, rc)
+
+
+def _tokens(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if t.dtype is not torch.int64:
+        raise TypeError(f"{name} must be int64, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _matrix(name: str, t: torch.Tensor, width: int, unit: int = 1) -> torch.Tensor:
+    """``t [..., width]`` as rows that the kernels read where they lie, or a copy: neighbouring values, rows apart by a multiple of ``unit``
+    values that do not overlap (``unit`` > 1: on 16-byte boundaries)."""
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise ValueError(f"{name} must be [..., {width}], got {list(t.shape)}")
+    rows = t if t.dim() == 2 else t.reshape(-1, width)
+    apart = rows.shape[0] > 1 and (rows.stride(0) < width or rows.stride(0) % unit)
+    if (rows.stride(1) != 1 and width > 1) or apart or (unit > 1 and rows.data_ptr() % 16):
+        rows = rows.clone(memory_format=torch.contiguous_format)
+    return rows
+
+
+def _apart(rows: torch.Tensor) -> int:
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
+
+
+# ----------------------------------------------------------------------------- embedding
+def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``table[ids] * scale``: rows of ``table [n_rows, width]`` (bf16, fp16 or fp32) for int64 ``ids`` of any shape, ``[*ids.shape, width]``.  The
+    product is formed in fp32 and rounded once.  An id outside the table (-1: padding) reads zeros.  ``out`` (contiguous) receives the
+    result.  Differentiable in ``table`` (``embed_grad``)."""
+    _check_table("table", table)
+    ids = _tokens("ids", ids, table.device)
+    grad = table.requires_grad and torch.is_grad_enabled()
+    if out is not None:
+        if out.shape != (*ids.shape, table.shape[1]) or out.dtype is not table.dtype or out.device != table.device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {table.dtype} {[*ids.shape, table.shape[1]]} on {table.device}")
+        if grad or (out.requires_grad and torch.is_grad_enabled()):
+            raise RuntimeError("out cannot take a result that requires a gradient")
+    if grad:
+        leaves = _on_one_stream("embed", table)              # (alive until the graph holds them itself)
+        return _Embed.apply(ids, table, float(scale))
+    return _embed(ids, table, float(scale), out)
+
+
+def _on_one_stream(name: str, *inputs: torch.Tensor):
+    """A captured backward pass must not reach a leaf through an autograd graph of another stream that still lives: torch would wait for that
+    stream, which invalidates the capture (or ends the process, where nothing catches it).  Said before, as far as these functions made that graph."""
+    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in inputs if t.requires_grad and t.is_leaf]
+    if nodes:
+        stream = _raw_stream(inputs[0].get_device())
+        for node in nodes:
+            seen = node.metadata.setdefault("cobalt_stream", stream)
+            if seen != stream and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{name}: a graph of this leaf that was made on another stream is still alive; drop it before the capture, or capture "
+                                   "embed_grad / head_loss_and_grad, which need none")
+    return nodes
+
+
+def _check_table(name: str, t: torch.Tensor):
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor; there is no CPU path")
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if t.dim() != 2 or 0 in t.shape:
+        raise ValueError(f"{name} must be [n_rows, width], got {list(t.shape)}")
+
+
+def _embed(ids, table, scale, out=None):
+    width = table.shape[1]
+    rows = _matrix("table", table, width)
+    if out is None:
+        out = table.new_empty((*ids.shape, width))
+    n = ids.numel()
+    if n:
+        _call(table.get_device(), "cobalt_embed", ids.data_ptr(), n, rows.data_ptr(), _apart(rows), _TYPES[table.dtype], rows.shape[0], width, scale,
+              out.data_ptr(), width)
+    return out
+
+
+def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of ``embed`` with respect to its table, dense ``[n_rows, width]`` of ``grad``'s type: ``scale`` times the sum of the rows of
+    ``grad [*ids.shape, width]`` by token, in fp32 and in the tokens' order.  Tokens outside the table are left out."""
+    if not grad.is_cuda:
+        raise RuntimeError("grad must be a CUDA tensor; there is no CPU path")
+    if grad.dtype not in _TYPES:
+        raise TypeError(f"grad must be bfloat16, float16 or float32, got {grad.dtype}")
+    ids = _tokens("ids", ids, grad.device)
+    if grad.dim() < 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] < 1 or n_rows < 1:
+        raise ValueError(f"grad must be [*ids.shape, width] = {[*ids.shape, 'width']} and n_rows at least 1, got {list(grad.shape)} and {n_rows}")
+    width, n = grad.shape[-1], ids.numel()
+    if n == 0:
+        return grad.new_zeros((n_rows, width))
+    rows = _matrix("grad", grad, width)
+    out = grad.new_empty((n_rows, width))
+    need = _lib.load().cobalt_embed_grad_scratch_bytes(n, width)
+    scratch = out.new_empty(need, dtype=torch.uint8)         # per call, from the stream's own pool: overlapping calls never share one
+    _call(out.get_device(), "cobalt_embed_grad", ids.data_ptr(), n, rows.data_ptr(), _apart(rows), _TYPES[grad.dtype], n_rows, width, float(scale), out.data_ptr(),
+          scratch.data_ptr(), need)
+    return out
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale):
+        ctx.save_for_backward(ids)
+        ctx.n_rows, ctx.scale = table.shape[0], scale
+        return _embed(ids, table, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return None, embed_grad(grad, ctx.saved_tensors[0], ctx.n_rows, ctx.scale), None
+
+
+# ----------------------------------------------------------------------------- head loss
+def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str = "mean", status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Softmax cross entropy of the logits ``x @ weight.T``, which are never held: ``x [..., hidden]`` and ``weight [vocab, hidden]`` bf16 (hidden a
+    multiple of 8), int64 ``targets`` of ``x``'s leading shape.  fp32 result: of every token (``"none"``), their ``"sum"``, or their ``"mean"`` over the
+    tokens that count.  A target outside the vocabulary (-1, -100: padding, a prompt) does not count: loss and gradient zero, whatever
+    its row holds.  If none counts, the mean is 0.  Differentiable in ``x`` and ``weight``; the backward pass forms the logits once more.
+    ``status`` (int32 ``[1]``, zero) takes the code of a bounded wait that gave up, as ``head_loss_status`` tells it without one."""
+    _check_loss(x, weight, targets, reduction, status)
+    targets = _tokens("targets", targets, x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        leaves = _on_one_stream("head_loss", x, weight)      # (alive until the graph holds them itself)
+        return _HeadLoss.apply(x, weight, targets, reduction, status)
+    return _head_loss(x, weight, targets, reduction, status, False)[0]
+
+
+def head_loss_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str = "mean", grad: Optional[torch.Tensor] = None,
+                       need_x: bool = True, need_weight: bool = True, status: Optional[torch.Tensor] = None):
+    """``(loss, dx, dw)`` of ``head_loss`` without autograd, for captured steps and loops of one's own.  ``grad``: fp32 gradient of the result (of
+    its shape; ones by default).  ``need_x`` and ``need_weight``: which gradients are formed (``None`` else)."""
+    _check_loss(x, weight, targets, reduction, status)
+    targets = _tokens("targets", targets, x.device)
+    shape = targets.shape if reduction == "none" else ()
+    if grad is None:
+        grad = x.new_ones((), dtype=torch.float32).expand(shape)
+    elif grad.dtype is not torch.float32 or grad.shape != shape or grad.device != x.device:
+        raise ValueError(f"grad must be float32 {list(shape)} on {x.device}, got {grad.dtype} {list(grad.shape)} on {grad.device}")
+    with torch.no_grad():
+        loss, stats = _head_loss(x, weight, targets, reduction, status, True)
+        dx, dw = _head_loss_grad(x, weight, targets, stats, grad, reduction, status, need_x, need_weight) if need_x or need_weight else (None, None)
+    return loss, dx, dw
+
+
+def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str, status: Optional[torch.Tensor]):
+    for name, t in (("x", x), ("weight", weight)):
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor; there is no CPU path")
+        if t.dtype is not torch.bfloat16:
+            raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if weight.device != x.device:
+        raise ValueError(f"weight is on {weight.device}, x on {x.device}")
+    if weight.dim() != 2 or 0 in weight.shape or weight.shape[1] % 8:
+        raise ValueError(f"weight must be [vocab, hidden] with hidden a multiple of 8, got {list(weight.shape)}")
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x must be [..., {weight.shape[1]}], got {list(x.shape)}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
+    if targets.shape != x.shape[:-1]:
+        raise ValueError(f"targets must be {list(x.shape[:-1])}, got {list(targets.shape)}")
+    if status is not None and (status.dtype is not torch.int32 or status.shape != (1,) or status.device != x.device):
+        raise ValueError(f"status must be int32 [1] on {x.device}, got {status.dtype} {list(status.shape)} on {status.device}")
+
+
+def _head_loss(x, weight, targets, reduction, status, keep):
+    """(result, what the gradient needs: ``[n, 2]`` if ``keep``)"""
+    V, H = weight.shape
+    n = targets.numel()
+    if n == 0:
+        empty = x.new_zeros(targets.shape if reduction == "none" else (), dtype=torch.float32)
+        return empty, x.new_empty((0, 2), dtype=torch.float32) if keep else None
+    rows, w = _matrix("x", x, H, 8), _matrix("weight", weight, H, 8)
+    loss = x.new_empty(targets.shape, dtype=torch.float32)
+    stats = x.new_empty((n, 2), dtype=torch.float32) if keep else None
+    total = x.new_empty((), dtype=torch.float32) if reduction != "none" else None
+    need = _lib.load().cobalt_head_loss_scratch_bytes(n, H, V)
+    scratch = x.new_empty(need, dtype=torch.uint8)
+    _call(x.get_device(), "cobalt_head_loss", rows.data_ptr(), _apart(rows), w.data_ptr(), _apart(w), targets.data_ptr(), n, H, V, loss.data_ptr(),
+          None if stats is None else stats.data_ptr(), None if total is None else total.data_ptr(), 1 if reduction == "mean" else 0, scratch.data_ptr(), need,
+          None if status is None else status.data_ptr())
+    return loss if total is None else total, stats
+
+
+def _head_loss_grad(x, weight, targets, stats, grad, reduction, status, want_x, want_w):
+    V, H = weight.shape
+    n = targets.numel()
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else None
+    dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_w else None
+    if n == 0:
+        return dx, None if dw is None else dw.zero_()
+    rows, w = _matrix("x", x, H, 8), _matrix("weight", weight, H, 8)
+    each = reduction == "none" and any(grad.stride(i) for i in range(grad.dim()) if grad.shape[i] > 1)      # (a sum's gradient is one value, expanded)
+    if each:
+        grad = grad.contiguous()
+    index = x.get_device()
+    with torch.cuda.device(index):
+        need = _lib.load().cobalt_head_loss_grad_scratch_bytes(n, H, V, 1 if want_x else 0)
+    scratch = x.new_empty(need, dtype=torch.uint8)
+    _call(index, "cobalt_head_loss_grad", rows.data_ptr(), _apart(rows), w.data_ptr(), _apart(w), targets.data_ptr(), stats.data_ptr(), grad.data_ptr(), 1 if each else 0,
+          1 if reduction == "mean" else 0, n, H, V, None if dx is None else dx.data_ptr(), H, None if dw is None else dw.data_ptr(), H, scratch.data_ptr(), need,
+          None if status is None else status.data_ptr())
+    return dx, dw
+
+
+class _HeadLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets, reduction, status):
+        result, stats = _head_loss(x, weight, targets, reduction, status, True)
+        ctx.save_for_backward(x, weight, targets, stats)
+        ctx.reduction, ctx.status = reduction, status                # (the word is no input of the result)
+        return result
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        want_x, want_w = ctx.needs_input_grad[:2]
+        dx, dw = _head_loss_grad(*ctx.saved_tensors, grad, ctx.reduction, ctx.status, want_x, want_w) if want_x or want_w else (None, None)
+        return dx, dw, None, None, None
+
+
+def head_loss_status(device=None) -> int:
+    """0, or the code of the first bounded wait of ``head_loss`` or its gradient on ``device`` that gave up since the last question, of
+    those without a status word of their own; what it concerns is NaN.  Waits for the current stream."""
+    word = ctypes.c_uint32(0)
+    with torch.cuda.device(device):
+        rc = _lib.load().cobalt_vocab_status(_raw_stream(torch.cuda.current_device()), ctypes.byref(word))
+    if rc not in (0, _lib.ETIMEOUT):
+        _lib.check("cobalt_vocab_status", rc)
+    return int(word.value)

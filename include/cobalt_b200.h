@@ -389,6 +389,44 @@ int cobalt_kv4_attend_watched(const void* q, int64_t ld_q, const void* tiles, in
                               int sinks, float scale, void* scratch, size_t scratch_bytes, void* status, void* stream);
 int cobalt_kv4_status(void* stream, uint32_t* status_out);
 
+/* The two dense ends of a vocabulary: embedding lookup and softmax cross entropy against a head, with their gradients.
+ * Embedding calls: tables, rows and gradients of one type (COBALT_BF16, COBALT_FP16, COBALT_FP32), row strides ld in elements; any width,
+ * any alignment of a value (16-byte rows are faster).  An id outside [0, n_rows) (-1: padding) reads zeros and has no gradient.
+ *   cobalt_embed      : out[t] = table[ids[t]] * scale, the product in fp32, rounded once (scale 1: the bits of the table).
+ *   cobalt_embed_grad : out [n_rows][width] (contiguous, 16-byte aligned, every value written) = scale * sum of the rows grad[t] with ids[t] = row, in fp32,
+ *                       rounded once.  The same inputs give the same bits.  n <= 2^24.
+ * Head calls: x [n][hidden] and weight [vocab][hidden] bf16 (hidden a multiple of 8, rows 16-byte aligned), l[t, v] = x[t] . weight[v] in fp32,
+ * loss[t] = log(sum over v of exp l[t, v]) - l[t, targets[t]].  A target outside [0, vocab) (-1: padding, a prompt) means that the token does
+ * not count: its loss and its row of dx are zeros, and nothing in its row of x reaches a sum.  No logits are kept: scratch holds tile
+ * statistics (the loss) or two pieces of the gradient of the logits, at most 256 MB each unless a piece of 256 rows is larger.  n <= 2^20, hidden <= 2^16.
+ *   cobalt_head_loss      : loss fp32 [n]; stats (fp32 [n][2], 8-byte aligned; may be NULL) is what the gradient needs; total (fp32 [1]; may be NULL) = the
+ *                           sum of the losses or, with mean, their mean over the tokens that count (0 if none does).
+ *   cobalt_head_loss_grad : gradients for the same x, weight and targets.  grad fp32: of every token's loss (grad_step 1), or one value (grad_step 0)
+ *                           of the sum or, with mean, of the mean.  dx [n][hidden] and dw [vocab][hidden] bf16 (rows 16-byte aligned; either may be
+ *                           NULL), every value written.  The gradient of the logits is rounded to bf16 on the way, sums are fp32.
+ *                           status of both (may be NULL: the device's word): device memory, 4-byte aligned, zeroed by the caller; a bounded wait of
+ *                           the call that gives up leaves its code there while it is 0, and NaN in what it concerns.
+ *   cobalt_vocab_status   : 0, or the code of the first bounded wait that gave up since the last question, of the head calls on the current device
+ *                           without a word of their own.  Synchronises `stream`; not during capture.
+ * scratch: as many bytes as the _scratch_bytes call says, 256-byte aligned, contents irrelevant; calls that may overlap on the GPU need buffers
+ * of their own.  The reference looks up rows and forms logits in its megakernel (src/cobaltkernel/csrc/megakernel.cu:1652-2003) and has no loss. */
+#define COBALT_FP32 0
+#define COBALT_FP16 1
+#define COBALT_BF16 2
+int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out,
+                 int64_t ld_out, void* stream);
+size_t cobalt_embed_grad_scratch_bytes(int64_t n, int width);
+int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out,
+                      void* scratch, size_t scratch_bytes, void* stream);
+size_t cobalt_head_loss_scratch_bytes(int n, int hidden, int64_t vocab);
+int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, int n, int hidden, int64_t vocab,
+                     float* loss, float* stats, float* total, int mean, void* scratch, size_t scratch_bytes, void* status, void* stream);
+size_t cobalt_head_loss_grad_scratch_bytes(int n, int hidden, int64_t vocab, int want_x);
+int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, const float* stats,
+                          const float* grad, int64_t grad_step, int mean, int n, int hidden, int64_t vocab, void* dx, int64_t ld_dx, void* dw,
+                          int64_t ld_dw, void* scratch, size_t scratch_bytes, void* status, void* stream);
+int cobalt_vocab_status(void* stream, uint32_t* status_out);
+
 /* All-reduce (sum) of the fp32 partial outputs of a row-parallel layer over peer memory, for tensor-parallel decode
  * (the reference has no distributed code; this replaces the NCCL all-reduce that would follow cobalt_linear_f32).
  * Every rank owns one symmetric buffer mapped into all processes: [staging: slot_stride bytes][slot 0: world rows of
