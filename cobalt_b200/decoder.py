@@ -3,7 +3,8 @@
 This is the caller side of the hot path (the seven projections of every block): residual add +
 RMSNorm, RoPE + KV-cache append and SwiGLU are small fused CUDA kernels of the library;
 grouped-query attention over the preallocated KV cache and the dense ``lm_head`` (the reference
-leaves ``lm_head`` uncompressed: sinq/patch_model.py:49) are PyTorch matmuls.  The dtype policy follows the reference's executable spec
+leaves ``lm_head`` uncompressed: sinq/patch_model.py:49) are PyTorch matmuls.  ``score`` takes the cross entropy of a text without
+forming logits.  The dtype policy follows the reference's executable spec
 src/cobaltkernel/ref_llama.py:10-16, 82-143: fp32 normalise -> bf16 -> times w; bf16 RoPE
 tables; bf16 score/context matmuls with an fp32 softmax cast back to bf16; bf16 residuals.
 With ``model_type == "gemma3_text"`` the block follows src/cobaltkernel/ref_gemma3.py:138-294 instead:
@@ -32,6 +33,7 @@ from .compress import SparseQuantConfig, compress_weight
 from . import _lib
 from .kvcache import KVCache4
 from .linear import CobaltSparseLinear, FusedProjections, called_plainly, status_word
+from .vocab import embed, head_loss
 
 PROJ = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj",
         "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
@@ -153,6 +155,7 @@ class CobaltDecoder:
             raise ValueError("attention_sinks must not be negative, and needs kv_bits = 4")
         self.sinks = int(attention_sinks)
         self.prompt_status = torch.zeros(1, dtype=torch.int32, device=device)          # non-zero: a bounded wait of a prompt's attention (4-bit cache: of any) gave up
+        self.score_status = torch.zeros(1, dtype=torch.int32, device=device)           # the same of the losses of score() and their gradients
         self.kv4 = [KVCache4(self.B, nkv, max_ctx, D, device, status=self.prompt_status) for _ in range(L)] if kv_bits == 4 else None
         self.k_cache = self.v_cache = None
         if self.kv4 is None:
@@ -163,8 +166,8 @@ class CobaltDecoder:
         self.types = layer_types(cfg)
         self.inv_freq = {lt: rope_inv_freq(cfg, lt, device) for lt in set(self.types)}
         self.scale = float(cfg["query_pre_attn_scalar"]) ** -0.5 if self.gemma else float(D) ** -0.5
-        if self.gemma:
-            self.embed_scale = torch.tensor(float(cfg["hidden_size"]) ** 0.5, dtype=torch.bfloat16, device=device)
+        # of the embeddings; Gemma's is rounded to bf16 first
+        self.embed_factor = float(torch.tensor(float(cfg["hidden_size"]) ** 0.5, dtype=torch.bfloat16)) if self.gemma else 1.0
         self.kv_pos = torch.arange(max_ctx, device=device)
         need = _lib.load().cobalt_attn_decode_scratch_bytes(self.nh, D, max_ctx) * self.B
         self.att_scratch = torch.empty(need, dtype=torch.uint8, device=device) if self.kv4 is None and self.nh // self.nkv <= 8 and D % 64 == 0 \
@@ -366,12 +369,14 @@ class CobaltDecoder:
         return self._row_parallel(lin, self._swiglu(g, u))
 
     # ------------------------------------------------------------------ one forward over T tokens
+    def _dense_head(self) -> torch.Tensor:
+        return self.P["model.embed_tokens.weight"] if self.gemma else self.P["lm_head.weight"]              # Gemma ties the head
+
     def _head_logits(self, x: torch.Tensor) -> torch.Tensor:
         """Head: dense bf16 matmul, or the compressed head (GEMV up to 16 rows, tcgen05 GEMM above); with a vocabulary
         split over the ranks the local logits are gathered in rank order."""
         if self.head is None:
-            w = self.P["model.embed_tokens.weight"] if self.gemma else self.P["lm_head.weight"]   # Gemma ties the head
-            return F.linear(x, w)
+            return F.linear(x, self._dense_head())
         lg = self.head(x)
         if self.world > 1:
             import torch.distributed as dist
@@ -380,8 +385,8 @@ class CobaltDecoder:
             lg = torch.cat(parts, dim=-1)
         return lg
 
-    def _forward(self, ids: torch.Tensor, positions: torch.Tensor, attend_len: int, seq: Optional[int] = 0) -> torch.Tensor:
-        """ids, positions: [T] device tensors.  Keys/values are written at ``positions``; attention
+    def _forward(self, ids: torch.Tensor, positions: torch.Tensor, attend_len: int, seq: Optional[int] = 0, hidden: bool = False) -> torch.Tensor:
+        """Logits ``[1, T, V]``, or with ``hidden`` what the head takes, ``[1, T, H]``.  ids, positions: [T] device tensors.  Keys/values are written at ``positions``; attention
         looks at cache slots [0, attend_len) under the causal mask ``slot <= position``.  ``seq`` names the sequence
         whose cache is used; ``seq=None`` is the batched decode step: token t is the next token of sequence t."""
         cfg, P = self.cfg, self.P
@@ -451,18 +456,20 @@ class CobaltDecoder:
             delta = self._glu_down(i, g, u)
             if self.gemma:
                 delta_w = P[p + "post_feedforward_layernorm.weight"]
-        return self._logits_of(h, delta, delta_w).unsqueeze(0)                              # [1, T, V]
+        return (self._head_input if hidden else self._logits_of)(h, delta, delta_w).unsqueeze(0)
 
     def _logits_of(self, h, delta, delta_w):
         """What follows the last block: the branch joins, final norm, head; ``[T, V]``."""
         w = self.P["model.norm.weight"]
         if self.head_f is not None and self.world == 1:                                # final norm folded into the compressed head
             return self._norm_then(self.head_f, h, delta, w, delta_w)[1][0]
-        return self._head_logits(self._add_rmsnorm(h, self._settled(delta), w, delta_w)[1])
+        return self._head_logits(self._head_input(h, delta, delta_w))
+
+    def _head_input(self, h, delta, delta_w):
+        return self._add_rmsnorm(h, self._settled(delta), self.P["model.norm.weight"], delta_w)[1]
 
     def _embed(self, ids: torch.Tensor) -> torch.Tensor:
-        h = self.P["model.embed_tokens.weight"].index_select(0, ids)                   # [T, H]
-        return h * self.embed_scale if self.gemma else h                               # scale rounded to bf16 first
+        return embed(ids.long(), self.P["model.embed_tokens.weight"], self.embed_factor)                    # [T, H]
 
     def _greedy(self, rows: torch.Tensor, out: torch.Tensor):
         """``out [B]`` = the greedy token of every row of logits."""
@@ -475,13 +482,15 @@ class CobaltDecoder:
 
     def device_status(self) -> int:
         """The worst status word of everything this decoder launches (0 = healthy): modules, fused launches, prompt and one-kernel
-        attention, peer all-reduce.  A launch whose bounded wait gave up leaves its output unwritten and its code here."""
+        attention, losses, peer all-reduce.  A launch whose bounded wait gave up leaves its output unwritten and its code here."""
         words = [m.device_status() for m in self.lin.values()] + [int(self.prompt_status.item()), status_word(self.att_fused)]
         words += [f.device_status() for fs in (self.qkv, self.gate_up, self.o_f, self.down) for f in fs]
         if self.head_f is not None:
             words += [self.head.device_status(), self.head_f.device_status()]
         if self.reducer is not None:
             words.append(self.reducer.device_status())
+        if getattr(self, "score_status", None) is not None:
+            words.append(int(self.score_status.item()))
         return max(words)
 
     def _check_prompt_attention(self):
@@ -533,8 +542,9 @@ class CobaltDecoder:
             return 1
         return max(1, min(self.B, self.prompt_rows // T))
 
-    def _forward_prompts(self, ids: torch.Tensor, positions: torch.Tensor, first: int) -> torch.Tensor:
-        """``ids [n, T]``: the prompts of sequences ``first`` .. ``first + n - 1`` at the same ``positions [T]``; logits ``[n, T, V]``."""
+    def _forward_prompts(self, ids: torch.Tensor, positions: torch.Tensor, first: int, hidden: bool = False) -> torch.Tensor:
+        """``ids [n, T]``: the prompts of sequences ``first`` .. ``first + n - 1`` at the same ``positions [T]``; logits ``[n, T, V]`` or,
+        with ``hidden``, what the head takes, ``[n, T, H]``."""
         cfg, P = self.cfg, self.P
         n, T = ids.shape
         h = self._embed(ids.reshape(-1))                                               # [n*T, H]
@@ -556,7 +566,9 @@ class CobaltDecoder:
             else:
                 h, x = self._add_rmsnorm(h, o, P[p + "post_attention_layernorm.weight"])
             (delta,) = self.down[i](self._swiglu(*self.gate_up[i](x, T)), T)
-        h, x = self._add_rmsnorm(h, delta, P["model.norm.weight"], delta_w)
+        x = self._head_input(h, delta, delta_w)
+        if hidden:
+            return x.view(n, T, -1)
         if self.head_f is not None:
             return self.head_f(x, T)[0].view(n, T, -1)
         return torch.stack([self._head_logits(x[b * T:(b + 1) * T]) for b in range(n)])        # the library's GEMM, one shape for all
@@ -570,27 +582,48 @@ class CobaltDecoder:
         """Run the prompt(s), fill the cache(s), return the logits: ``ids [T]`` -> ``[T, V]`` (sequence 0), or
         ``ids [B, T]`` (one prompt per sequence, equal lengths) -> ``[B, T, V]``.  Waits for nothing; ``device_status()`` says
         whether the launches were healthy."""
-        ids = ids.to(self.dev)
         single = ids.dim() == 1
-        ids2 = ids.view(1, -1) if single else ids
+        logits = self._prefill(ids.to(self.dev).view(1, -1) if single else ids.to(self.dev), False)
+        return logits[0] if single else logits
+
+    def _prefill(self, ids2: torch.Tensor, hidden: bool) -> torch.Tensor:
+        """``ids2 [n, T]`` through all layers: logits ``[n, T, V]``, or with ``hidden`` what the head takes, ``[n, T, H]``."""
         if ids2.shape[0] > self.B:
             raise ValueError(f"{ids2.shape[0]} prompts for a decoder built for {self.B} sequences")
         T = ids2.shape[1]
         self._check_room(T)
         pos = torch.arange(T, device=self.dev)
         n, at_once = ids2.shape[0], self._prompts_at_once(T)
-        logits = None
+        out = None
         if at_once > 1 and n > 1:
             try:
-                parts = [self._forward_prompts(ids2[b:b + at_once], pos, b) for b in range(0, n, at_once)]
-                logits = parts[0] if len(parts) == 1 else torch.cat(parts)
+                parts = [self._forward_prompts(ids2[b:b + at_once], pos, b, hidden) for b in range(0, n, at_once)]
+                out = parts[0] if len(parts) == 1 else torch.cat(parts)
             except torch.cuda.OutOfMemoryError:              # one at a time needs less, and writes the same again over what is in the caches (4-bit ones: to within the order of sums)
                 parts = None
-        if logits is None:
-            parts = [self._forward(ids2[b], pos, T, seq=b) for b in range(n)]              # [1, T, V] each
-            logits = parts[0] if n == 1 else torch.cat(parts)
+        if out is None:
+            parts = [self._forward(ids2[b], pos, T, seq=b, hidden=hidden) for b in range(n)]
+            out = parts[0] if n == 1 else torch.cat(parts)
         self.pos.fill_(T)
-        return logits[0] if single else logits
+        return out
+
+    def score(self, ids: torch.Tensor, reduction: str = "none") -> torch.Tensor:
+        """Negative log-likelihood (natural logarithm, fp32) of every token but the first, given those before it: ``ids [T]`` -> ``[T - 1]``,
+        ``ids [B, T]`` (one text per sequence) -> ``[B, T - 1]``; with ``reduction`` ``"sum"`` or ``"mean"`` of all of them (``exp`` of the mean is the
+        perplexity).  A next token outside the vocabulary (-1: padding at the end) is not counted.  The caches are filled as by ``prefill``; no
+        logits are formed and none rounded, and the head is the dense one (``compress_head`` leaves its dequantised matrix there).  The blocks have no
+        backward pass, but where the dense head requires a gradient, the result has one with respect to it (``head_loss``)."""
+        if ids.dim() not in (1, 2) or ids.shape[-1] < 1:
+            raise ValueError(f"ids must be [T] or [B, T], got {list(ids.shape)}")
+        ids = ids.to(self.dev, torch.int64)
+        ids2 = ids.view(1, -1) if ids.dim() == 1 else ids
+        with torch.no_grad():
+            x = self._prefill(ids2, True)
+            targets = torch.cat([ids2[:, 1:], ids2.new_full((ids2.shape[0], 1), -1)], dim=1)
+        loss = head_loss(x, self._dense_head(), targets, reduction, status=self.score_status)
+        if reduction != "none":
+            return loss
+        return loss[0, :-1] if ids.dim() == 1 else loss[:, :-1]
 
     @torch.no_grad()
     def step(self) -> torch.Tensor:
