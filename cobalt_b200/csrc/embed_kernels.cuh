@@ -2,39 +2,106 @@
 //
 // An id outside the table (-1: padding) reads zeros and takes part in no sum; its row of dy is not read.
 //
+// Lookup: bound by memory.  32 bytes a thread, converted in pairs: 8192 rows of 5376 bf16 values in 25.8 us, 176 MB at 6.8 TB/s; a value
+// at a time with 16-byte loads took 50 us.
+//
 // The gradient is dense and mostly zeros: what bounds it is writing them.  It goes by sorted tokens, so that every sum has one owner and one
-// order (ascending n) and no atomics are needed:
-//   1. blocks of 2048 ids sort (id, n) in shared memory, while all others write the zeros of the whole table;
-//   2. more than one block: every element finds its place among all by binary searches in the other blocks' sorted ids;
-//   3. tiles of 32 sorted tokens add up the rows of each run of equal ids (fp32) and write the table rows of runs that lie inside the tile;
-//      what a run has in tiles that it leaves or enters goes to scratch, one row at either end of a tile;
-//   4. one block per run that crosses tiles adds those rows in order.
-// The zeros of rows that are overwritten in 3 and 4 are written twice: a few per cent of the table, for which the sort costs nothing.
+// order (ascending n) and no atomics on values are needed:
+//   1. blocks of 2048 ids sort (id, n) in registers and shared memory, while all other blocks write zeros to the whole table;
+//   2. more than one block: every element finds its place among all by binary searches in the other blocks' sorted ids (the rest of the
+//      zeros is written beside it);
+//   3. tiles of 16 sorted tokens add up the rows of each run of equal ids (fp32) and write the table rows of runs that lie inside the tile;
+//      what a run has in tiles that it leaves or enters goes to scratch, one row at either end of a tile, and the tile where it begins to a list;
+//   4. the runs of the list add those rows in order.
+// The zeros of rows that are overwritten in 3 and 4 are written twice: a few per cent of the table, for which sorting costs nothing.
+// Zeros go out as one 32-byte store a thread of blocks that hold 32 KB each: 7.5 TB/s over 2.8 GB, where a grid that strides over the table
+// reaches 6.2 TB/s whatever the width of its stores (bulk copies from shared memory: 6.3).
 #pragma once
 #include <cuda_fp16.h>
 #include "common.cuh"
+#include "staged_input.cuh"
 
 namespace cb {
 
 constexpr int EMB_THREADS = 256;
 constexpr int EG_BLOCK = 2048;             // ids that a block sorts
 constexpr int EG_SORT_THREADS = 1024;
-constexpr int EG_TILE = 32;                // sorted tokens of a tile
+constexpr int EG_TILE = 16;                // sorted tokens of a tile
+constexpr int EG_JOIN_GRID = 256;          // blocks along the list of runs that cross tiles
+constexpr int EG_PLACE_THREADS = 256;
 constexpr int EG_SUM_THREADS = 128;
 constexpr uint32_t EG_NONE = 0xFFFFFFFFu;  // sorts behind every row
 
 struct Bf16 { uint16_t v; };
 struct Fp16 { uint16_t v; };
 
-// N values of a type as they lie in memory, to fp32 and back (one rounding to nearest)
+// A 32-bit word of a type's values as they lie in memory: to fp32 and back (one rounding to nearest), and single values
+template <typename T> constexpr int PER_WORD = 4 / sizeof(T);
+__device__ __forceinline__ void word_values(Bf16, uint32_t w, float* v) { v[0] = __uint_as_float(w << 16); v[1] = __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ void word_values(Fp16, uint32_t w, float* v) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    v[0] = f.x; v[1] = f.y;
+}
+__device__ __forceinline__ void word_values(float, uint32_t w, float* v) { v[0] = __uint_as_float(w); }
+__device__ __forceinline__ uint32_t word_of(Bf16, const float* v) { return pack_bf16x2(v[0], v[1]); }
+__device__ __forceinline__ uint32_t word_of(Fp16, const float* v) {
+    const __half2 h = __floats2half2_rn(v[0], v[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t word_of(float, const float* v) { return __float_as_uint(v[0]); }
 __device__ __forceinline__ float value_of(float x) { return x; }
 __device__ __forceinline__ float value_of(Bf16 x) { return bf16_to_float(x.v); }
 __device__ __forceinline__ float value_of(Fp16 x) { return __half2float(__ushort_as_half(x.v)); }
 __device__ __forceinline__ void set_value(float& d, float x) { d = x; }
 __device__ __forceinline__ void set_value(Bf16& d, float x) { d.v = float_to_bf16(x); }
 __device__ __forceinline__ void set_value(Fp16& d, float x) { d.v = __half_as_ushort(__float2half_rn(x)); }
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+// W words of a row at a time (rows on such boundaries), or a value (W = 0)
+template <typename T, int W> constexpr int PACK = W ? W * PER_WORD<T> : 1;
+template <typename T, int W>
+struct Pack {
+    uint32_t w[W];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (W == 8) {
+            asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+        } else {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (W == 8)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+        else
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ void values(float (&v)[PACK<T, W>]) const {
+#pragma unroll
+        for (int i = 0; i < W; ++i) word_values(T{}, w[i], v + i * PER_WORD<T>);
+    }
+    __device__ __forceinline__ void set(const float (&v)[PACK<T, W>], float scale) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            float x[PER_WORD<T>];
+#pragma unroll
+            for (int e = 0; e < PER_WORD<T>; ++e) x[e] = v[i * PER_WORD<T> + e] * scale;
+            w[i] = word_of(T{}, x);
+        }
+    }
+};
+template <typename T>
+struct Pack<T, 0> {
+    T x;
+    __device__ __forceinline__ void clear() { x = T{}; }
+    __device__ __forceinline__ void load(const T* p) { x = *p; }
+    __device__ __forceinline__ void store(T* p) const { *p = x; }
+    __device__ __forceinline__ void values(float (&v)[1]) const { v[0] = value_of(x); }
+    __device__ __forceinline__ void set(const float (&v)[1], float scale) { set_value(x, v[0] * scale); }
+};
 
 struct EmbedParams {
     const long long* ids;
@@ -46,30 +113,28 @@ struct EmbedParams {
     bool plain;                            // scale 1: bits are copied
 };
 
-// `threads_per_row` threads a token, four packs of each in flight
-template <typename T, int N>
+// `threads_per_row` threads a token
+template <typename T, int W>
 __global__ void __launch_bounds__(EMB_THREADS) embed_kernel(const EmbedParams P) {
     const int per = P.threads_per_row, lane = threadIdx.x & (per - 1);
     const long long t = (long long)blockIdx.x * (EMB_THREADS / per) + threadIdx.x / per;
     if (t >= P.n) return;
     const long long id = P.ids[t];
     const bool in = id >= 0 && id < P.n_rows;
-    const Pack<T, N>* src = reinterpret_cast<const Pack<T, N>*>(reinterpret_cast<const T*>(P.table) + (in ? id : 0) * P.ld);
-    Pack<T, N>* dst = reinterpret_cast<Pack<T, N>*>(reinterpret_cast<T*>(P.out) + t * P.ld_out);
-    for (int c = lane; c < P.chunks; c += 4 * per) {
-        Pack<T, N> v[4] = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (in && c + i * per < P.chunks) v[i] = src[c + i * per];
-        if (!P.plain && in) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < N; ++e) set_value(v[i].v[e], value_of(v[i].v[e]) * P.scale);
+    const T* src = reinterpret_cast<const T*>(P.table) + (in ? id : 0) * P.ld;
+    T* dst = reinterpret_cast<T*>(P.out) + t * P.ld_out;
+    for (int c = lane; c < P.chunks; c += per) {
+        Pack<T, W> v;
+        v.clear();
+        if (in) {
+            v.load(src + c * PACK<T, W>);
+            if (!P.plain) {
+                float x[PACK<T, W>];
+                v.values(x);
+                v.set(x, P.scale);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i * per < P.chunks) dst[c + i * per] = v[i];
+        v.store(dst + c * PACK<T, W>);
     }
 }
 
@@ -85,53 +150,87 @@ struct EmbedGradParams {
     uint32_t* ids_sorted;                  // [n] (one block: the same memory as block_ids)
     uint32_t* pos_sorted;
     float* part;                           // [tiles][2][width]: what a tile has of the run that entered it, of the one that leaves it
+    uint32_t* runs;                        // [0]: number of runs that cross tiles, [1..]: the tiles where they begin
+    long long out_bytes, zero_first;       // of them, those that are cleared beside the sort; the rest beside step 2
 };
 
-// Step 1.  Bitonic sort of (id, n) in shared memory: unique keys, so the order of equal ids is that of the tokens.
-__global__ void __launch_bounds__(EG_SORT_THREADS) embed_grad_sort_kernel(const EmbedGradParams P, long long out_bytes) {
-    if ((int)blockIdx.x >= P.blocks) {                     // zeros
-        uint4* out = reinterpret_cast<uint4*>(P.out);
-        const long long packs = out_bytes / 16, step = (long long)(gridDim.x - P.blocks) * EG_SORT_THREADS;
-        const long long first = (long long)(blockIdx.x - P.blocks) * EG_SORT_THREADS + threadIdx.x;
-        for (long long i = first; i < packs; i += step) out[i] = make_uint4(0, 0, 0, 0);
-        if (first < out_bytes % 16) reinterpret_cast<uint8_t*>(P.out)[packs * 16 + first] = 0;
+constexpr int EG_ZERO_BYTES = 32 * EG_SORT_THREADS;        // of a block
+// block `b` of those that clear the bytes [from, to); both multiples of 16
+__device__ __forceinline__ void embed_grad_zero(const EmbedGradParams& P, long long b, int threads, long long from, long long to) {
+    const long long at = from + (b * threads + threadIdx.x) * 32;
+    if (at >= to) return;
+    uint8_t* p = reinterpret_cast<uint8_t*>(P.out) + at;
+    if (at + 32 <= to && !((uintptr_t)p & 31)) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};" ::"l"(p), "r"(0) : "memory");
+    } else {
+        for (int i = 0; i < 32 && at + i < to; i += 16) {
+            if (at + i + 16 <= to) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+            else
+                for (int k = i; at + k < to; ++k) p[k] = 0;            // the last bytes of the table
+        }
+    }
+}
+
+// Step 1.  Bitonic sort of the keys (id, n): unique, so the order of equal ids is that of the tokens.  A thread holds two neighbouring elements;
+// partners up to 32 apart are in its warp, others meet in shared memory.
+__global__ void __launch_bounds__(EG_SORT_THREADS) embed_grad_sort_kernel(const EmbedGradParams P) {
+    if ((int)blockIdx.x >= P.blocks) {
+        embed_grad_zero(P, blockIdx.x - P.blocks, EG_SORT_THREADS, 0, P.zero_first);
         return;
     }
-    __shared__ unsigned long long key[EG_BLOCK];
+    __shared__ ulonglong2 key_s[EG_SORT_THREADS];
     const long long base = (long long)blockIdx.x * EG_BLOCK;
     const int here = (int)min((long long)EG_BLOCK, P.n - base);
-    int size = 2;
-    while (size < here) size *= 2;
-    for (int i = threadIdx.x; i < size; i += EG_SORT_THREADS) {
+    const uint32_t i0 = 2 * threadIdx.x;
+    if (blockIdx.x == 0 && threadIdx.x == 0) P.runs[0] = 0;
+    unsigned long long key[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
         uint32_t id = EG_NONE;
-        if (i < here) {
-            const long long v = P.ids[base + i];
+        if ((int)i0 + e < here) {
+            const long long v = P.ids[base + i0 + e];
             if (v >= 0 && v < P.n_rows) id = (uint32_t)v;
         }
-        key[i] = (unsigned long long)id << 32 | (uint32_t)i;
+        key[e] = (unsigned long long)id << 32 | (i0 + e);
     }
-    __syncthreads();
-    for (int k = 2; k <= size; k *= 2) {
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = threadIdx.x; t < size / 2; t += EG_SORT_THREADS) {
-                const int a = 2 * t - (t & (j - 1)), b = a + j;
-                const unsigned long long x = key[a], y = key[b];
-                if ((x > y) == ((a & k) == 0)) { key[a] = y; key[b] = x; }
+    uint32_t size = 2;
+    while ((int)size < here) size *= 2;
+    for (uint32_t k = 2; k <= size; k *= 2) {
+        const bool up = (i0 & k) == 0;                     // (k = 2: the two elements of a thread are one group)
+        for (uint32_t j = k / 2; j > 1; j /= 2) {
+            unsigned long long other[2];
+            if (j <= 32) {
+                other[0] = __shfl_xor_sync(0xFFFFFFFFu, key[0], j / 2);
+                other[1] = __shfl_xor_sync(0xFFFFFFFFu, key[1], j / 2);
+            } else {
+                key_s[threadIdx.x] = make_ulonglong2(key[0], key[1]);
+                __syncthreads();
+                const ulonglong2 o = key_s[threadIdx.x ^ (j / 2)];
+                other[0] = o.x; other[1] = o.y;
+                __syncthreads();
             }
-            __syncthreads();
+            const bool low = ((i0 & j) == 0) == up;        // keeps the smaller one
+#pragma unroll
+            for (int e = 0; e < 2; ++e) key[e] = (key[e] < other[e]) == low ? key[e] : other[e];
         }
+        if ((key[0] > key[1]) == up) { const unsigned long long t = key[0]; key[0] = key[1]; key[1] = t; }
     }
-    for (int i = threadIdx.x; i < EG_BLOCK; i += EG_SORT_THREADS) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int i = (int)i0 + e;
         const bool in = i < here;
-        if (!in && P.blocks == 1) break;
-        P.block_ids[base + i] = in ? (uint32_t)(key[i] >> 32) : EG_NONE;
-        if (in) P.block_pos[base + i] = (uint32_t)(base + (uint32_t)key[i]);
+        if (in || P.blocks > 1) P.block_ids[base + i] = in ? (uint32_t)(key[e] >> 32) : EG_NONE;
+        if (in) P.block_pos[base + i] = (uint32_t)(base + (uint32_t)key[e]);
     }
 }
 
 // Step 2.  An element's place: its own in its block, plus how many of every other block come before it (equal ids: of earlier blocks).
-__global__ void __launch_bounds__(256) embed_grad_place_kernel(const EmbedGradParams P) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(EG_PLACE_THREADS) embed_grad_place_kernel(const EmbedGradParams P, int place_blocks) {
+    if ((int)blockIdx.x >= place_blocks) {
+        embed_grad_zero(P, blockIdx.x - place_blocks, EG_PLACE_THREADS, P.zero_first, P.out_bytes);
+        return;
+    }
+    const long long i = (long long)blockIdx.x * EG_PLACE_THREADS + threadIdx.x;
     if (i >= P.n) return;
     const int mine = (int)(i / EG_BLOCK);
     const uint32_t id = P.block_ids[i];
@@ -156,17 +255,21 @@ __global__ void __launch_bounds__(256) embed_grad_place_kernel(const EmbedGradPa
 }
 
 // Step 3.
-template <typename T, int N>
+template <typename T, int W>
 __global__ void __launch_bounds__(EG_SUM_THREADS) embed_grad_sum_kernel(const EmbedGradParams P) {
+    constexpr int N = PACK<T, W>, AHEAD = 8;               // rows in flight
     __shared__ uint32_t id_s[EG_TILE + 2], pos_s[EG_TILE];
     const long long t0 = (long long)blockIdx.x * EG_TILE;
     const int here = (int)min((long long)EG_TILE, P.n - t0);
-    for (int i = threadIdx.x; i < EG_TILE + 2; i += EG_SUM_THREADS) {       // the tile's ids and one on either side
+    if (threadIdx.x < EG_TILE + 2) {                       // the tile's ids and one on either side
+        const int i = threadIdx.x;
         const long long at = t0 + i - 1;
         id_s[i] = at >= 0 && at < P.n ? P.ids_sorted[at] : EG_NONE;
         if (i < here) pos_s[i] = P.pos_sorted[t0 + i];
     }
     __syncthreads();
+    const uint32_t tail = id_s[here];
+    if (blockIdx.y == 0 && threadIdx.x == 0 && tail != EG_NONE && id_s[here + 1] == tail && id_s[0] != tail) P.runs[1 + atomicAdd(P.runs, 1u)] = blockIdx.x;
     const int col = ((int)blockIdx.y * EG_SUM_THREADS + (int)threadIdx.x) * N;
     if (col >= P.width) return;
     const T* grad = reinterpret_cast<const T*>(P.grad) + col;
@@ -174,29 +277,34 @@ __global__ void __launch_bounds__(EG_SUM_THREADS) embed_grad_sum_kernel(const Em
     float* part = P.part + (long long)blockIdx.x * 2 * P.width + col;
     float sum[N] = {};
     bool entered = id_s[0] == id_s[1];                     // the run began in an earlier tile
-    for (int i0 = 0; i0 < here; i0 += 8) {
-        Pack<T, N> v[8] = {};
+    for (int i0 = 0; i0 < here; i0 += AHEAD) {
+        Pack<T, W> v[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i0 + i < here && id_s[i0 + i + 1] != EG_NONE) v[i] = *reinterpret_cast<const Pack<T, N>*>(grad + (long long)pos_s[i0 + i] * P.ld);
+        for (int i = 0; i < AHEAD; ++i) {
+            v[i].clear();
+            if (i0 + i < here && id_s[i0 + i + 1] != EG_NONE) v[i].load(grad + (long long)pos_s[i0 + i] * P.ld);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (i0 + i >= here) continue;
-            const uint32_t id = id_s[i0 + i + 1];
-            if (id == EG_NONE) return;
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t id = i0 + i < here ? id_s[i0 + i + 1] : EG_NONE;
+            float x[N];
+            v[i].values(x);
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += value_of(v[i].v[e]);
-            const bool last = i0 + i + 1 == here, ends = id_s[i0 + i + 2] != id;
-            if (!last && !ends) continue;
+            for (int e = 0; e < N; ++e) sum[e] += x[e];
+            const bool last = i0 + i + 1 == here, ends = id_s[min(i0 + i + 2, EG_TILE + 1)] != id;
+            if (id == EG_NONE || (!last && !ends)) continue;
             if (entered || !ends) {
                 float* p = part + (entered ? 0 : P.width);
+                if constexpr (N % 4 == 0) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) p[e] = sum[e];
+                    for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(sum[e], sum[e + 1], sum[e + 2], sum[e + 3]);
+                } else {
+                    p[0] = sum[0];
+                }
             } else {
-                Pack<T, N> o;
-#pragma unroll
-                for (int e = 0; e < N; ++e) set_value(o.v[e], sum[e] * P.scale);
-                *reinterpret_cast<Pack<T, N>*>(out + (long long)id * P.width) = o;
+                Pack<T, W> o;
+                o.set(sum, P.scale);
+                o.store(out + (long long)id * P.width);
             }
             entered = false;
 #pragma unroll
@@ -208,39 +316,47 @@ __global__ void __launch_bounds__(EG_SUM_THREADS) embed_grad_sum_kernel(const Em
 // Step 4.  A run that leaves tile a for the first time: its rows in the tiles a .. b.  Eight warps take a part of them each.
 template <typename T>
 __global__ void __launch_bounds__(256) embed_grad_join_kernel(const EmbedGradParams P) {
-    const long long a = blockIdx.x, end = (a + 1) * EG_TILE;
-    if (end >= P.n) return;
-    const uint32_t id = P.ids_sorted[end - 1];
-    if (id == EG_NONE || P.ids_sorted[end] != id) return;
-    if (a > 0 && P.ids_sorted[end - EG_TILE] == id && P.ids_sorted[end - EG_TILE - 1] == id) return;      // it came from an earlier tile
-    long long lo = end, hi = P.n;                          // first element behind the run
-    while (lo < hi) {
-        const long long mid = (lo + hi) / 2;
-        if (P.ids_sorted[mid] <= id) lo = mid + 1;
-        else hi = mid;
-    }
-    const int rows = (int)((lo - 1) / EG_TILE - a);        // tiles that it enters
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col = ((int)blockIdx.y * 32 + lane) * 4;
     __shared__ float sum_s[8][128];
-    float sum[4] = {};
-    const int first = (int)((long long)rows * warp / 8), last = (int)((long long)rows * (warp + 1) / 8);
-    const float* part = P.part + (a + 1) * 2 * P.width + col;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int col = ((int)blockIdx.y * 32 + lane) * 4, c = (int)blockIdx.y * 128 + (int)threadIdx.x;
+    const int n_runs = (int)P.runs[0];
+    for (int k = blockIdx.x; k < n_runs; k += gridDim.x) {
+        const long long a = P.runs[1 + k], end = (a + 1) * EG_TILE;
+        const uint32_t id = P.ids_sorted[end];
+        int rows = 0;                                      // tiles that it enters: those that begin with its id
+        for (int more = 256; more == 256; rows += more) {
+            const long long at = (a + 1 + rows + threadIdx.x) * EG_TILE;
+            more = __syncthreads_count(at < P.n && P.ids_sorted[at] == id);
+        }
+        const int first = (int)((long long)rows * warp / 8), last = (int)((long long)rows * (warp + 1) / 8);
+        const float* part = P.part + (a + 1) * 2 * P.width + col;
+        float sum[4] = {};
+        if (P.width % 4 == 0) {
+            if (col < P.width) {
+#pragma unroll 8
+                for (int r = first; r < last; ++r) {
+                    const float4 v = *reinterpret_cast<const float4*>(part + (long long)r * 2 * P.width);
+                    sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+                }
+            }
+        } else {
 #pragma unroll 4
-    for (int r = first; r < last; ++r)
+            for (int r = first; r < last; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (col + e < P.width) sum[e] += part[(long long)r * 2 * P.width + e];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum_s[warp][lane * 4 + e] = sum[e];
-    __syncthreads();
-    const int c = (int)blockIdx.y * 128 + threadIdx.x;
-    if (threadIdx.x >= 128 || c >= P.width) return;
-    float total = P.part[a * 2 * P.width + P.width + c];
-    for (int w = 0; w < 8; ++w) total += sum_s[w][threadIdx.x];
-    T o;
-    set_value(o, total * P.scale);
-    reinterpret_cast<T*>(P.out)[(long long)id * P.width + c] = o;
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < P.width) sum[e] += part[(long long)r * 2 * P.width + e];
+        }
+        *reinterpret_cast<float4*>(&sum_s[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        __syncthreads();
+        if (threadIdx.x < 128 && c < P.width) {
+            float total = P.part[a * 2 * P.width + P.width + c];
+            for (int w = 0; w < 8; ++w) total += sum_s[w][threadIdx.x];
+            T o;
+            set_value(o, total * P.scale);
+            reinterpret_cast<T*>(P.out)[(long long)id * P.width + c] = o;
+        }
+        __syncthreads();
+    }
 }
 
 }  // namespace cb

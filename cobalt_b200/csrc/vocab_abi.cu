@@ -42,15 +42,17 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // bytes of a value of a type of the embedding calls, 0: no such type
 int type_bytes(int type) { return type == COBALT_FP32 ? 4 : type == COBALT_FP16 || type == COBALT_BF16 ? 2 : 0; }
-// Calls CALL with T, the type as it lies in memory, and N, the values of a 16-byte pack (1: rows do not lie on 16-byte boundaries)
-#define EMBED_DISPATCH(TYPE, PACKED, CALL)                                                   \
-    if ((TYPE) == COBALT_FP32) { using T = float; if (PACKED) { constexpr int N = 4; CALL; } else { constexpr int N = 1; CALL; } } \
-    else if ((TYPE) == COBALT_FP16) { using T = Fp16; if (PACKED) { constexpr int N = 8; CALL; } else { constexpr int N = 1; CALL; } } \
-    else { using T = Bf16; if (PACKED) { constexpr int N = 8; CALL; } else { constexpr int N = 1; CALL; } }
+// The statements with T, the type as it lies in memory, and W, the 32-bit words that its rows can be read in at a time (0: a value at a time)
+#define EMBED_TYPES(TYPE, ...)                                              \
+    if ((TYPE) == COBALT_FP32) { using T = float; __VA_ARGS__; }                   \
+    else if ((TYPE) == COBALT_FP16) { using T = Fp16; __VA_ARGS__; }               \
+    else { using T = Bf16; __VA_ARGS__; }
+// the largest of 8, 4 and 0 words that divides all addresses and strides
+int words_at_once(uintptr_t all) { return !(all & 31) ? 8 : !(all & 15) ? 4 : 0; }
 
 struct EmbedGradScratch {
     int blocks, tiles;
-    size_t block_ids, block_pos, ids, pos, part, bytes;
+    size_t block_ids, block_pos, ids, pos, runs, part, bytes;
 };
 EmbedGradScratch embed_grad_scratch(int64_t n, int width) {
     EmbedGradScratch s = {};
@@ -61,7 +63,8 @@ EmbedGradScratch embed_grad_scratch(int64_t n, int width) {
     s.block_pos = list;
     s.ids = s.blocks > 1 ? 2 * list : s.block_ids;
     s.pos = s.blocks > 1 ? 3 * list : s.block_pos;
-    s.part = (s.blocks > 1 ? 4 : 2) * list;
+    s.runs = (s.blocks > 1 ? 4 : 2) * list;
+    s.part = s.runs + align256(((size_t)s.tiles + 1) * 4);
     s.bytes = s.part + (s.tiles > 1 ? align256((size_t)s.tiles * 2 * width * 4) : 0);
     return s;
 }
@@ -175,19 +178,24 @@ int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, i
     int sms = 0;
     const int rc = sm_count(&sms);
     if (rc) return rc;
-    const bool packed = !(((uintptr_t)table | (uintptr_t)out | (uintptr_t)(ld * size) | (uintptr_t)(ld_out * size) | (uintptr_t)((int64_t)width * size)) & 15);
+    const int words = words_at_once((uintptr_t)table | (uintptr_t)out | (uintptr_t)(ld * size) | (uintptr_t)(ld_out * size) | (uintptr_t)((int64_t)width * size));
     EmbedParams P;
     P.ids = (const long long*)ids;
     P.table = table; P.out = out;
     P.n = n; P.ld = ld; P.ld_out = ld_out; P.n_rows = n_rows;
-    P.chunks = packed ? width * size / 16 : width;
+    P.chunks = words ? width * size / (4 * words) : width;
     P.threads_per_row = 8;
-    while (P.threads_per_row < EMB_THREADS && 4 * P.threads_per_row < P.chunks) P.threads_per_row *= 2;
+    while (P.threads_per_row < EMB_THREADS && P.threads_per_row < P.chunks) P.threads_per_row *= 2;
     P.scale = scale;
     P.plain = scale == 1.0f;
     const int64_t blocks = ceil_div(n, EMB_THREADS / P.threads_per_row);
     if (blocks > 0x7FFFFFFFll) return COBALT_ETOOBIG;
-    EMBED_DISPATCH(type, packed, (embed_kernel<T, N><<<(unsigned)blocks, EMB_THREADS, 0, (cudaStream_t)stream>>>(P)));
+    cudaStream_t st = (cudaStream_t)stream;
+    EMBED_TYPES(type, {
+        if (words == 8) embed_kernel<T, 8><<<(unsigned)blocks, EMB_THREADS, 0, st>>>(P);
+        else if (words == 4) embed_kernel<T, 4><<<(unsigned)blocks, EMB_THREADS, 0, st>>>(P);
+        else embed_kernel<T, 0><<<(unsigned)blocks, EMB_THREADS, 0, st>>>(P);
+    });
     return launched();
 }
 
@@ -218,25 +226,33 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
     P.ids_sorted = (uint32_t*)(base + s.ids);
     P.pos_sorted = (uint32_t*)(base + s.pos);
     P.part = (float*)(base + s.part);
+    P.runs = (uint32_t*)(base + s.runs);
+    // Placing takes about 1.5 us a block of ids; zeros are written at 7 MB in a microsecond meanwhile
+    P.out_bytes = n_rows * width * size;
+    P.zero_first = s.blocks > 1 ? P.out_bytes - std::min<int64_t>(P.out_bytes / 2, (int64_t)s.blocks * (10 << 20)) / 32 * 32 : P.out_bytes;
+    if (P.zero_first < P.out_bytes) P.zero_first = P.zero_first / 32 * 32;
     cudaStream_t st = (cudaStream_t)stream;
-    const int64_t out_bytes = n_rows * width * size;
-    const int zeros = (int)std::min<int64_t>(ceil_div(out_bytes, 16 * EG_SORT_THREADS), 2 * sms);
-    embed_grad_sort_kernel<<<s.blocks + zeros, EG_SORT_THREADS, 0, st>>>(P, out_bytes);
+    const int64_t zeros = ceil_div(P.zero_first, EG_ZERO_BYTES);
+    if (zeros > 0x3FFFFFFFll) return COBALT_ETOOBIG;
+    embed_grad_sort_kernel<<<(unsigned)(s.blocks + zeros), EG_SORT_THREADS, 0, st>>>(P);
     if ((rc = launched())) return rc;
     if (s.blocks > 1) {
-        embed_grad_place_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(P);
+        const int64_t places = ceil_div(n, EG_PLACE_THREADS);
+        embed_grad_place_kernel<<<(unsigned)(places + ceil_div(P.out_bytes - P.zero_first, 32 * EG_PLACE_THREADS)), EG_PLACE_THREADS, 0, st>>>(P, (int)places);
         if ((rc = launched())) return rc;
     }
-    const bool packed = !(((uintptr_t)grad | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)width * size)) & 15);
-    const int per_block = EG_SUM_THREADS * (packed ? 16 / size : 1);
+    const int words = std::min(words_at_once((uintptr_t)grad | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)width * size)), 4);
+    const int per_block = EG_SUM_THREADS * (words ? 16 / size : 1);
     if (ceil_div(width, per_block) > 65535) return COBALT_ETOOBIG;
-    EMBED_DISPATCH(type, packed, (embed_grad_sum_kernel<T, N><<<dim3((unsigned)s.tiles, (unsigned)ceil_div(width, per_block)), EG_SUM_THREADS, 0, st>>>(P)));
+    const dim3 grid((unsigned)s.tiles, (unsigned)ceil_div(width, per_block));
+    EMBED_TYPES(type, {
+        if (words) embed_grad_sum_kernel<T, 4><<<grid, EG_SUM_THREADS, 0, st>>>(P);
+        else embed_grad_sum_kernel<T, 0><<<grid, EG_SUM_THREADS, 0, st>>>(P);
+    });
     if ((rc = launched())) return rc;
     if (s.tiles > 1) {
-        const dim3 grid((unsigned)s.tiles, (unsigned)ceil_div(width, 128));
-        if (type == COBALT_FP32) embed_grad_join_kernel<float><<<grid, 256, 0, st>>>(P);
-        else if (type == COBALT_FP16) embed_grad_join_kernel<Fp16><<<grid, 256, 0, st>>>(P);
-        else embed_grad_join_kernel<Bf16><<<grid, 256, 0, st>>>(P);
+        const dim3 join((unsigned)std::min(s.tiles, EG_JOIN_GRID), (unsigned)ceil_div(width, 128));
+        EMBED_TYPES(type, { embed_grad_join_kernel<T><<<join, 256, 0, st>>>(P); });
     }
     return launched();
 }

@@ -8,6 +8,8 @@ The kernels' contract is in ``include/cobalt_b200.h``.  There is no torch fallba
 from __future__ import annotations
 
 import ctypes
+import functools
+import weakref
 from typing import Optional
 
 import torch
@@ -22,38 +24,51 @@ _REDUCTIONS = ("none", "sum", "mean")
 
 def _call(index: int, name: str, *args):
     """A library call on device ``index`` and its current stream (the last argument)."""
-    lib = _lib.load()
+    fn = getattr(_lib.load(), name)
     if index == torch._C._cuda_getDevice():
-        rc = getattr(lib, name)(*args, _raw_stream(index))
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = getattr(lib, name)(*args, _raw_stream(index))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(name, rc)
 
 
-def _tokens(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(index: int, name: str, *sizes: int) -> int:
+    with torch.cuda.device(index):
+        return getattr(_lib.load(), name)(*sizes)
+
+
+def _gpu(name: str, t: torch.Tensor) -> int:
+    index = t.get_device()
+    if index < 0 or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor; there is no CPU path")
+    return index
+
+
+def _tokens(name: str, t: torch.Tensor, index: int) -> torch.Tensor:
     if t.dtype is not torch.int64:
         raise TypeError(f"{name} must be int64, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _matrix(name: str, t: torch.Tensor, width: int, unit: int = 1) -> torch.Tensor:
-    """``t [..., width]`` as rows that the kernels read where they lie, or a copy: neighbouring values, rows apart by a multiple of ``unit``
-    values that do not overlap (``unit`` > 1: on 16-byte boundaries)."""
-    if t.dim() < 1 or t.shape[-1] != width:
-        raise ValueError(f"{name} must be [..., {width}], got {list(t.shape)}")
-    rows = t if t.dim() == 2 else t.reshape(-1, width)
-    apart = rows.shape[0] > 1 and (rows.stride(0) < width or rows.stride(0) % unit)
-    if (rows.stride(1) != 1 and width > 1) or apart or (unit > 1 and rows.data_ptr() % 16):
+def _matrix(name: str, t: torch.Tensor, width: int, unit: int = 1):
+    """``(rows, their distance)``: ``t [..., width]`` as rows that the kernels read where they lie, or a copy: neighbouring values, rows apart by
+    a multiple of ``unit`` values that do not overlap (``unit`` > 1: on 16-byte boundaries)."""
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        raise ValueError(f"{name} must be [..., {width}], got {list(shape)}")
+    if t.is_contiguous() and (unit == 1 or t.data_ptr() % 16 == 0):
+        return t, width
+    rows = t if len(shape) == 2 else t.reshape(-1, width)
+    n, apart = rows.shape[0], rows.stride(0)
+    if (rows.stride(1) != 1 and width > 1) or (n > 1 and (apart < width or apart % unit)) or (unit > 1 and rows.data_ptr() % 16):
         rows = rows.clone(memory_format=torch.contiguous_format)
-    return rows
-
-
-def _apart(rows: torch.Tensor) -> int:
-    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
+        apart = width
+    return rows, apart if n > 1 else width
 
 
 # ----------------------------------------------------------------------------- embedding
@@ -61,74 +76,83 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
     """``table[ids] * scale``: rows of ``table [n_rows, width]`` (bf16, fp16 or fp32) for int64 ``ids`` of any shape, ``[*ids.shape, width]``.  The
     product is formed in fp32 and rounded once.  An id outside the table (-1: padding) reads zeros.  ``out`` (contiguous) receives the
     result.  Differentiable in ``table`` (``embed_grad``)."""
-    _check_table("table", table)
-    ids = _tokens("ids", ids, table.device)
-    grad = table.requires_grad and torch.is_grad_enabled()
+    index = _gpu("table", table)
+    shape, kind = table.shape, _TYPES.get(table.dtype)
+    if kind is None:
+        raise TypeError(f"table must be bfloat16, float16 or float32, got {table.dtype}")
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError(f"table must be [n_rows, width], got {list(shape)}")
+    ids = _tokens("ids", ids, index)
+    grad = torch.is_grad_enabled() and table.requires_grad
     if out is not None:
-        if out.shape != (*ids.shape, table.shape[1]) or out.dtype is not table.dtype or out.device != table.device or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {table.dtype} {[*ids.shape, table.shape[1]]} on {table.device}")
+        if out.shape != (*ids.shape, shape[1]) or out.dtype is not table.dtype or out.get_device() != index or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {table.dtype} {[*ids.shape, shape[1]]} on {table.device}")
         if grad or (out.requires_grad and torch.is_grad_enabled()):
             raise RuntimeError("out cannot take a result that requires a gradient")
     if grad:
-        leaves = _on_one_stream("embed", table)              # (alive until the graph holds them itself)
-        return _Embed.apply(ids, table, float(scale))
+        leaves = _leaves("embed", table)
+        return _seen(_Embed.apply(ids, table, float(scale)), leaves)
     return _embed(ids, table, float(scale), out)
 
 
-def _on_one_stream(name: str, *inputs: torch.Tensor):
-    """A captured backward pass must not reach a leaf through an autograd graph of another stream that still lives: torch would wait for that
-    stream, which invalidates the capture (or ends the process, where nothing catches it).  Said before, as far as these functions made that graph."""
-    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in inputs if t.requires_grad and t.is_leaf]
-    if nodes:
-        stream = _raw_stream(inputs[0].get_device())
-        for node in nodes:
-            seen = node.metadata.setdefault("cobalt_stream", stream)
-            if seen != stream and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"{name}: a graph of this leaf that was made on another stream is still alive; drop it before the capture, or capture "
-                                   "embed_grad / head_loss_and_grad, which need none")
-    return nodes
-
-
-def _check_table(name: str, t: torch.Tensor):
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor; there is no CPU path")
-    if t.dtype not in _TYPES:
-        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
-    if t.dim() != 2 or 0 in t.shape:
-        raise ValueError(f"{name} must be [n_rows, width], got {list(t.shape)}")
-
-
 def _embed(ids, table, scale, out=None):
-    width = table.shape[1]
-    rows = _matrix("table", table, width)
+    n_rows, width = table.shape
+    rows, apart = _matrix("table", table, width)
     if out is None:
         out = table.new_empty((*ids.shape, width))
     n = ids.numel()
     if n:
-        _call(table.get_device(), "cobalt_embed", ids.data_ptr(), n, rows.data_ptr(), _apart(rows), _TYPES[table.dtype], rows.shape[0], width, scale,
-              out.data_ptr(), width)
+        _call(table.get_device(), "cobalt_embed", ids.data_ptr(), n, rows.data_ptr(), apart, _TYPES[table.dtype], n_rows, width, scale, out.data_ptr(), width)
     return out
+
+
+_graphs = {}                                                 # by id of a leaf: (it, weakly; the stream of the last graph made here; that graph, weakly)
+
+
+def _leaves(name: str, *inputs: torch.Tensor):
+    """The inputs that are leaves, for ``_seen``.  A captured backward pass must not reach a leaf through an autograd graph of another stream that
+    still lives: torch would wait for that stream, which invalidates the capture (or ends the process, where nothing catches it).  Said
+    before, as far as these functions made that graph."""
+    leaves = [t for t in inputs if t.requires_grad and t.is_leaf]
+    if leaves and torch.cuda.is_current_stream_capturing():
+        stream = _raw_stream(leaves[0].get_device())
+        for t in leaves:
+            leaf, made, graph = _graphs.get(id(t), (None, stream, None))
+            if made != stream and leaf() is t and graph() is not None:
+                raise RuntimeError(f"{name}: a graph of this leaf that was made on another stream is still alive; drop it before the capture, or capture "
+                                   "embed_grad / head_loss_and_grad, which need none")
+    return leaves
+
+
+def _seen(result: torch.Tensor, leaves) -> torch.Tensor:
+    if leaves:
+        stream, graph = _raw_stream(leaves[0].get_device()), weakref.ref(result.grad_fn)
+        for t in leaves:
+            _graphs[id(t)] = weakref.ref(t), stream, graph
+        if len(_graphs) > 256:
+            for key in [k for k, (leaf, _, g) in _graphs.items() if leaf() is None or g() is None]:
+                _graphs.pop(key, None)
+    return result
 
 
 def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``embed`` with respect to its table, dense ``[n_rows, width]`` of ``grad``'s type: ``scale`` times the sum of the rows of
     ``grad [*ids.shape, width]`` by token, in fp32 and in the tokens' order.  Tokens outside the table are left out."""
-    if not grad.is_cuda:
-        raise RuntimeError("grad must be a CUDA tensor; there is no CPU path")
-    if grad.dtype not in _TYPES:
+    index, kind = _gpu("grad", grad), _TYPES.get(grad.dtype)
+    if kind is None:
         raise TypeError(f"grad must be bfloat16, float16 or float32, got {grad.dtype}")
-    ids = _tokens("ids", ids, grad.device)
-    if grad.dim() < 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] < 1 or n_rows < 1:
-        raise ValueError(f"grad must be [*ids.shape, width] = {[*ids.shape, 'width']} and n_rows at least 1, got {list(grad.shape)} and {n_rows}")
-    width, n = grad.shape[-1], ids.numel()
+    ids = _tokens("ids", ids, index)
+    shape = grad.shape
+    if not shape or shape[:-1] != ids.shape or shape[-1] < 1 or n_rows < 1:
+        raise ValueError(f"grad must be [*ids.shape, width] = {[*ids.shape, 'width']} and n_rows at least 1, got {list(shape)} and {n_rows}")
+    width, n = shape[-1], ids.numel()
     if n == 0:
         return grad.new_zeros((n_rows, width))
-    rows = _matrix("grad", grad, width)
+    rows, apart = _matrix("grad", grad, width)
     out = grad.new_empty((n_rows, width))
-    need = _lib.load().cobalt_embed_grad_scratch_bytes(n, width)
+    need = _scratch_bytes(index, "cobalt_embed_grad_scratch_bytes", n, width)
     scratch = out.new_empty(need, dtype=torch.uint8)         # per call, from the stream's own pool: overlapping calls never share one
-    _call(out.get_device(), "cobalt_embed_grad", ids.data_ptr(), n, rows.data_ptr(), _apart(rows), _TYPES[grad.dtype], n_rows, width, float(scale), out.data_ptr(),
-          scratch.data_ptr(), need)
+    _call(index, "cobalt_embed_grad", ids.data_ptr(), n, rows.data_ptr(), apart, kind, n_rows, width, float(scale), out.data_ptr(), scratch.data_ptr(), need)
     return out
 
 
@@ -152,11 +176,10 @@ def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, redu
     tokens that count.  A target outside the vocabulary (-1, -100: padding, a prompt) does not count: loss and gradient zero, whatever
     its row holds.  If none counts, the mean is 0.  Differentiable in ``x`` and ``weight``; the backward pass forms the logits once more.
     ``status`` (int32 ``[1]``, zero) takes the code of a bounded wait that gave up, as ``head_loss_status`` tells it without one."""
-    _check_loss(x, weight, targets, reduction, status)
-    targets = _tokens("targets", targets, x.device)
+    targets = _check_loss(x, weight, targets, reduction, status)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        leaves = _on_one_stream("head_loss", x, weight)      # (alive until the graph holds them itself)
-        return _HeadLoss.apply(x, weight, targets, reduction, status)
+        leaves = _leaves("head_loss", x, weight)
+        return _seen(_HeadLoss.apply(x, weight, targets, reduction, status), leaves)
     return _head_loss(x, weight, targets, reduction, status, False)[0]
 
 
@@ -164,8 +187,7 @@ def head_loss_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
                        need_x: bool = True, need_weight: bool = True, status: Optional[torch.Tensor] = None):
     """``(loss, dx, dw)`` of ``head_loss`` without autograd, for captured steps and loops of one's own.  ``grad``: fp32 gradient of the result (of
     its shape; ones by default).  ``need_x`` and ``need_weight``: which gradients are formed (``None`` else)."""
-    _check_loss(x, weight, targets, reduction, status)
-    targets = _tokens("targets", targets, x.device)
+    targets = _check_loss(x, weight, targets, reduction, status)
     shape = targets.shape if reduction == "none" else ()
     if grad is None:
         grad = x.new_ones((), dtype=torch.float32).expand(shape)
@@ -177,61 +199,62 @@ def head_loss_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     return loss, dx, dw
 
 
-def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str, status: Optional[torch.Tensor]):
-    for name, t in (("x", x), ("weight", weight)):
-        if not t.is_cuda:
-            raise RuntimeError(f"{name} must be a CUDA tensor; there is no CPU path")
-        if t.dtype is not torch.bfloat16:
-            raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
-    if weight.device != x.device:
+def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, reduction: str, status: Optional[torch.Tensor]) -> torch.Tensor:
+    """``targets`` as the kernels read them, if the arguments are in order."""
+    index = _gpu("x", x)
+    shape, head = x.shape, weight.shape
+    if x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
+        raise TypeError(f"x and weight must be bfloat16, got {x.dtype} and {weight.dtype}")
+    if _gpu("weight", weight) != index:
         raise ValueError(f"weight is on {weight.device}, x on {x.device}")
-    if weight.dim() != 2 or 0 in weight.shape or weight.shape[1] % 8:
-        raise ValueError(f"weight must be [vocab, hidden] with hidden a multiple of 8, got {list(weight.shape)}")
-    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x must be [..., {weight.shape[1]}], got {list(x.shape)}")
+    if len(head) != 2 or 0 in head or head[1] % 8:
+        raise ValueError(f"weight must be [vocab, hidden] with hidden a multiple of 8, got {list(head)}")
+    if not shape or shape[-1] != head[1]:
+        raise ValueError(f"x must be [..., {head[1]}], got {list(shape)}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
-    if targets.shape != x.shape[:-1]:
-        raise ValueError(f"targets must be {list(x.shape[:-1])}, got {list(targets.shape)}")
-    if status is not None and (status.dtype is not torch.int32 or status.shape != (1,) or status.device != x.device):
+    targets = _tokens("targets", targets, index)
+    if targets.shape != shape[:-1]:
+        raise ValueError(f"targets must be {list(shape[:-1])}, got {list(targets.shape)}")
+    if status is not None and (status.dtype is not torch.int32 or status.shape != (1,) or status.get_device() != index):
         raise ValueError(f"status must be int32 [1] on {x.device}, got {status.dtype} {list(status.shape)} on {status.device}")
+    return targets
 
 
 def _head_loss(x, weight, targets, reduction, status, keep):
     """(result, what the gradient needs: ``[n, 2]`` if ``keep``)"""
     V, H = weight.shape
     n = targets.numel()
+    new = functools.partial(x.new_empty, dtype=torch.float32)
     if n == 0:
-        empty = x.new_zeros(targets.shape if reduction == "none" else (), dtype=torch.float32)
-        return empty, x.new_empty((0, 2), dtype=torch.float32) if keep else None
-    rows, w = _matrix("x", x, H, 8), _matrix("weight", weight, H, 8)
-    loss = x.new_empty(targets.shape, dtype=torch.float32)
-    stats = x.new_empty((n, 2), dtype=torch.float32) if keep else None
-    total = x.new_empty((), dtype=torch.float32) if reduction != "none" else None
-    need = _lib.load().cobalt_head_loss_scratch_bytes(n, H, V)
+        return x.new_zeros(targets.shape if reduction == "none" else (), dtype=torch.float32), new((0, 2)) if keep else None
+    rows, apart = _matrix("x", x, H, 8)
+    w, apart_w = _matrix("weight", weight, H, 8)
+    loss, stats, total = new(targets.shape), new((n, 2)) if keep else None, new(()) if reduction != "none" else None
+    index = x.get_device()
+    need = _scratch_bytes(index, "cobalt_head_loss_scratch_bytes", n, H, V)
     scratch = x.new_empty(need, dtype=torch.uint8)
-    _call(x.get_device(), "cobalt_head_loss", rows.data_ptr(), _apart(rows), w.data_ptr(), _apart(w), targets.data_ptr(), n, H, V, loss.data_ptr(),
-          None if stats is None else stats.data_ptr(), None if total is None else total.data_ptr(), 1 if reduction == "mean" else 0, scratch.data_ptr(), need,
-          None if status is None else status.data_ptr())
+    _call(index, "cobalt_head_loss", rows.data_ptr(), apart, w.data_ptr(), apart_w, targets.data_ptr(), n, H, V, loss.data_ptr(), None if stats is None else stats.data_ptr(),
+          None if total is None else total.data_ptr(), 1 if reduction == "mean" else 0, scratch.data_ptr(), need, None if status is None else status.data_ptr())
     return loss if total is None else total, stats
 
 
 def _head_loss_grad(x, weight, targets, stats, grad, reduction, status, want_x, want_w):
     V, H = weight.shape
     n = targets.numel()
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else None
-    dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_w else None
+    dx = x.new_empty(x.shape) if want_x else None
+    dw = weight.new_empty((V, H)) if want_w else None
     if n == 0:
         return dx, None if dw is None else dw.zero_()
-    rows, w = _matrix("x", x, H, 8), _matrix("weight", weight, H, 8)
-    each = reduction == "none" and any(grad.stride(i) for i in range(grad.dim()) if grad.shape[i] > 1)      # (a sum's gradient is one value, expanded)
+    rows, apart = _matrix("x", x, H, 8)
+    w, apart_w = _matrix("weight", weight, H, 8)
+    each = reduction == "none" and any(step for step, size in zip(grad.stride(), grad.shape) if size > 1)   # (a sum's gradient is one value, expanded)
     if each:
         grad = grad.contiguous()
     index = x.get_device()
-    with torch.cuda.device(index):
-        need = _lib.load().cobalt_head_loss_grad_scratch_bytes(n, H, V, 1 if want_x else 0)
+    need = _scratch_bytes(index, "cobalt_head_loss_grad_scratch_bytes", n, H, V, 1 if want_x else 0)
     scratch = x.new_empty(need, dtype=torch.uint8)
-    _call(index, "cobalt_head_loss_grad", rows.data_ptr(), _apart(rows), w.data_ptr(), _apart(w), targets.data_ptr(), stats.data_ptr(), grad.data_ptr(), 1 if each else 0,
+    _call(index, "cobalt_head_loss_grad", rows.data_ptr(), apart, w.data_ptr(), apart_w, targets.data_ptr(), stats.data_ptr(), grad.data_ptr(), 1 if each else 0,
           1 if reduction == "mean" else 0, n, H, V, None if dx is None else dx.data_ptr(), H, None if dw is None else dw.data_ptr(), H, scratch.data_ptr(), need,
           None if status is None else status.data_ptr())
     return dx, dw

@@ -222,3 +222,13 @@ def test_refusals():
             bad()
     with pytest.raises(TypeError):
         cb.embed_grad(table[:3].int(), ids, 5)
+
+
+def test_a_table_that_was_used_can_be_copied_and_saved(tmp_path):
+    import copy
+    table = torch.nn.Parameter(torch.randn(5, 8, device="cuda"))
+    y = cb.embed(torch.tensor([1, 2], device="cuda"), table)
+    assert torch.equal(copy.deepcopy(table), table)
+    torch.save(table, tmp_path / "t.pt")
+    y.sum().backward()
+    assert float(table.grad.sum()) == 16

@@ -18,13 +18,14 @@ def test_tensors_off_the_gpu_are_refused():
 
 def test_rows_are_taken_where_they_lie_or_copied():
     m = torch.arange(7 * 24, dtype=torch.float32).view(7, 24).bfloat16()
-    assert vocab._matrix("x", m, 24, 8).data_ptr() == m.data_ptr()
+    assert vocab._matrix("x", m, 24, 8)[0].data_ptr() == m.data_ptr()
     for odd in (m[:, 1:17], m.t()[:, :7].t()[:, :16].flip(1), m[:, ::2][:, :8], m[:1, :16].expand(3, 16), m.as_strided((5, 16), (12, 1))):
         width = odd.shape[1]
-        got = vocab._matrix("x", odd, width, 8)
-        assert torch.equal(got, odd) and got.stride(1) == 1 and got.data_ptr() % 16 == 0 and (got.stride(0) % 8 == 0 and got.stride(0) >= width)
+        got, apart = vocab._matrix("x", odd, width, 8)
+        assert torch.equal(got, odd) and got.stride(1) == 1 and got.data_ptr() % 16 == 0 and apart % 8 == 0 and apart >= width
     part = m[:, 8:24]                                                  # a slice on 16-byte boundaries stays where it is
-    assert vocab._matrix("x", part, 16, 8).data_ptr() == part.data_ptr() and vocab._apart(part) == 24
+    got, apart = vocab._matrix("x", part, 16, 8)
+    assert got.data_ptr() == part.data_ptr() and apart == 24
     with pytest.raises(ValueError):
         vocab._matrix("x", m, 23)
 
