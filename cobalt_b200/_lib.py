@@ -127,7 +127,7 @@ EXPORTS = {
     "cobalt_head_loss_scratch_bytes": (c_size_t, [c_int, c_int, c_int64]),
     "cobalt_head_loss": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                  c_size_t, c_void_p, c_void_p]),
-    "cobalt_head_loss_grad_scratch_bytes": (c_size_t, [c_int, c_int, c_int64, c_int]),
+    "cobalt_head_loss_grad_scratch_bytes": (c_size_t, [c_int, c_int, c_int64, c_int, c_int]),
     "cobalt_head_loss_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int64, c_void_p,
                                       c_int64, c_void_p, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cobalt_vocab_status": (c_int, [c_void_p, POINTER(c_uint32)]),

@@ -1,0 +1,265 @@
+// The products of head_loss.cuh for few tokens (up to 128), which are bound by reading W once: the other way round.  W is the M side, 256 rows (or hidden
+// columns) a stage of 32 KB, and the tokens are the N side, 32 to 128 columns.
+//
+// In the pair kernel's tile the tokens are the 256 rows of A, most of them zeros that take half of every stage: five stages hold 70 KB of W in
+// flight, and 32000 x 4096 took 68 us for one token (3.9 TB/s).  Here six stages hold up to 192 KB.
+//
+//   stats, dlogits   A = W, two blocks of up to 128 of its rows; B = x.  A unit of work is `rows` rows, so many that the units go round the CTAs evenly.
+//                    TMEM lane = row of W, column = token: a warp's statistics are reductions over its lanes, 32 tokens at a time.
+//   dx               A = W with hidden columns as M (M-major as it lies), K = rows of W; B = d.  A unit is 256 hidden columns and a range of rows.
+//   warps 0-7  epilogue: warp w owns lanes 32 * (w % 4).. of block w / 4        warp 8  TMA        warp 9  MMA
+#pragma once
+#include "head_loss.cuh"
+
+namespace cb {
+
+constexpr int HF_TOKENS = 128;             // at most
+constexpr int HF_EPI_WARPS = 8;
+constexpr int HF_THREADS = HF_EPI_WARPS * 32 + 64;
+constexpr uint32_t HF_A_BYTES = 4 * HL_BOX;
+constexpr int hf_stages(int n_pad) { return n_pad <= 32 ? 6 : n_pad <= 96 ? 5 : 4; }
+constexpr uint32_t hf_stage_bytes(int n_pad) { return HF_A_BYTES + (uint32_t)n_pad * 128u; }
+constexpr uint32_t HF_SMEM = hf_stages(96) * hf_stage_bytes(96) + 256 + 1024;
+static_assert(hf_stages(32) * hf_stage_bytes(32) + 1280 <= HF_SMEM && hf_stages(64) * hf_stage_bytes(64) + 1280 <= HF_SMEM &&
+              hf_stages(128) * hf_stage_bytes(128) + 1280 <= HF_SMEM && HF_SMEM <= 227 * 1024, "stages of every size fit");
+
+struct HfParams {
+    int kind;                              // HL_STATS, HL_DLOGITS or HL_DX
+    int n, n_pad;                          // tokens; the N of the products, a multiple of 32
+    const int* count;                      // tokens that count, or null: all of n (their targets say so themselves)
+    int v0, cols;                          // piece of the vocabulary: its first row, and its rows inside the vocabulary
+    int units, rows;                       // stats, dlogits: rows of W a unit, a multiple of 16
+    int h_tiles, splits, add;              // dx: tiles of 256 hidden columns; ranges of the piece; the slabs hold the sums of earlier pieces
+    int hidden;
+    const long long* targets;              // stats: of every token
+    long long vocab;
+    const int* target;                     // dlogits: by place
+    int* counted;                          // stats: [0] tokens that count, [1] zero, for the kernel that joins
+    float2* part;                          // stats: [8 * units][n_pad]
+    float* at;
+    const float4* row;
+    uint16_t* d;
+    int ld_d;
+    float* slab;                           // [split][n][hidden]
+    uint32_t* status;
+};
+
+// Over the lanes of a warp and 32 values a lane: lane c gets the reduction of every lane's value c.  31 exchanges, each step halves the values.
+template <typename F>
+__device__ __forceinline__ float reduce_columns(float (&v)[32], int lane, F f) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        const bool up = (lane & s) != 0;
+#pragma unroll
+        for (int i = 0; i < s; ++i) {
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, up ? v[i] : v[i + s], s);
+            v[i] = f(up ? v[i + s] : v[i], got);
+        }
+    }
+    return v[0];
+}
+
+__global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_constant__ HfParams P, const __grid_constant__ CUtensorMap amap,
+                                                                 const __grid_constant__ CUtensorMap bmap) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full_mask = 0xFFFFFFFFu;
+    const uint32_t s0 = (smem_u32(smem) + 1023u) & ~1023u;
+    const uint32_t stages = (uint32_t)hf_stages(P.n_pad), stage_bytes = hf_stage_bytes(P.n_pad);
+    const uint32_t bars = s0 + stages * stage_bytes;
+    auto bar_full = [&](uint32_t s) { return bars + 8u * s; };
+    auto bar_empty = [&](uint32_t s) { return bars + 64u + 8u * s; };
+    auto bar_acc = [&](uint32_t b) { return bars + 128u + 8u * b; };
+    auto bar_free = [&](uint32_t b) { return bars + 144u + 8u * b; };
+    const uint32_t tmem_slot = bars + 160u;
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < stages; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
+        for (uint32_t b = 0; b < 2; ++b) { mbar_init(bar_acc(b), 1); mbar_init(bar_free(b), HF_EPI_WARPS); }
+        mbar_fence_init();
+        fence_proxy_async();
+    }
+    if (warp == HF_EPI_WARPS + 1) { tmem_alloc<false>(tmem_slot, 512); tmem_relinquish<false>(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = lds32(tmem_slot);
+    pdl_next();
+    pdl_wait();
+    const bool logits = P.kind != HL_DX;
+    const int k_all = ((logits ? P.hidden : P.cols) + HL_KS - 1) / HL_KS;
+    auto k_range = [&](int u, int* k0, int* k1) {
+        const int split = logits ? 0 : u / P.h_tiles;
+        *k0 = logits ? 0 : (int)((long long)k_all * split / P.splits);
+        *k1 = logits ? k_all : (int)((long long)k_all * (split + 1) / P.splits);
+    };
+
+    if (warp < HF_EPI_WARPS) {
+        // =========================================================== epilogue
+        const int block = warp >> 2, in_block = (warp & 3) * 32 + lane;
+        const uint32_t my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(block * P.n_pad);
+        const int tokens = P.count ? *P.count : P.n;
+        if (P.kind == HL_STATS && blockIdx.x == 0 && warp == 0) {
+            int counted = 0;
+            for (int i = lane; i < P.n; i += 32) counted += P.targets[i] >= 0 && P.targets[i] < P.vocab ? 1 : 0;
+            counted = __reduce_add_sync(full_mask, counted);
+            if (lane == 0) { P.counted[0] = counted; P.counted[1] = 0; }
+        }
+        bool healthy = true;
+        uint32_t buf = 0, ph = 0;
+        for (int u = blockIdx.x; u < P.units; u += gridDim.x) {
+            int k0, k1;
+            k_range(u, &k0, &k1);
+            float acc[HF_TOKENS];
+#pragma unroll
+            for (int q = 0; q < HF_TOKENS; ++q) acc[q] = 0.0f;
+            for (int k = k0; k < k1; k += logits ? HL_SUM_STAGES : k1 - k0) {
+                if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded(bar_acc(buf), ph, P.status, DEV_TIMEOUT_ACC));
+                tc_fence_after();
+#pragma unroll
+                for (int q = 0; q < HF_TOKENS / 32; ++q) {
+                    if (32 * q >= P.n_pad) continue;
+                    uint32_t v[32];
+                    tmem_ld32(my_tmem + buf * 2u * (uint32_t)P.n_pad + 32u * q, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) acc[32 * q + e] += healthy ? __uint_as_float(v[e]) : __uint_as_float(0x7FC00000u);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0 && healthy) mbar_arrive(bar_free(buf));
+                buf ^= 1u;
+                if (buf == 0) ph ^= 1u;
+            }
+            if (logits) {
+                const int half = P.rows / 2, in_piece = u * P.rows + block * half + in_block, row = P.v0 + in_piece;
+                const bool mine = in_block < half && in_piece < P.cols;
+#pragma unroll
+                for (int q = 0; q < HF_TOKENS / 32; ++q) {
+                    if (32 * q >= P.n_pad) continue;
+                    const int token = 32 * q + lane;
+                    if (P.kind == HL_STATS) {
+                        float v[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = acc[32 * q + e] = mine ? acc[32 * q + e] : -INFINITY;
+                        const float top = reduce_columns(v, lane, [](float a, float b) { return fmaxf(a, b); });
+                        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = exp2_fast((acc[32 * q + e] - __shfl_sync(full_mask, base, e)) * LOG2E);
+                        const float sum = reduce_columns(v, lane, [](float a, float b) { return a + b; });
+                        P.part[((long long)u * HF_EPI_WARPS + warp) * P.n_pad + token] = make_float2(top, sum);
+                        // the token whose target is this row: its logit
+                        const long long t = token < P.n ? P.targets[token] : -1;
+                        const int rel = t >= 0 && t < P.vocab ? (int)t - (row - lane) : -1;      // lane of this warp that holds it
+                        for (unsigned left = __ballot_sync(full_mask, rel >= 0 && rel < 32); left; left &= left - 1) {
+                            const int e = __ffs(left) - 1, holder = __shfl_sync(full_mask, rel, e);
+                            float own = 0.0f;
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) own = c == e ? acc[32 * q + c] : own;
+                            if (lane == holder && mine) P.at[32 * q + e] = own;
+                        }
+                    } else {
+                        const bool in_d = in_block < half && in_piece < P.ld_d;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int c = 32 * q + e;
+                            if (c >= P.n) continue;
+                            float g = 0.0f;
+                            if (c < tokens && mine) {
+                                const float4 r = P.row[c];
+                                g = exp2_fast(fmaf(acc[c] - r.x, LOG2E, -r.y));
+                                if (P.target[c] == row) g -= 1.0f;
+                                g *= r.z;
+                            }
+                            if (in_d) P.d[(long long)c * P.ld_d + in_piece] = float_to_bf16(g);
+                        }
+                    }
+                }
+            } else {
+                const int split = u / P.h_tiles, h = (u - split * P.h_tiles) * HL_TILE + block * 128 + in_block;
+                float* dst = P.slab + (long long)split * P.n * P.hidden + h;
+                if (h < P.hidden) {
+#pragma unroll
+                    for (int c = 0; c < HF_TOKENS; ++c) {
+                        if (c >= P.n) continue;
+                        float* at = dst + (long long)c * P.hidden;
+                        *at = P.add ? *at + acc[c] : acc[c];
+                    }
+                }
+            }
+        }
+    } else if (warp == HF_EPI_WARPS) {
+        // =========================================================== TMA
+        bool good = true;
+        uint32_t s = 0, ph = 0;
+        const uint32_t bytes = (logits ? (uint32_t)P.rows * 128u : HF_A_BYTES) + (uint32_t)P.n_pad * 128u;
+        for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
+            int k0, k1;
+            k_range(u, &k0, &k1);
+            const int h0 = logits ? 0 : u % P.h_tiles * HL_TILE, r0 = P.v0 + (logits ? u * P.rows : 0);
+            for (int k = k0; k < k1; ++k) {
+                good = __all_sync(full_mask, mbar_wait_bounded(bar_empty(s), ph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
+                if (!good) break;
+                const uint32_t dst = s0 + s * stage_bytes, bar = bar_full(s);
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bar, bytes);
+                    if (logits) {
+                        tma_load_2d<false>(dst, &amap, k * HL_KS, r0, bar);
+                        tma_load_2d<false>(dst + 2 * HL_BOX, &amap, k * HL_KS, r0 + P.rows / 2, bar);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) tma_load_2d<false>(dst + b * HL_BOX, &amap, h0 + 64 * b, r0 + k * HL_KS, bar);
+                    }
+                    tma_load_2d<false>(dst + HF_A_BYTES, &bmap, k * HL_KS, 0, bar);
+                }
+                __syncwarp();
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else {
+        // =========================================================== MMA
+        bool good = true;
+        uint32_t s = 0, ph = 0, buf = 0, aph = 0;
+        const uint32_t idesc = umma_idesc((uint32_t)P.n_pad) | (logits ? 0u : 1u << 15);
+        const uint64_t a_step = logits ? 32 >> 4 : 2048 >> 4;
+        for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
+            int first, last;
+            k_range(u, &first, &last);
+            const int per = logits ? HL_SUM_STAGES : last - first;
+            for (int k0 = first; good && k0 < last; k0 += per) {
+                good = __all_sync(full_mask, mbar_wait_bounded(bar_free(buf), aph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
+                if (!good) break;
+                tc_fence_after();
+                const uint32_t d = tmem + buf * 2u * (uint32_t)P.n_pad;
+                const int k1 = min(last, k0 + per);
+                for (int k = k0; k < k1; ++k) {
+                    good = __all_sync(full_mask, mbar_wait_bounded(bar_full(s), ph, P.status, DEV_TIMEOUT_FULL));
+                    if (!good) break;
+                    tc_fence_after();
+                    const uint32_t at = s0 + s * stage_bytes;
+                    const uint64_t bd = umma_smem_desc(at + HF_A_BYTES);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const uint64_t ad = logits ? umma_smem_desc(at + b * 2 * HL_BOX) : umma_smem_desc_mn(at + b * 2 * HL_BOX, HL_BOX);
+#pragma unroll
+                            for (int q = 0; q < HL_KS / 16; ++q)
+                                umma_bf16<false>(d + (uint32_t)(b * P.n_pad), ad + a_step * q, bd + (uint64_t)(2 * q), idesc, (k > k0 || q > 0) ? 1u : 0u);
+                        }
+                        umma_commit<false>(bar_empty(s));
+                    }
+                    __syncwarp();
+                    if (++s == stages) { s = 0; ph ^= 1u; }
+                }
+                if (good && elect_one()) umma_commit<false>(bar_acc(buf));
+                __syncwarp();
+                buf ^= 1u;
+                if (buf == 0) aph ^= 1u;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == HF_EPI_WARPS + 1) { tc_fence_after(); tmem_dealloc<false>(tmem, 512); }
+}
+
+}  // namespace cb

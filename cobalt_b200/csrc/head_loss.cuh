@@ -10,7 +10,9 @@
 // Operands come by TMA in boxes of 64 x 64, whatever their order: a box is 64 rows of 128 swizzled bytes, and which of its sides is K is
 // the descriptor's business.
 //   warps 0-7  epilogue: warp w owns TMEM lanes 32 * (w % 4).. (a thread = a row) and columns 128 * (w / 4)..
-//   warp 8     TMA         warp 9     MMA (of the pair's first CTA)
+//   warp 8     TMA         warp 9     MMA (of the pair's first CTA)        warps 10, 11     none: they fill a warpgroup
+// An epilogue thread holds 128 sums.  The 168 registers that 384 threads have each do not hold them and what belongs to them, and what is
+// spilled goes to the L2 (227 KB of shared memory leave little L1): warps 8-11 hand registers over, 216 to 72.
 // Two accumulators of 256 columns: the epilogue of a tile runs under the next one's products.
 //
 // Tokens without a target are left out beforehand (prepare kernel: targets and rows of x that count, packed in order), so a prompt that is not
@@ -30,13 +32,17 @@ namespace cb {
 
 constexpr int HL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int HL_KS = 64;                  // K per stage
-constexpr int HL_STAGES = 6;
+constexpr int HL_STAGES = 5;
 constexpr uint32_t HL_BOX = 64 * 128;      // bytes of 64 rows x 64 bf16
 constexpr uint32_t HL_STAGE_BYTES = 4 * HL_BOX;
 constexpr int HL_EPI_WARPS = 8;
-constexpr int HL_THREADS = HL_EPI_WARPS * 32 + 64;
+constexpr int HL_COLS = 128;               // columns of an epilogue warp
+constexpr int HL_THREADS = HL_EPI_WARPS * 32 + 128;
+constexpr int HL_REGS = 168, HL_EPI_REGS = 216, HL_ROLE_REGS = 72;     // of a thread: at the launch, epilogue, the others
+static_assert(HL_EPI_REGS * HL_EPI_WARPS * 32 + HL_ROLE_REGS * 128 <= HL_REGS * HL_THREADS, "no more than the block was launched with");
 constexpr int HL_SUM_STAGES = 8;           // stages of logits that are summed in tensor memory
-constexpr uint32_t HL_SMEM = HL_STAGES * HL_STAGE_BYTES + 256 + 1024;
+constexpr uint32_t HL_OUT_BYTES = 32 * 128;                // results of a warp on their way out: 32 rows of 128 swizzled bytes, twice
+constexpr uint32_t HL_SMEM = HL_STAGES * HL_STAGE_BYTES + HL_EPI_WARPS * 2 * HL_OUT_BYTES + 256 + 1024;
 constexpr int HL_JOBS = 3;
 constexpr float LOG2E = 1.44269504088896341f;
 
@@ -47,6 +53,7 @@ struct HlJob {
     int kind;
     int v0, cols;                          // piece of the vocabulary: its first row, and its rows inside the vocabulary
     int n_tiles;                           // tiles along B's side: of the piece (stats, dlogits) or of hidden columns (dx, dw)
+    int width;                             // their columns: 256, of logits any multiple of 16 up to that
     int splits;                            // dx: ranges of the piece that are summed in slabs of their own
     int add;                               // dx: the slabs hold the sums of earlier pieces
     int buf;                               // which of the two scratch pieces holds d
@@ -67,65 +74,142 @@ struct HlParams {
     const float* factor;                   // dw: of the sums
     uint16_t* d[2];                        // [rounded rows][ld_d]
     int ld_d;
-    float* slab;                           // dx
-    uint16_t* dw;
-    long long ld_dw;
-    int wide;                              // dw's rows are 32-byte aligned
     uint32_t* status;
 };
+struct HlMaps {
+    CUtensorMap x, w, w_tile, d[2];        // bf16, boxes of 64 x 64; w_tile: 64 columns of half a tile's rows
+    CUtensorMap slab, dw;                  // results: fp32 [split][token][hidden], boxes of 32 x 32; bf16, boxes of 64 columns x 32 rows
+};
 
-struct HlTile { int job, kind, m, n, k0, k1; };
+struct HlTile { int m, n, split, k0, k1; };
 
-// Tile i of the launch's list.  Jobs follow one another.  Logits: tokens in groups of at most 12 tiles, so that a group's x stays in the L2
-// while the vocabulary streams by, once a group; gradients: neighbours share the operand that is longer.
-__device__ __forceinline__ bool hl_tile(const HlParams& P, int tokens, int i, HlTile* t) {
-    const int nt = min(max((tokens - P.tok0 + HL_TILE - 1) / HL_TILE, 1), P.tok_tiles);
-#pragma unroll
-    for (int j = 0; j < HL_JOBS; ++j) {
-        if (j >= P.n_jobs) return false;
-        const HlJob& J = P.job[j];
-        const int m_tiles = J.kind == HL_DW ? (J.cols + HL_TILE - 1) / HL_TILE : nt;
-        const int all = m_tiles * J.n_tiles * J.splits;
-        if (i >= all) { i -= all; continue; }
-        t->job = j;
-        t->kind = J.kind;
+// The tiles of a pair of CTAs, one after another.  Jobs follow one another, a job's tiles go round the pairs.  dx comes first, in few long tiles: the pairs
+// that get one less than others take that many more tiles of dw, so that all end together (2458 tokens of 4096 x 32000, 160 tiles of
+// dx on 74 pairs: 1012 -> TIME_SCHED us for both products).
+struct HlList {
+    int pair, pairs, tokens, token_tiles;
+    int job, next;                         // current job, and the number of the next tile that the pair takes of it
+    HlJob J;                               // the job, in registers
+    int m_tiles, tiles;
+    int shift;                             // the pair's place in the round of the current job
+    int extra, few_from, few;              // rounds that only the pairs from few_from on take part in, `few` of them
+    int at_m, at_n, step_m, step_n;        // gradients: the last tile (at_m < 0: none yet), and the way to the next
+
+    __device__ __forceinline__ HlList(const HlParams& P, int pair_, int pairs_, int tokens_) {
+        pair = pair_; pairs = pairs_; tokens = tokens_;
+        token_tiles = min(max((tokens - P.tok0 + HL_TILE - 1) / HL_TILE, 1), P.tok_tiles);
+        next = 0;
+        shift = pair;
+        extra = few_from = 0;
+        few = pairs;
+        open(P, 0);
+    }
+    __device__ __forceinline__ void open(const HlParams& P, int j) {
+        job = j;
+        at_m = -1;
+        if (j < P.n_jobs) J = P.job[j];
+        m_tiles = J.kind == HL_DW ? (J.cols + HL_TILE - 1) / HL_TILE : token_tiles;
+        tiles = m_tiles * J.n_tiles * J.splits;
+    }
+    __device__ __forceinline__ int stages(const HlParams& P) const {
+        return J.kind <= HL_DLOGITS ? (P.hidden + HL_KS - 1) / HL_KS : J.kind == HL_DX ? (J.cols + HL_KS - 1) / HL_KS / J.splits : max((tokens + HL_KS - 1) / HL_KS, 1);
+    }
+    __device__ __forceinline__ bool take(const HlParams& P, HlTile* t) {
+        if (at_m >= 0) {                                               // rounds of all pairs in a gradient of one range
+            at_m += step_m;
+            at_n += step_n;
+            if (at_n >= J.n_tiles) { at_n -= J.n_tiles; ++at_m; }
+            if (at_m < m_tiles) {
+                t->m = at_m;
+                t->n = at_n;
+                return true;
+            }
+            next = tiles;                                              // none is left
+        }
+        while (job < P.n_jobs) {
+            int i = tiles;
+            if (next < extra) {
+                if (pair >= few_from) i = pair - few_from + next * few;
+                else next = extra;                                     // (not in these rounds)
+            }
+            if (next >= extra && next < tiles) i = extra * few + shift + (next - extra) * pairs;
+            if (i < tiles) {
+                place(P, i, t);
+                if (next >= extra && J.kind >= HL_DX && J.splits == 1) {
+                    at_m = t->m;
+                    at_n = t->n;
+                    step_m = pairs / J.n_tiles;
+                    step_n = pairs - step_m * J.n_tiles;
+                }
+                ++next;
+                return true;
+            }
+            // the next job: who is ahead, and by how many of its tiles
+            const int rest = max(tiles - extra * few, 0) % pairs;      // places of the last round that were taken
+            const int ahead = rest && J.kind == HL_DX ? stages(P) : 0;
+            next = extra = 0;
+            shift = shift >= rest ? shift - rest : shift - rest + pairs;       // the others go first
+            open(P, job + 1);
+            if (job < P.n_jobs && ahead) {
+                few_from = rest;
+                few = pairs - rest;
+                const int each = stages(P);
+                extra = min((ahead + each / 2) / each, tiles / few);
+            }
+        }
+        return false;
+    }
+    // Tile i of a job.  Logits: tokens in groups of at most 12 tiles, so that a group's x stays in the L2 while the vocabulary streams by, once a
+    // group; gradients: neighbours share the operand that is longer.
+    __device__ __forceinline__ void place(const HlParams& P, int i, HlTile* t) const {
         t->k0 = 0;
+        t->split = 0;
         if (J.kind <= HL_DLOGITS) {
-            const int groups = (nt + 11) / 12, per = (nt + groups - 1) / groups;
-            const int g = i / (per * J.n_tiles), in = i - g * per * J.n_tiles, width = min(per, nt - g * per);
+            const int groups = (token_tiles + 11) / 12, per = (token_tiles + groups - 1) / groups;
+            const int g = i / (per * J.n_tiles), in = i - g * per * J.n_tiles, width = min(per, token_tiles - g * per);
             t->n = in / width;
             t->m = g * per + in - t->n * width;
             t->k1 = (P.hidden + HL_KS - 1) / HL_KS;
         } else if (J.kind == HL_DX) {
-            const int ks = (J.cols + HL_KS - 1) / HL_KS, s = i / (m_tiles * J.n_tiles), in = i - s * m_tiles * J.n_tiles;
+            const int ks = (J.cols + HL_KS - 1) / HL_KS, one = token_tiles * J.n_tiles, s = i / one, in = i - s * one;
+            t->split = s;
             t->m = in / J.n_tiles;
             t->n = in - t->m * J.n_tiles;
             t->k0 = (int)((long long)ks * s / J.splits);
             t->k1 = (int)((long long)ks * (s + 1) / J.splits);
-            t->m |= s << 20;                               // the split rides along
         } else {
             t->m = i / J.n_tiles;
             t->n = i - t->m * J.n_tiles;
             t->k1 = max((tokens + HL_KS - 1) / HL_KS, 1);
         }
-        return true;
     }
-    return false;
-}
+};
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+}
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }       // all but the last one
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
-__global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __grid_constant__ HlParams P, const __grid_constant__ CUtensorMap xmap,
-                                                                     const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap dmap0,
-                                                                     const __grid_constant__ CUtensorMap dmap1) {
+__global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __grid_constant__ HlParams P, const __grid_constant__ HlMaps M) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full_mask = 0xFFFFFFFFu;
     const uint32_t s0 = (smem_u32(smem) + 1023u) & ~1023u;
-    const uint32_t bars = s0 + HL_STAGES * HL_STAGE_BYTES;
+    const uint32_t outs = s0 + HL_STAGES * HL_STAGE_BYTES, bars = outs + HL_EPI_WARPS * 2 * HL_OUT_BYTES;
     auto bar_full = [&](uint32_t s) { return bars + 8u * s; };
     auto bar_empty = [&](uint32_t s) { return bars + 64u + 8u * s; };
     auto bar_acc = [&](uint32_t b) { return bars + 128u + 8u * b; };
@@ -146,179 +230,225 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
     cluster_sync_all();                                    // the other CTA's barriers are in place before anyone arrives on them
     tc_fence_after();
     const uint32_t tmem = lds32(tmem_slot);
+    pdl_next();
+    pdl_wait();
     const int tokens = *P.count;
+    HlList list(P, pair, pairs, tokens);
     HlTile t;
 
     if (warp < HL_EPI_WARPS) {
         // =========================================================== epilogue
-        const uint32_t my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(warp >> 2) * 128u;
-        const int my_row = (int)rank * 128 + (warp & 3) * 32 + lane, my_col = (warp >> 2) * 128;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(HL_EPI_REGS));
+        const int part = warp >> 2;                        // which columns of the tile
+        const uint32_t my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)part * HL_COLS;
+        const int my_row = (int)rank * 128 + (warp & 3) * 32 + lane, my_col = part * HL_COLS;
+        const uint32_t out = outs + (uint32_t)warp * 2 * HL_OUT_BYTES, my_out = out + (uint32_t)lane * 128u;
+        const uint32_t x7 = (uint32_t)(lane & 7);
+        const float factor = P.factor ? *P.factor : 0.0f;
         bool healthy = true;
-        uint32_t buf = 0, ph = 0;
-        for (int i = pair; hl_tile(P, tokens, i, &t); i += pairs) {
-            const HlJob& J = P.job[t.job];
-            const bool logits = t.kind <= HL_DLOGITS;
-            const int split = t.m >> 20, row = (t.m & 0xFFFFF) * HL_TILE + my_row, col = t.n * HL_TILE + my_col;
-            const int r = t.kind == HL_STATS ? P.tok0 + row : row;
-            // what a row of logits needs; requested under the products
-            int target = -1;
-            float4 rowv = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (logits && r < tokens) {
-                target = P.target[r] - J.v0 - col;
-                if (t.kind == HL_DLOGITS) rowv = P.row[r];
+        uint32_t buf = 0, ph = 0, side = 0;                // which accumulator comes next, and which half of `out`
+        auto wait_acc = [&]() {
+            if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded<true>(bar_acc(buf), ph, P.status, DEV_TIMEOUT_ACC));
+            tc_fence_after();
+        };
+        auto free_acc = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && healthy) mbar_arrive_cluster(map_to_rank(bar_free(buf), 0));
+            buf ^= 1u;
+            if (buf == 0) ph ^= 1u;
+        };
+        float acc[HL_COLS];
+        auto spoil = [&]() {                               // a wait gave up: everything that this tile feeds becomes NaN
+            if (healthy) return;
+#pragma unroll
+            for (int e = 0; e < HL_COLS; ++e) acc[e] = __uint_as_float(0x7FC00000u);
+        };
+        auto take_columns = [&]() {                        // the accumulator's columns
+            wait_acc();
+            uint32_t(&v)[4][32] = *reinterpret_cast<uint32_t(*)[4][32]>(&acc);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tmem_ld32(my_tmem + buf * 256u + 32u * q, v[q]);
+            tmem_ld_wait();
+            free_acc();
+        };
+        auto add_columns = [&]() {                         // on top of what there is
+            wait_acc();
+#pragma unroll
+            for (int q = 0; q < HL_COLS; q += 32) {
+                uint32_t v[32];
+                tmem_ld32(my_tmem + buf * 256u + (uint32_t)q, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) acc[q + e] += __uint_as_float(v[e]);
             }
-            float acc[128];
+            free_acc();
+        };
+        while (list.take(P, &t)) {
+            const HlJob& J = list.J;
+            const int row = t.m * HL_TILE + my_row, col = t.n * J.width + my_col;
+            if (J.kind <= HL_DLOGITS) {
+                const int r = J.kind == HL_STATS ? P.tok0 + row : row;
+                // what a row of logits needs; requested under the products
+                int target = -1;
+                float4 rowv = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (r < tokens) {
+                    target = P.target[r] - J.v0 - col;
+                    if (J.kind == HL_DLOGITS) rowv = P.row[r];
+                }
+                take_columns();
+                for (int k = t.k0 + HL_SUM_STAGES; k < t.k1; k += HL_SUM_STAGES) add_columns();
+                spoil();
+                int here = min(J.width - my_col, HL_COLS);             // columns of this warp that are the tile's
+                if (J.kind == HL_DLOGITS) here = min(here, P.ld_d - col);
+                const int valid = min(here, J.cols - col);             // ... and inside the vocabulary
+                if (target >= here) target = -1;
+                if (J.kind == HL_STATS) {
+                    if (valid < HL_COLS) {
 #pragma unroll
-            for (int q = 0; q < 128; ++q) acc[q] = 0.0f;
-            for (int k = t.k0; k < t.k1; k += logits ? HL_SUM_STAGES : t.k1 - t.k0) {
-                if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded<true>(bar_acc(buf), ph, P.status, DEV_TIMEOUT_ACC));
-                if (healthy) {
-                    tc_fence_after();
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t v[32];
-                        tmem_ld32(my_tmem + buf * 256u + 32u * q, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) acc[32 * q + e] += __uint_as_float(v[e]);
+                        for (int q = 0; q < HL_COLS; ++q)
+                            if (q >= valid) acc[q] = -INFINITY;
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(map_to_rank(bar_free(buf), 0));
-                }
-                buf ^= 1u;
-                if (buf == 0) ph ^= 1u;
-            }
-            if (!healthy) {                                // a wait gave up: everything that this tile feeds becomes NaN
+                    float m[4] = {acc[0], acc[1], acc[2], acc[3]};
 #pragma unroll
-                for (int q = 0; q < 128; ++q) acc[q] = __uint_as_float(0x7FC00000u);
-            }
-            if (t.kind == HL_STATS) {
-                const int valid = J.cols - col;            // columns of this half inside the vocabulary
-                if (valid < 128) {
+                    for (int q = 4; q < HL_COLS; ++q) m[q & 3] = fmaxf(m[q & 3], acc[q]);
+                    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), base = top == -INFINITY ? 0.0f : top;
+                    if (__any_sync(full_mask, target >= 0)) {
+                        float own = 0.0f;
 #pragma unroll
-                    for (int q = 0; q < 128; ++q)
-                        if (q >= valid) acc[q] = -INFINITY;
-                }
-                float m[4] = {acc[0], acc[1], acc[2], acc[3]};
-#pragma unroll
-                for (int q = 4; q < 128; ++q) m[q & 3] = fmaxf(m[q & 3], acc[q]);
-                const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), base = top == -INFINITY ? 0.0f : top;
-                if (__any_sync(full_mask, target >= 0 && target < 128)) {
-                    float own = 0.0f;
-#pragma unroll
-                    for (int q = 0; q < 128; ++q) own = q == target ? acc[q] : own;
-                    if (target >= 0 && target < 128) P.at[r] = own;
-                }
-                // (the difference first: the product of a large logit with log2(e) would be rounded where the difference is exact)
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int q = 0; q < 128; ++q) s[q & 3] += exp2_fast((acc[q] - base) * LOG2E);
-                P.part[(long long)(2 * t.n + (warp >> 2)) * P.ld_part + row] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
-            } else if (t.kind == HL_DLOGITS) {
-                const bool in = row < tokens;
-                const int valid = in ? J.cols - col : 0;
-                uint16_t* dst = P.d[J.buf] + (long long)row * P.ld_d + col;
-                const bool mine = __any_sync(full_mask, target >= 0 && target < 128);
-#pragma unroll
-                for (int q = 0; q < 128; q += 16) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float p[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int c = q + 2 * e + h;
-                            p[h] = exp2_fast(fmaf(acc[c] - rowv.x, LOG2E, -rowv.y));
-                            if (mine && c == target) p[h] -= 1.0f;
-                            p[h] = c < valid ? p[h] * rowv.z : 0.0f;
-                        }
-                        w[e] = pack_bf16x2(p[0], p[1]);
+                        for (int q = 0; q < HL_COLS; ++q) own = q == target ? acc[q] : own;
+                        if (target >= 0) P.at[r] = own;
                     }
-                    store32(dst + q, w);
-                }
-            } else if (t.kind == HL_DX) {
-                if (row < tokens) {
-                    float* dst = P.slab + ((long long)split * P.n_rows + row) * P.hidden + col;
+                    // (the difference first: the product of a large logit with log2(e) would be rounded where the difference is exact)
+                    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int q = 0; q < 128; q += 4) {
-                        if (col + q >= P.hidden) continue;
-                        float4 v = make_float4(acc[q], acc[q + 1], acc[q + 2], acc[q + 3]);
-                        if (J.add) {
-                            const float4 o = *reinterpret_cast<const float4*>(dst + q);
-                            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+                    for (int q = 0; q < HL_COLS; ++q) s[q & 3] += exp2_fast((acc[q] - base) * LOG2E);
+                    const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+                    P.part[(long long)(2 * t.n + part) * P.ld_part + row] = make_float2(top, sum);
+                } else if (row < P.n_rows) {
+                    const int kept = row < tokens ? valid : 0;
+                    uint16_t* dst = P.d[J.buf] + (long long)row * P.ld_d + col;
+#pragma unroll
+                    for (int q = 0; q < HL_COLS; q += 16) {
+                        if (q >= here) continue;
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float p[2];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int c = q + 2 * e + h;
+                                p[h] = exp2_fast(fmaf(acc[c] - rowv.x, LOG2E, -rowv.y));
+                                if (c == target) p[h] -= 1.0f;
+                                p[h] = c < kept ? p[h] * rowv.z : 0.0f;
+                            }
+                            w[e] = pack_bf16x2(p[0], p[1]);
                         }
-                        *reinterpret_cast<float4*>(dst + q) = v;
+                        store32(dst + q, w);
                     }
                 }
             } else {
-                const float g = *P.factor;
-                if (row < J.cols) {
-                    uint16_t* dst = P.dw + (long long)(J.v0 + row) * P.ld_dw + col;
+                take_columns();
+                spoil();
+                if (col >= P.hidden) continue;
+                // out by the copy engine, over shared memory: 64 columns of dw at a time; 32 of dx, which it adds up: one addition a piece, in their order
+                if (J.kind == HL_DX) {
 #pragma unroll
-                    for (int q = 0; q < 128; q += 16) {
-                        uint32_t w[8];
+                    for (int q = 0; q < 4; ++q) {
+                        if (col + 32 * q >= P.hidden) continue;
+                        if (lane == 0) bulk_wait_read();               // the last copy but one is out of here
+                        __syncwarp();
+                        const float* v = acc + 32 * q;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(acc[q + 2 * e] * g, acc[q + 2 * e + 1] * g);
-                        if (P.wide && col + q + 16 <= P.hidden) {
-                            store32(dst + q, w);
-                        } else {                           // (the width is a multiple of 8)
-                            if (col + q < P.hidden) *reinterpret_cast<uint4*>(dst + q) = make_uint4(w[0], w[1], w[2], w[3]);
-                            if (col + q + 8 < P.hidden) *reinterpret_cast<uint4*>(dst + q + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                        for (int c = 0; c < 8; ++c)
+                            sts128(my_out + side + (((uint32_t)c ^ x7) << 4), __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]),
+                                   __float_as_uint(v[4 * c + 3]));
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (J.add) tma_add_3d(&M.slab, out + side, col + 32 * q, row, t.split);
+                            else tma_store_3d(&M.slab, out + side, col + 32 * q, row, t.split);
+                            bulk_commit();
                         }
+                        side ^= HL_OUT_BYTES;
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        if (col + 64 * q >= P.hidden) continue;
+                        if (lane == 0) bulk_wait_read();
+                        __syncwarp();
+                        const float* v = acc + 64 * q;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            sts128(my_out + side + (((uint32_t)c ^ x7) << 4), pack_bf16x2(v[8 * c] * factor, v[8 * c + 1] * factor),
+                                   pack_bf16x2(v[8 * c + 2] * factor, v[8 * c + 3] * factor), pack_bf16x2(v[8 * c + 4] * factor, v[8 * c + 5] * factor),
+                                   pack_bf16x2(v[8 * c + 6] * factor, v[8 * c + 7] * factor));
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&M.dw, out + side, col + 64 * q, J.v0 + row);
+                            bulk_commit();
+                        }
+                        side ^= HL_OUT_BYTES;
                     }
                 }
             }
         }
-    } else if (warp == HL_EPI_WARPS) {
+        if (lane == 0) bulk_wait_all();
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(HL_ROLE_REGS));
+    if (warp == HL_EPI_WARPS) {
         // =========================================================== TMA
         bool good = true;
         uint32_t s = 0, ph = 0;
         const int mine = (int)rank * 128;
-        for (int i = pair; good && hl_tile(P, tokens, i, &t); i += pairs) {
-            const HlJob& J = P.job[t.job];
-            const int m0 = (t.m & 0xFFFFF) * HL_TILE + mine, n0 = t.n * HL_TILE + mine;
-            const CUtensorMap* const dmap = J.buf ? &dmap1 : &dmap0;
+        while (good && list.take(P, &t)) {
+            const HlJob& J = list.J;
+            const int m0 = t.m * HL_TILE + mine, n0 = t.n * J.width + (int)rank * (J.width / 2);
+            const CUtensorMap* const dmap = &M.d[J.buf];
             const CUtensorMap *am, *bm;
             bool a_rows, b_rows;                           // the operand's rows are the tensor's rows (K-major), else its columns
             int ax, ay, bx, by;                            // at K = 0
-            if (t.kind <= HL_DLOGITS) {
-                am = &xmap; a_rows = true; ax = 0; ay = m0 + (t.kind == HL_STATS ? P.tok0 : 0);
-                bm = &wmap; b_rows = true; bx = 0; by = J.v0 + n0;
-            } else if (t.kind == HL_DX) {
+            if (J.kind <= HL_DLOGITS) {
+                am = &M.x; a_rows = true; ax = 0; ay = m0 + (J.kind == HL_STATS ? P.tok0 : 0);
+                bm = &M.w_tile; b_rows = true; bx = 0; by = J.v0 + n0;
+            } else if (J.kind == HL_DX) {
                 am = dmap; a_rows = true; ax = 0; ay = m0;
-                bm = &wmap; b_rows = false; bx = n0; by = J.v0;
+                bm = &M.w; b_rows = false; bx = n0; by = J.v0;
             } else {
                 am = dmap; a_rows = false; ax = m0; ay = 0;
-                bm = &xmap; b_rows = false; bx = n0; by = 0;
+                bm = &M.x; b_rows = false; bx = n0; by = 0;
             }
+            const uint32_t bytes = 2 * (2 * HL_BOX + (uint32_t)J.width * 64u);             // of both CTAs
             for (int k = t.k0; k < t.k1; ++k) {
                 good = __all_sync(full_mask, mbar_wait_bounded<true>(bar_empty(s), ph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
                 if (!good) break;
                 const uint32_t bar = map_to_rank(bar_full(s), 0), dst = s0 + s * HL_STAGE_BYTES;
                 const int kk = k * HL_KS;
                 if (elect_one()) {
-                    if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * HL_STAGE_BYTES);
+                    if (rank == 0) mbar_arrive_expect_tx(bar_full(s), bytes);
                     const int x = a_rows ? ax + kk : ax, y = a_rows ? ay : ay + kk;
                     tma_load_2d<true>(dst, am, x, y, bar);
                     tma_load_2d<true>(dst + HL_BOX, am, a_rows ? x : x + 64, a_rows ? y + 64 : y, bar);
                     const int u = b_rows ? bx + kk : bx, v = b_rows ? by : by + kk;
                     tma_load_2d<true>(dst + 2 * HL_BOX, bm, u, v, bar);
-                    tma_load_2d<true>(dst + 3 * HL_BOX, bm, b_rows ? u : u + 64, b_rows ? v + 64 : v, bar);
+                    if (!b_rows) tma_load_2d<true>(dst + 3 * HL_BOX, bm, u + 64, v, bar);
                 }
                 __syncwarp();
                 if (++s == HL_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (rank == 0) {
+    } else if (warp == HL_EPI_WARPS + 1 && rank == 0) {
         // =========================================================== MMA
         bool good = true;
         uint32_t s = 0, ph = 0, buf = 0, aph = 0;
-        for (int i = pair; good && hl_tile(P, tokens, i, &t); i += pairs) {
-            const bool a_mn = t.kind == HL_DW, b_mn = t.kind >= HL_DX;
-            const uint32_t idesc = umma_idesc(HL_TILE, HL_TILE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+        while (good && list.take(P, &t)) {
+            const HlJob& J = list.J;
+            const bool a_mn = J.kind == HL_DW, b_mn = J.kind >= HL_DX;
+            const uint32_t idesc = umma_idesc((uint32_t)J.width, HL_TILE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
             const uint64_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
-            const int per = t.kind <= HL_DLOGITS ? HL_SUM_STAGES : t.k1 - t.k0;
+            const int per = J.kind <= HL_DLOGITS ? HL_SUM_STAGES : t.k1 - t.k0;
             for (int k0 = t.k0; good && k0 < t.k1; k0 += per) {
                 good = __all_sync(full_mask, mbar_wait_bounded<true>(bar_free(buf), aph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
                 if (!good) break;
@@ -348,6 +478,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
             }
         }
     }
+    }
     tc_fence_before();
     __syncwarp();
     cluster_sync_all();                                    // the pair frees its tensor memory together
@@ -376,6 +507,7 @@ constexpr int HL_PREP_THREADS = 256;
 // Tokens that count, packed in their order.  Every block counts those before its own for itself (the targets are a few KB, and in the L2).
 __global__ void __launch_bounds__(HL_PREP_THREADS) head_prepare_kernel(const HlPrepareParams P) {
     __shared__ int before_s, total_s, slots_s[HL_PREP_THREADS], sums_s[HL_PREP_THREADS / 32];
+    pdl_next();
     const int first = blockIdx.x * P.per_block, last = min(first + P.per_block, P.n);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) before_s = total_s = 0;
@@ -440,7 +572,9 @@ __global__ void __launch_bounds__(HL_PREP_THREADS) head_prepare_kernel(const HlP
 struct HlJoinParams {
     const float2* part;
     const float* at;
-    const int* slot;
+    const int* slot;                       // null: every token is at its own place, and counts if its target is inside the vocabulary
+    const long long* targets;
+    long long vocab;
     int* count;
     int n, parts, ld_part, tok0, tokens;   // places tok0 .. tok0 + tokens are in `part`
     float* loss;                           // [n]
@@ -452,11 +586,21 @@ struct HlJoinParams {
 constexpr int HL_JOIN_THREADS = 512, HL_JOIN_TOKENS = 8, HL_JOIN_SLICES = HL_JOIN_THREADS / HL_JOIN_TOKENS;
 // The tiles' statistics of eight tokens, joined in a fixed order; the last block to finish adds up the losses.
 __global__ void __launch_bounds__(HL_JOIN_THREADS) head_join_kernel(const HlJoinParams P) {
+    pdl_next();
+    pdl_wait();
     __shared__ float m_s[HL_JOIN_SLICES][HL_JOIN_TOKENS], s_s[HL_JOIN_SLICES][HL_JOIN_TOKENS];
     __shared__ bool last_s;
     const int which = threadIdx.x % HL_JOIN_TOKENS, slice = threadIdx.x / HL_JOIN_TOKENS;
     const int i = blockIdx.x * HL_JOIN_TOKENS + which;
-    const int p = i < P.n ? P.slot[i] : -1;
+    int p = -1;
+    if (i < P.n) {
+        if (P.slot) {
+            p = P.slot[i];
+        } else {
+            const long long t = P.targets[i];
+            if (t >= 0 && t < P.vocab) p = i;
+        }
+    }
     const bool here = p >= P.tok0 && p < P.tok0 + P.tokens;
     float m = -INFINITY, s = 0.0f;
     if (here) {
@@ -514,6 +658,7 @@ __global__ void __launch_bounds__(HL_JOIN_THREADS) head_join_kernel(const HlJoin
 // dx of every token: the sum of its slabs times the factor that all share, or zeros
 __global__ void __launch_bounds__(256) head_dx_kernel(const float* slab, const int* slot, int n_rows, int hidden, int splits, const float* factor, uint16_t* dx,
                                                     long long ld) {
+    pdl_wait();
     const int i = blockIdx.x, p = slot[i];
     const float g = *factor;
     for (int c = threadIdx.x * 8; c < hidden; c += 256 * 8) {

@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "embed_kernels.cuh"
+#include "head_few.cuh"
 #include "head_loss.cuh"
 
 using namespace cb;
@@ -77,9 +78,10 @@ constexpr size_t HEAD_PIECE_BYTES = (size_t)256 << 20;
 
 typedef CUresult (*TensorMapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                       const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// bf16 [rows][cols], row stride ld elements: boxes of 64 x 64, 128-byte swizzle, zeros outside.  Encoding is a driver call and needs the device's context
-// on this thread, which a thread that has launched nothing yet (autograd's) does not have: cudaSetDevice() of the current device sees to it.
-int make_map(CUtensorMap* map, const void* p, int64_t ld, int64_t rows, int64_t cols) {
+// A matrix (or `depth` of them in a row, ld * rows apart) with boxes of 128 swizzled bytes x box_rows; zeros outside, nothing written there.  Encoding is a
+// driver call and needs the device's context on this thread, which a thread that has launched nothing yet (autograd's) does not have: cudaSetDevice()
+// of the current device sees to it.
+int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, int64_t ld, int64_t rows, int64_t cols, int box_rows, int depth = 0) {
     static TensorMapEncodeFn encode = nullptr;
     if (!encode) {
         void* fn = nullptr;
@@ -89,10 +91,26 @@ int make_map(CUtensorMap* map, const void* p, int64_t ld, int64_t rows, int64_t 
     }
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return COBALT_ELAUNCH;
-    const cuuint64_t dim[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64, 64}, one[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint64_t size = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
+    const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)depth}, stride[2] = {(cuuint64_t)ld * size, (cuuint64_t)ld * size * (cuuint64_t)rows};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+    return encode(map, type, depth ? 3 : 2, const_cast<void*>(p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? COBALT_OK : COBALT_EINVAL;
+}
+int bf16_map(CUtensorMap* map, const void* p, int64_t ld, int64_t rows, int64_t cols, int box_rows = 64) {
+    return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, ld, rows, cols, box_rows);
+}
+
+// Columns of a tile of logits.  Tiles go round the pairs; with few of them the last round is far from full, and narrower tiles fill it: the
+// rounds times a tile's cost (its columns, and 16 for what it costs besides) are smallest.
+int tile_width(int64_t token_tiles, int64_t cols, int pairs) {
+    int best = HL_TILE;
+    int64_t least = INT64_MAX;
+    for (int w = HL_TILE; w >= 96; w -= 16) {
+        const int64_t cost = ceil_div(token_tiles * ceil_div(cols, w), pairs) * (w + 16);
+        if (cost < least) { least = cost; best = w; }
+    }
+    return best;
 }
 
 bool head_rows_ok(const void* p, int64_t ld, int64_t width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
@@ -102,15 +120,44 @@ int head_sizes(int n, int hidden, int64_t vocab) {
     return COBALT_OK;
 }
 
+// Rows of W of a unit of the few-token kernel: as few rounds of the CTAs as units of at most 256 rows allow, and these evenly filled
+int few_rows(int64_t cols, int sms) {
+    const int64_t rounds = ceil_div(cols, (int64_t)256 * sms);
+    return (int)(ceil_div(ceil_div(cols, rounds * sms), 16) * 16);
+}
+
 struct HeadScratch {
-    int piece, pieces, splits, stats_tokens;
+    bool few;                              // the few-token kernel forms the logits and dx
+    int piece, pieces, splits, stats_tokens, width;      // width: of a tile of logits; few: rows of a unit
     size_t count, slot, target, at, row, packed, part, slab, d[2], bytes;
 };
-HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool want_x, int sms) {
+// Ranges of a piece that dx is summed over separately: with dw's tiles to fill up the rounds, so many that every pair has one; without, as gives the
+// shortest last round (a range more costs about 3 % of a round: its slab is written and read)
+int dx_splits(int64_t tiles, bool want_w, int pairs) {
+    int best = 1;
+    if (want_w) return (int)std::max<int64_t>(pairs / tiles, 1);
+    double least = 1e30;
+    for (int s = 1; s <= std::max<int64_t>(2 * pairs / tiles, 4); ++s) {
+        const double cost = (double)ceil_div(tiles * s, pairs) / s + 0.03 * s;
+        if (cost < least) { least = cost; best = s; }
+    }
+    return best;
+}
+HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool want_x, bool want_w, int sms) {
     HeadScratch s = {};
     const size_t rows = (size_t)ceil_div(n, HL_TILE) * HL_TILE;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t p = at; at += align256(bytes); return p; };
+    s.few = n <= HF_TOKENS;
+    if (!backward && s.few) {                              // x is read where it lies
+        s.stats_tokens = ceil_div(n, 32) * 32;
+        s.width = few_rows(vocab, sms);
+        s.count = take(256);
+        s.at = take((size_t)n * 4);
+        s.part = take((size_t)ceil_div(vocab, s.width) * HF_EPI_WARPS * s.stats_tokens * 8);
+        s.bytes = at;
+        return s;
+    }
     s.count = take(256);
     s.slot = take((size_t)n * 4);
     s.target = take((size_t)n * 4);
@@ -118,18 +165,23 @@ HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool w
     if (!backward) {
         s.stats_tokens = (int)std::min<size_t>(rows, HEAD_STATS_TOKENS);
         s.at = take((size_t)n * 4);
-        s.part = take((size_t)ceil_div(vocab, HL_TILE) * 2 * s.stats_tokens * 8);
+        s.width = tile_width(ceil_div(s.stats_tokens, HL_TILE), vocab, sms / 2);
+        s.part = take((size_t)ceil_div(vocab, s.width) * 2 * s.stats_tokens * 8);
     } else {
         s.row = take((size_t)n * 16);
         // pieces of equal size, each within HEAD_PIECE_BYTES of scratch
-        const int64_t most = std::max<int64_t>(HEAD_PIECE_BYTES / 2 / rows / HL_TILE * HL_TILE, HL_TILE);
+        const int64_t most = std::max<int64_t>(HEAD_PIECE_BYTES / 2 / n / HL_TILE * HL_TILE, HL_TILE);
         s.pieces = (int)ceil_div(vocab, most);
         s.piece = (int)(ceil_div(ceil_div(vocab, s.pieces), HL_TILE) * HL_TILE);
         s.pieces = (int)ceil_div(vocab, s.piece);
-        for (int b = 0; b < 2; ++b) s.d[b] = b < s.pieces ? take(rows * s.piece * 2) : s.d[0];
+        for (int b = 0; b < 2; ++b) s.d[b] = b < s.pieces ? take((size_t)n * s.piece * 2) : s.d[0];
+        s.width = s.few ? few_rows(s.piece, sms) : tile_width(rows / HL_TILE, s.piece, sms / 2);
         if (want_x) {
             const int64_t tiles = (int64_t)(rows / HL_TILE) * ceil_div(hidden, HL_TILE);
-            s.splits = (int)std::min<int64_t>(std::max<int64_t>(sms / tiles, 1), std::max(s.piece / 512, 1));
+            // (a range of at least one stage, of the last piece too)
+            const int64_t last = vocab - (int64_t)(s.pieces - 1) * s.piece;
+            const int most = s.few ? std::max((int)(sms / ceil_div(hidden, HL_TILE)), 1) : dx_splits(tiles, want_w, sms / 2);
+            s.splits = (int)std::min<int64_t>({most, std::max(s.piece / 512, 1), ceil_div(last, HL_KS)});
             s.slab = take((size_t)s.splits * n * hidden * 4);
         }
     }
@@ -143,27 +195,50 @@ int prepare(const HlPrepareParams& in, cudaStream_t st) {
     head_prepare_kernel<<<ceil_div(P.n, P.per_block), HL_PREP_THREADS, 0, st>>>(P);
     return launched();
 }
-int product(const HlParams& P, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& d0, const CUtensorMap& d1, int64_t tiles, int sms, cudaStream_t st) {
+// a kernel whose start may overlap the end of the one before (it waits for that one's results itself)
+template <typename... Params, typename... Args>
+int launch_next(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, const Args&... args) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+}
+int few(const HfParams& P, const CUtensorMap& a, const CUtensorMap& b, int sms, bool first, cudaStream_t st) {
+    static bool configured[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)HF_SMEM) != cudaSuccess) return COBALT_ELAUNCH;
+        configured[dev] = true;
+    }
+    const dim3 grid((unsigned)std::min(P.units, sms));
+    if (!first) return launch_next(head_few_kernel, grid, HF_THREADS, HF_SMEM, 1, st, P, a, b);
+    head_few_kernel<<<grid, HF_THREADS, HF_SMEM, st>>>(P, a, b);
+    return launched();
+}
+int product(const HlParams& P, const HlMaps& M, int64_t tiles, int sms, cudaStream_t st) {
     static bool configured[MAX_DEVICES];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
     if (!configured[dev]) {
         if (cudaFuncSetAttribute(head_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)HL_SMEM) != cudaSuccess) return COBALT_ELAUNCH;
+        // warps that ask for registers wait for them: never launch a build that does not bring as many as are handed around
+        cudaFuncAttributes built;
+        if (cudaFuncGetAttributes(&built, head_product_kernel) != cudaSuccess || built.numRegs != HL_REGS) return COBALT_ELAUNCH;
         configured[dev] = true;
     }
     if (tiles > 0x3FFFFFFF) return COBALT_ETOOBIG;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
-    cfg.blockDim = dim3(HL_THREADS);
-    cfg.dynamicSmemBytes = HL_SMEM;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, head_product_kernel, P, x, w, d0, d1) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
+    return launch_next(head_product_kernel, dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2))), HL_THREADS, HL_SMEM, 2, st, P, M);
 }
 
 }  // namespace
@@ -258,7 +333,8 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
 }
 
 size_t cobalt_head_loss_scratch_bytes(int n, int hidden, int64_t vocab) {
-    return head_sizes(n, hidden, vocab) ? 0 : head_scratch(n, hidden, vocab, false, false, 0).bytes;
+    int sms = 0;
+    return head_sizes(n, hidden, vocab) || sm_count(&sms) ? 0 : head_scratch(n, hidden, vocab, false, false, false, sms).bytes;
 }
 
 int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, int n, int hidden, int64_t vocab, float* loss,
@@ -267,31 +343,61 @@ int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw
     if (rc) return rc;
     if (!head_rows_ok(x, ldx, hidden) || !head_rows_ok(weight, ldw, hidden) || !targets || !loss) return COBALT_EINVAL;
     if (((uintptr_t)targets & 7) || (((uintptr_t)loss | (uintptr_t)total) & 3) || ((uintptr_t)stats & 7) || ((uintptr_t)status & 3)) return COBALT_EINVAL;
-    const HeadScratch s = head_scratch(n, hidden, vocab, false, false, 0);
-    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
+    const HeadScratch s = head_scratch(n, hidden, vocab, false, false, false, sms);
+    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
     uint8_t* base = (uint8_t*)scratch;
     cudaStream_t st = (cudaStream_t)stream;
+    uint32_t* const word = status ? (uint32_t*)status : status_word();
+    if (!word) return COBALT_ELAUNCH;
+    HlJoinParams J = {};
+    J.targets = (const long long*)targets;
+    J.vocab = vocab;
+    J.part = (float2*)(base + s.part);
+    J.at = (float*)(base + s.at);
+    J.count = (int*)(base + s.count);
+    J.n = n; J.ld_part = s.stats_tokens;
+    J.loss = loss; J.stats = (float2*)stats; J.mean = mean;
+    if (s.few) {
+        HfParams F = {};
+        F.kind = HL_STATS;
+        F.n = n; F.n_pad = s.stats_tokens;
+        F.cols = (int)vocab; F.rows = s.width;
+        F.units = (int)ceil_div(vocab, s.width);
+        F.hidden = hidden;
+        F.targets = J.targets; F.vocab = vocab;
+        F.counted = J.count;
+        F.part = (float2*)(base + s.part);
+        F.at = (float*)(base + s.at);
+        F.status = word;
+        CUtensorMap wm, xm;
+        if ((rc = bf16_map(&wm, weight, ldw, vocab, hidden, s.width / 2)) || (rc = bf16_map(&xm, x, ldx, n, hidden, F.n_pad))) return rc;
+        if ((rc = few(F, wm, xm, sms, true, st))) return rc;
+        J.parts = F.units * HF_EPI_WARPS;
+        J.tokens = n;
+        J.total = total;
+        return launch_next(head_join_kernel, dim3((unsigned)ceil_div(n, HL_JOIN_TOKENS)), HL_JOIN_THREADS, 0, 1, st, J);
+    }
     HlPrepareParams A = {};
     A.x = (const uint16_t*)x; A.ldx = ldx;
     A.targets = (const long long*)targets;
     A.n = n; A.hidden = hidden; A.vocab = vocab;
-    A.count = (int*)(base + s.count);
+    A.count = J.count;
     A.slot = (int*)(base + s.slot);
     A.target = (int*)(base + s.target);
     A.packed = (uint16_t*)(base + s.packed);
     HlParams P = {};
-    P.status = status ? (uint32_t*)status : status_word();
-    if (!P.status) return COBALT_ELAUNCH;
-    CUtensorMap xm, wm;
-    if ((rc = make_map(&xm, A.packed, hidden, n, hidden)) || (rc = make_map(&wm, weight, ldw, vocab, hidden))) return rc;
+    P.status = word;
+    HlMaps M = {};
+    if ((rc = bf16_map(&M.x, A.packed, hidden, n, hidden)) || (rc = bf16_map(&M.w_tile, weight, ldw, vocab, hidden, s.width / 2))) return rc;
     if ((rc = prepare(A, st))) return rc;
-    const int v_tiles = (int)ceil_div(vocab, HL_TILE);
+    const int v_tiles = (int)ceil_div(vocab, s.width);
     P.n_jobs = 1;
     P.job[0].kind = HL_STATS;
     P.job[0].cols = (int)vocab;
     P.job[0].n_tiles = v_tiles;
+    P.job[0].width = s.width;
     P.job[0].splits = 1;
     P.count = A.count;
     P.n_rows = n; P.hidden = hidden;
@@ -299,25 +405,22 @@ int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw
     P.part = (float2*)(base + s.part);
     P.at = (float*)(base + s.at);
     P.ld_part = s.stats_tokens;
-    HlJoinParams J = {};
-    J.part = P.part; J.at = P.at; J.slot = A.slot; J.count = A.count;
-    J.n = n; J.parts = 2 * v_tiles; J.ld_part = P.ld_part;
-    J.loss = loss; J.stats = (float2*)stats; J.mean = mean;
+    J.slot = A.slot;
+    J.parts = 2 * v_tiles;
     for (int tok0 = 0; tok0 < n; tok0 += s.stats_tokens) {
         J.tok0 = P.tok0 = tok0;
         J.tokens = std::min(n - tok0, s.stats_tokens);
         P.tok_tiles = ceil_div(J.tokens, HL_TILE);
         J.total = tok0 + s.stats_tokens >= n ? total : nullptr;
-        if ((rc = product(P, xm, wm, xm, xm, (int64_t)P.tok_tiles * v_tiles, sms, st))) return rc;
-        head_join_kernel<<<ceil_div(n, HL_JOIN_TOKENS), HL_JOIN_THREADS, 0, st>>>(J);
-        if ((rc = launched())) return rc;
+        if ((rc = product(P, M, (int64_t)P.tok_tiles * v_tiles, sms, st))) return rc;
+        if ((rc = launch_next(head_join_kernel, dim3((unsigned)ceil_div(n, HL_JOIN_TOKENS)), HL_JOIN_THREADS, 0, 1, st, J))) return rc;
     }
     return COBALT_OK;
 }
 
-size_t cobalt_head_loss_grad_scratch_bytes(int n, int hidden, int64_t vocab, int want_x) {
+size_t cobalt_head_loss_grad_scratch_bytes(int n, int hidden, int64_t vocab, int want_x, int want_w) {
     int sms = 0;
-    return head_sizes(n, hidden, vocab) || sm_count(&sms) ? 0 : head_scratch(n, hidden, vocab, true, want_x != 0, sms).bytes;
+    return head_sizes(n, hidden, vocab) || sm_count(&sms) ? 0 : head_scratch(n, hidden, vocab, true, want_x != 0, want_w != 0, sms).bytes;
 }
 
 int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, const float* stats, const float* grad,
@@ -330,7 +433,7 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     if (((uintptr_t)targets & 7) || ((uintptr_t)stats & 7) || (((uintptr_t)grad | (uintptr_t)status) & 3) || grad_step < 0 || grad_step > 1) return COBALT_EINVAL;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
-    const HeadScratch s = head_scratch(n, hidden, vocab, true, dx != nullptr, sms);
+    const HeadScratch s = head_scratch(n, hidden, vocab, true, dx != nullptr, dw != nullptr, sms);
     if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
     uint8_t* base = (uint8_t*)scratch;
     cudaStream_t st = (cudaStream_t)stream;
@@ -349,23 +452,24 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     HlParams P = {};
     P.status = status ? (uint32_t*)status : status_word();
     if (!P.status) return COBALT_ELAUNCH;
-    const int64_t rows = (int64_t)ceil_div(n, HL_TILE) * HL_TILE;
-    CUtensorMap xm, wm, dm[2];
-    if ((rc = make_map(&xm, A.packed, hidden, n, hidden)) || (rc = make_map(&wm, weight, ldw, vocab, hidden))) return rc;
+    HlMaps M = {};
+    if ((rc = bf16_map(&M.x, A.packed, hidden, n, hidden)) || (rc = bf16_map(&M.w, weight, ldw, vocab, hidden)) ||
+        (rc = bf16_map(&M.w_tile, weight, ldw, vocab, hidden, s.width / 2))) return rc;
+    CUtensorMap x_few, d_few[2];
+    if (s.few && (rc = bf16_map(&x_few, A.packed, hidden, n, hidden, ceil_div(n, 32) * 32))) return rc;
     for (int b = 0; b < 2; ++b)
-        if ((rc = make_map(&dm[b], base + s.d[b], s.piece, rows, s.piece))) return rc;
+        if ((rc = bf16_map(&M.d[b], base + s.d[b], s.piece, n, s.piece)) || (s.few && (rc = bf16_map(&d_few[b], base + s.d[b], s.piece, n, s.piece, ceil_div(n, 32) * 32)))) return rc;
+    if (dx && (rc = make_map(&M.slab, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base + s.slab, hidden, n, hidden, 32, s.splits))) return rc;
+    if (dw && (rc = bf16_map(&M.dw, dw, ld_dw, vocab, hidden, 32))) return rc;
     if ((rc = prepare(A, st))) return rc;
     P.count = A.count;
-    P.tok_tiles = (int)(rows / HL_TILE);
+    P.tok_tiles = ceil_div(n, HL_TILE);
     P.n_rows = n; P.hidden = hidden;
     P.target = A.target;
     P.row = A.row;
     P.factor = A.factor;
     P.d[0] = (uint16_t*)(base + s.d[0]); P.d[1] = (uint16_t*)(base + s.d[1]);
     P.ld_d = s.piece;
-    P.slab = (float*)(base + s.slab);
-    P.dw = (uint16_t*)dw; P.ld_dw = ld_dw;
-    P.wide = !((uintptr_t)dw & 31) && !(ld_dw & 15);
     // One launch per piece and one more: the products with piece i's d beside the logits of piece i + 1
     const int h_tiles = ceil_div(hidden, HL_TILE);
     for (int i = 0; i <= s.pieces; ++i) {
@@ -379,9 +483,31 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
             j.cols = (int)std::min<int64_t>(s.piece, vocab - j.v0);
             j.splits = 1;
             j.buf = k & 1;
+            j.width = HL_TILE;
             return j;
         };
-        if (i > 0 && dx) {
+        // few tokens: logits and dx by their own kernel
+        HfParams F = {};
+        F.n = n; F.n_pad = ceil_div(n, 32) * 32;
+        F.count = A.count;
+        F.hidden = hidden;
+        F.target = A.target; F.row = A.row;
+        F.ld_d = s.piece;
+        F.slab = (float*)(base + s.slab);
+        F.status = P.status;
+        auto few_piece = [&](int kind, int k) {
+            F.kind = kind;
+            F.v0 = k * s.piece;
+            F.cols = (int)std::min<int64_t>(s.piece, vocab - F.v0);
+            F.d = P.d[k & 1];
+        };
+        if (s.few && i > 0 && dx) {
+            few_piece(HL_DX, i - 1);
+            F.h_tiles = h_tiles; F.splits = s.splits; F.add = i > 1;
+            F.units = h_tiles * s.splits;
+            if ((rc = few(F, M.w, d_few[(i - 1) & 1], sms, false, st))) return rc;
+        }
+        if (!s.few && i > 0 && dx) {
             HlJob& j = piece(HL_DX, i - 1);
             j.n_tiles = h_tiles;
             j.splits = s.splits;
@@ -393,15 +519,23 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
             j.n_tiles = h_tiles;
             tiles += (int64_t)ceil_div(j.cols, HL_TILE) * h_tiles;
         }
-        if (i < s.pieces) {
+        if (s.few && i < s.pieces) {
+            few_piece(HL_DLOGITS, i);
+            F.rows = s.width;
+            F.units = ceil_div(ceil_div(F.cols, HL_KS) * HL_KS, s.width);
+            if ((rc = few(F, M.w_tile, x_few, sms, false, st))) return rc;
+        }
+        if (!s.few && i < s.pieces) {
             HlJob& j = piece(HL_DLOGITS, i);
-            j.n_tiles = ceil_div(j.cols, HL_TILE);
+            j.width = s.width;
+            j.n_tiles = ceil_div(ceil_div(j.cols, HL_KS) * HL_KS, s.width);    // (dx reads whole stages of d)
             tiles += (int64_t)P.tok_tiles * j.n_tiles;
         }
-        if ((rc = product(P, xm, wm, dm[0], dm[1], tiles, sms, st))) return rc;
+        if (P.n_jobs && (rc = product(P, M, tiles, sms, st))) return rc;
     }
-    if (dx) head_dx_kernel<<<n, 256, 0, st>>>(P.slab, A.slot, n, hidden, s.splits, A.factor, (uint16_t*)dx, ld_dx);
-    return launched();
+    return dx ? launch_next(head_dx_kernel, dim3((unsigned)n), 256, 0, 1, st, (const float*)(base + s.slab), (const int*)A.slot, n, hidden, s.splits, (const float*)A.factor,
+                            (uint16_t*)dx, (long long)ld_dx)
+              : COBALT_OK;
 }
 
 int cobalt_vocab_status(void* stream, uint32_t* status_out) {

@@ -252,7 +252,7 @@ def _head_loss_grad(x, weight, targets, stats, grad, reduction, status, want_x, 
     if each:
         grad = grad.contiguous()
     index = x.get_device()
-    need = _scratch_bytes(index, "cobalt_head_loss_grad_scratch_bytes", n, H, V, 1 if want_x else 0)
+    need = _scratch_bytes(index, "cobalt_head_loss_grad_scratch_bytes", n, H, V, 1 if want_x else 0, 1 if want_w else 0)
     scratch = x.new_empty(need, dtype=torch.uint8)
     _call(index, "cobalt_head_loss_grad", rows.data_ptr(), apart, w.data_ptr(), apart_w, targets.data_ptr(), stats.data_ptr(), grad.data_ptr(), 1 if each else 0,
           1 if reduction == "mean" else 0, n, H, V, None if dx is None else dx.data_ptr(), H, None if dw is None else dw.data_ptr(), H, scratch.data_ptr(), need,

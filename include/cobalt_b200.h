@@ -421,7 +421,7 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
 size_t cobalt_head_loss_scratch_bytes(int n, int hidden, int64_t vocab);
 int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, int n, int hidden, int64_t vocab,
                      float* loss, float* stats, float* total, int mean, void* scratch, size_t scratch_bytes, void* status, void* stream);
-size_t cobalt_head_loss_grad_scratch_bytes(int n, int hidden, int64_t vocab, int want_x);
+size_t cobalt_head_loss_grad_scratch_bytes(int n, int hidden, int64_t vocab, int want_x, int want_w);
 int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_t ldw, const int64_t* targets, const float* stats,
                           const float* grad, int64_t grad_step, int mean, int n, int hidden, int64_t vocab, void* dx, int64_t ld_dx, void* dw,
                           int64_t ld_dw, void* scratch, size_t scratch_bytes, void* status, void* stream);
