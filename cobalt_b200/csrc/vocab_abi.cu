@@ -343,10 +343,11 @@ int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw
     if (rc) return rc;
     if (!head_rows_ok(x, ldx, hidden) || !head_rows_ok(weight, ldw, hidden) || !targets || !loss) return COBALT_EINVAL;
     if (((uintptr_t)targets & 7) || (((uintptr_t)loss | (uintptr_t)total) & 3) || ((uintptr_t)stats & 7) || ((uintptr_t)status & 3)) return COBALT_EINVAL;
+    if (!scratch || ((uintptr_t)scratch & 255)) return COBALT_ESCRATCH;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
     const HeadScratch s = head_scratch(n, hidden, vocab, false, false, false, sms);
-    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
+    if (scratch_bytes < s.bytes) return COBALT_ESCRATCH;
     uint8_t* base = (uint8_t*)scratch;
     cudaStream_t st = (cudaStream_t)stream;
     uint32_t* const word = status ? (uint32_t*)status : status_word();
@@ -431,10 +432,11 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     if (!head_rows_ok(x, ldx, hidden) || !head_rows_ok(weight, ldw, hidden) || !targets || !stats || !grad || (!dx && !dw)) return COBALT_EINVAL;
     if ((dx && !head_rows_ok(dx, ld_dx, hidden)) || (dw && !head_rows_ok(dw, ld_dw, hidden))) return COBALT_EINVAL;
     if (((uintptr_t)targets & 7) || ((uintptr_t)stats & 7) || (((uintptr_t)grad | (uintptr_t)status) & 3) || grad_step < 0 || grad_step > 1) return COBALT_EINVAL;
+    if (!scratch || ((uintptr_t)scratch & 255)) return COBALT_ESCRATCH;
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
     const HeadScratch s = head_scratch(n, hidden, vocab, true, dx != nullptr, dw != nullptr, sms);
-    if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
+    if (scratch_bytes < s.bytes) return COBALT_ESCRATCH;
     uint8_t* base = (uint8_t*)scratch;
     cudaStream_t st = (cudaStream_t)stream;
     HlPrepareParams A = {};

@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import cobalt_b200 as cb
+from cobalt_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -340,3 +341,22 @@ def test_refusals():
             cb.head_loss_and_grad(x, w, t, grad=bad)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     assert torch.equal(cb.head_loss(x, w, t, status=status), cb.head_loss(x, w, t)) and int(status) == 0
+
+
+def test_scratch():
+    """Per token and 128 columns of the vocabulary 8 bytes, of at most 16384 tokens at once: a 64th of fp32 logits, and less for more tokens; two pieces of
+    at most 256 MB for the gradient.  Too little is refused."""
+    L, (n, H, V) = _lib.load(), (2048, 1024, 262144)
+    sizes = L.cobalt_head_loss_scratch_bytes, L.cobalt_head_loss_grad_scratch_bytes
+    assert 0 < sizes[0](n, H, V) < n * V * 4 // 64 + n * H * 2 + (1 << 20)
+    assert 0 < sizes[0](1 << 18, 64, V) < 16384 * (V // 128) * 8 + (1 << 18) * 64 * 2 + (4 << 20)
+    assert 0 < sizes[1](n, H, V, 1, 1) < (512 << 20) + n * H * 2 + 4 * n * H * 4 + (1 << 20)
+    assert sizes[0](n, 60, V) == sizes[1](n, 60, V, 1, 1) == 0
+    x, w, t = inputs(200, 300, 64, 16)
+    out = torch.empty(200, device="cuda")
+    need = sizes[0](200, 64, 300)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    call = lambda size: L.cobalt_head_loss(x.data_ptr(), 64, w.data_ptr(), 64, t.data_ptr(), 200, 64, 300, out.data_ptr(), None, None, 0, scratch.data_ptr(), size, None,  # noqa: E731
+                                           torch.cuda.current_stream().cuda_stream)
+    assert call(need - 1) == -2 and call(need) == 0
+    assert torch.equal(out, cb.head_loss(x, w, t, "none"))

@@ -53,23 +53,15 @@ def test_head_arguments_at_the_c_entry():
     bad = [(dict(x=None), -1), (dict(w=None), -1), (dict(targets=None), -1), (dict(loss=None), -1), (dict(x=A + 8), -1), (dict(w=A + 8), -1), (dict(ldx=60), -1),
            (dict(ldx=68), -1), (dict(ldw=56), -1), (dict(n=0), -1), (dict(hidden=0), -1), (dict(hidden=60), -1), (dict(vocab=0), -1), (dict(targets=A + 4), -1),
            (dict(loss=A + 2), -1), (dict(stats=A + 4), -1), (dict(total=A + 2), -1), (dict(status=A + 2), -1), (dict(n=(1 << 20) + 1), -6),
-           (dict(hidden=(1 << 16) + 8, ldx=1 << 17, ldw=1 << 17), -6), (dict(vocab=1 << 31), -6), (dict(scratch=None), -2), (dict(scratch=A + 128), -2), (dict(bytes=64), -2)]
+           (dict(hidden=(1 << 16) + 8, ldx=1 << 17, ldw=1 << 17), -6), (dict(vocab=1 << 31), -6), (dict(scratch=None), -2), (dict(scratch=A + 128), -2)]
     for change, rc in bad:
         assert L.cobalt_head_loss(*{**good, **change}.values(), None) == rc, change
     good = dict(x=A, ldx=64, w=A, ldw=64, targets=A, stats=A, grad=A, step=0, mean=1, n=4, hidden=64, vocab=100, dx=A, ld_dx=64, dw=A, ld_dw=64, scratch=A,
                 bytes=1 << 30, status=None)
     bad = [(dict(x=None), -1), (dict(w=None), -1), (dict(targets=None), -1), (dict(stats=None), -1), (dict(grad=None), -1), (dict(dx=None, dw=None), -1),
            (dict(step=2), -1), (dict(step=-1), -1), (dict(dx=A + 8), -1), (dict(dw=A + 8), -1), (dict(ld_dx=56), -1), (dict(ld_dw=68), -1), (dict(hidden=4), -1),
-           (dict(grad=A + 2), -1), (dict(status=A + 1), -1), (dict(vocab=1 << 31), -6)]
+           (dict(grad=A + 2), -1), (dict(status=A + 1), -1), (dict(vocab=1 << 31), -6), (dict(scratch=None), -2), (dict(scratch=A + 128), -2)]
     for change, rc in bad:
         assert L.cobalt_head_loss_grad(*{**good, **change}.values(), None) == rc, change
     assert L.cobalt_head_loss_scratch_bytes(4, 60, 100) == 0 and L.cobalt_head_loss_scratch_bytes(0, 64, 100) == 0
     assert L.cobalt_vocab_status(None, None) == -1
-
-
-def test_scratch_of_the_loss_does_not_hold_logits():
-    """Per token and 128 columns of the vocabulary 8 bytes, of at most 16384 tokens at once: a 64th of fp32 logits, and less for more tokens."""
-    L = _lib.load()
-    n, H, V = 2048, 1024, 262144
-    assert L.cobalt_head_loss_scratch_bytes(n, H, V) < n * V * 4 // 64 + n * H * 2 + (1 << 20)
-    assert L.cobalt_head_loss_scratch_bytes(1 << 18, 64, V) < 16384 * (V // 128) * 8 + (1 << 18) * 64 * 2 + (4 << 20)
