@@ -6,6 +6,8 @@
 //
 //   stats, dlogits   A = W, two blocks of up to 128 of its rows; B = x.  A unit of work is `rows` rows, so many that the units go round the CTAs evenly.
 //                    TMEM lane = row of W, column = token: a warp's statistics are reductions over its lanes, 32 tokens at a time.
+//                    Tokens stay where they are (none are packed): what a row without a target holds reaches its own column alone, which is not used.
+//                    dlogits also leaves what dw takes beside d: x with zeros for those rows, and the factor of the sums.
 //   dx               A = W with hidden columns as M (M-major as it lies), K = rows of W; B = d.  A unit is 256 hidden columns and a range of rows.
 //   warps 0-7  epilogue: warp w owns lanes 32 * (w % 4).. of block w / 4        warp 8  TMA        warp 9  MMA
 #pragma once
@@ -19,25 +21,30 @@ constexpr int HF_THREADS = HF_EPI_WARPS * 32 + 64;
 constexpr uint32_t HF_A_BYTES = 4 * HL_BOX;
 constexpr int hf_stages(int n_pad) { return n_pad <= 32 ? 6 : n_pad <= 96 ? 5 : 4; }
 constexpr uint32_t hf_stage_bytes(int n_pad) { return HF_A_BYTES + (uint32_t)n_pad * 128u; }
-constexpr uint32_t HF_SMEM = hf_stages(96) * hf_stage_bytes(96) + 256 + 1024;
-static_assert(hf_stages(32) * hf_stage_bytes(32) + 1280 <= HF_SMEM && hf_stages(64) * hf_stage_bytes(64) + 1280 <= HF_SMEM &&
-              hf_stages(128) * hf_stage_bytes(128) + 1280 <= HF_SMEM && HF_SMEM <= 227 * 1024, "stages of every size fit");
+constexpr uint32_t HF_TAIL = 256 + HF_TOKENS * 16;         // barriers, then maximum, log2 of the sum, factor and target of every token
+constexpr uint32_t HF_SMEM = hf_stages(96) * hf_stage_bytes(96) + HF_TAIL + 1024;
+static_assert(hf_stages(32) * hf_stage_bytes(32) + HF_TAIL + 1024 <= HF_SMEM && hf_stages(64) * hf_stage_bytes(64) + HF_TAIL + 1024 <= HF_SMEM &&
+              hf_stages(128) * hf_stage_bytes(128) + HF_TAIL + 1024 <= HF_SMEM && HF_SMEM <= 227 * 1024, "stages of every size fit");
 
 struct HfParams {
     int kind;                              // HL_STATS, HL_DLOGITS or HL_DX
     int n, n_pad;                          // tokens; the N of the products, a multiple of 32
-    const int* count;                      // tokens that count, or null: all of n (their targets say so themselves)
     int v0, cols;                          // piece of the vocabulary: its first row, and its rows inside the vocabulary
     int units, rows;                       // stats, dlogits: rows of W a unit, a multiple of 16
     int h_tiles, splits, add;              // dx: tiles of 256 hidden columns; ranges of the piece; the slabs hold the sums of earlier pieces
     int hidden;
-    const long long* targets;              // stats: of every token
+    const long long* targets;              // stats, dlogits: of every token; one outside the vocabulary does not count
     long long vocab;
-    const int* target;                     // dlogits: by place
-    int* counted;                          // stats: [0] tokens that count, [1] zero, for the kernel that joins
+    int* counted;                          // stats: [0] tokens that count, [1] zero, for the kernel that joins; dlogits: [0] all tokens, for dw
     float2* part;                          // stats: [8 * units][n_pad]
     float* at;
-    const float4* row;
+    const float2* stats;                   // dlogits: maximum and log2 of the sum
+    const float* grad;                     // gradient of the loss, of every token (grad_step 1) or of the sum or mean (0)
+    int grad_step, mean;
+    float* factor;
+    const uint16_t* x;
+    long long ldx;
+    uint16_t* packed;                      // [n][hidden]
     uint16_t* d;
     int ld_d;
     float* slab;                           // [split][n][hidden]
@@ -97,12 +104,30 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         // =========================================================== epilogue
         const int block = warp >> 2, in_block = (warp & 3) * 32 + lane;
         const uint32_t my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(block * P.n_pad);
-        const int tokens = P.count ? *P.count : P.n;
-        if (P.kind == HL_STATS && blockIdx.x == 0 && warp == 0) {
+        float4* const token_s = reinterpret_cast<float4*>(smem + (bars + 256u - smem_u32(smem)));
+        auto counts = [&](long long t) { return t >= 0 && t < P.vocab; };
+        if (logits && blockIdx.x == 0 && warp == 0) {
             int counted = 0;
-            for (int i = lane; i < P.n; i += 32) counted += P.targets[i] >= 0 && P.targets[i] < P.vocab ? 1 : 0;
+            for (int i = lane; i < P.n; i += 32) counted += counts(P.targets[i]) ? 1 : 0;
             counted = __reduce_add_sync(full_mask, counted);
-            if (lane == 0) { P.counted[0] = counted; P.counted[1] = 0; }
+            if (lane == 0) {
+                P.counted[0] = P.kind == HL_STATS ? counted : P.n;
+                P.counted[1] = 0;
+                if (P.kind == HL_DLOGITS) *P.factor = P.grad_step ? 1.0f : P.mean ? P.grad[0] / (float)max(counted, 1) : P.grad[0];
+            }
+        }
+        if (P.kind == HL_DLOGITS) {
+            if (threadIdx.x < P.n) {
+                const long long t = P.targets[threadIdx.x];
+                const float2 s = P.stats[threadIdx.x];
+                token_s[threadIdx.x] = make_float4(s.x, s.y, P.grad_step ? P.grad[threadIdx.x] : 1.0f, __int_as_float(counts(t) ? (int)t : -1));
+            }
+            for (int i = blockIdx.x; i < P.n; i += gridDim.x) {
+                const bool in = counts(P.targets[i]);
+                for (int c = threadIdx.x; c < P.hidden / 8; c += HF_EPI_WARPS * 32)
+                    reinterpret_cast<uint4*>(P.packed + (long long)i * P.hidden)[c] = in ? reinterpret_cast<const uint4*>(P.x + i * P.ldx)[c] : make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");             // the epilogue warps
         }
         bool healthy = true;
         uint32_t buf = 0, ph = 0;
@@ -164,10 +189,10 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                             const int c = 32 * q + e;
                             if (c >= P.n) continue;
                             float g = 0.0f;
-                            if (c < tokens && mine) {
-                                const float4 r = P.row[c];
+                            const float4 r = token_s[c];
+                            if (mine && __float_as_int(r.w) >= 0) {
                                 g = exp2_fast(fmaf(acc[c] - r.x, LOG2E, -r.y));
-                                if (P.target[c] == row) g -= 1.0f;
+                                if (__float_as_int(r.w) == row) g -= 1.0f;
                                 g *= r.z;
                             }
                             if (in_d) P.d[(long long)c * P.ld_d + in_piece] = float_to_bf16(g);
@@ -196,10 +221,11 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
             int k0, k1;
             k_range(u, &k0, &k1);
             const int h0 = logits ? 0 : u % P.h_tiles * HL_TILE, r0 = P.v0 + (logits ? u * P.rows : 0);
-            for (int k = k0; k < k1; ++k) {
+            for (int i = k0; i < k1; ++i) {
                 good = __all_sync(full_mask, mbar_wait_bounded(bar_empty(s), ph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
                 if (!good) break;
                 const uint32_t dst = s0 + s * stage_bytes, bar = bar_full(s);
+                const int k = P.kind == HL_DLOGITS ? k1 - 1 - i : i;   // backwards: the L2 still holds the columns that the loss read last
                 if (elect_one()) {
                     mbar_arrive_expect_tx(bar, bytes);
                     if (logits) {

@@ -655,15 +655,17 @@ __global__ void __launch_bounds__(HL_JOIN_THREADS) head_join_kernel(const HlJoin
     if (threadIdx.x == 0) *P.total = P.mean ? sum_s[0] / (float)max(P.count[0], 1) : sum_s[0];
 }
 
-// dx of every token: the sum of its slabs times the factor that all share, or zeros
-__global__ void __launch_bounds__(256) head_dx_kernel(const float* slab, const int* slot, int n_rows, int hidden, int splits, const float* factor, uint16_t* dx,
+// dx of every token: the sum of its slabs times the factor that all share, or zeros.  Without slots every token is at its own place, and counts if its
+// target is inside the vocabulary.
+__global__ void __launch_bounds__(256) head_dx_kernel(const float* slab, const int* slot, const long long* targets, long long vocab, int n_rows, int hidden, int splits, const float* factor, uint16_t* dx,
                                                     long long ld) {
     pdl_wait();
-    const int i = blockIdx.x, p = slot[i];
+    const int i = blockIdx.x, p = slot ? slot[i] : targets[i] >= 0 && targets[i] < vocab ? i : -1;
     const float g = *factor;
     for (int c = threadIdx.x * 8; c < hidden; c += 256 * 8) {
         float v[8] = {};
         if (p >= 0) {
+#pragma unroll 8
             for (int s = 0; s < splits; ++s) {
                 const float4* q = reinterpret_cast<const float4*>(slab + ((long long)s * n_rows + p) * hidden + c);
                 const float4 a = q[0], b = q[1];

@@ -78,9 +78,7 @@ constexpr size_t HEAD_PIECE_BYTES = (size_t)256 << 20;
 
 typedef CUresult (*TensorMapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                       const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// A matrix (or `depth` of them in a row, ld * rows apart) with boxes of 128 swizzled bytes x box_rows; zeros outside, nothing written there.  Encoding is a
-// driver call and needs the device's context on this thread, which a thread that has launched nothing yet (autograd's) does not have: cudaSetDevice()
-// of the current device sees to it.
+// A matrix (or `depth` of them in a row, ld * rows apart) with boxes of 128 swizzled bytes x box_rows; zeros outside, nothing written there
 int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, int64_t ld, int64_t rows, int64_t cols, int box_rows, int depth = 0) {
     static TensorMapEncodeFn encode = nullptr;
     if (!encode) {
@@ -89,8 +87,6 @@ int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, int64_t 
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return COBALT_ELAUNCH;
         encode = (TensorMapEncodeFn)fn;
     }
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return COBALT_ELAUNCH;
     const cuuint64_t size = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
     const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)depth}, stride[2] = {(cuuint64_t)ld * size, (cuuint64_t)ld * size * (cuuint64_t)rows};
     const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
@@ -99,6 +95,12 @@ int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, int64_t 
 }
 int bf16_map(CUtensorMap* map, const void* p, int64_t ld, int64_t rows, int64_t cols, int box_rows = 64) {
     return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, ld, rows, cols, box_rows);
+}
+
+// Encoding a map is a driver call and needs the device's context on this thread, which a thread that has launched nothing yet (autograd's) does not have
+int bind_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
 }
 
 // Columns of a tile of logits.  Tiles go round the pairs; with few of them the last round is far from full, and narrower tiles fill it: the
@@ -191,7 +193,7 @@ HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool w
 
 int prepare(const HlPrepareParams& in, cudaStream_t st) {
     HlPrepareParams P = in;
-    P.per_block = std::max((int)ceil_div(P.n, 1024), 4);
+    P.per_block = (int)ceil_div(P.n, 1024);
     head_prepare_kernel<<<ceil_div(P.n, P.per_block), HL_PREP_THREADS, 0, st>>>(P);
     return launched();
 }
@@ -348,6 +350,7 @@ int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw
     if ((rc = sm_count(&sms))) return rc;
     const HeadScratch s = head_scratch(n, hidden, vocab, false, false, false, sms);
     if (scratch_bytes < s.bytes) return COBALT_ESCRATCH;
+    if ((rc = bind_device())) return rc;
     uint8_t* base = (uint8_t*)scratch;
     cudaStream_t st = (cudaStream_t)stream;
     uint32_t* const word = status ? (uint32_t*)status : status_word();
@@ -437,6 +440,7 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     if ((rc = sm_count(&sms))) return rc;
     const HeadScratch s = head_scratch(n, hidden, vocab, true, dx != nullptr, dw != nullptr, sms);
     if (scratch_bytes < s.bytes) return COBALT_ESCRATCH;
+    if ((rc = bind_device())) return rc;
     uint8_t* base = (uint8_t*)scratch;
     cudaStream_t st = (cudaStream_t)stream;
     HlPrepareParams A = {};
@@ -454,16 +458,19 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     HlParams P = {};
     P.status = status ? (uint32_t*)status : status_word();
     if (!P.status) return COBALT_ELAUNCH;
+    const int n_pad = ceil_div(n, 32) * 32;
+    const bool two = s.pieces > 1;
     HlMaps M = {};
-    if ((rc = bf16_map(&M.x, A.packed, hidden, n, hidden)) || (rc = bf16_map(&M.w, weight, ldw, vocab, hidden)) ||
-        (rc = bf16_map(&M.w_tile, weight, ldw, vocab, hidden, s.width / 2))) return rc;
     CUtensorMap x_few, d_few[2];
-    if (s.few && (rc = bf16_map(&x_few, A.packed, hidden, n, hidden, ceil_div(n, 32) * 32))) return rc;
-    for (int b = 0; b < 2; ++b)
-        if ((rc = bf16_map(&M.d[b], base + s.d[b], s.piece, n, s.piece)) || (s.few && (rc = bf16_map(&d_few[b], base + s.d[b], s.piece, n, s.piece, ceil_div(n, 32) * 32)))) return rc;
-    if (dx && (rc = make_map(&M.slab, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base + s.slab, hidden, n, hidden, 32, s.splits))) return rc;
+    if ((rc = bf16_map(&M.w_tile, weight, ldw, vocab, hidden, s.width / 2)) || ((dw || !s.few) && (rc = bf16_map(&M.x, A.packed, hidden, n, hidden))) ||
+        (s.few && (rc = bf16_map(&x_few, x, ldx, n, hidden, n_pad))) || (dx && (rc = bf16_map(&M.w, weight, ldw, vocab, hidden)))) return rc;
+    for (int b = 0; b <= two; ++b) {
+        if ((dw || !s.few) && (rc = bf16_map(&M.d[b], base + s.d[b], s.piece, n, s.piece))) return rc;
+        if (s.few && dx && (rc = bf16_map(&d_few[b], base + s.d[b], s.piece, n, s.piece, n_pad))) return rc;
+    }
+    if (dx && !s.few && (rc = make_map(&M.slab, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base + s.slab, hidden, n, hidden, 32, s.splits))) return rc;
     if (dw && (rc = bf16_map(&M.dw, dw, ld_dw, vocab, hidden, 32))) return rc;
-    if ((rc = prepare(A, st))) return rc;
+    if (!s.few && (rc = prepare(A, st))) return rc;
     P.count = A.count;
     P.tok_tiles = ceil_div(n, HL_TILE);
     P.n_rows = n; P.hidden = hidden;
@@ -490,10 +497,15 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
         };
         // few tokens: logits and dx by their own kernel
         HfParams F = {};
-        F.n = n; F.n_pad = ceil_div(n, 32) * 32;
-        F.count = A.count;
+        F.n = n; F.n_pad = n_pad;
         F.hidden = hidden;
-        F.target = A.target; F.row = A.row;
+        F.targets = A.targets; F.vocab = vocab;
+        F.counted = A.count;
+        F.stats = A.stats;
+        F.grad = A.grad; F.grad_step = A.grad_step; F.mean = mean;
+        F.factor = A.factor;
+        F.x = A.x; F.ldx = ldx;
+        F.packed = A.packed;
         F.ld_d = s.piece;
         F.slab = (float*)(base + s.slab);
         F.status = P.status;
@@ -525,7 +537,7 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
             few_piece(HL_DLOGITS, i);
             F.rows = s.width;
             F.units = ceil_div(ceil_div(F.cols, HL_KS) * HL_KS, s.width);
-            if ((rc = few(F, M.w_tile, x_few, sms, false, st))) return rc;
+            if ((rc = few(F, M.w_tile, x_few, sms, i == 0, st))) return rc;
         }
         if (!s.few && i < s.pieces) {
             HlJob& j = piece(HL_DLOGITS, i);
@@ -535,7 +547,8 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
         }
         if (P.n_jobs && (rc = product(P, M, tiles, sms, st))) return rc;
     }
-    return dx ? launch_next(head_dx_kernel, dim3((unsigned)n), 256, 0, 1, st, (const float*)(base + s.slab), (const int*)A.slot, n, hidden, s.splits, (const float*)A.factor,
+    return dx ? launch_next(head_dx_kernel, dim3((unsigned)n), 256, 0, 1, st, (const float*)(base + s.slab), s.few ? (const int*)nullptr : (const int*)A.slot, A.targets,
+                            (long long)vocab, n, hidden, s.splits, (const float*)A.factor,
                             (uint16_t*)dx, (long long)ld_dx)
               : COBALT_OK;
 }

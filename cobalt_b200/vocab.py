@@ -225,18 +225,22 @@ def _head_loss(x, weight, targets, reduction, status, keep):
     """(result, what the gradient needs: ``[n, 2]`` if ``keep``)"""
     V, H = weight.shape
     n = targets.numel()
-    new = functools.partial(x.new_empty, dtype=torch.float32)
+    each = reduction == "none"
     if n == 0:
-        return x.new_zeros(targets.shape if reduction == "none" else (), dtype=torch.float32), new((0, 2)) if keep else None
+        return x.new_zeros(targets.shape if each else (), dtype=torch.float32), x.new_empty((0, 2), dtype=torch.float32) if keep else None
     rows, apart = _matrix("x", x, H, 8)
     w, apart_w = _matrix("weight", weight, H, 8)
-    loss, stats, total = new(targets.shape), new((n, 2)) if keep else None, new(()) if reduction != "none" else None
     index = x.get_device()
+    result = x.new_empty(targets.shape if each else (), dtype=torch.float32)
+    stats = x.new_empty((n, 2), dtype=torch.float32) if keep else None
     need = _scratch_bytes(index, "cobalt_head_loss_scratch_bytes", n, H, V)
-    scratch = x.new_empty(need, dtype=torch.uint8)
-    _call(index, "cobalt_head_loss", rows.data_ptr(), apart, w.data_ptr(), apart_w, targets.data_ptr(), n, H, V, loss.data_ptr(), None if stats is None else stats.data_ptr(),
-          None if total is None else total.data_ptr(), 1 if reduction == "mean" else 0, scratch.data_ptr(), need, None if status is None else status.data_ptr())
-    return loss if total is None else total, stats
+    scratch = x.new_empty(need if each else need + 4 * n, dtype=torch.uint8)       # per call, from the stream's own pool: overlapping calls never share one
+    at = scratch.data_ptr()
+    # (the tokens' losses, where only their sum is asked for, go behind the scratch)
+    _call(index, "cobalt_head_loss", rows.data_ptr(), apart, w.data_ptr(), apart_w, targets.data_ptr(), n, H, V, result.data_ptr() if each else at + need,
+          None if stats is None else stats.data_ptr(), None if each else result.data_ptr(), 1 if reduction == "mean" else 0, at, need,
+          None if status is None else status.data_ptr())
+    return result, stats
 
 
 def _head_loss_grad(x, weight, targets, stats, grad, reduction, status, want_x, want_w):
