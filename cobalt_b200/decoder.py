@@ -594,15 +594,15 @@ class CobaltDecoder:
         self._check_room(T)
         pos = torch.arange(T, device=self.dev)
         n, at_once = ids2.shape[0], self._prompts_at_once(T)
-        out = None
+        out, what = None, {"hidden": True} if hidden else {}
         if at_once > 1 and n > 1:
             try:
-                parts = [self._forward_prompts(ids2[b:b + at_once], pos, b, hidden) for b in range(0, n, at_once)]
+                parts = [self._forward_prompts(ids2[b:b + at_once], pos, b, **what) for b in range(0, n, at_once)]
                 out = parts[0] if len(parts) == 1 else torch.cat(parts)
             except torch.cuda.OutOfMemoryError:              # one at a time needs less, and writes the same again over what is in the caches (4-bit ones: to within the order of sums)
                 parts = None
         if out is None:
-            parts = [self._forward(ids2[b], pos, T, seq=b, hidden=hidden) for b in range(n)]
+            parts = [self._forward(ids2[b], pos, T, seq=b, **what) for b in range(n)]
             out = parts[0] if n == 1 else torch.cat(parts)
         self.pos.fill_(T)
         return out

@@ -90,8 +90,8 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
         if grad or (out.requires_grad and torch.is_grad_enabled()):
             raise RuntimeError("out cannot take a result that requires a gradient")
     if grad:
-        leaves = _leaves("embed", table)
-        return _seen(_Embed.apply(ids, table, float(scale)), leaves)
+        leaves, elsewhere = _leaves(table)
+        return _seen(_Embed.apply(ids, table, float(scale), elsewhere), leaves)
     return _embed(ids, table, float(scale), out)
 
 
@@ -109,19 +109,24 @@ def _embed(ids, table, scale, out=None):
 _graphs = {}                                                 # by id of a leaf: (it, weakly; the stream of the last graph made here; that graph, weakly)
 
 
-def _leaves(name: str, *inputs: torch.Tensor):
-    """The inputs that are leaves, for ``_seen``.  A captured backward pass must not reach a leaf through an autograd graph of another stream that
-    still lives: torch would wait for that stream, which invalidates the capture (or ends the process, where nothing catches it).  Said
-    before, as far as these functions made that graph."""
+def _leaves(*inputs: torch.Tensor):
+    """(the inputs that are leaves, for ``_seen``; whether a captured backward pass must not reach them)"""
     leaves = [t for t in inputs if t.requires_grad and t.is_leaf]
+    elsewhere = False
     if leaves and torch.cuda.is_current_stream_capturing():
         stream = _raw_stream(leaves[0].get_device())
         for t in leaves:
             leaf, made, graph = _graphs.get(id(t), (None, stream, None))
-            if made != stream and leaf() is t and graph() is not None:
-                raise RuntimeError(f"{name}: a graph of this leaf that was made on another stream is still alive; drop it before the capture, or capture "
-                                   "embed_grad / head_loss_and_grad, which need none")
-    return leaves
+            elsewhere |= made != stream and leaf() is t and graph() is not None
+    return leaves, elsewhere
+
+
+def _refuse_captured(name: str, elsewhere: bool):
+    """A captured backward pass must not reach a leaf through an autograd graph of another stream that still lives: torch would wait for that stream,
+    which invalidates the capture (or ends the process, where nothing catches it).  Said before, as far as these functions made that graph."""
+    if elsewhere and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name}: a graph of this leaf that was made on another stream is still alive; drop it before the capture, or capture "
+                           "embed_grad / head_loss_and_grad, which need none")
 
 
 def _seen(result: torch.Tensor, leaves) -> torch.Tensor:
@@ -158,15 +163,16 @@ def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float 
 
 class _Embed(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale):
+    def forward(ctx, ids, table, scale, elsewhere):
         ctx.save_for_backward(ids)
-        ctx.n_rows, ctx.scale = table.shape[0], scale
+        ctx.n_rows, ctx.scale, ctx.elsewhere = table.shape[0], scale, elsewhere
         return _embed(ids, table, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return None, embed_grad(grad, ctx.saved_tensors[0], ctx.n_rows, ctx.scale), None
+        _refuse_captured("embed", ctx.elsewhere)
+        return None, embed_grad(grad, ctx.saved_tensors[0], ctx.n_rows, ctx.scale), None, None
 
 
 # ----------------------------------------------------------------------------- head loss
@@ -178,8 +184,8 @@ def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, redu
     ``status`` (int32 ``[1]``, zero) takes the code of a bounded wait that gave up, as ``head_loss_status`` tells it without one."""
     targets = _check_loss(x, weight, targets, reduction, status)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        leaves = _leaves("head_loss", x, weight)
-        return _seen(_HeadLoss.apply(x, weight, targets, reduction, status), leaves)
+        leaves, elsewhere = _leaves(x, weight)
+        return _seen(_HeadLoss.apply(x, weight, targets, reduction, status, elsewhere), leaves)
     return _head_loss(x, weight, targets, reduction, status, False)[0]
 
 
@@ -266,18 +272,19 @@ def _head_loss_grad(x, weight, targets, stats, grad, reduction, status, want_x, 
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, targets, reduction, status):
+    def forward(ctx, x, weight, targets, reduction, status, elsewhere):
         result, stats = _head_loss(x, weight, targets, reduction, status, True)
         ctx.save_for_backward(x, weight, targets, stats)
-        ctx.reduction, ctx.status = reduction, status                # (the word is no input of the result)
+        ctx.reduction, ctx.status, ctx.elsewhere = reduction, status, elsewhere      # (the word is no input of the result)
         return result
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        _refuse_captured("head_loss", ctx.elsewhere)
         want_x, want_w = ctx.needs_input_grad[:2]
         dx, dw = _head_loss_grad(*ctx.saved_tensors, grad, ctx.reduction, ctx.status, want_x, want_w) if want_x or want_w else (None, None)
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None
 
 
 def head_loss_status(device=None) -> int:

@@ -183,9 +183,11 @@ def test_streams_and_graphs():
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
     kept = cb.embed(some_ids(n, V, 1), table)                          # an eager graph of the same leaf: its gradient is captured without one
-    with pytest.raises(RuntimeError, match="still alive"):
-        with torch.cuda.graph(torch.cuda.CUDAGraph()):
-            cb.embed(ids, table, 2.0)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        y = cb.embed(ids, table, 2.0)
+        with pytest.raises(RuntimeError, match="still alive"):
+            torch.autograd.grad(y, table, grad)
+    del y
     plain = torch.cuda.CUDAGraph()
     with torch.cuda.graph(plain):
         d0 = cb.embed_grad(grad, ids, V, 2.0)

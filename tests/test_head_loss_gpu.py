@@ -138,6 +138,12 @@ def test_pieces_of_the_vocabulary_and_of_the_tokens():
     dx, dw = torch.autograd.grad(loss, (x, w))
     near(dx, e.dx, e.dx_tol)
     near(dw, e.dw, e.dw_tol)
+    n, V, H = 100, 1400007, 64                                         # few tokens, two pieces
+    x, w, t = inputs(n, V, H, 17, 0.2, 3.0)
+    e = Exact(x, w, t, torch.ones(n, device="cuda"))
+    loss, dx, dw = cb.head_loss_and_grad(x, w, t, "sum")
+    near(dx, e.dx, e.dx_tol)
+    near(dw, e.dw, e.dw_tol)
     n = 33000
     x, w, t = inputs(n, 300, 72, 4, 0.3)
     e = Exact(x, w, t)
@@ -281,9 +287,11 @@ def test_streams_and_graphs():
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
     graphs = []
     kept = cb.head_loss(x, w, t)                                       # an eager graph of the same leaves: captured without autograd alone
-    with pytest.raises(RuntimeError, match="still alive"):
-        with torch.cuda.graph(torch.cuda.CUDAGraph()):
-            cb.head_loss(x, w, t)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        loss = cb.head_loss(x, w, t)
+        with pytest.raises(RuntimeError, match="still alive"):
+            torch.autograd.grad(loss, (x, w))
+    del loss
     for _ in range(2):                                                 # two graphs of the same call, replayed in turn
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
