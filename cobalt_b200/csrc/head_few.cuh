@@ -19,12 +19,11 @@ constexpr int HF_TOKENS = 128;             // at most
 constexpr int HF_EPI_WARPS = 8;
 constexpr int HF_THREADS = HF_EPI_WARPS * 32 + 64;
 constexpr uint32_t HF_A_BYTES = 4 * HL_BOX;
-constexpr int hf_stages(int n_pad) { return n_pad <= 32 ? 6 : n_pad <= 96 ? 5 : 4; }
+constexpr int hf_stages(int n_pad) { return n_pad <= 32 ? 6 : n_pad <= 64 ? 5 : 4; }
 constexpr uint32_t hf_stage_bytes(int n_pad) { return HF_A_BYTES + (uint32_t)n_pad * 128u; }
-constexpr uint32_t HF_TAIL = 256 + HF_TOKENS * 16;         // barriers, then maximum, log2 of the sum, factor and target of every token
-constexpr uint32_t HF_SMEM = hf_stages(96) * hf_stage_bytes(96) + HF_TAIL + 1024;
-static_assert(hf_stages(32) * hf_stage_bytes(32) + HF_TAIL + 1024 <= HF_SMEM && hf_stages(64) * hf_stage_bytes(64) + HF_TAIL + 1024 <= HF_SMEM &&
-              hf_stages(128) * hf_stage_bytes(128) + HF_TAIL + 1024 <= HF_SMEM && HF_SMEM <= 227 * 1024, "stages of every size fit");
+// stages, barriers, what belongs to a token (16 bytes), the warps' statistics of it (8 bytes each), room for the alignment
+constexpr uint32_t hf_smem(int n_pad) { return (uint32_t)hf_stages(n_pad) * hf_stage_bytes(n_pad) + 256 + (uint32_t)n_pad * (16 + 8 * HF_EPI_WARPS) + 1024; }
+static_assert(hf_smem(32) <= 227 * 1024 && hf_smem(64) <= 227 * 1024 && hf_smem(96) <= 227 * 1024 && hf_smem(128) <= 227 * 1024, "stages of every size fit");
 
 struct HfParams {
     int kind;                              // HL_STATS, HL_DLOGITS or HL_DX
@@ -36,7 +35,7 @@ struct HfParams {
     const long long* targets;              // stats, dlogits: of every token; one outside the vocabulary does not count
     long long vocab;
     int* counted;                          // stats: [0] tokens that count, [1] zero, for the kernel that joins; dlogits: [0] all tokens, for dw
-    float2* part;                          // stats: [8 * units][n_pad]
+    float2* part;                          // stats: [units][n_pad]
     float* at;
     const float2* stats;                   // dlogits: maximum and log2 of the sum
     const float* grad;                     // gradient of the loss, of every token (grad_step 1) or of the sum or mean (0)
@@ -105,6 +104,8 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         const int block = warp >> 2, in_block = (warp & 3) * 32 + lane;
         const uint32_t my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(block * P.n_pad);
         float4* const token_s = reinterpret_cast<float4*>(smem + (bars + 256u - smem_u32(smem)));
+        float2* const part_s = reinterpret_cast<float2*>(token_s + P.n_pad);           // [warp][n_pad]
+        auto epilogue_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         auto counts = [&](long long t) { return t >= 0 && t < P.vocab; };
         if (logits && blockIdx.x == 0 && warp == 0) {
             int counted = 0;
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                 for (int c = threadIdx.x; c < P.hidden / 8; c += HF_EPI_WARPS * 32)
                     reinterpret_cast<uint4*>(P.packed + (long long)i * P.hidden)[c] = in ? reinterpret_cast<const uint4*>(P.x + i * P.ldx)[c] : make_uint4(0, 0, 0, 0);
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");             // the epilogue warps
+            epilogue_sync();
         }
         bool healthy = true;
         uint32_t buf = 0, ph = 0;
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = exp2_fast((acc[32 * q + e] - __shfl_sync(full_mask, base, e)) * LOG2E);
                         const float sum = reduce_columns(v, lane, [](float a, float b) { return a + b; });
-                        P.part[((long long)u * HF_EPI_WARPS + warp) * P.n_pad + token] = make_float2(top, sum);
+                        part_s[warp * P.n_pad + token] = make_float2(top, sum);
                         // the token whose target is this row: its logit
                         const long long t = token < P.n ? P.targets[token] : -1;
                         const int rel = t >= 0 && t < P.vocab ? (int)t - (row - lane) : -1;      // lane of this warp that holds it
@@ -198,6 +199,20 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                             if (in_d) P.d[(long long)c * P.ld_d + in_piece] = float_to_bf16(g);
                         }
                     }
+                }
+                if (P.kind == HL_STATS) {                              // the warps' statistics joined, a thread a token
+                    epilogue_sync();
+                    if ((int)threadIdx.x < P.n_pad) {
+                        float top = -INFINITY, sum = 0.0f;
+                        for (int w = 0; w < HF_EPI_WARPS; ++w) top = fmaxf(top, part_s[w * P.n_pad + threadIdx.x].x);
+                        const float base = top == -INFINITY ? 0.0f : top;
+                        for (int w = 0; w < HF_EPI_WARPS; ++w) {
+                            const float2 v = part_s[w * P.n_pad + threadIdx.x];
+                            sum += v.y * exp2_fast((v.x - base) * LOG2E);
+                        }
+                        P.part[(long long)u * P.n_pad + threadIdx.x] = make_float2(top, sum);
+                    }
+                    epilogue_sync();
                 }
             } else {
                 const int split = u / P.h_tiles, h = (u - split * P.h_tiles) * HL_TILE + block * 128 + in_block;

@@ -156,7 +156,7 @@ HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool w
         s.width = few_rows(vocab, sms);
         s.count = take(256);
         s.at = take((size_t)n * 4);
-        s.part = take((size_t)ceil_div(vocab, s.width) * HF_EPI_WARPS * s.stats_tokens * 8);
+        s.part = take((size_t)ceil_div(vocab, s.width) * s.stats_tokens * 8);
         s.bytes = at;
         return s;
     }
@@ -220,12 +220,12 @@ int few(const HfParams& P, const CUtensorMap& a, const CUtensorMap& b, int sms, 
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)HF_SMEM) != cudaSuccess) return COBALT_ELAUNCH;
+        if (cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return COBALT_ELAUNCH;
         configured[dev] = true;
     }
     const dim3 grid((unsigned)std::min(P.units, sms));
-    if (!first) return launch_next(head_few_kernel, grid, HF_THREADS, HF_SMEM, 1, st, P, a, b);
-    head_few_kernel<<<grid, HF_THREADS, HF_SMEM, st>>>(P, a, b);
+    if (!first) return launch_next(head_few_kernel, grid, HF_THREADS, hf_smem(P.n_pad), 1, st, P, a, b);
+    head_few_kernel<<<grid, HF_THREADS, hf_smem(P.n_pad), st>>>(P, a, b);
     return launched();
 }
 int product(const HlParams& P, const HlMaps& M, int64_t tiles, int sms, cudaStream_t st) {
@@ -378,7 +378,7 @@ int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw
         CUtensorMap wm, xm;
         if ((rc = bf16_map(&wm, weight, ldw, vocab, hidden, s.width / 2)) || (rc = bf16_map(&xm, x, ldx, n, hidden, F.n_pad))) return rc;
         if ((rc = few(F, wm, xm, sms, true, st))) return rc;
-        J.parts = F.units * HF_EPI_WARPS;
+        J.parts = F.units;
         J.tokens = n;
         J.total = total;
         return launch_next(head_join_kernel, dim3((unsigned)ceil_div(n, HL_JOIN_TOKENS)), HL_JOIN_THREADS, 0, 1, st, J);
