@@ -28,6 +28,7 @@ constexpr int EG_BLOCK = 2048;             // ids that a block sorts
 constexpr int EG_SORT_THREADS = 1024;
 constexpr int EG_TILE = 16;                // sorted tokens of a tile
 constexpr int EG_JOIN_GRID = 256;          // blocks along the list of runs that cross tiles
+constexpr int EG_JOIN_THREADS = 256, EG_JOIN_COLS = 4 * EG_JOIN_THREADS;
 constexpr int EG_PLACE_THREADS = 256;
 constexpr int EG_SUM_THREADS = 128;
 constexpr uint32_t EG_NONE = 0xFFFFFFFFu;  // sorts behind every row
@@ -155,18 +156,21 @@ struct EmbedGradParams {
 };
 
 constexpr int EG_ZERO_BYTES = 32 * EG_SORT_THREADS;        // of a block
-// block `b` of those that clear the bytes [from, to); both multiples of 16
-__device__ __forceinline__ void embed_grad_zero(const EmbedGradParams& P, long long b, int threads, long long from, long long to) {
-    const long long at = from + (b * threads + threadIdx.x) * 32;
-    if (at >= to) return;
-    uint8_t* p = reinterpret_cast<uint8_t*>(P.out) + at;
-    if (at + 32 <= to && !((uintptr_t)p & 31)) {
-        asm volatile("st.global.v8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};" ::"l"(p), "r"(0) : "memory");
-    } else {
-        for (int i = 0; i < 32 && at + i < to; i += 16) {
-            if (at + i + 16 <= to) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
-            else
-                for (int k = i; at + k < to; ++k) p[k] = 0;            // the last bytes of the table
+// block `b` of those that clear the bytes [from, to), EG_ZERO_BYTES each; `from` is a multiple of 32
+template <int THREADS>
+__device__ __forceinline__ void embed_grad_zero(const EmbedGradParams& P, long long b, long long from, long long to) {
+#pragma unroll
+    for (int step = 0; step < EG_ZERO_BYTES / 32 / THREADS; ++step) {
+        const long long at = from + b * EG_ZERO_BYTES + (step * THREADS + (int)threadIdx.x) * 32;
+        uint8_t* p = reinterpret_cast<uint8_t*>(P.out) + at;
+        if (at + 32 <= to && !((uintptr_t)p & 31)) {
+            asm volatile("st.global.v8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};" ::"l"(p), "r"(0) : "memory");
+        } else {
+            for (int i = 0; i < 32 && at + i < to; i += 16) {
+                if (at + i + 16 <= to) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+                else
+                    for (int k = i; at + k < to; ++k) p[k] = 0;        // the last bytes of the table
+            }
         }
     }
 }
@@ -175,7 +179,7 @@ __device__ __forceinline__ void embed_grad_zero(const EmbedGradParams& P, long l
 // partners up to 32 apart are in its warp, others meet in shared memory.
 __global__ void __launch_bounds__(EG_SORT_THREADS) embed_grad_sort_kernel(const EmbedGradParams P) {
     if ((int)blockIdx.x >= P.blocks) {
-        embed_grad_zero(P, blockIdx.x - P.blocks, EG_SORT_THREADS, 0, P.zero_first);
+        embed_grad_zero<EG_SORT_THREADS>(P, blockIdx.x - P.blocks, 0, P.zero_first);
         return;
     }
     __shared__ ulonglong2 key_s[EG_SORT_THREADS];
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(EG_SORT_THREADS) embed_grad_sort_kernel(const 
 // Step 2.  An element's place: its own in its block, plus how many of every other block come before it (equal ids: of earlier blocks).
 __global__ void __launch_bounds__(EG_PLACE_THREADS) embed_grad_place_kernel(const EmbedGradParams P, int place_blocks) {
     if ((int)blockIdx.x >= place_blocks) {
-        embed_grad_zero(P, blockIdx.x - place_blocks, EG_PLACE_THREADS, P.zero_first, P.out_bytes);
+        embed_grad_zero<EG_PLACE_THREADS>(P, blockIdx.x - place_blocks, P.zero_first, P.out_bytes);
         return;
     }
     const long long i = (long long)blockIdx.x * EG_PLACE_THREADS + threadIdx.x;
@@ -313,47 +317,81 @@ __global__ void __launch_bounds__(EG_SUM_THREADS) embed_grad_sum_kernel(const Em
     }
 }
 
-// Step 4.  A run that leaves tile a for the first time: its rows in the tiles a .. b.  Eight warps take a part of them each.
+// Step 4.  A run that leaves tile a for the first time: its rows in the tiles a .. b.  A block takes 1024 columns: of short runs a thread four of them,
+// of long ones eight warps a part of the rows each.
 template <typename T>
-__global__ void __launch_bounds__(256) embed_grad_join_kernel(const EmbedGradParams P) {
-    __shared__ float sum_s[8][128];
+__device__ __forceinline__ void embed_grad_write(const EmbedGradParams& P, uint32_t id, int col, const float (&v)[4]) {
+    T o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) set_value(o[e], v[e] * P.scale);
+    T* out = reinterpret_cast<T*>(P.out) + (long long)id * P.width + col;
+    if (P.width % 4 == 0) {                                // rows of whole packs, and the table begins on a 16-byte boundary
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
+        else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < P.width) out[e] = o[e];
+    }
+}
+// four columns of `rows` rows of `part`, two rows apart each, on top of v
+__device__ __forceinline__ void embed_grad_rows(const EmbedGradParams& P, const float* part, int col, int rows, float (&v)[4]) {
+    if (P.width % 4 == 0) {
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) {
+            const float4 x = *reinterpret_cast<const float4*>(part + (long long)r * 2 * P.width + col);
+            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        }
+    } else {
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < P.width) v[e] += part[(long long)r * 2 * P.width + col + e];
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(EG_JOIN_THREADS) embed_grad_join_kernel(const EmbedGradParams P) {
+    __shared__ alignas(16) float sum_s[8][EG_JOIN_COLS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col = ((int)blockIdx.y * 32 + lane) * 4, c = (int)blockIdx.y * 128 + (int)threadIdx.x;
-    const int n_runs = (int)P.runs[0];
+    const int col0 = (int)blockIdx.y * EG_JOIN_COLS, n_runs = (int)P.runs[0];
     for (int k = blockIdx.x; k < n_runs; k += gridDim.x) {
         const long long a = P.runs[1 + k], end = (a + 1) * EG_TILE;
         const uint32_t id = P.ids_sorted[end];
         int rows = 0;                                      // tiles that it enters: those that begin with its id
-        for (int more = 256; more == 256; rows += more) {
+        for (int more = EG_JOIN_THREADS; more == EG_JOIN_THREADS; rows += more) {
             const long long at = (a + 1 + rows + threadIdx.x) * EG_TILE;
             more = __syncthreads_count(at < P.n && P.ids_sorted[at] == id);
         }
-        const int first = (int)((long long)rows * warp / 8), last = (int)((long long)rows * (warp + 1) / 8);
-        const float* part = P.part + (a + 1) * 2 * P.width + col;
-        float sum[4] = {};
-        if (P.width % 4 == 0) {
+        const float* first = P.part + (a * 2 + 1) * P.width;           // of the tile where it begins
+        const float* others = P.part + (a + 1) * 2 * P.width;
+        const int col = col0 + (int)threadIdx.x * 4;
+        if (rows <= 64) {
             if (col < P.width) {
-#pragma unroll 8
-                for (int r = first; r < last; ++r) {
-                    const float4 v = *reinterpret_cast<const float4*>(part + (long long)r * 2 * P.width);
-                    sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
-                }
+                float v[4] = {};
+                embed_grad_rows(P, first, col, 1, v);
+                embed_grad_rows(P, others, col, rows, v);
+                embed_grad_write<T>(P, id, col, v);
             }
-        } else {
-#pragma unroll 4
-            for (int r = first; r < last; ++r)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < P.width) sum[e] += part[(long long)r * 2 * P.width + e];
+            continue;
         }
-        *reinterpret_cast<float4*>(&sum_s[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        const int from = (int)((long long)rows * warp / 8), to = (int)((long long)rows * (warp + 1) / 8);
+        float v[8][4] = {};
+#pragma unroll 2
+        for (int r = from; r < to; ++r)
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+                if (col0 + g * 128 + lane * 4 < P.width) embed_grad_rows(P, others + (long long)r * 2 * P.width, col0 + g * 128 + lane * 4, 1, v[g]);
+#pragma unroll
+        for (int g = 0; g < 8; ++g) *reinterpret_cast<float4*>(&sum_s[warp][g * 128 + lane * 4]) = make_float4(v[g][0], v[g][1], v[g][2], v[g][3]);
         __syncthreads();
-        if (threadIdx.x < 128 && c < P.width) {
-            float total = P.part[a * 2 * P.width + P.width + c];
-            for (int w = 0; w < 8; ++w) total += sum_s[w][threadIdx.x];
-            T o;
-            set_value(o, total * P.scale);
-            reinterpret_cast<T*>(P.out)[(long long)id * P.width + c] = o;
+        if (col < P.width) {
+            float total[4] = {};
+            embed_grad_rows(P, first, col, 1, total);
+            for (int w = 0; w < 8; ++w)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) total[e] += sum_s[w][threadIdx.x * 4 + e];
+            embed_grad_write<T>(P, id, col, total);
         }
         __syncthreads();
     }

@@ -315,7 +315,7 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
     if ((rc = launched())) return rc;
     if (s.blocks > 1) {
         const int64_t places = ceil_div(n, EG_PLACE_THREADS);
-        embed_grad_place_kernel<<<(unsigned)(places + ceil_div(P.out_bytes - P.zero_first, 32 * EG_PLACE_THREADS)), EG_PLACE_THREADS, 0, st>>>(P, (int)places);
+        embed_grad_place_kernel<<<(unsigned)(places + ceil_div(P.out_bytes - P.zero_first, EG_ZERO_BYTES)), EG_PLACE_THREADS, 0, st>>>(P, (int)places);
         if ((rc = launched())) return rc;
     }
     const int words = std::min(words_at_once((uintptr_t)grad | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)width * size)), 4);
@@ -328,8 +328,8 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
     });
     if ((rc = launched())) return rc;
     if (s.tiles > 1) {
-        const dim3 join((unsigned)std::min(s.tiles, EG_JOIN_GRID), (unsigned)ceil_div(width, 128));
-        EMBED_TYPES(type, { embed_grad_join_kernel<T><<<join, 256, 0, st>>>(P); });
+        const dim3 join((unsigned)std::min(s.tiles, EG_JOIN_GRID), (unsigned)ceil_div(width, EG_JOIN_COLS));
+        EMBED_TYPES(type, { embed_grad_join_kernel<T><<<join, EG_JOIN_THREADS, 0, st>>>(P); });
     }
     return launched();
 }
