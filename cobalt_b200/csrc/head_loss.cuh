@@ -7,8 +7,8 @@
 //   dlogits   the same product again; d, rounded to bf16, goes to the piece's scratch [tokens][columns]
 //   dx        A = d (K-major), B = W with the vocabulary as K (N-major as it lies): fp32 sums over the pieces, in slabs [split][token][hidden]
 //   dw        A = d with the tokens as K (M-major as it lies), B = x the same: dW, rounded once
-// Operands come by TMA in boxes of 64 x 64, whatever their order: a box is 64 rows of 128 swizzled bytes, and which of its sides is K is
-// the descriptor's business.
+// Operands come by TMA in boxes of 64 columns, whatever their order: a box is rows of 128 swizzled bytes, and which of its sides is K is the
+// descriptor's business.
 //   warps 0-7  epilogue: warp w owns TMEM lanes 32 * (w % 4).. (a thread = a row) and columns 128 * (w / 4)..
 //   warp 8     TMA         warp 9     MMA (of the pair's first CTA)        warps 10, 11     none: they fill a warpgroup
 // An epilogue thread holds 128 sums.  The 168 registers that 384 threads have each do not hold them and what belongs to them, and what is
@@ -77,7 +77,8 @@ struct HlParams {
     uint32_t* status;
 };
 struct HlMaps {
-    CUtensorMap x, w, w_tile, d[2];        // bf16, boxes of 64 x 64; w_tile: 64 columns of half a tile's rows
+    CUtensorMap x, w, d[2];                // bf16, boxes of 64 x 64: operands whose rows are K
+    CUtensorMap x_rows, w_rows, d_rows[2]; // 64 columns of 128 rows, of w half a tile's: operands whose columns are K
     CUtensorMap slab, dw;                  // results: fp32 [split][token][hidden], boxes of 32 x 32; bf16, boxes of 64 columns x 32 rows
 };
 
@@ -204,23 +205,103 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
+// where the barriers of a block lie, from `bars` on: stage full, stage empty, accumulator complete, accumulator free
+__device__ __forceinline__ uint32_t hl_full(uint32_t bars, uint32_t s) { return bars + 8u * s; }
+__device__ __forceinline__ uint32_t hl_empty(uint32_t bars, uint32_t s) { return bars + 64u + 8u * s; }
+__device__ __forceinline__ uint32_t hl_acc(uint32_t bars, uint32_t b) { return bars + 128u + 8u * b; }
+__device__ __forceinline__ uint32_t hl_free(uint32_t bars, uint32_t b) { return bars + 144u + 8u * b; }
+
+// The warp that loads the operands, both CTAs each its half; the bytes of both are counted on the first one's barrier
+struct HlLoad {
+    uint32_t s0, bars, first_full, rank;
+    uint32_t* status;
+    uint32_t s, ph;                                        // stage that comes next, and its phase
+    bool ready;                                            // the stage was seen empty
+
+    template <bool A_MN, bool B_MN>
+    __device__ __forceinline__ bool tile(const CUtensorMap* a, int ax, int ay, const CUtensorMap* b, int bx, int by, int stages, uint32_t bytes) {
+        const uint32_t full_mask = 0xFFFFFFFFu;
+        for (int k = 0; k < stages; ++k) {
+            if (!ready && !__all_sync(full_mask, mbar_wait_bounded<true>(hl_empty(bars, s), ph ^ 1u, status, DEV_TIMEOUT_EMPTY))) return false;
+            const uint32_t next = s + 1 == HL_STAGES ? 0 : s + 1, next_ph = next ? ph : ph ^ 1u;
+            const bool seen = mbar_test_cluster(hl_empty(bars, next), next_ph ^ 1u);
+            const uint32_t dst = s0 + s * HL_STAGE_BYTES, bar = first_full + 8u * s;
+            if (elect_one()) {
+                if (rank == 0) mbar_arrive_expect_tx(hl_full(bars, s), bytes);
+                tma_load_2d<true>(dst, a, ax, ay, bar);
+                if (A_MN) tma_load_2d<true>(dst + HL_BOX, a, ax + 64, ay, bar);
+                tma_load_2d<true>(dst + 2 * HL_BOX, b, bx, by, bar);
+                if (B_MN) tma_load_2d<true>(dst + 3 * HL_BOX, b, bx + 64, by, bar);
+            }
+            __syncwarp();
+            ready = __all_sync(full_mask, seen);
+            (A_MN ? ay : ax) += HL_KS;
+            (B_MN ? by : bx) += HL_KS;
+            s = next;
+            ph = next_ph;
+        }
+        return true;
+    }
+};
+
+// The warp that issues the MMAs.  A stage is 512 clocks of MMA, and its wait, four MMAs and commit one after another took 630: so the next stage's
+// barrier is asked before the MMAs of this one are issued (without waiting), and the order of the operands is known at compile time
+// (descriptors differ in their low words alone).
+struct HlIssue {
+    uint32_t s0, bars, tmem;
+    uint32_t* status;
+    uint32_t s, ph, buf, aph;                              // stage and accumulator that come next, and their phases
+    bool ready;                                            // the stage was seen full
+
+    template <bool A_MN, bool B_MN>
+    __device__ __forceinline__ bool tile(int stages, int per, uint32_t width) {
+        const uint32_t full_mask = 0xFFFFFFFFu;
+        const uint32_t idesc = umma_idesc(width, HL_TILE) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+        constexpr uint32_t A_STEP = A_MN ? 2048 >> 4 : 32 >> 4, B_STEP = B_MN ? 2048 >> 4 : 32 >> 4;
+        for (int k0 = 0; k0 < stages; k0 += per) {
+            if (!__all_sync(full_mask, mbar_wait_bounded<true>(hl_free(bars, buf), aph ^ 1u, status, DEV_TIMEOUT_EMPTY))) return false;
+            tc_fence_after();
+            const uint32_t d = tmem + buf * 256u;
+            for (int k = k0; k < min(stages, k0 + per); ++k) {
+                if (!ready && !__all_sync(full_mask, mbar_wait_bounded<true>(hl_full(bars, s), ph, status, DEV_TIMEOUT_FULL))) return false;
+                cluster_acquire();                         // the other CTA's half
+                tc_fence_after();
+                const uint32_t next = s + 1 == HL_STAGES ? 0 : s + 1, next_ph = next ? ph : ph ^ 1u;
+                const bool seen = mbar_test_cluster(hl_full(bars, next), next_ph);
+                const uint32_t at = (s0 >> 4) + s * (HL_STAGE_BYTES >> 4);
+                const uint32_t a = at | (A_MN ? (HL_BOX >> 4) << 16 : 1u << 16), b = (at + (2 * HL_BOX >> 4)) | (B_MN ? (HL_BOX >> 4) << 16 : 1u << 16);
+                if (elect_one()) {
+#pragma unroll
+                    for (int q = 0; q < HL_KS / 16; ++q) umma_pair(d, a + A_STEP * q, b + B_STEP * q, idesc, (k > k0 || q > 0) ? 1u : 0u);
+                    umma_commit<true>(hl_empty(bars, s), 3);
+                }
+                __syncwarp();
+                ready = __all_sync(full_mask, seen);
+                s = next;
+                ph = next_ph;
+            }
+            if (elect_one()) umma_commit<true>(hl_acc(bars, buf), 3);
+            __syncwarp();
+            buf ^= 1u;
+            if (buf == 0) aph ^= 1u;
+        }
+        return true;
+    }
+};
+
 __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __grid_constant__ HlParams P, const __grid_constant__ HlMaps M) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full_mask = 0xFFFFFFFFu;
     const uint32_t s0 = (smem_u32(smem) + 1023u) & ~1023u;
     const uint32_t outs = s0 + HL_STAGES * HL_STAGE_BYTES, bars = outs + HL_EPI_WARPS * 2 * HL_OUT_BYTES;
-    auto bar_full = [&](uint32_t s) { return bars + 8u * s; };
-    auto bar_empty = [&](uint32_t s) { return bars + 64u + 8u * s; };
-    auto bar_acc = [&](uint32_t b) { return bars + 128u + 8u * b; };
-    auto bar_free = [&](uint32_t b) { return bars + 144u + 8u * b; };
     const uint32_t tmem_slot = bars + 160u;
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < HL_STAGES; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
-        for (uint32_t b = 0; b < 2; ++b) { mbar_init(bar_acc(b), 1); mbar_init(bar_free(b), 2 * HL_EPI_WARPS); }
+        for (uint32_t s = 0; s < HL_STAGES; ++s) { mbar_init(hl_full(bars, s), 1); mbar_init(hl_empty(bars, s), 1); }
+        for (uint32_t b = 0; b < 2; ++b) { mbar_init(hl_acc(bars, b), 1); mbar_init(hl_free(bars, b), 2 * HL_EPI_WARPS); }
         mbar_fence_init();
         fence_proxy_async();
     }
@@ -248,13 +329,13 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
         bool healthy = true;
         uint32_t buf = 0, ph = 0, side = 0;                // which accumulator comes next, and which half of `out`
         auto wait_acc = [&]() {
-            if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded<true>(bar_acc(buf), ph, P.status, DEV_TIMEOUT_ACC));
+            if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded<true>(hl_acc(bars, buf), ph, P.status, DEV_TIMEOUT_ACC));
             tc_fence_after();
         };
         auto free_acc = [&]() {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0 && healthy) mbar_arrive_cluster(map_to_rank(bar_free(buf), 0));
+            if (lane == 0 && healthy) mbar_arrive_cluster(map_to_rank(hl_free(bars, buf), 0));
             buf ^= 1u;
             if (buf == 0) ph ^= 1u;
         };
@@ -400,82 +481,26 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(HL_ROLE_REGS));
     if (warp == HL_EPI_WARPS) {
         // =========================================================== TMA
+        HlLoad L = {s0, bars, map_to_rank(hl_full(bars, 0), 0), rank, P.status, 0, 0, false};
         bool good = true;
-        uint32_t s = 0, ph = 0;
         const int mine = (int)rank * 128;
         while (good && list.take(P, &t)) {
             const HlJob& J = list.J;
-            const int m0 = t.m * HL_TILE + mine, n0 = t.n * J.width + (int)rank * (J.width / 2);
-            const CUtensorMap* const dmap = &M.d[J.buf];
-            const CUtensorMap *am, *bm;
-            bool a_rows, b_rows;                           // the operand's rows are the tensor's rows (K-major), else its columns
-            int ax, ay, bx, by;                            // at K = 0
-            if (J.kind <= HL_DLOGITS) {
-                am = &M.x; a_rows = true; ax = 0; ay = m0 + (J.kind == HL_STATS ? P.tok0 : 0);
-                bm = &M.w_tile; b_rows = true; bx = 0; by = J.v0 + n0;
-            } else if (J.kind == HL_DX) {
-                am = dmap; a_rows = true; ax = 0; ay = m0;
-                bm = &M.w; b_rows = false; bx = n0; by = J.v0;
-            } else {
-                am = dmap; a_rows = false; ax = m0; ay = 0;
-                bm = &M.x; b_rows = false; bx = n0; by = 0;
-            }
+            const int m0 = t.m * HL_TILE + mine, n0 = t.n * J.width + (int)rank * (J.width / 2), k0 = t.k0 * HL_KS, stages = t.k1 - t.k0;
             const uint32_t bytes = 2 * (2 * HL_BOX + (uint32_t)J.width * 64u);             // of both CTAs
-            for (int k = t.k0; k < t.k1; ++k) {
-                good = __all_sync(full_mask, mbar_wait_bounded<true>(bar_empty(s), ph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
-                if (!good) break;
-                const uint32_t bar = map_to_rank(bar_full(s), 0), dst = s0 + s * HL_STAGE_BYTES;
-                const int kk = k * HL_KS;
-                if (elect_one()) {
-                    if (rank == 0) mbar_arrive_expect_tx(bar_full(s), bytes);
-                    const int x = a_rows ? ax + kk : ax, y = a_rows ? ay : ay + kk;
-                    tma_load_2d<true>(dst, am, x, y, bar);
-                    tma_load_2d<true>(dst + HL_BOX, am, a_rows ? x : x + 64, a_rows ? y + 64 : y, bar);
-                    const int u = b_rows ? bx + kk : bx, v = b_rows ? by : by + kk;
-                    tma_load_2d<true>(dst + 2 * HL_BOX, bm, u, v, bar);
-                    if (!b_rows) tma_load_2d<true>(dst + 3 * HL_BOX, bm, u + 64, v, bar);
-                }
-                __syncwarp();
-                if (++s == HL_STAGES) { s = 0; ph ^= 1u; }
-            }
+            if (J.kind <= HL_DLOGITS) good = L.tile<false, false>(&M.x_rows, k0, m0 + (J.kind == HL_STATS ? P.tok0 : 0), &M.w_rows, k0, J.v0 + n0, stages, bytes);
+            else if (J.kind == HL_DX) good = L.tile<false, true>(&M.d_rows[J.buf], k0, m0, &M.w, n0, J.v0 + k0, stages, bytes);
+            else good = L.tile<true, true>(&M.d[J.buf], m0, k0, &M.x, n0, k0, stages, bytes);
         }
     } else if (warp == HL_EPI_WARPS + 1 && rank == 0) {
         // =========================================================== MMA
+        HlIssue I = {s0, bars, tmem, P.status, 0, 0, 0, 0, false};
         bool good = true;
-        uint32_t s = 0, ph = 0, buf = 0, aph = 0;
         while (good && list.take(P, &t)) {
-            const HlJob& J = list.J;
-            const bool a_mn = J.kind == HL_DW, b_mn = J.kind >= HL_DX;
-            const uint32_t idesc = umma_idesc((uint32_t)J.width, HL_TILE) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
-            const uint64_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
-            const int per = J.kind <= HL_DLOGITS ? HL_SUM_STAGES : t.k1 - t.k0;
-            for (int k0 = t.k0; good && k0 < t.k1; k0 += per) {
-                good = __all_sync(full_mask, mbar_wait_bounded<true>(bar_free(buf), aph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
-                if (!good) break;
-                tc_fence_after();
-                const uint32_t d = tmem + buf * 256u;
-                const int k1 = min(t.k1, k0 + per);
-                for (int k = k0; k < k1; ++k) {
-                    good = __all_sync(full_mask, mbar_wait_bounded<true>(bar_full(s), ph, P.status, DEV_TIMEOUT_FULL));
-                    if (!good) break;
-                    cluster_acquire();                     // the other CTA's half
-                    tc_fence_after();
-                    const uint32_t at = s0 + s * HL_STAGE_BYTES;
-                    const uint64_t ad = a_mn ? umma_smem_desc_mn(at, HL_BOX) : umma_smem_desc(at);
-                    const uint64_t bd = b_mn ? umma_smem_desc_mn(at + 2 * HL_BOX, HL_BOX) : umma_smem_desc(at + 2 * HL_BOX);
-                    if (elect_one()) {
-#pragma unroll
-                        for (int q = 0; q < HL_KS / 16; ++q) umma_bf16<true>(d, ad + a_step * q, bd + b_step * q, idesc, (k > k0 || q > 0) ? 1u : 0u);
-                        umma_commit<true>(bar_empty(s), 3);
-                    }
-                    __syncwarp();
-                    if (++s == HL_STAGES) { s = 0; ph ^= 1u; }
-                }
-                if (good && elect_one()) umma_commit<true>(bar_acc(buf), 3);
-                __syncwarp();
-                buf ^= 1u;
-                if (buf == 0) aph ^= 1u;
-            }
+            const int kind = list.J.kind, stages = t.k1 - t.k0;
+            const uint32_t width = (uint32_t)list.J.width;
+            good = kind <= HL_DLOGITS ? I.tile<false, false>(stages, HL_SUM_STAGES, width) : kind == HL_DX ? I.tile<false, true>(stages, stages, width)
+                                                                                                         : I.tile<true, true>(stages, stages, width);
         }
     }
     }

@@ -394,7 +394,7 @@ int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw
     HlParams P = {};
     P.status = word;
     HlMaps M = {};
-    if ((rc = bf16_map(&M.x, A.packed, hidden, n, hidden)) || (rc = bf16_map(&M.w_tile, weight, ldw, vocab, hidden, s.width / 2))) return rc;
+    if ((rc = bf16_map(&M.x_rows, A.packed, hidden, n, hidden, 128)) || (rc = bf16_map(&M.w_rows, weight, ldw, vocab, hidden, s.width / 2))) return rc;
     if ((rc = prepare(A, st))) return rc;
     const int v_tiles = (int)ceil_div(vocab, s.width);
     P.n_jobs = 1;
@@ -461,12 +461,14 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     const int n_pad = ceil_div(n, 32) * 32;
     const bool two = s.pieces > 1;
     HlMaps M = {};
-    CUtensorMap x_few, d_few[2];
-    if ((rc = bf16_map(&M.w_tile, weight, ldw, vocab, hidden, s.width / 2)) || ((dw || !s.few) && (rc = bf16_map(&M.x, A.packed, hidden, n, hidden))) ||
-        (s.few && (rc = bf16_map(&x_few, x, ldx, n, hidden, n_pad))) || (dx && (rc = bf16_map(&M.w, weight, ldw, vocab, hidden)))) return rc;
+    // what a kernel reads by rows it takes in boxes of 128 (few tokens: all of them), x where it lies if they are few
+    const int box = s.few ? n_pad : 128;
+    if ((rc = bf16_map(&M.w_rows, weight, ldw, vocab, hidden, s.width / 2)) ||
+        (rc = s.few ? bf16_map(&M.x_rows, x, ldx, n, hidden, box) : bf16_map(&M.x_rows, A.packed, hidden, n, hidden, box)) ||
+        (dw && (rc = bf16_map(&M.x, A.packed, hidden, n, hidden))) || (dx && (rc = bf16_map(&M.w, weight, ldw, vocab, hidden)))) return rc;
     for (int b = 0; b <= two; ++b) {
-        if ((dw || !s.few) && (rc = bf16_map(&M.d[b], base + s.d[b], s.piece, n, s.piece))) return rc;
-        if (s.few && dx && (rc = bf16_map(&d_few[b], base + s.d[b], s.piece, n, s.piece, n_pad))) return rc;
+        if (dw && (rc = bf16_map(&M.d[b], base + s.d[b], s.piece, n, s.piece))) return rc;
+        if (dx && (rc = bf16_map(&M.d_rows[b], base + s.d[b], s.piece, n, s.piece, box))) return rc;
     }
     if (dx && !s.few && (rc = make_map(&M.slab, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base + s.slab, hidden, n, hidden, 32, s.splits))) return rc;
     if (dw && (rc = bf16_map(&M.dw, dw, ld_dw, vocab, hidden, 32))) return rc;
@@ -519,7 +521,7 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
             few_piece(HL_DX, i - 1);
             F.h_tiles = h_tiles; F.splits = s.splits; F.add = i > 1;
             F.units = h_tiles * s.splits;
-            if ((rc = few(F, M.w, d_few[(i - 1) & 1], sms, false, st))) return rc;
+            if ((rc = few(F, M.w, M.d_rows[(i - 1) & 1], sms, false, st))) return rc;
         }
         if (!s.few && i > 0 && dx) {
             HlJob& j = piece(HL_DX, i - 1);
@@ -537,7 +539,7 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
             few_piece(HL_DLOGITS, i);
             F.rows = s.width;
             F.units = ceil_div(ceil_div(F.cols, HL_KS) * HL_KS, s.width);
-            if ((rc = few(F, M.w_tile, x_few, sms, i == 0, st))) return rc;
+            if ((rc = few(F, M.w_rows, M.x_rows, sms, i == 0, st))) return rc;
         }
         if (!s.few && i < s.pieces) {
             HlJob& j = piece(HL_DLOGITS, i);
