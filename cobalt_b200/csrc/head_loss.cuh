@@ -53,7 +53,7 @@ struct HlJob {
     int kind;
     int v0, cols;                          // piece of the vocabulary: its first row, and its rows inside the vocabulary
     int n_tiles;                           // tiles along B's side: of the piece (stats, dlogits) or of hidden columns (dx, dw)
-    int width;                             // their columns: 256, of logits any multiple of 16 up to that
+    int width;                             // their columns: 256, of logits any multiple of 32 up to that (what the instruction of a pair takes)
     int splits;                            // dx: ranges of the piece that are summed in slabs of their own
     int add;                               // dx: the slabs hold the sums of earlier pieces
     int buf;                               // which of the two scratch pieces holds d

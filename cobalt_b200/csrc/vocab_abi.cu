@@ -70,6 +70,7 @@ EmbedGradScratch embed_grad_scratch(int64_t n, int width) {
     return s;
 }
 constexpr int64_t EMBED_MAX_TOKENS = 1 << 24;
+constexpr int EMBED_MAX_WIDTH = 1 << 28;
 
 // ----------------------------------------------------------------------------- head loss
 constexpr int HEAD_MAX_TOKENS = 1 << 20, HEAD_MAX_HIDDEN = 1 << 16;
@@ -108,7 +109,7 @@ int bind_device() {
 int tile_width(int64_t token_tiles, int64_t cols, int pairs) {
     int best = HL_TILE;
     int64_t least = INT64_MAX;
-    for (int w = HL_TILE; w >= 96; w -= 16) {
+    for (int w = HL_TILE; w >= 96; w -= 32) {
         const int64_t cost = ceil_div(token_tiles * ceil_div(cols, w), pairs) * (w + 16);
         if (cost < least) { least = cost; best = w; }
     }
@@ -252,6 +253,7 @@ int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, i
     const int size = type_bytes(type);
     if (!ids || !table || !out || !size || n <= 0 || n_rows <= 0 || width <= 0 || ld < width || ld_out < width) return COBALT_EINVAL;
     if (((uintptr_t)ids & 7) || (((uintptr_t)table | (uintptr_t)out) & (size - 1))) return COBALT_EINVAL;
+    if (width > EMBED_MAX_WIDTH) return COBALT_ETOOBIG;
     int sms = 0;
     const int rc = sm_count(&sms);
     if (rc) return rc;
@@ -277,7 +279,7 @@ int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, i
 }
 
 size_t cobalt_embed_grad_scratch_bytes(int64_t n, int width) {
-    return n <= 0 || n > EMBED_MAX_TOKENS || width <= 0 ? 0 : embed_grad_scratch(n, width).bytes;
+    return n <= 0 || n > EMBED_MAX_TOKENS || width <= 0 || width > EMBED_MAX_WIDTH ? 0 : embed_grad_scratch(n, width).bytes;
 }
 
 int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out, void* scratch,
@@ -285,7 +287,7 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
     const int size = type_bytes(type);
     if (!ids || !grad || !out || !size || n <= 0 || n_rows <= 0 || width <= 0 || ld < width) return COBALT_EINVAL;
     if (((uintptr_t)ids & 7) || ((uintptr_t)grad & (size - 1)) || ((uintptr_t)out & 15)) return COBALT_EINVAL;
-    if (n > EMBED_MAX_TOKENS || n_rows > 0x7FFFFFFFll) return COBALT_ETOOBIG;
+    if (n > EMBED_MAX_TOKENS || n_rows > 0x7FFFFFFFll || width > EMBED_MAX_WIDTH) return COBALT_ETOOBIG;
     const EmbedGradScratch s = embed_grad_scratch(n, width);
     if (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < s.bytes) return COBALT_ESCRATCH;
     int sms = 0;

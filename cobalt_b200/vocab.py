@@ -20,6 +20,7 @@ from .linear import _raw_stream
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _REDUCTIONS = ("none", "sum", "mean")
+_WIDEST = 1 << 28                                            # columns of a table; larger sizes would not pass the C ABI's 32 bits
 
 
 def _call(index: int, name: str, *args):
@@ -80,8 +81,8 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
     shape, kind = table.shape, _TYPES.get(table.dtype)
     if kind is None:
         raise TypeError(f"table must be bfloat16, float16 or float32, got {table.dtype}")
-    if len(shape) != 2 or 0 in shape:
-        raise ValueError(f"table must be [n_rows, width], got {list(shape)}")
+    if len(shape) != 2 or 0 in shape or shape[1] > _WIDEST:
+        raise ValueError(f"table must be [n_rows, width] with width at most {_WIDEST}, got {list(shape)}")
     ids = _tokens("ids", ids, index)
     grad = torch.is_grad_enabled() and table.requires_grad
     if out is not None:
@@ -135,7 +136,7 @@ def _seen(result: torch.Tensor, leaves) -> torch.Tensor:
         for t in leaves:
             _graphs[id(t)] = weakref.ref(t), stream, graph
         if len(_graphs) > 256:
-            for key in [k for k, (leaf, _, g) in _graphs.items() if leaf() is None or g() is None]:
+            for key in [k for k, (leaf, _, g) in list(_graphs.items()) if leaf() is None or g() is None]:
                 _graphs.pop(key, None)
     return result
 
@@ -148,8 +149,9 @@ def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float 
         raise TypeError(f"grad must be bfloat16, float16 or float32, got {grad.dtype}")
     ids = _tokens("ids", ids, index)
     shape = grad.shape
-    if not shape or shape[:-1] != ids.shape or shape[-1] < 1 or n_rows < 1:
-        raise ValueError(f"grad must be [*ids.shape, width] = {[*ids.shape, 'width']} and n_rows at least 1, got {list(shape)} and {n_rows}")
+    if not shape or shape[:-1] != ids.shape or not 1 <= shape[-1] <= _WIDEST or n_rows < 1:
+        raise ValueError(f"grad must be [*ids.shape, width] = {[*ids.shape, 'width']}, width at most {_WIDEST}, and n_rows at least 1, got {list(shape)} "
+                         f"and {n_rows}")
     width, n = shape[-1], ids.numel()
     if n == 0:
         return grad.new_zeros((n_rows, width))
@@ -219,6 +221,8 @@ def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, re
         raise ValueError(f"x must be [..., {head[1]}], got {list(shape)}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
+    if targets.numel() >= 1 << 31:
+        raise ValueError(f"{targets.numel()} tokens in one call")
     targets = _tokens("targets", targets, index)
     if targets.shape != shape[:-1]:
         raise ValueError(f"targets must be {list(shape[:-1])}, got {list(targets.shape)}")

@@ -390,8 +390,8 @@ int cobalt_kv4_attend_watched(const void* q, int64_t ld_q, const void* tiles, in
 int cobalt_kv4_status(void* stream, uint32_t* status_out);
 
 /* The two dense ends of a vocabulary: embedding lookup and softmax cross entropy against a head, with their gradients.
- * Embedding calls: tables, rows and gradients of one type (COBALT_BF16, COBALT_FP16, COBALT_FP32), row strides ld in elements; any width,
- * any alignment of a value (16-byte rows are faster).  An id outside [0, n_rows) (-1: padding) reads zeros and has no gradient.
+ * Embedding calls: tables, rows and gradients of one type (COBALT_BF16, COBALT_FP16, COBALT_FP32), row strides ld in elements; any width
+ * up to 2^28, any alignment of a value (16-byte rows are faster).  An id outside [0, n_rows) (-1: padding) reads zeros and has no gradient.
  *   cobalt_embed      : out[t] = table[ids[t]] * scale, the product in fp32, rounded once (scale 1: the bits of the table).
  *   cobalt_embed_grad : out [n_rows][width] (contiguous, 16-byte aligned, every value written) = scale * sum of the rows grad[t] with ids[t] = row, in fp32,
  *                       rounded once.  The same inputs give the same bits.  n <= 2^24.

@@ -224,6 +224,11 @@ def test_refusals():
             bad()
     with pytest.raises(TypeError):
         cb.embed_grad(table[:3].int(), ids, 5)
+    wide = table[:1, :1].expand(3, 2 ** 32 + 8)                        # (a width of 8 in 32 bits)
+    with pytest.raises(ValueError):
+        cb.embed(ids, wide)
+    with pytest.raises(ValueError):
+        cb.embed_grad(wide, ids, 5)
 
 
 def test_a_table_that_was_used_can_be_copied_and_saved(tmp_path):

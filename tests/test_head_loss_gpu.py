@@ -341,6 +341,7 @@ def test_refusals():
                         (lambda: cb.head_loss(x, w[:, :56], t), ValueError), (lambda: cb.head_loss(x[:, :60], w[:, :60], t), ValueError),
                         (lambda: cb.head_loss(x, w, t[:3]), ValueError), (lambda: cb.head_loss(x, w, t.cpu()), ValueError), (lambda: cb.head_loss(x, w.cpu(), t), RuntimeError),
                         (lambda: cb.head_loss(x, w, t, "median"), ValueError), (lambda: cb.head_loss(x, w[0], t), ValueError), (lambda: cb.head_loss(x, w[:0], t), ValueError),
+                        (lambda: cb.head_loss(x[:1].expand(2 ** 32 + 4, 64), w, t[:1].expand(2 ** 32 + 4)), ValueError),       # (4 tokens in 32 bits)
                         (lambda: cb.head_loss(x, w, t, status=torch.zeros(1, device="cuda")), ValueError)):
         with pytest.raises(error):
             call()

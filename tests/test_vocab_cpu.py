@@ -37,10 +37,12 @@ def test_embedding_arguments_at_the_c_entry():
            dict(ids=A + 4), dict(table=A + 1), dict(out=A + 1), dict(type=0, table=A + 2)]
     for change in bad:
         assert L.cobalt_embed(*{**good, **change}.values(), None) == -1, change
+    wide = dict(width=(1 << 28) + 1, ld=1 << 29)
+    assert L.cobalt_embed(*{**good, **wide, 'ld_out': 1 << 29}.values(), None) == -6
     good = dict(ids=A, n=4, grad=A, ld=64, type=2, n_rows=10, width=64, scale=1.0, out=A, scratch=A, bytes=1 << 30)
     bad = [(dict(ids=None), -1), (dict(grad=None), -1), (dict(out=None), -1), (dict(out=A + 8), -1), (dict(n=0), -1), (dict(type=-1), -1), (dict(n_rows=0), -1),
            (dict(ld=60), -1), (dict(grad=A + 1), -1), (dict(scratch=None), -2), (dict(scratch=A + 16), -2), (dict(bytes=100), -2), (dict(n=(1 << 24) + 1), -6),
-           (dict(n_rows=1 << 31), -6)]
+           (dict(n_rows=1 << 31), -6), (wide, -6)]
     for change, rc in bad:
         assert L.cobalt_embed_grad(*{**good, **change}.values(), None) == rc, change
     assert L.cobalt_embed_grad_scratch_bytes(0, 64) == 0 and L.cobalt_embed_grad_scratch_bytes((1 << 24) + 1, 64) == 0
