@@ -59,11 +59,11 @@ EmbedGradScratch embed_grad_scratch(int64_t n, int width) {
     EmbedGradScratch s = {};
     s.blocks = (int)ceil_div(n, EG_BLOCK);
     s.tiles = (int)ceil_div(n, EG_TILE);
-    const size_t list = align256((size_t)s.blocks * EG_BLOCK * 4);
+    const size_t list = align256((size_t)n * 4);
     s.block_ids = 0;
     s.block_pos = list;
-    s.ids = s.blocks > 1 ? 2 * list : s.block_ids;
-    s.pos = s.blocks > 1 ? 3 * list : s.block_pos;
+    s.ids = 2 * list;
+    s.pos = 3 * list;
     s.runs = (s.blocks > 1 ? 4 : 2) * list;
     s.part = s.runs + align256(((size_t)s.tiles + 1) * 4);
     s.bytes = s.part + (s.tiles > 1 ? align256((size_t)s.tiles * 2 * width * 4) : 0);
@@ -71,6 +71,7 @@ EmbedGradScratch embed_grad_scratch(int64_t n, int width) {
 }
 constexpr int64_t EMBED_MAX_TOKENS = 1 << 24;
 constexpr int EMBED_MAX_WIDTH = 1 << 28;
+static_assert(EG_BLOCK == 1 << 11 && EG_GROUP == 1 << 4 && EMBED_MAX_TOKENS <= 1 << 27, "steps of placing");
 
 // ----------------------------------------------------------------------------- head loss
 constexpr int HEAD_MAX_TOKENS = 1 << 20, HEAD_MAX_HIDDEN = 1 << 16;
@@ -302,23 +303,32 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
     P.scale = scale;
     P.block_ids = (uint32_t*)(base + s.block_ids);
     P.block_pos = (uint32_t*)(base + s.block_pos);
-    P.ids_sorted = (uint32_t*)(base + s.ids);
-    P.pos_sorted = (uint32_t*)(base + s.pos);
+    P.ids_sorted = P.block_ids;
+    P.pos_sorted = P.block_pos;
     P.part = (float*)(base + s.part);
     P.runs = (uint32_t*)(base + s.runs);
-    // Placing takes about 1.5 us a block of ids; zeros are written at 7 MB in a microsecond meanwhile
+    // The first step of placing takes about 1.5 us a block of ids that it looks through; zeros are written at 7 MB in a microsecond meanwhile
     P.out_bytes = n_rows * width * size;
-    P.zero_first = s.blocks > 1 ? P.out_bytes - std::min<int64_t>(P.out_bytes / 2, (int64_t)s.blocks * (10 << 20)) / 32 * 32 : P.out_bytes;
+    P.zero_first = s.blocks > 1 ? P.out_bytes - std::min<int64_t>(P.out_bytes / 2, (int64_t)std::min(s.blocks, EG_GROUP) * (10 << 20)) / 32 * 32 : P.out_bytes;
     if (P.zero_first < P.out_bytes) P.zero_first = P.zero_first / 32 * 32;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t zeros = ceil_div(P.zero_first, EG_ZERO_BYTES);
     if (zeros > 0x3FFFFFFFll) return COBALT_ETOOBIG;
     embed_grad_sort_kernel<<<(unsigned)(s.blocks + zeros), EG_SORT_THREADS, 0, st>>>(P);
     if ((rc = launched())) return rc;
-    if (s.blocks > 1) {
-        const int64_t places = ceil_div(n, EG_PLACE_THREADS);
-        embed_grad_place_kernel<<<(unsigned)(places + ceil_div(P.out_bytes - P.zero_first, EG_ZERO_BYTES)), EG_PLACE_THREADS, 0, st>>>(P, (int)places);
+    uint32_t *ids_to = (uint32_t*)(base + s.ids), *pos_to = (uint32_t*)(base + s.pos);
+    for (int64_t run = EG_BLOCK; run < n; run *= EG_GROUP) {
+        const int64_t places = ceil_div(n, EG_PLACE_THREADS), rest = run == EG_BLOCK ? ceil_div(P.out_bytes - P.zero_first, EG_ZERO_BYTES) : 0;
+        // (the runs that tokens up to EMBED_MAX_TOKENS need)
+        const auto place = run == EG_BLOCK ? embed_grad_place_kernel<11> : run == EG_BLOCK * EG_GROUP ? embed_grad_place_kernel<15>
+                           : run == EG_BLOCK * EG_GROUP * EG_GROUP ? embed_grad_place_kernel<19> : embed_grad_place_kernel<23>;
+        place<<<(unsigned)(places + rest), EG_PLACE_THREADS, 0, st>>>(P, (int)places, P.ids_sorted, P.pos_sorted, ids_to, pos_to);
         if ((rc = launched())) return rc;
+        uint32_t* const ids_was = const_cast<uint32_t*>(P.ids_sorted), *const pos_was = const_cast<uint32_t*>(P.pos_sorted);
+        P.ids_sorted = ids_to;
+        P.pos_sorted = pos_to;
+        ids_to = ids_was;
+        pos_to = pos_was;
     }
     const int words = std::min(words_at_once((uintptr_t)grad | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)width * size)), 4);
     const int per_block = EG_SUM_THREADS * (words ? 16 / size : 1);
