@@ -680,28 +680,30 @@ __global__ void __launch_bounds__(HL_JOIN_THREADS) head_join_kernel(const HlJoin
     if (threadIdx.x == 0) *P.total = P.mean ? sum_s[0] / (float)max(P.count[0], 1) : sum_s[0];
 }
 
-// dx of every token: the sum of its slabs times the factor that all share, or zeros.  Without slots every token is at its own place, and counts if its
-// target is inside the vocabulary.
-__global__ void __launch_bounds__(256) head_dx_kernel(const float* slab, const int* slot, const long long* targets, long long vocab, int n_rows, int hidden, int splits, const float* factor, uint16_t* dx,
-                                                    long long ld) {
+// dx of every token: the sum of its slabs times the factor that all share, or zeros.  A thread has eight columns.  Without slots every token is at its own
+// place, and counts if its target is inside the vocabulary.
+constexpr int HL_DX_THREADS = 256;
+__global__ void __launch_bounds__(HL_DX_THREADS) head_dx_kernel(const float* slab, const int* slot, const long long* targets, long long vocab, int n_rows, int hidden,
+                                                               int splits, const float* factor, uint16_t* dx, long long ld) {
+    pdl_next();
     pdl_wait();
-    const int i = blockIdx.x, p = slot ? slot[i] : targets[i] >= 0 && targets[i] < vocab ? i : -1;
+    const int i = blockIdx.x, c = ((int)blockIdx.y * HL_DX_THREADS + (int)threadIdx.x) * 8;
+    const int p = slot ? slot[i] : targets[i] >= 0 && targets[i] < vocab ? i : -1;
+    if (c >= hidden) return;
     const float g = *factor;
-    for (int c = threadIdx.x * 8; c < hidden; c += 256 * 8) {
-        float v[8] = {};
-        if (p >= 0) {
+    float v[8] = {};
+    if (p >= 0) {
 #pragma unroll 8
-            for (int s = 0; s < splits; ++s) {
-                const float4* q = reinterpret_cast<const float4*>(slab + ((long long)s * n_rows + p) * hidden + c);
-                const float4 a = q[0], b = q[1];
-                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-                v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-            }
+        for (int s = 0; s < splits; ++s) {
+            const float4* q = reinterpret_cast<const float4*>(slab + ((long long)s * n_rows + p) * hidden + c);
+            const float4 a = q[0], b = q[1];
+            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+            v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
         }
-        *reinterpret_cast<uint4*>(dx + (long long)i * ld + c) =
-            p < 0 ? make_uint4(0, 0, 0, 0)
-                  : make_uint4(pack_bf16x2(v[0] * g, v[1] * g), pack_bf16x2(v[2] * g, v[3] * g), pack_bf16x2(v[4] * g, v[5] * g), pack_bf16x2(v[6] * g, v[7] * g));
     }
+    *reinterpret_cast<uint4*>(dx + (long long)i * ld + c) =
+        p < 0 ? make_uint4(0, 0, 0, 0)
+              : make_uint4(pack_bf16x2(v[0] * g, v[1] * g), pack_bf16x2(v[2] * g, v[3] * g), pack_bf16x2(v[4] * g, v[5] * g), pack_bf16x2(v[6] * g, v[7] * g));
 }
 
 }  // namespace cb

@@ -493,6 +493,11 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     P.factor = A.factor;
     P.d[0] = (uint16_t*)(base + s.d[0]); P.d[1] = (uint16_t*)(base + s.d[1]);
     P.ld_d = s.piece;
+    auto join_dx = [&](const int* slot) {
+        const dim3 grid((unsigned)n, (unsigned)ceil_div(hidden, 8 * HL_DX_THREADS));
+        return launch_next(head_dx_kernel, grid, HL_DX_THREADS, 0, 1, st, (const float*)(base + s.slab), slot, A.targets, (long long)vocab, n, hidden, s.splits,
+                           (const float*)A.factor, (uint16_t*)dx, (long long)ld_dx);
+    };
     // One launch per piece and one more: the products with piece i's d beside the logits of piece i + 1
     const int h_tiles = ceil_div(hidden, HL_TILE);
     for (int i = 0; i <= s.pieces; ++i) {
@@ -534,6 +539,8 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
             F.h_tiles = h_tiles; F.splits = s.splits; F.add = i > 1;
             F.units = h_tiles * s.splits;
             if ((rc = few(F, M.w, M.d_rows[(i - 1) & 1], sms, false, st))) return rc;
+            // (before dw: its writes fill the L2, and reading the slabs behind them took 17 us where it takes 8)
+            if (i == s.pieces && (rc = join_dx(nullptr))) return rc;
         }
         if (!s.few && i > 0 && dx) {
             HlJob& j = piece(HL_DX, i - 1);
@@ -561,10 +568,7 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
         }
         if (P.n_jobs && (rc = product(P, M, tiles, sms, st))) return rc;
     }
-    return dx ? launch_next(head_dx_kernel, dim3((unsigned)n), 256, 0, 1, st, (const float*)(base + s.slab), s.few ? (const int*)nullptr : (const int*)A.slot, A.targets,
-                            (long long)vocab, n, hidden, s.splits, (const float*)A.factor,
-                            (uint16_t*)dx, (long long)ld_dx)
-              : COBALT_OK;
+    return dx && !s.few ? join_dx(A.slot) : COBALT_OK;
 }
 
 int cobalt_vocab_status(void* stream, uint32_t* status_out) {
