@@ -32,7 +32,7 @@ namespace cb {
 
 constexpr int HL_TILE = 256;               // rows and columns of a pair's tile
 constexpr int HL_KS = 64;                  // K per stage
-constexpr int HL_STAGES = 5;
+constexpr int HL_STAGES = 5, HL_LOGIT_STAGES = 7;         // of logits alone: nothing goes out by shared memory
 constexpr uint32_t HL_BOX = 64 * 128;      // bytes of 64 rows x 64 bf16
 constexpr uint32_t HL_STAGE_BYTES = 4 * HL_BOX;
 constexpr int HL_EPI_WARPS = 8;
@@ -43,6 +43,7 @@ static_assert(HL_EPI_REGS * HL_EPI_WARPS * 32 + HL_ROLE_REGS * 128 <= HL_REGS * 
 constexpr int HL_SUM_STAGES = 8;           // stages of logits that are summed in tensor memory
 constexpr uint32_t HL_OUT_BYTES = 32 * 128;                // results of a warp on their way out: 32 rows of 128 swizzled bytes, twice
 constexpr uint32_t HL_SMEM = HL_STAGES * HL_STAGE_BYTES + HL_EPI_WARPS * 2 * HL_OUT_BYTES + 256 + 1024;
+static_assert(HL_LOGIT_STAGES * HL_STAGE_BYTES <= HL_STAGES * HL_STAGE_BYTES + HL_EPI_WARPS * 2 * HL_OUT_BYTES && HL_LOGIT_STAGES <= 8, "room and barriers");
 constexpr int HL_JOBS = 3;
 constexpr float LOG2E = 1.44269504088896341f;
 
@@ -62,6 +63,7 @@ struct HlJob {
 struct HlParams {
     HlJob job[HL_JOBS];
     int n_jobs;
+    int stages;
     const int* count;                      // tokens that count
     int tok0, tok_tiles;                   // stats: first token, and at most this many tiles of tokens
     int n_rows;                            // rows of the packed x (and of a slab)
@@ -213,7 +215,7 @@ __device__ __forceinline__ uint32_t hl_free(uint32_t bars, uint32_t b) { return 
 
 // The warp that loads the operands, both CTAs each its half; the bytes of both are counted on the first one's barrier
 struct HlLoad {
-    uint32_t s0, bars, first_full, rank;
+    uint32_t s0, bars, first_full, rank, depth;            // depth: how many stages there are
     uint32_t* status;
     uint32_t s, ph;                                        // stage that comes next, and its phase
     bool ready;                                            // the stage was seen empty
@@ -223,7 +225,7 @@ struct HlLoad {
         const uint32_t full_mask = 0xFFFFFFFFu;
         for (int k = 0; k < stages; ++k) {
             if (!ready && !__all_sync(full_mask, mbar_wait_bounded<true>(hl_empty(bars, s), ph ^ 1u, status, DEV_TIMEOUT_EMPTY))) return false;
-            const uint32_t next = s + 1 == HL_STAGES ? 0 : s + 1, next_ph = next ? ph : ph ^ 1u;
+            const uint32_t next = s + 1 == depth ? 0 : s + 1, next_ph = next ? ph : ph ^ 1u;
             const bool seen = mbar_test_cluster(hl_empty(bars, next), next_ph ^ 1u);
             const uint32_t dst = s0 + s * HL_STAGE_BYTES, bar = first_full + 8u * s;
             if (elect_one()) {
@@ -248,7 +250,7 @@ struct HlLoad {
 // barrier is asked before the MMAs of this one are issued (without waiting), and the order of the operands is known at compile time
 // (descriptors differ in their low words alone).
 struct HlIssue {
-    uint32_t s0, bars, tmem;
+    uint32_t s0, bars, tmem, depth;
     uint32_t* status;
     uint32_t s, ph, buf, aph;                              // stage and accumulator that come next, and their phases
     bool ready;                                            // the stage was seen full
@@ -266,7 +268,7 @@ struct HlIssue {
                 if (!ready && !__all_sync(full_mask, mbar_wait_bounded<true>(hl_full(bars, s), ph, status, DEV_TIMEOUT_FULL))) return false;
                 cluster_acquire();                         // the other CTA's half
                 tc_fence_after();
-                const uint32_t next = s + 1 == HL_STAGES ? 0 : s + 1, next_ph = next ? ph : ph ^ 1u;
+                const uint32_t next = s + 1 == depth ? 0 : s + 1, next_ph = next ? ph : ph ^ 1u;
                 const bool seen = mbar_test_cluster(hl_full(bars, next), next_ph);
                 const uint32_t at = (s0 >> 4) + s * (HL_STAGE_BYTES >> 4);
                 const uint32_t a = at | (A_MN ? (HL_BOX >> 4) << 16 : 1u << 16), b = (at + (2 * HL_BOX >> 4)) | (B_MN ? (HL_BOX >> 4) << 16 : 1u << 16);
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < HL_STAGES; ++s) { mbar_init(hl_full(bars, s), 1); mbar_init(hl_empty(bars, s), 1); }
+        for (uint32_t s = 0; s < (uint32_t)P.stages; ++s) { mbar_init(hl_full(bars, s), 1); mbar_init(hl_empty(bars, s), 1); }
         for (uint32_t b = 0; b < 2; ++b) { mbar_init(hl_acc(bars, b), 1); mbar_init(hl_free(bars, b), 2 * HL_EPI_WARPS); }
         mbar_fence_init();
         fence_proxy_async();
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(HL_ROLE_REGS));
     if (warp == HL_EPI_WARPS) {
         // =========================================================== TMA
-        HlLoad L = {s0, bars, map_to_rank(hl_full(bars, 0), 0), rank, P.status, 0, 0, false};
+        HlLoad L = {s0, bars, map_to_rank(hl_full(bars, 0), 0), rank, (uint32_t)P.stages, P.status, 0, 0, false};
         bool good = true;
         const int mine = (int)rank * 128;
         while (good && list.take(P, &t)) {
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
         }
     } else if (warp == HL_EPI_WARPS + 1 && rank == 0) {
         // =========================================================== MMA
-        HlIssue I = {s0, bars, tmem, P.status, 0, 0, 0, 0, false};
+        HlIssue I = {s0, bars, tmem, (uint32_t)P.stages, P.status, 0, 0, 0, 0, false};
         bool good = true;
         while (good && list.take(P, &t)) {
             const int kind = list.J.kind, stages = t.k1 - t.k0;

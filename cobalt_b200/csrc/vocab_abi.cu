@@ -411,6 +411,7 @@ int cobalt_head_loss(const void* x, int64_t ldx, const void* weight, int64_t ldw
     if ((rc = prepare(A, st))) return rc;
     const int v_tiles = (int)ceil_div(vocab, s.width);
     P.n_jobs = 1;
+    P.stages = HL_LOGIT_STAGES;
     P.job[0].kind = HL_STATS;
     P.job[0].cols = (int)vocab;
     P.job[0].n_tiles = v_tiles;
@@ -567,6 +568,7 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
             j.n_tiles = ceil_div(ceil_div(j.cols, HL_KS) * HL_KS, s.width);    // (dx reads whole stages of d)
             tiles += (int64_t)P.tok_tiles * j.n_tiles;
         }
+        P.stages = i == 0 ? HL_LOGIT_STAGES : HL_STAGES;
         if (P.n_jobs && (rc = product(P, M, tiles, sms, st))) return rc;
     }
     return dx && !s.few ? join_dx(A.slot) : COBALT_OK;
