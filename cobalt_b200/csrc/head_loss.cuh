@@ -96,7 +96,9 @@ struct HlList {
     int m_tiles, tiles;
     int shift;                             // the pair's place in the round of the current job
     int extra, few_from, few;              // rounds that only the pairs from few_from on take part in, `few` of them
-    int at_m, at_n, step_m, step_n;        // gradients: the last tile (at_m < 0: none yet), and the way to the next
+    // The last tile as (outer, base + inner): gradients of one range (token or row tile, hidden tile), logits (vocabulary tile, token tile of the group that
+    // begins at `base`).  The next one is a step away; outer < 0: work it out from its number.
+    int outer, inner, base, outers, inners, step_out, step_in;
 
     __device__ __forceinline__ HlList(const HlParams& P, int pair_, int pairs_, int tokens_) {
         pair = pair_; pairs = pairs_; tokens = tokens_;
@@ -109,7 +111,7 @@ struct HlList {
     }
     __device__ __forceinline__ void open(const HlParams& P, int j) {
         job = j;
-        at_m = -1;
+        outer = -1;
         if (j < P.n_jobs) J = P.job[j];
         m_tiles = J.kind == HL_DW ? (J.cols + HL_TILE - 1) / HL_TILE : token_tiles;
         tiles = m_tiles * J.n_tiles * J.splits;
@@ -118,16 +120,17 @@ struct HlList {
         return J.kind <= HL_DLOGITS ? (P.hidden + HL_KS - 1) / HL_KS : J.kind == HL_DX ? (J.cols + HL_KS - 1) / HL_KS / J.splits : max((tokens + HL_KS - 1) / HL_KS, 1);
     }
     __device__ __forceinline__ bool take(const HlParams& P, HlTile* t) {
-        if (at_m >= 0) {                                               // rounds of all pairs in a gradient of one range
-            at_m += step_m;
-            at_n += step_n;
-            if (at_n >= J.n_tiles) { at_n -= J.n_tiles; ++at_m; }
-            if (at_m < m_tiles) {
-                t->m = at_m;
-                t->n = at_n;
+        if (outer >= 0) {
+            outer += step_out;
+            inner += step_in;
+            if (inner >= inners) { inner -= inners; ++outer; }
+            if (outer < outers) {
+                t->m = J.kind <= HL_DLOGITS ? base + inner : outer;
+                t->n = J.kind <= HL_DLOGITS ? outer : inner;
+                ++next;
                 return true;
             }
-            next = tiles;                                              // none is left
+            outer = -1;                                                // none is left, or in another group
         }
         while (job < P.n_jobs) {
             int i = tiles;
@@ -138,11 +141,12 @@ struct HlList {
             if (next >= extra && next < tiles) i = extra * few + shift + (next - extra) * pairs;
             if (i < tiles) {
                 place(P, i, t);
-                if (next >= extra && J.kind >= HL_DX && J.splits == 1) {
-                    at_m = t->m;
-                    at_n = t->n;
-                    step_m = pairs / J.n_tiles;
-                    step_n = pairs - step_m * J.n_tiles;
+                if (next >= extra && (J.kind <= HL_DLOGITS || J.splits == 1)) {
+                    outer = J.kind <= HL_DLOGITS ? t->n : t->m;
+                    inner = J.kind <= HL_DLOGITS ? t->m - base : t->n;
+                    if (J.kind > HL_DLOGITS) { outers = m_tiles; inners = J.n_tiles; }
+                    step_out = pairs / inners;
+                    step_in = pairs - step_out * inners;
                 }
                 ++next;
                 return true;
@@ -164,14 +168,17 @@ struct HlList {
     }
     // Tile i of a job.  Logits: tokens in groups of at most 12 tiles, so that a group's x stays in the L2 while the vocabulary streams by, once a
     // group; gradients: neighbours share the operand that is longer.
-    __device__ __forceinline__ void place(const HlParams& P, int i, HlTile* t) const {
+    __device__ __forceinline__ void place(const HlParams& P, int i, HlTile* t) {
         t->k0 = 0;
         t->split = 0;
         if (J.kind <= HL_DLOGITS) {
             const int groups = (token_tiles + 11) / 12, per = (token_tiles + groups - 1) / groups;
-            const int g = i / (per * J.n_tiles), in = i - g * per * J.n_tiles, width = min(per, token_tiles - g * per);
-            t->n = in / width;
-            t->m = g * per + in - t->n * width;
+            const int g = i / (per * J.n_tiles), in = i - g * per * J.n_tiles;
+            base = g * per;
+            inners = min(per, token_tiles - base);
+            outers = J.n_tiles;
+            t->n = in / inners;
+            t->m = base + in - t->n * inners;
             t->k1 = (P.hidden + HL_KS - 1) / HL_KS;
         } else if (J.kind == HL_DX) {
             const int ks = (J.cols + HL_KS - 1) / HL_KS, one = token_tiles * J.n_tiles, s = i / one, in = i - s * one;
