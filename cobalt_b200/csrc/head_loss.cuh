@@ -637,6 +637,7 @@ __global__ void __launch_bounds__(HL_JOIN_THREADS) head_join_kernel(const HlJoin
     }
     const bool here = p >= P.tok0 && p < P.tok0 + P.tokens;
     float m = -INFINITY, s = 0.0f;
+    const float own = here && slice == 0 ? P.at[p] : 0.0f; // (asked for early)
     if (here) {
         const float2* part = P.part + (p - P.tok0);
 #pragma unroll 8
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(HL_JOIN_THREADS) head_join_kernel(const HlJoin
     }
     if (slice == 0 && i < P.n) {
         if (here) {
-            P.loss[i] = (m - P.at[p]) + logf(s);
+            P.loss[i] = (m - own) + logf(s);
             if (P.stats) P.stats[i] = make_float2(m, log2f(s));
         } else if (p < 0) {
             P.loss[i] = 0.0f;
@@ -671,12 +672,15 @@ __global__ void __launch_bounds__(HL_JOIN_THREADS) head_join_kernel(const HlJoin
         }
     }
     if (!P.total) return;
-    __threadfence();
+    if (gridDim.x > 1) {
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) last_s = atomicAdd(&P.count[1], 1) == (int)gridDim.x - 1;
+        __syncthreads();
+        if (!last_s) return;
+        __threadfence();
+    }
     __syncthreads();
-    if (threadIdx.x == 0) last_s = atomicAdd(&P.count[1], 1) == (int)gridDim.x - 1;
-    __syncthreads();
-    if (!last_s) return;
-    __threadfence();
     float* sum_s = &s_s[0][0];
     float sum = 0.0f;
     for (int k = threadIdx.x; k < P.n; k += HL_JOIN_THREADS) sum += __ldcg(P.loss + k);
