@@ -78,7 +78,7 @@ def near(got, want, tol):
 
 
 SIZES = [(1, 1, 8), (1, 2, 8), (1, 32000, 128), (2, 255, 72), (3, 257, 64), (17, 511, 136), (63, 1000, 512), (64, 512, 520), (65, 130, 1000), (127, 2049, 320),
-         (129, 384, 256), (255, 700, 192), (256, 256, 256), (257, 257, 264), (333, 10007, 1000), (600, 5000, 2048), (1025, 513, 640)]
+         (129, 384, 256), (255, 700, 192), (256, 256, 256), (257, 257, 264), (333, 10007, 1000), (400, 7000, 320), (600, 5000, 2048), (1025, 513, 640)]
 
 
 @pytest.mark.parametrize("n,V,H", SIZES)
