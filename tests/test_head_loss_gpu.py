@@ -272,9 +272,10 @@ def test_shapes_and_strides():
     assert dx.shape == (0, H) and not bool(dw.any())
 
 
-def test_streams_and_graphs():
+@pytest.mark.parametrize("n", [20, 400])
+def test_streams_and_graphs(n):
     """Two streams at once; loss and gradients captured, by autograd and without it, and replayed on new inputs."""
-    n, V, H = 400, 3000, 256
+    V, H = 3000, 256
     x, w, t = inputs(n, V, H, 11, 0.3)
     x.requires_grad_(), w.requires_grad_()
     want = torch.autograd.grad(cb.head_loss(x, w, t), (x, w))
@@ -311,6 +312,29 @@ def test_streams_and_graphs():
         ref = cb.head_loss(x, w, t)
         for _, loss, dx, dw in graphs:
             assert torch.equal(loss, ref) and all(torch.equal(a, b) for a, b in zip((dx, dw), torch.autograd.grad(ref, (x, w), retain_graph=True)))
+
+
+def test_threads():
+    """Four host threads on streams of their own, few tokens and many."""
+    import threading
+    cases = [inputs(n, 3000, 256, n, 0.3) for n in (20, 100, 400, 700)]
+    want = [cb.head_loss_and_grad(*c) for c in cases]
+    torch.cuda.synchronize()
+    bad, done = [], []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [cb.head_loss_and_grad(*cases[i]) for _ in range(8)]
+            torch.cuda.current_stream().synchronize()
+            bad.extend(i for g in got if not all(torch.equal(a, b) for a, b in zip(g, want[i])))
+        done.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and sorted(done) == [0, 1, 2, 3] and cb.head_loss_status() == 0
 
 
 def test_offsets_beyond_32_bits():
