@@ -93,7 +93,7 @@ def test_lookup_strides_shapes_and_results():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,V,H,kind", [(1, 1, 1, "some"), (1, 5, 8, "some"), (5, 2, 16, "none"), (31, 9, 64, "one"), (32, 40, 72, "few"), (33, 40, 65, "few"),
-                                        (64, 3, 1001, "one"), (100, 30000, 128, "some"), (2048, 100, 40, "few"), (2049, 100, 40, "few"), (4096, 7, 24, "one"),
+                                        (64, 3, 1001, "one"), (100, 30000, 128, "some"), (2048, 100, 40, "few"), (2049, 100, 40, "few"), (4096, 7, 24, "one"), (6143, 500, 24, "few"), (6144, 9, 40, "some"), (6145, 500, 24, "few"),
                                         (7000, 5000, 264, "few"), (20001, 333, 33, "few"),
                                         (32769, 40000, 16, "some"), (600001, 5000, 8, "few"),
                                         (8388611, 100000, 2, "some")])
