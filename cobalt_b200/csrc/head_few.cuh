@@ -70,6 +70,51 @@ __device__ __forceinline__ float reduce_columns(float (&v)[32], int lane, F f) {
     return v[0];
 }
 
+// The warp that issues the MMAs, as HlIssue does: eight of them and a commit a stage, the next stage's barrier asked ahead (barriers lie where the pair kernel has them)
+struct HfIssue {
+    uint32_t s0, bars, tmem, stage_bytes, depth, n_pad;
+    uint32_t* status;
+    uint32_t s, ph, buf, aph;
+    bool ready;
+
+    template <bool A_MN>
+    __device__ __forceinline__ bool unit(int stages, int per) {
+        const uint32_t full_mask = 0xFFFFFFFFu;
+        const uint32_t idesc = umma_idesc(n_pad) | (A_MN ? 1u << 15 : 0u);
+        constexpr uint32_t A_STEP = A_MN ? 2048 >> 4 : 32 >> 4;
+        for (int k0 = 0; k0 < stages; k0 += per) {
+            if (!__all_sync(full_mask, mbar_wait_bounded(hl_free(bars, buf), aph ^ 1u, status, DEV_TIMEOUT_EMPTY))) return false;
+            tc_fence_after();
+            const uint32_t d = tmem + buf * 2u * n_pad;
+            for (int k = k0; k < min(stages, k0 + per); ++k) {
+                if (!ready && !__all_sync(full_mask, mbar_wait_bounded(hl_full(bars, s), ph, status, DEV_TIMEOUT_FULL))) return false;
+                tc_fence_after();
+                const uint32_t next = s + 1 == depth ? 0 : s + 1, next_ph = next ? ph : ph ^ 1u;
+                const bool seen = mbar_test(hl_full(bars, next), next_ph);
+                const uint32_t at = (s0 + s * stage_bytes) >> 4, b = (at + (HF_A_BYTES >> 4)) | 1u << 16;
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t block = 0; block < 2; ++block) {
+                        const uint32_t a = (at + block * (2 * HL_BOX >> 4)) | (A_MN ? (HL_BOX >> 4) << 16 : 1u << 16);
+#pragma unroll
+                        for (int q = 0; q < HL_KS / 16; ++q) umma_low<false>(d + block * n_pad, a + A_STEP * q, b + 2u * q, idesc, (k > k0 || q > 0) ? 1u : 0u);
+                    }
+                    umma_commit<false>(hl_empty(bars, s));
+                }
+                __syncwarp();
+                ready = __all_sync(full_mask, seen);
+                s = next;
+                ph = next_ph;
+            }
+            if (elect_one()) umma_commit<false>(hl_acc(bars, buf));
+            __syncwarp();
+            buf ^= 1u;
+            if (buf == 0) aph ^= 1u;
+        }
+        return true;
+    }
+};
+
 __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_constant__ HfParams P, const __grid_constant__ CUtensorMap amap,
                                                                  const __grid_constant__ CUtensorMap bmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -78,14 +123,10 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
     const uint32_t s0 = (smem_u32(smem) + 1023u) & ~1023u;
     const uint32_t stages = (uint32_t)hf_stages(P.n_pad), stage_bytes = hf_stage_bytes(P.n_pad);
     const uint32_t bars = s0 + stages * stage_bytes;
-    auto bar_full = [&](uint32_t s) { return bars + 8u * s; };
-    auto bar_empty = [&](uint32_t s) { return bars + 64u + 8u * s; };
-    auto bar_acc = [&](uint32_t b) { return bars + 128u + 8u * b; };
-    auto bar_free = [&](uint32_t b) { return bars + 144u + 8u * b; };
     const uint32_t tmem_slot = bars + 160u;
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < stages; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
-        for (uint32_t b = 0; b < 2; ++b) { mbar_init(bar_acc(b), 1); mbar_init(bar_free(b), HF_EPI_WARPS); }
+        for (uint32_t s = 0; s < stages; ++s) { mbar_init(hl_full(bars, s), 1); mbar_init(hl_empty(bars, s), 1); }
+        for (uint32_t b = 0; b < 2; ++b) { mbar_init(hl_acc(bars, b), 1); mbar_init(hl_free(bars, b), HF_EPI_WARPS); }
         mbar_fence_init();
         fence_proxy_async();
     }
@@ -144,7 +185,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
 #pragma unroll
             for (int q = 0; q < HF_TOKENS; ++q) acc[q] = 0.0f;
             for (int k = k0; k < k1; k += logits ? HF_SUM_STAGES : k1 - k0) {
-                if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded(bar_acc(buf), ph, P.status, DEV_TIMEOUT_ACC));
+                if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded(hl_acc(bars, buf), ph, P.status, DEV_TIMEOUT_ACC));
                 tc_fence_after();
 #pragma unroll
                 for (int q = 0; q < HF_TOKENS / 32; ++q) {
@@ -157,7 +198,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0 && healthy) mbar_arrive(bar_free(buf));
+                if (lane == 0 && healthy) mbar_arrive(hl_free(bars, buf));
                 buf ^= 1u;
                 if (buf == 0) ph ^= 1u;
             }
@@ -242,9 +283,9 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
             k_range(u, &k0, &k1);
             const int h0 = logits ? 0 : u % P.h_tiles * HL_TILE, r0 = P.v0 + (logits ? u * P.rows : 0);
             for (int i = k0; i < k1; ++i) {
-                good = __all_sync(full_mask, mbar_wait_bounded(bar_empty(s), ph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
+                good = __all_sync(full_mask, mbar_wait_bounded(hl_empty(bars, s), ph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
                 if (!good) break;
-                const uint32_t dst = s0 + s * stage_bytes, bar = bar_full(s);
+                const uint32_t dst = s0 + s * stage_bytes, bar = hl_full(bars, s);
                 const int k = P.kind == HL_DLOGITS ? k1 - 1 - i : i;   // backwards: the L2 still holds the columns that the loss read last
                 if (elect_one()) {
                     mbar_arrive_expect_tx(bar, bytes);
@@ -263,44 +304,12 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         }
     } else {
         // =========================================================== MMA
+        HfIssue I = {s0, bars, tmem, stage_bytes, stages, (uint32_t)P.n_pad, P.status, 0, 0, 0, 0, false};
         bool good = true;
-        uint32_t s = 0, ph = 0, buf = 0, aph = 0;
-        const uint32_t idesc = umma_idesc((uint32_t)P.n_pad) | (logits ? 0u : 1u << 15);
-        const uint64_t a_step = logits ? 32 >> 4 : 2048 >> 4;
         for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
             int first, last;
             k_range(u, &first, &last);
-            const int per = logits ? HF_SUM_STAGES : last - first;
-            for (int k0 = first; good && k0 < last; k0 += per) {
-                good = __all_sync(full_mask, mbar_wait_bounded(bar_free(buf), aph ^ 1u, P.status, DEV_TIMEOUT_EMPTY));
-                if (!good) break;
-                tc_fence_after();
-                const uint32_t d = tmem + buf * 2u * (uint32_t)P.n_pad;
-                const int k1 = min(last, k0 + per);
-                for (int k = k0; k < k1; ++k) {
-                    good = __all_sync(full_mask, mbar_wait_bounded(bar_full(s), ph, P.status, DEV_TIMEOUT_FULL));
-                    if (!good) break;
-                    tc_fence_after();
-                    const uint32_t at = s0 + s * stage_bytes;
-                    const uint64_t bd = umma_smem_desc(at + HF_A_BYTES);
-                    if (elect_one()) {
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            const uint64_t ad = logits ? umma_smem_desc(at + b * 2 * HL_BOX) : umma_smem_desc_mn(at + b * 2 * HL_BOX, HL_BOX);
-#pragma unroll
-                            for (int q = 0; q < HL_KS / 16; ++q)
-                                umma_bf16<false>(d + (uint32_t)(b * P.n_pad), ad + a_step * q, bd + (uint64_t)(2 * q), idesc, (k > k0 || q > 0) ? 1u : 0u);
-                        }
-                        umma_commit<false>(bar_empty(s));
-                    }
-                    __syncwarp();
-                    if (++s == stages) { s = 0; ph ^= 1u; }
-                }
-                if (good && elect_one()) umma_commit<false>(bar_acc(buf));
-                __syncwarp();
-                buf ^= 1u;
-                if (buf == 0) aph ^= 1u;
-            }
+            good = logits ? I.unit<false>(last - first, HF_SUM_STAGES) : I.unit<true>(last - first, last - first);
         }
     }
     tc_fence_before();

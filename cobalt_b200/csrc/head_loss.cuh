@@ -286,7 +286,7 @@ struct HlIssue {
                 const uint32_t a = at | (A_MN ? (HL_BOX >> 4) << 16 : 1u << 16), b = (at + (2 * HL_BOX >> 4)) | (B_MN ? (HL_BOX >> 4) << 16 : 1u << 16);
                 if (elect_one()) {
 #pragma unroll
-                    for (int q = 0; q < HL_KS / 16; ++q) umma_pair(d, a + A_STEP * q, b + B_STEP * q, idesc, (k > k0 || q > 0) ? 1u : 0u);
+                    for (int q = 0; q < HL_KS / 16; ++q) umma_low<true>(d, a + A_STEP * q, b + B_STEP * q, idesc, (k > k0 || q > 0) ? 1u : 0u);
                     umma_commit<true>(hl_empty(bars, s), 3);
                 }
                 __syncwarp();

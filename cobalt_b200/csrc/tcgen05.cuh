@@ -35,13 +35,20 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint6
             "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
             ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// The same for a pair, with descriptors by their low words: the high word says 8-row groups 1024 bytes apart, 128-byte swizzle, version 1, as
+// The same with descriptors by their low words: the high word says 8-row groups 1024 bytes apart, 128-byte swizzle, version 1, as
 // umma_smem_desc() and umma_smem_desc_mn() do
-__device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint32_t alo, uint32_t blo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(alo), "r"(blo), "r"(idesc), "r"(accumulate), "n"((1024 >> 4) | 1 << 14 | 2 << 29) : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void umma_low(uint32_t tmem_d, uint32_t alo, uint32_t blo, uint32_t idesc, uint32_t accumulate) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(alo), "r"(blo), "r"(idesc), "r"(accumulate), "n"((1024 >> 4) | 1 << 14 | 2 << 29) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(alo), "r"(blo), "r"(idesc), "r"(accumulate), "n"((1024 >> 4) | 1 << 14 | 2 << 29) : "memory");
 }
 // completion of the MMAs issued so far -> the barrier at this offset (pair: in both CTAs, `mask` = their cluster ranks)
 template <bool PAIR>
