@@ -151,9 +151,9 @@ struct EmbedGradParams {
     long long n, ld, n_rows;
     int width, blocks, tiles;              // blocks of ids, tiles of sorted tokens
     float scale;
-    uint32_t* block_ids;                   // [blocks][EG_BLOCK] sorted within each block
+    uint32_t* block_ids;                   // [n] sorted within blocks of EG_BLOCK, or all of them
     uint32_t* block_pos;
-    const uint32_t* ids_sorted;            // [n] (one block: the same memory as block_ids)
+    const uint32_t* ids_sorted;            // [n] (one block, or placed by counting: the same memory as block_ids)
     const uint32_t* pos_sorted;
     float* part;                           // [tiles][2][width]: what a tile has of the run that entered it, of the one that leaves it
     uint32_t* runs;                        // [0]: number of runs that cross tiles, [1..]: the tiles where they begin
