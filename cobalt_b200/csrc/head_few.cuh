@@ -4,13 +4,15 @@
 // In the pair kernel's tile the tokens are the 256 rows of A, most of them zeros that take half of every stage: five stages hold 70 KB of W in
 // flight, and 32000 x 4096 took 68 us for one token (3.9 TB/s).  Here six stages hold up to 192 KB: 46 us (5.7 TB/s; the loss with the kernel that joins
 // its statistics 50.4), of which 39 stream W and the rest is the start, the last unit's epilogue and the launch.  With gradients (16 tokens): logits
-// again 43 us, 40 % of them from the L2, dx 52, dw (head_loss.cuh) 55, 27 tiles a pair of 1 us each behind 9 us of first passes through code.
+// again 43 us, 40 % of them from the L2, dx 52 (one value of d), dw (head_loss.cuh) 55, 27 tiles a pair of 1 us each behind 9 us of first passes through code.
 //
 //   stats, dlogits   A = W, two blocks of up to 128 of its rows; B = x.  A unit of work is `rows` rows, so many that the units go round the CTAs evenly.
 //                    TMEM lane = row of W, column = token: a warp's statistics are reductions over its lanes, 32 tokens at a time.
 //                    Tokens stay where they are (none are packed): what a row without a target holds reaches its own column alone, which is not used.
-//                    dlogits also leaves what dw takes beside d: x with zeros for those rows, and the factor of the sums.
-//   dx               A = W with hidden columns as M (M-major as it lies), K = rows of W; B = d.  A unit is 256 hidden columns and a range of rows.
+//                    dlogits leaves d in rows 0 .. n - 1 of the piece's scratch (a second bf16 value of it in rows n .. 2n - 1), and what dw takes beside
+//                    it: x with zeros for those rows, as often, and the factor of the sums.
+//   dx               A = W with hidden columns as M (M-major as it lies), K = rows of W; B = d, both values of a stage one after the other on the same A.  A
+//                    unit is 256 hidden columns and a range of rows.
 //   warps 0-7  epilogue: warp w owns lanes 32 * (w % 4).. of block w / 4        warp 8  TMA        warp 9  MMA
 #pragma once
 #include "head_loss.cuh"
@@ -24,11 +26,20 @@ constexpr int HF_EPI_WARPS = 8;
 constexpr int HF_SUM_STAGES = 4;
 constexpr int HF_THREADS = HF_EPI_WARPS * 32 + 64;
 constexpr uint32_t HF_A_BYTES = 4 * HL_BOX;
-constexpr int hf_stages(int n_pad) { return n_pad <= 32 ? 6 : n_pad <= 64 ? 5 : 4; }
-constexpr uint32_t hf_stage_bytes(int n_pad) { return HF_A_BYTES + (uint32_t)n_pad * 128u; }
+// Up to 64 tokens d goes out as hi + lo, each rounded to bf16: 2^-16 of d is lost where one value loses 2^-8, as much as the result's own rounding (dw of one
+// token is d times its row of x).  W is read once all the same, and the tensor pipe has the time: gradients of 16 tokens of 32000 x 4096, error in 2-norm 1.9e-3 -> 1.7e-3,
+// with the shorter code of the kernel for 64 tokens 219 -> 212 us.  More tokens than that are bound by reading d for every 256 hidden columns: 128 tokens would
+// take 313 us instead of 273, 100 of 262144 x 5376 2.55 ms instead of 2.07, and have one value.
+constexpr int hf_parts(int n) { return n <= HF_TOKENS / 2 ? 2 : 1; }
+// A stage holds W and `parts` operands of the tokens' side (dx: hi and lo; logits: x)
+constexpr int hf_stages(int n_pad, int parts) { return n_pad * parts <= 32 ? 6 : n_pad * parts <= 64 ? 5 : 4; }
+constexpr uint32_t hf_stage_bytes(int n_pad, int parts) { return HF_A_BYTES + (uint32_t)(n_pad * parts) * 128u; }
 // stages, barriers, what belongs to a token (16 bytes), the warps' statistics of it (8 bytes each), room for the alignment
-constexpr uint32_t hf_smem(int n_pad) { return (uint32_t)hf_stages(n_pad) * hf_stage_bytes(n_pad) + 256 + (uint32_t)n_pad * (16 + 8 * HF_EPI_WARPS) + 1024; }
-static_assert(hf_smem(32) <= 227 * 1024 && hf_smem(64) <= 227 * 1024 && hf_smem(96) <= 227 * 1024 && hf_smem(128) <= 227 * 1024, "stages of every size fit");
+constexpr uint32_t hf_smem(int n_pad, int parts) {
+    return (uint32_t)hf_stages(n_pad, parts) * hf_stage_bytes(n_pad, parts) + 256 + (uint32_t)n_pad * (16 + 8 * HF_EPI_WARPS) + 1024;
+}
+static_assert(hf_smem(32, 1) <= 227 * 1024 && hf_smem(64, 1) <= 227 * 1024 && hf_smem(96, 1) <= 227 * 1024 && hf_smem(128, 1) <= 227 * 1024 &&
+              hf_smem(32, 2) <= 227 * 1024 && hf_smem(64, 2) <= 227 * 1024, "stages of every size fit");
 
 struct HfParams {
     int kind;                              // HL_STATS, HL_DLOGITS or HL_DX
@@ -39,7 +50,7 @@ struct HfParams {
     int hidden;
     const long long* targets;              // stats, dlogits: of every token; one outside the vocabulary does not count
     long long vocab;
-    int* counted;                          // stats: [0] tokens that count, [1] zero, for the kernel that joins; dlogits: [0] all tokens, for dw
+    int* counted;                          // stats: [0] tokens that count, [1] zero, for the kernel that joins; dlogits: [0] rows of d, for dw
     float2* part;                          // stats: [units][n_pad]
     float* at;
     const float2* stats;                   // dlogits: maximum and log2 of the sum
@@ -48,8 +59,8 @@ struct HfParams {
     float* factor;
     const uint16_t* x;
     long long ldx;
-    uint16_t* packed;                      // [n][hidden]
-    uint16_t* d;
+    uint16_t* packed;                      // [values of d][n][hidden]
+    uint16_t* d;                           // [values of d][n][ld_d]
     int ld_d;
     float* slab;                           // [split][n][hidden]
     uint32_t* status;
@@ -77,7 +88,8 @@ struct HfIssue {
     uint32_t s, ph, buf, aph;
     bool ready;
 
-    template <bool A_MN>
+    // PARTS operands B of a stage go onto the same sums
+    template <bool A_MN, int PARTS>
     __device__ __forceinline__ bool unit(int stages, int per) {
         const uint32_t full_mask = 0xFFFFFFFFu;
         const uint32_t idesc = umma_idesc(n_pad) | (A_MN ? 1u << 15 : 0u);
@@ -98,6 +110,10 @@ struct HfIssue {
                         const uint32_t a = (at + block * (2 * HL_BOX >> 4)) | (A_MN ? (HL_BOX >> 4) << 16 : 1u << 16);
 #pragma unroll
                         for (int q = 0; q < HL_KS / 16; ++q) umma_low<false>(d + block * n_pad, a + A_STEP * q, b + 2u * q, idesc, (k > k0 || q > 0) ? 1u : 0u);
+                        if constexpr (PARTS > 1) {
+#pragma unroll
+                            for (int q = 0; q < HL_KS / 16; ++q) umma_low<false>(d + block * n_pad, a + A_STEP * q, b + (n_pad * 128u >> 4) + 2u * q, idesc, 1u);
+                        }
                     }
                     umma_commit<false>(hl_empty(bars, s));
                 }
@@ -115,13 +131,18 @@ struct HfIssue {
     }
 };
 
+// TOKENS: at most.  A CTA passes most of the code once, so its length is time: that for 64 tokens takes 206 us for the gradients of one token, that for 128 216.
+template <int TOKENS>
 __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_constant__ HfParams P, const __grid_constant__ CUtensorMap amap,
                                                                  const __grid_constant__ CUtensorMap bmap) {
+    constexpr int PARTS = hf_parts(TOKENS);
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full_mask = 0xFFFFFFFFu;
     const uint32_t s0 = (smem_u32(smem) + 1023u) & ~1023u;
-    const uint32_t stages = (uint32_t)hf_stages(P.n_pad), stage_bytes = hf_stage_bytes(P.n_pad);
+    const bool logits = P.kind != HL_DX;
+    const int parts = logits ? 1 : PARTS;                  // operands of a stage's tokens' side
+    const uint32_t stages = (uint32_t)hf_stages(P.n_pad, parts), stage_bytes = hf_stage_bytes(P.n_pad, parts);
     const uint32_t bars = s0 + stages * stage_bytes;
     const uint32_t tmem_slot = bars + 160u;
     if (threadIdx.x == 0) {
@@ -137,7 +158,6 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
     const uint32_t tmem = lds32(tmem_slot);
     pdl_next();
     pdl_wait();
-    const bool logits = P.kind != HL_DX;
     const int k_all = ((logits ? P.hidden : P.cols) + HL_KS - 1) / HL_KS;
     auto k_range = [&](int u, int* k0, int* k1) {
         const int split = logits ? 0 : u / P.h_tiles;
@@ -158,7 +178,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
             for (int i = lane; i < P.n; i += 32) counted += counts(P.targets[i]) ? 1 : 0;
             counted = __reduce_add_sync(full_mask, counted);
             if (lane == 0) {
-                P.counted[0] = P.kind == HL_STATS ? counted : P.n;
+                P.counted[0] = P.kind == HL_STATS ? counted : PARTS * P.n;
                 P.counted[1] = 0;
                 if (P.kind == HL_DLOGITS) *P.factor = P.grad_step ? 1.0f : P.mean ? P.grad[0] / (float)max(counted, 1) : P.grad[0];
             }
@@ -171,8 +191,11 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
             }
             for (int i = blockIdx.x; i < P.n; i += gridDim.x) {
                 const bool in = counts(P.targets[i]);
-                for (int c = threadIdx.x; c < P.hidden / 8; c += HF_EPI_WARPS * 32)
-                    reinterpret_cast<uint4*>(P.packed + (long long)i * P.hidden)[c] = in ? reinterpret_cast<const uint4*>(P.x + i * P.ldx)[c] : make_uint4(0, 0, 0, 0);
+                for (int c = threadIdx.x; c < P.hidden / 8; c += HF_EPI_WARPS * 32) {
+                    const uint4 v = in ? reinterpret_cast<const uint4*>(P.x + i * P.ldx)[c] : make_uint4(0, 0, 0, 0);
+                    reinterpret_cast<uint4*>(P.packed + (long long)i * P.hidden)[c] = v;
+                    if (PARTS > 1) reinterpret_cast<uint4*>(P.packed + (long long)(P.n + i) * P.hidden)[c] = v;
+                }
             }
             epilogue_sync();
         }
@@ -181,14 +204,14 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         for (int u = blockIdx.x; u < P.units; u += gridDim.x) {
             int k0, k1;
             k_range(u, &k0, &k1);
-            float acc[HF_TOKENS];
+            float acc[TOKENS];
 #pragma unroll
-            for (int q = 0; q < HF_TOKENS; ++q) acc[q] = 0.0f;
+            for (int q = 0; q < TOKENS; ++q) acc[q] = 0.0f;
             for (int k = k0; k < k1; k += logits ? HF_SUM_STAGES : k1 - k0) {
                 if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded(hl_acc(bars, buf), ph, P.status, DEV_TIMEOUT_ACC));
                 tc_fence_after();
 #pragma unroll
-                for (int q = 0; q < HF_TOKENS / 32; ++q) {
+                for (int q = 0; q < TOKENS / 32; ++q) {
                     if (32 * q >= P.n_pad) continue;
                     uint32_t v[32];
                     tmem_ld32(my_tmem + buf * 2u * (uint32_t)P.n_pad + 32u * q, v);
@@ -206,7 +229,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                 const int half = P.rows / 2, in_piece = u * P.rows + block * half + in_block, row = P.v0 + in_piece;
                 const bool mine = in_block < half && in_piece < P.cols;
 #pragma unroll
-                for (int q = 0; q < HF_TOKENS / 32; ++q) {
+                for (int q = 0; q < TOKENS / 32; ++q) {
                     if (32 * q >= P.n_pad) continue;
                     const int token = 32 * q + lane;
                     if (P.kind == HL_STATS) {
@@ -231,6 +254,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                         }
                     } else {
                         const bool in_d = in_block < half && in_piece < P.ld_d;
+                        const long long lo_rows = (long long)P.n * P.ld_d;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             const int c = 32 * q + e;
@@ -242,7 +266,16 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                                 if (__float_as_int(r.w) == row) g -= 1.0f;
                                 g *= r.z;
                             }
-                            if (in_d) P.d[(long long)c * P.ld_d + in_piece] = float_to_bf16(g);
+                            if (!in_d) continue;
+                            uint16_t* at = P.d + (long long)c * P.ld_d + in_piece;
+                            if (PARTS == 1) {
+                                *at = float_to_bf16(g);
+                            } else {
+                                const float hi = bf16_round(g), rest = g - hi;         // (exact)
+                                const uint32_t both = pack_bf16x2(hi, fabsf(hi) < INFINITY ? rest : 0.0f);
+                                *at = (uint16_t)both;
+                                at[lo_rows] = (uint16_t)(both >> 16);
+                            }
                         }
                     }
                 }
@@ -265,7 +298,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                 float* dst = P.slab + (long long)split * P.n * P.hidden + h;
                 if (h < P.hidden) {
 #pragma unroll
-                    for (int c = 0; c < HF_TOKENS; ++c) {
+                    for (int c = 0; c < TOKENS; ++c) {
                         if (c >= P.n) continue;
                         float* at = dst + (long long)c * P.hidden;
                         *at = P.add ? *at + acc[c] : acc[c];
@@ -277,7 +310,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         // =========================================================== TMA
         bool good = true;
         uint32_t s = 0, ph = 0;
-        const uint32_t bytes = (logits ? (uint32_t)P.rows * 128u : HF_A_BYTES) + (uint32_t)P.n_pad * 128u;
+        const uint32_t bytes = (logits ? (uint32_t)P.rows * 128u : HF_A_BYTES) + (uint32_t)(P.n_pad * parts) * 128u;
         for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
             int k0, k1;
             k_range(u, &k0, &k1);
@@ -297,6 +330,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                         for (int b = 0; b < 4; ++b) tma_load_2d<false>(dst + b * HL_BOX, &amap, h0 + 64 * b, r0 + k * HL_KS, bar);
                     }
                     tma_load_2d<false>(dst + HF_A_BYTES, &bmap, k * HL_KS, 0, bar);
+                    if (PARTS > 1 && !logits) tma_load_2d<false>(dst + HF_A_BYTES + (uint32_t)P.n_pad * 128u, &bmap, k * HL_KS, P.n, bar);
                 }
                 __syncwarp();
                 if (++s == stages) { s = 0; ph ^= 1u; }
@@ -309,7 +343,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
             int first, last;
             k_range(u, &first, &last);
-            good = logits ? I.unit<false>(last - first, HF_SUM_STAGES) : I.unit<true>(last - first, last - first);
+            good = logits ? I.unit<false, 1>(last - first, HF_SUM_STAGES) : I.unit<true, PARTS>(last - first, last - first);
         }
     }
     tc_fence_before();

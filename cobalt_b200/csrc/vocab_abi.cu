@@ -167,7 +167,8 @@ HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool w
     s.count = take(256);
     s.slot = take((size_t)n * 4);
     s.target = take((size_t)n * 4);
-    s.packed = take((size_t)n * hidden * 2);
+    const size_t d_rows = (size_t)n * (backward && s.few ? hf_parts(n) : 1);  // of d, and of x beside it
+    s.packed = take(d_rows * hidden * 2);
     if (!backward) {
         s.stats_tokens = (int)std::min<size_t>(rows, HEAD_STATS_TOKENS);
         s.at = take((size_t)n * 4);
@@ -176,11 +177,11 @@ HeadScratch head_scratch(int n, int hidden, int64_t vocab, bool backward, bool w
     } else {
         s.row = take((size_t)n * 16);
         // pieces of equal size, each within HEAD_PIECE_BYTES of scratch
-        const int64_t most = std::max<int64_t>(HEAD_PIECE_BYTES / 2 / n / HL_TILE * HL_TILE, HL_TILE);
+        const int64_t most = std::max<int64_t>(HEAD_PIECE_BYTES / 2 / d_rows / HL_TILE * HL_TILE, HL_TILE);
         s.pieces = (int)ceil_div(vocab, most);
         s.piece = (int)(ceil_div(ceil_div(vocab, s.pieces), HL_TILE) * HL_TILE);
         s.pieces = (int)ceil_div(vocab, s.piece);
-        for (int b = 0; b < 2; ++b) s.d[b] = b < s.pieces ? take((size_t)n * s.piece * 2) : s.d[0];
+        for (int b = 0; b < 2; ++b) s.d[b] = b < s.pieces ? take(d_rows * s.piece * 2) : s.d[0];
         s.width = s.few ? few_rows(s.piece, sms) : tile_width(rows / HL_TILE, s.piece, sms / 2);
         if (want_x) {
             const int64_t tiles = (int64_t)(rows / HL_TILE) * ceil_div(hidden, HL_TILE);
@@ -219,18 +220,23 @@ int launch_next(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, 
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? COBALT_OK : COBALT_ELAUNCH;
 }
-int few(const HfParams& P, const CUtensorMap& a, const CUtensorMap& b, int sms, bool first, cudaStream_t st) {
+template <int TOKENS>
+int few_sized(const HfParams& P, const CUtensorMap& a, const CUtensorMap& b, int sms, bool first, cudaStream_t st) {
     static bool configured[MAX_DEVICES];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return COBALT_ELAUNCH;
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return COBALT_ELAUNCH;
+        if (cudaFuncSetAttribute(head_few_kernel<TOKENS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return COBALT_ELAUNCH;
         configured[dev] = true;
     }
     const dim3 grid((unsigned)std::min(P.units, sms));
-    if (!first) return launch_next(head_few_kernel, grid, HF_THREADS, hf_smem(P.n_pad), 1, st, P, a, b);
-    head_few_kernel<<<grid, HF_THREADS, hf_smem(P.n_pad), st>>>(P, a, b);
+    const uint32_t smem = hf_smem(P.n_pad, P.kind == HL_DX ? hf_parts(TOKENS) : 1);
+    if (!first) return launch_next(head_few_kernel<TOKENS>, grid, HF_THREADS, smem, 1, st, P, a, b);
+    head_few_kernel<TOKENS><<<grid, HF_THREADS, smem, st>>>(P, a, b);
     return launched();
+}
+int few(const HfParams& P, const CUtensorMap& a, const CUtensorMap& b, int sms, bool first, cudaStream_t st) {
+    return P.n <= HF_TOKENS / 2 ? few_sized<HF_TOKENS / 2>(P, a, b, sms, first, st) : few_sized<HF_TOKENS>(P, a, b, sms, first, st);
 }
 int product(const HlParams& P, const HlMaps& M, int64_t tiles, int sms, cudaStream_t st) {
     static bool configured[MAX_DEVICES];
@@ -485,12 +491,13 @@ int cobalt_head_loss_grad(const void* x, int64_t ldx, const void* weight, int64_
     HlMaps M = {};
     // what a kernel reads by rows it takes in boxes of 128 (few tokens: all of them), x where it lies if they are few
     const int box = s.few ? n_pad : 128;
+    const int64_t d_rows = (int64_t)n * (s.few ? hf_parts(n) : 1);
     if ((rc = bf16_map(&M.w_rows, weight, ldw, vocab, hidden, s.width / 2)) ||
         (rc = s.few ? bf16_map(&M.x_rows, x, ldx, n, hidden, box) : bf16_map(&M.x_rows, A.packed, hidden, n, hidden, box)) ||
-        (dw && (rc = bf16_map(&M.x, A.packed, hidden, n, hidden))) || (dx && (rc = bf16_map(&M.w, weight, ldw, vocab, hidden)))) return rc;
+        (dw && (rc = bf16_map(&M.x, A.packed, hidden, d_rows, hidden))) || (dx && (rc = bf16_map(&M.w, weight, ldw, vocab, hidden)))) return rc;
     for (int b = 0; b <= two; ++b) {
-        if (dw && (rc = bf16_map(&M.d[b], base + s.d[b], s.piece, n, s.piece))) return rc;
-        if (dx && (rc = bf16_map(&M.d_rows[b], base + s.d[b], s.piece, n, s.piece, box))) return rc;
+        if (dw && (rc = bf16_map(&M.d[b], base + s.d[b], s.piece, d_rows, s.piece))) return rc;
+        if (dx && (rc = bf16_map(&M.d_rows[b], base + s.d[b], s.piece, d_rows, s.piece, box))) return rc;
     }
     if (dx && !s.few && (rc = make_map(&M.slab, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base + s.slab, hidden, n, hidden, 32, s.splits))) return rc;
     if (dw && (rc = bf16_map(&M.dw, dw, ld_dw, vocab, hidden, 32))) return rc;

@@ -403,7 +403,7 @@ int cobalt_kv4_status(void* stream, uint32_t* status_out);
  *                           sum of the losses or, with mean, their mean over the tokens that count (0 if none does).
  *   cobalt_head_loss_grad : gradients for the same x, weight and targets.  grad fp32: of every token's loss (grad_step 1), or one value (grad_step 0)
  *                           of the sum or, with mean, of the mean.  dx [n][hidden] and dw [vocab][hidden] bf16 (rows 16-byte aligned; either may be
- *                           NULL), every value written.  The gradient of the logits is rounded to bf16 on the way, sums are fp32.
+ *                           NULL), every value written.  The gradient of the logits is rounded to bf16 on the way (up to 64 tokens: to two bf16 values, 2^-16 of it), sums are fp32.
  *                           status of both (may be NULL: the device's word): device memory, 4-byte aligned, zeroed by the caller; a bounded wait of
  *                           the call that gives up leaves its code there while it is 0, and NaN in what it concerns.
  *   cobalt_vocab_status   : 0, or the code of the first bounded wait that gave up since the last question, of the head calls on the current device

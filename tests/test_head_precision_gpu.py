@@ -1,0 +1,41 @@
+"""Head loss: how many bits its gradients keep (needs a B200).  The bounds are those of the formulas in 64 bits; a rounding to bf16 is off by half a step at
+most, 2^-8 of the value."""
+import pytest
+import torch
+
+import cobalt_b200 as cb
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+@pytest.mark.parametrize("n,V,H", [(1, 1000, 8), (1, 4099, 64), (2, 700, 16), (5, 3001, 8), (32, 2000, 8), (33, 513, 16), (63, 260, 8), (64, 300, 8)])
+def test_gradients_of_few_tokens_round_their_results_alone(n, V, H):
+    """Up to 64 tokens the gradient of the logits goes into both products as two bf16 values: 2^-8 of it, and 2^-8 of the rest, so 2^-16.  A logit is off by
+    (2^-15.9 + 2^-24) of the sum of its magnitudes S (the tensor core's cuts, see test_head_loss_gpu.py), a loss or a normaliser by twice that and a few
+    fp32 roundings, a probability by both of them.  The products cut 17 / 16 * 2^-25 of the magnitudes for each of their columns, twice as many as there
+    are tokens or rows; what is left is the result's own rounding.  (Rounded once, d alone would be off by as much as the result.)"""
+    g = gen(n + V + H)
+    x = torch.randn(n, H, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(V, H, generator=g, device="cuda") * H ** -0.5).bfloat16()
+    t = torch.randint(0, V, (n,), generator=g, device="cuda")
+    f = torch.rand(n, generator=g, device="cuda") + 0.5
+    xd, wd = x.double(), w.double()
+    l = xd @ wd.T
+    lse = torch.logsumexp(l, 1, keepdim=True)
+    off = (2.0 ** -15.9 + 2.0 ** -24) * (xd.abs() @ wd.abs().T).amax(1, keepdim=True)
+    tol = 2 * off + 2.0 ** -21 + 2.0 ** -22 * (l.abs().amax(1, keepdim=True) * 2 + lse.abs() + 1)
+    p = torch.exp(l - lse)
+    d = p.clone()
+    d[torch.arange(n), t] -= 1.0
+    size = d.abs() * f.double()[:, None]
+    err = (d.abs() * 2.0 ** -16 * 1.01 + p * (2 * tol + 2.0 ** -20) + 2.0 ** -22) * f.double()[:, None]
+    d = d * f.double()[:, None]
+    cut = 17 / 16 * 2.0 ** -25
+    _, dx, dw = cb.head_loss_and_grad(x, w, t, "none", f)
+    for got, want, slack in ((dx, d @ wd, err @ wd.abs() + 2 * V * cut * (size @ wd.abs())), (dw, d.T @ xd, err.T @ xd.abs() + 2 * n * cut * (size.T @ xd.abs()))):
+        worst = ((got.double() - want).abs() - 1.01 * slack - want.abs() * 2.0 ** -8 - 1e-38).max()
+        assert float(worst) <= 0, float(worst)
