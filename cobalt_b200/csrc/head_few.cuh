@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
             float acc[TOKENS];
 #pragma unroll
             for (int q = 0; q < TOKENS; ++q) acc[q] = 0.0f;
-            for (int k = k0; k < k1; k += logits ? HF_SUM_STAGES : k1 - k0) {
+            for (int k = k0; k < k1; k += logits ? HF_SUM_STAGES : HL_GRAD_STAGES) {
                 if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded(hl_acc(bars, buf), ph, P.status, DEV_TIMEOUT_ACC));
                 tc_fence_after();
 #pragma unroll
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
             int first, last;
             k_range(u, &first, &last);
-            good = logits ? I.unit<false, 1>(last - first, HF_SUM_STAGES) : I.unit<true, PARTS>(last - first, last - first);
+            good = logits ? I.unit<false, 1>(last - first, HF_SUM_STAGES) : I.unit<true, PARTS>(last - first, HL_GRAD_STAGES);
         }
     }
     tc_fence_before();

@@ -25,7 +25,8 @@
 // them are not visited.
 //
 // Precision.  The tensor core cuts every product at its running sum's last bits, always towards zero: over 5376 columns that is 1e-5 of a
-// logit, all in one direction.  So logits are summed in tensor memory over 512 columns at a time, and these sums in fp32 registers.  d is rounded
+// logit, all in one direction.  So logits are summed in tensor memory over 512 columns at a time, and these sums in fp32 registers; gradients, which are
+// rounded to bf16 in the end, over 4096 tokens or rows of the vocabulary (all at once, dx of 2^19 equal weights is off by 1.2e-3 of its terms, as much as by the rounding).  d is rounded
 // to bf16 (2^-8 of an element at most, at random), because the tensor core multiplies two operands of one type: gradients are off by 1.8e-3 to 1.9e-3 in 2-norm, 1.7e-3
 // of it their own last rounding.  As hi + lo it would be 12 n V H operations instead of 8 here, where the tensor pipe is the bound; up to 64 tokens, where it
 // is not, have both (head_few.cuh).  A factor g that all tokens share
@@ -48,6 +49,7 @@ constexpr int HL_THREADS = HL_EPI_WARPS * 32 + 128;
 constexpr int HL_REGS = 168, HL_EPI_REGS = 216, HL_ROLE_REGS = 72;     // of a thread: at the launch, epilogue, the others
 static_assert(HL_EPI_REGS * HL_EPI_WARPS * 32 + HL_ROLE_REGS * 128 <= HL_REGS * HL_THREADS, "no more than the block was launched with");
 constexpr int HL_SUM_STAGES = 8;           // stages of logits that are summed in tensor memory
+constexpr int HL_GRAD_STAGES = 64;         // ... of gradients, whose results are rounded to bf16
 constexpr uint32_t HL_OUT_BYTES = 32 * 128;                // results of a warp on their way out: 32 rows of 128 swizzled bytes, twice
 constexpr uint32_t HL_SMEM = HL_STAGES * HL_STAGE_BYTES + HL_EPI_WARPS * 2 * HL_OUT_BYTES + 256 + 1024;
 static_assert(HL_LOGIT_STAGES * HL_STAGE_BYTES <= HL_STAGES * HL_STAGE_BYTES + HL_EPI_WARPS * 2 * HL_OUT_BYTES && HL_LOGIT_STAGES <= 8, "room and barriers");
@@ -444,8 +446,9 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
                         store32(dst + q, w);
                     }
                 }
-            } else {
+            } else {                                       // (a copy of its own: shared with the logits it spills, dw of 16 tokens 55 -> 68 us)
                 take_columns();
+                for (int k = t.k0 + HL_GRAD_STAGES; k < t.k1; k += HL_GRAD_STAGES) add_columns();
                 spoil();
                 if (col >= P.hidden) continue;
                 // out by the copy engine, over shared memory: 64 columns of dw at a time; 32 of dx, which it adds up: one addition a piece, in their order
@@ -515,8 +518,8 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
         while (good && list.take(P, &t)) {
             const int kind = list.J.kind, stages = t.k1 - t.k0;
             const uint32_t width = (uint32_t)list.J.width;
-            good = kind <= HL_DLOGITS ? I.tile<false, false>(stages, HL_SUM_STAGES, width) : kind == HL_DX ? I.tile<false, true>(stages, stages, width)
-                                                                                                         : I.tile<true, true>(stages, stages, width);
+            good = kind <= HL_DLOGITS ? I.tile<false, false>(stages, HL_SUM_STAGES, width) : kind == HL_DX ? I.tile<false, true>(stages, HL_GRAD_STAGES, width)
+                                                                                                         : I.tile<true, true>(stages, HL_GRAD_STAGES, width);
         }
     }
     }

@@ -39,3 +39,41 @@ def test_gradients_of_few_tokens_round_their_results_alone(n, V, H):
     for got, want, slack in ((dx, d @ wd, err @ wd.abs() + 2 * V * cut * (size @ wd.abs())), (dw, d.T @ xd, err.T @ xd.abs() + 2 * n * cut * (size.T @ xd.abs()))):
         worst = ((got.double() - want).abs() - 1.01 * slack - want.abs() * 2.0 ** -8 - 1e-38).max()
         assert float(worst) <= 0, float(worst)
+
+
+def long_sum(size, columns):
+    """Bound of a sum of ``columns`` products of magnitudes ``size`` in all, cut in the tensor core over 4096 columns at a time (17 / 16 * 2^-25 of
+    the magnitudes for each column) and added up in fp32"""
+    return size * (4096 * 17 / 16 * 2.0 ** -25 + columns / 4096 * 2.0 ** -24)
+
+
+def test_the_heads_gradient_over_very_many_tokens():
+    """2^19 tokens, the first half pulling one way and the second the other: what is left is small against what was added up.  The rows of the head are zero, so
+    probabilities are 1/2 and d = +-1/2, without an error."""
+    n, H = 1 << 19, 64
+    x = torch.randn(n, H, generator=gen(1), device="cuda").abs().bfloat16()
+    w = torch.zeros(2, H, dtype=torch.bfloat16, device="cuda")
+    t = (torch.arange(n, device="cuda") >= n // 2).long()
+    _, _, dw = cb.head_loss_and_grad(x, w, t, "sum", need_x=False)
+    half = 0.5 * x.double()
+    want = half[n // 2:].sum(0) - half[:n // 2].sum(0)
+    want = torch.stack([want, -want])
+    worst = ((dw.double() - want).abs() - long_sum(half.sum(0), n) - want.abs() * 2.0 ** -8).max()
+    assert float(worst) <= 0, float(worst)
+
+
+@pytest.mark.parametrize("n,V,H", [(3, 1 << 18, 19200), (256, 1 << 19, 10240)])
+def test_the_hidden_gradient_over_a_large_vocabulary(n, V, H):
+    """x = 0: every probability is 1 / V, a power of two, so dx is the mean of the rows less the target's, which is made to be that mean as far as bf16 has it.  The rounding
+    of 1 / V - 1 costs at most 1 / V."""
+    x = torch.zeros(n, H, dtype=torch.bfloat16, device="cuda")
+    w = torch.randn(V, H, generator=gen(2), device="cuda", dtype=torch.bfloat16).abs_()
+    mean = sum(w[i:i + 4096].double().sum(0) for i in range(0, V, 4096)) / V
+    w[V - 1] = mean.bfloat16()
+    mean = sum(w[i:i + 4096].double().sum(0) for i in range(0, V, 4096)) / V
+    t = torch.full((n,), V - 1, device="cuda")
+    _, dx, _ = cb.head_loss_and_grad(x, w, t, "sum")
+    want = mean - w[V - 1].double()
+    slack = long_sum(mean + w[V - 1].double(), V) + w[V - 1].double() / V + want.abs() * 2.0 ** -8
+    worst = ((dx.double() - want).abs() - slack).max()
+    assert float(worst) <= 0, float(worst)
