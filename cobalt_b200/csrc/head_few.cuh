@@ -85,7 +85,7 @@ __device__ __forceinline__ float reduce_columns(float (&v)[32], int lane, F f) {
 struct HfIssue {
     uint32_t s0, bars, tmem, stage_bytes, depth, n_pad;
     uint32_t* status;
-    uint32_t s, ph, buf, aph;
+    uint32_t s, ph, buf, aph, uses;
     bool ready;
 
     // PARTS operands B of a stage go onto the same sums
@@ -118,6 +118,7 @@ struct HfIssue {
                     umma_commit<false>(hl_empty(bars, s));
                 }
                 __syncwarp();
+                ++uses;
                 ready = __all_sync(full_mask, seen);
                 s = next;
                 ph = next_ph;
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
     } else if (warp == HF_EPI_WARPS) {
         // =========================================================== TMA
         bool good = true;
-        uint32_t s = 0, ph = 0;
+        uint32_t s = 0, ph = 0, fills = 0;
         const uint32_t bytes = (logits ? (uint32_t)P.rows * 128u : HF_A_BYTES) + (uint32_t)(P.n_pad * parts) * 128u;
         for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
             int k0, k1;
@@ -333,18 +334,21 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
                     if (PARTS > 1 && !logits) tma_load_2d<false>(dst + HF_A_BYTES + (uint32_t)P.n_pad * 128u, &bmap, k * HL_KS, P.n, bar);
                 }
                 __syncwarp();
+                ++fills;
                 if (++s == stages) { s = 0; ph ^= 1u; }
             }
         }
+        hl_landed<false>(bars, fills, stages, P.status);
     } else {
         // =========================================================== MMA
-        HfIssue I = {s0, bars, tmem, stage_bytes, stages, (uint32_t)P.n_pad, P.status, 0, 0, 0, 0, false};
+        HfIssue I = {s0, bars, tmem, stage_bytes, stages, (uint32_t)P.n_pad, P.status, 0, 0, 0, 0, 0, false};
         bool good = true;
         for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
             int first, last;
             k_range(u, &first, &last);
             good = logits ? I.unit<false, 1>(last - first, HF_SUM_STAGES) : I.unit<true, PARTS>(last - first, HL_GRAD_STAGES);
         }
+        hl_multiplied<false>(bars, I.uses, stages, P.status);
     }
     tc_fence_before();
     __syncthreads();

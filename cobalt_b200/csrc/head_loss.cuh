@@ -229,11 +229,24 @@ __device__ __forceinline__ uint32_t hl_empty(uint32_t bars, uint32_t s) { return
 __device__ __forceinline__ uint32_t hl_acc(uint32_t bars, uint32_t b) { return bars + 128u + 8u * b; }
 __device__ __forceinline__ uint32_t hl_free(uint32_t bars, uint32_t b) { return bars + 144u + 8u * b; }
 
+// Nothing may be on its way when a CTA ends, also where a wait gave up: a copy would land in the shared memory of the block that comes next, a product in its tensor
+// memory.  `fills` stages were filled, one after another; each of the last `depth` has its barrier's latest phase.
+template <bool CLUSTER>
+__device__ __forceinline__ void hl_landed(uint32_t bars, uint32_t fills, uint32_t depth, uint32_t* status) {
+    for (uint32_t i = fills > depth ? fills - depth : 0; i < fills; ++i) mbar_wait_bounded<CLUSTER>(hl_full(bars, i % depth), i / depth & 1u, status, DEV_TIMEOUT_FULL);
+}
+// A commit follows all products before it, so the one behind the last stage that was used, the `uses`th, is enough
+template <bool CLUSTER>
+__device__ __forceinline__ void hl_multiplied(uint32_t bars, uint32_t uses, uint32_t depth, uint32_t* status) {
+    if (uses) mbar_wait_bounded<CLUSTER>(hl_empty(bars, (uses - 1) % depth), (uses - 1) / depth & 1u, status, DEV_TIMEOUT_ACC);
+}
+
 // The warp that loads the operands, both CTAs each its half; the bytes of both are counted on the first one's barrier
 struct HlLoad {
     uint32_t s0, bars, first_full, rank, depth;            // depth: how many stages there are
     uint32_t* status;
     uint32_t s, ph;                                        // stage that comes next, and its phase
+    uint32_t fills;                                        // how many were filled
     bool ready;                                            // the stage was seen empty
 
     template <bool A_MN, bool B_MN>
@@ -255,6 +268,7 @@ struct HlLoad {
             ready = __all_sync(full_mask, seen);
             (A_MN ? ay : ax) += HL_KS;
             (B_MN ? by : bx) += HL_KS;
+            ++fills;
             s = next;
             ph = next_ph;
         }
@@ -269,6 +283,7 @@ struct HlIssue {
     uint32_t s0, bars, tmem, depth;
     uint32_t* status;
     uint32_t s, ph, buf, aph;                              // stage and accumulator that come next, and their phases
+    uint32_t uses;                                         // how many stages were used
     bool ready;                                            // the stage was seen full
 
     template <bool A_MN, bool B_MN>
@@ -294,6 +309,7 @@ struct HlIssue {
                     umma_commit<true>(hl_empty(bars, s), 3);
                 }
                 __syncwarp();
+                ++uses;
                 ready = __all_sync(full_mask, seen);
                 s = next;
                 ph = next_ph;
@@ -500,7 +516,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(HL_ROLE_REGS));
     if (warp == HL_EPI_WARPS) {
         // =========================================================== TMA
-        HlLoad L = {s0, bars, map_to_rank(hl_full(bars, 0), 0), rank, (uint32_t)P.stages, P.status, 0, 0, false};
+        HlLoad L = {s0, bars, map_to_rank(hl_full(bars, 0), 0), rank, (uint32_t)P.stages, P.status, 0, 0, 0, false};
         bool good = true;
         const int mine = (int)rank * 128;
         while (good && list.take(P, &t)) {
@@ -511,9 +527,11 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
             else if (J.kind == HL_DX) good = L.tile<false, true>(&M.d_rows[J.buf], k0, m0, &M.w, n0, J.v0 + k0, stages, bytes);
             else good = L.tile<true, true>(&M.d[J.buf], m0, k0, &M.x, n0, k0, stages, bytes);
         }
+        // (the first CTA's barriers count the copies of both, and neither ends before the other)
+        if (rank == 0) hl_landed<true>(bars, L.fills, L.depth, P.status);
     } else if (warp == HL_EPI_WARPS + 1 && rank == 0) {
         // =========================================================== MMA
-        HlIssue I = {s0, bars, tmem, (uint32_t)P.stages, P.status, 0, 0, 0, 0, false};
+        HlIssue I = {s0, bars, tmem, (uint32_t)P.stages, P.status, 0, 0, 0, 0, 0, false};
         bool good = true;
         while (good && list.take(P, &t)) {
             const int kind = list.J.kind, stages = t.k1 - t.k0;
@@ -521,6 +539,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1) head_product_kernel(const __gri
             good = kind <= HL_DLOGITS ? I.tile<false, false>(stages, HL_SUM_STAGES, width) : kind == HL_DX ? I.tile<false, true>(stages, HL_GRAD_STAGES, width)
                                                                                                          : I.tile<true, true>(stages, HL_GRAD_STAGES, width);
         }
+        hl_multiplied<true>(bars, I.uses, I.depth, P.status);
     }
     }
     tc_fence_before();
