@@ -99,10 +99,12 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
 def _embed(ids, table, scale, out=None):
     n_rows, width = table.shape
     rows, apart = _matrix("table", table, width)
-    if out is None:
+    n, given = ids.numel(), out is not None
+    if not given:
         out = table.new_empty((*ids.shape, width))
-    n = ids.numel()
     if n:
+        if given:
+            torch.autograd.graph.increment_version(out)      # who saved what it held is told, as by an operation of torch
         _call(table.get_device(), "cobalt_embed", ids.data_ptr(), n, rows.data_ptr(), apart, _TYPES[table.dtype], n_rows, width, scale, out.data_ptr(), width)
     return out
 
