@@ -72,11 +72,19 @@ def _matrix(name: str, t: torch.Tensor, width: int, unit: int = 1):
     return rows, apart if n > 1 else width
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the bytes from the first value of ``a`` to its last meet those of ``b``."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 # ----------------------------------------------------------------------------- embedding
 def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``table[ids] * scale``: rows of ``table [n_rows, width]`` (bf16, fp16 or fp32) for int64 ``ids`` of any shape, ``[*ids.shape, width]``.  The
-    product is formed in fp32 and rounded once.  An id outside the table (-1: padding) reads zeros.  ``out`` (contiguous) receives the
-    result.  Differentiable in ``table`` (``embed_grad``)."""
+    product is formed in fp32 and rounded once.  An id outside the table (-1: padding) reads zeros.  ``out`` (contiguous, apart from ``ids`` and
+    ``table``) receives the result.  Differentiable in ``table`` (``embed_grad``)."""
     index = _gpu("table", table)
     shape, kind = table.shape, _TYPES.get(table.dtype)
     if kind is None:
@@ -90,6 +98,8 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
             raise ValueError(f"out must be a contiguous {table.dtype} {[*ids.shape, shape[1]]} on {table.device}")
         if grad or (out.requires_grad and torch.is_grad_enabled()):
             raise RuntimeError("out cannot take a result that requires a gradient")
+        if _overlap(out, table) or _overlap(out, ids):
+            raise ValueError("out must not overlap table or ids")
     if grad:
         leaves, elsewhere = _leaves(table)
         return _seen(_Embed.apply(ids, table, float(scale), elsewhere), leaves)

@@ -392,7 +392,7 @@ int cobalt_kv4_status(void* stream, uint32_t* status_out);
 /* The two dense ends of a vocabulary: embedding lookup and softmax cross entropy against a head, with their gradients.
  * Embedding calls: tables, rows and gradients of one type (COBALT_BF16, COBALT_FP16, COBALT_FP32), row strides ld in elements; any width
  * up to 2^28, any alignment of a value (16-byte rows are faster).  An id outside [0, n_rows) (-1: padding) reads zeros and has no gradient.
- *   cobalt_embed      : out[t] = table[ids[t]] * scale, the product in fp32, rounded once (scale 1: the bits of the table).
+ *   cobalt_embed      : out[t] = table[ids[t]] * scale, the product in fp32, rounded once (scale 1: the bits of the table).  out overlaps neither ids nor table.
  *   cobalt_embed_grad : out [n_rows][width] (contiguous, 16-byte aligned, every value written) = scale * sum of the rows grad[t] with ids[t] = row, in fp32,
  *                       rounded once.  The same inputs give the same bits.  n <= 2^24.
  * Head calls: x [n][hidden] and weight [vocab][hidden] bf16 (hidden a multiple of 8, rows 16-byte aligned), l[t, v] = x[t] . weight[v] in fp32,
@@ -403,7 +403,8 @@ int cobalt_kv4_status(void* stream, uint32_t* status_out);
  *                           sum of the losses or, with mean, their mean over the tokens that count (0 if none does).
  *   cobalt_head_loss_grad : gradients for the same x, weight and targets.  grad fp32: of every token's loss (grad_step 1), or one value (grad_step 0)
  *                           of the sum or, with mean, of the mean.  dx [n][hidden] and dw [vocab][hidden] bf16 (rows 16-byte aligned; either may be
- *                           NULL), every value written.  The gradient of the logits is rounded to bf16 on the way (up to 64 tokens: to two bf16 values, 2^-16 of it), sums are fp32.
+ *                           NULL), every value written, apart from what is read.  The gradient of the logits is rounded to bf16 on the way (up to 64
+ *                           tokens: to two bf16 values, 2^-16 of it), sums are fp32.
  *                           status of both (may be NULL: the device's word): device memory, 4-byte aligned, zeroed by the caller; a bounded wait of
  *                           the call that gives up leaves its code there while it is 0, and NaN in what it concerns.
  *   cobalt_vocab_status   : 0, or the code of the first bounded wait that gave up since the last question, of the head calls on the current device

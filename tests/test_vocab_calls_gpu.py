@@ -23,3 +23,25 @@ def test_a_result_written_in_place_moves_its_version():
     with torch.inference_mode():
         out = torch.empty(3, 16, device="cuda")
         assert torch.equal(cb.embed(ids, table, out=out), table[ids])
+
+
+def test_a_result_must_not_lie_in_what_is_read():
+    """Blocks would read rows that others have overwritten: refused before a launch."""
+    table = torch.randn(40, 16, device="cuda")
+    kept = table.clone()
+    ids = torch.arange(10, device="cuda")
+    for out in (table[:10], table[30:], table[5:15]):
+        with pytest.raises(ValueError, match="overlap"):
+            cb.embed(ids, table, out=out)
+    with pytest.raises(ValueError, match="overlap"):                   # rows of the table on either side of it
+        cb.embed(ids[:1], table[::2, :8], out=table[1, :8].view(1, 8))
+    flat = torch.zeros(90, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        cb.embed(flat[70:80], table, out=flat[:80].view(torch.float32).view(10, 16))
+    torch.cuda.synchronize()
+    assert torch.equal(table, kept) and not bool(flat.any())
+    both = torch.empty(50, 16, device="cuda")                          # behind one another is as good as apart
+    both[:40] = kept
+    assert torch.equal(cb.embed(ids, both[:40], out=both[40:]), kept[:10]) and torch.equal(both[:40], kept)
+    got = cb.embed(flat[80:], table, out=flat[:80].view(torch.float32).view(10, 16))
+    assert torch.equal(got, kept[:1].expand(10, 16))
