@@ -13,6 +13,7 @@ import weakref
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -46,6 +47,12 @@ def _gpu(name: str, t: torch.Tensor) -> int:
     if index < 0 or not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor; there is no CPU path")
     return index
+
+
+def _no_tangent(*tensors: torch.Tensor):
+    for t in tensors:
+        if fwAD.unpack_dual(t).tangent is not None:
+            raise RuntimeError("there are no forward-mode derivatives: a tensor that carries a tangent is not taken")
 
 
 def _tokens(name: str, t: torch.Tensor, index: int) -> torch.Tensor:
@@ -92,8 +99,10 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
     if len(shape) != 2 or 0 in shape or shape[1] > _WIDEST:
         raise ValueError(f"table must be [n_rows, width] with width at most {_WIDEST}, got {list(shape)}")
     ids = _tokens("ids", ids, index)
+    _no_tangent(table)
     grad = torch.is_grad_enabled() and table.requires_grad
     if out is not None:
+        _no_tangent(out)
         if out.shape != (*ids.shape, shape[1]) or out.dtype is not table.dtype or out.get_device() != index or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {table.dtype} {[*ids.shape, shape[1]]} on {table.device}")
         if grad or (out.requires_grad and torch.is_grad_enabled()):
@@ -155,7 +164,8 @@ def _seen(result: torch.Tensor, leaves) -> torch.Tensor:
 
 def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``embed`` with respect to its table, dense ``[n_rows, width]`` of ``grad``'s type: ``scale`` times the sum of the rows of
-    ``grad [*ids.shape, width]`` by token, in fp32 and in the tokens' order.  Tokens outside the table are left out."""
+    ``grad [*ids.shape, width]`` by token, in fp32 and in the tokens' order.  Tokens outside the table are left out.  No second
+    derivatives: a ``grad`` that requires one is refused."""
     index, kind = _gpu("grad", grad), _TYPES.get(grad.dtype)
     if kind is None:
         raise TypeError(f"grad must be bfloat16, float16 or float32, got {grad.dtype}")
@@ -164,6 +174,9 @@ def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float 
     if not shape or shape[:-1] != ids.shape or not 1 <= shape[-1] <= _WIDEST or n_rows < 1:
         raise ValueError(f"grad must be [*ids.shape, width] = {[*ids.shape, 'width']}, width at most {_WIDEST}, and n_rows at least 1, got {list(shape)} "
                          f"and {n_rows}")
+    _no_tangent(grad)
+    if grad.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("there are no second derivatives: grad must not require a gradient")
     width, n = shape[-1], ids.numel()
     if n == 0:
         return grad.new_zeros((n_rows, width))
@@ -213,6 +226,7 @@ def head_loss_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
         grad = x.new_ones((), dtype=torch.float32).expand(shape)
     elif grad.dtype is not torch.float32 or grad.shape != shape or grad.device != x.device:
         raise ValueError(f"grad must be float32 {list(shape)} on {x.device}, got {grad.dtype} {list(grad.shape)} on {grad.device}")
+    _no_tangent(grad)
     with torch.no_grad():
         loss, stats = _head_loss(x, weight, targets, reduction, status, True)
         dx, dw = _head_loss_grad(x, weight, targets, stats, grad, reduction, status, need_x, need_weight) if need_x or need_weight else (None, None)
@@ -238,6 +252,7 @@ def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, re
     targets = _tokens("targets", targets, index)
     if targets.shape != shape[:-1]:
         raise ValueError(f"targets must be {list(shape[:-1])}, got {list(targets.shape)}")
+    _no_tangent(x, weight)
     if status is not None and (status.dtype is not torch.int32 or status.shape != (1,) or status.get_device() != index):
         raise ValueError(f"status must be int32 [1] on {x.device}, got {status.dtype} {list(status.shape)} on {status.device}")
     return targets

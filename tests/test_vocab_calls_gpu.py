@@ -45,3 +45,25 @@ def test_a_result_must_not_lie_in_what_is_read():
     assert torch.equal(cb.embed(ids, both[:40], out=both[40:]), kept[:10]) and torch.equal(both[:40], kept)
     got = cb.embed(flat[80:], table, out=flat[:80].view(torch.float32).view(10, 16))
     assert torch.equal(got, kept[:1].expand(10, 16))
+
+
+def test_derivatives_that_there_are_none_of_are_refused():
+    """A tangent would be lost without a word, which reads as a derivative of zero; so would the second derivative of the embedding."""
+    import torch.autograd.forward_ad as fwAD
+    table, ids = torch.randn(9, 16, device="cuda"), torch.tensor([1, 8, 3], device="cuda")
+    x, w = torch.randn(3, 16, device="cuda").bfloat16(), torch.randn(9, 16, device="cuda").bfloat16()
+    with fwAD.dual_level():
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: cb.embed(ids, dual(table)), lambda: cb.embed(ids, dual(table.clone().requires_grad_())), lambda: cb.embed_grad(dual(table[:3]), ids, 9),
+                     lambda: cb.head_loss(dual(x), w, ids), lambda: cb.head_loss(x, dual(w), ids), lambda: cb.head_loss_and_grad(x, dual(w), ids),
+                     lambda: cb.head_loss_and_grad(x, w, ids, grad=dual(torch.ones((), device="cuda")))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            cb.embed(ids, table, out=dual(table[:3].clone()))
+        assert torch.equal(cb.embed(ids, table), table[ids])
+    grad = table[:3].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="second"):
+        cb.embed_grad(grad, ids, 9)
+    with torch.no_grad():
+        assert torch.equal(cb.embed_grad(grad, ids, 9)[ids], grad)
