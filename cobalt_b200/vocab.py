@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import weakref
 from typing import Optional
 
 import torch
@@ -110,8 +109,7 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
         if _overlap(out, table) or _overlap(out, ids):
             raise ValueError("out must not overlap table or ids")
     if grad:
-        leaves, elsewhere = _leaves(table)
-        return _seen(_Embed.apply(ids, table, float(scale), elsewhere), leaves)
+        return _seen(_Embed.apply(ids, table, float(scale)))
     return _embed(ids, table, float(scale), out)
 
 
@@ -128,38 +126,35 @@ def _embed(ids, table, scale, out=None):
     return out
 
 
-_graphs = {}                                                 # by id of a leaf: (it, weakly; the stream of the last graph made here; that graph, weakly)
+_STREAM = "cobalt_b200.stream"                               # in the metadata of a leaf's node: the stream that it was first seen on
 
 
-def _leaves(*inputs: torch.Tensor):
-    """(the inputs that are leaves, for ``_seen``; whether a captured backward pass must not reach them)"""
-    leaves = [t for t in inputs if t.requires_grad and t.is_leaf]
-    elsewhere = False
-    if leaves and torch.cuda.is_current_stream_capturing():
-        stream = _raw_stream(leaves[0].get_device())
-        for t in leaves:
-            leaf, made, graph = _graphs.get(id(t), (None, stream, None))
-            elsewhere |= made != stream and leaf() is t and graph() is not None
-    return leaves, elsewhere
+def _leaf_nodes(fn):
+    """The nodes of the leaves that ``fn`` takes, directly or behind casts and views (nodes with one input)."""
+    for node, _ in fn.next_functions:
+        while node is not None and type(node).__name__ != "AccumulateGrad":
+            nexts = node.next_functions
+            node = nexts[0][0] if len(nexts) == 1 else None
+        if node is not None:
+            yield node
 
 
-def _refuse_captured(name: str, elsewhere: bool):
-    """A captured backward pass must not reach a leaf through an autograd graph of another stream that still lives: torch would wait for that stream,
-    which invalidates the capture (or ends the process, where nothing catches it).  Said before, as far as these functions made that graph."""
-    if elsewhere and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{name}: a graph of this leaf that was made on another stream is still alive; drop it before the capture, or capture "
-                           "embed_grad / head_loss_and_grad, which need none")
-
-
-def _seen(result: torch.Tensor, leaves) -> torch.Tensor:
-    if leaves:
-        stream, graph = _raw_stream(leaves[0].get_device()), weakref.ref(result.grad_fn)
-        for t in leaves:
-            _graphs[id(t)] = weakref.ref(t), stream, graph
-        if len(_graphs) > 256:
-            for key in [k for k, (leaf, _, g) in list(_graphs.items()) if leaf() is None or g() is None]:
-                _graphs.pop(key, None)
+def _seen(result: torch.Tensor) -> torch.Tensor:
+    """``result`` of an operator's forward pass.  A leaf's node lives as long as any graph holds it, and what is written into it as long as itself."""
+    stream = _raw_stream(result.get_device())
+    for node in _leaf_nodes(result.grad_fn):
+        node.metadata.setdefault(_STREAM, stream)
     return result
+
+
+def _refuse_captured(name: str, fn, index: int):
+    """A captured backward pass must not reach a leaf through a node that was made on another stream: torch would wait for that stream, which
+    invalidates the capture (or ends the process, where nothing catches it).  Said before, as far as these functions saw the graph that holds the node."""
+    if torch.cuda.is_current_stream_capturing():
+        stream = _raw_stream(index)
+        if any(node.metadata.get(_STREAM, stream) != stream for node in _leaf_nodes(fn)):
+            raise RuntimeError(f"{name}: a graph of this leaf that was made on another stream is still alive; drop it before the capture, or capture "
+                               "embed_grad / head_loss_and_grad, which need none")
 
 
 def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0) -> torch.Tensor:
@@ -190,16 +185,16 @@ def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float 
 
 class _Embed(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale, elsewhere):
+    def forward(ctx, ids, table, scale):
         ctx.save_for_backward(ids)
-        ctx.n_rows, ctx.scale, ctx.elsewhere = table.shape[0], scale, elsewhere
+        ctx.n_rows, ctx.scale = table.shape[0], scale
         return _embed(ids, table, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        _refuse_captured("embed", ctx.elsewhere)
-        return None, embed_grad(grad, ctx.saved_tensors[0], ctx.n_rows, ctx.scale), None, None
+        _refuse_captured("embed", ctx, grad.get_device())
+        return None, embed_grad(grad, ctx.saved_tensors[0], ctx.n_rows, ctx.scale), None
 
 
 # ----------------------------------------------------------------------------- head loss
@@ -211,8 +206,7 @@ def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, redu
     ``status`` (int32 ``[1]``, zero) takes the code of a bounded wait that gave up, as ``head_loss_status`` tells it without one."""
     targets = _check_loss(x, weight, targets, reduction, status)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        leaves, elsewhere = _leaves(x, weight)
-        return _seen(_HeadLoss.apply(x, weight, targets, reduction, status, elsewhere), leaves)
+        return _seen(_HeadLoss.apply(x, weight, targets, reduction, status))
     return _head_loss(x, weight, targets, reduction, status, False)[0]
 
 
@@ -303,19 +297,19 @@ def _head_loss_grad(x, weight, targets, stats, grad, reduction, status, want_x, 
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, targets, reduction, status, elsewhere):
+    def forward(ctx, x, weight, targets, reduction, status):
         result, stats = _head_loss(x, weight, targets, reduction, status, True)
         ctx.save_for_backward(x, weight, targets, stats)
-        ctx.reduction, ctx.status, ctx.elsewhere = reduction, status, elsewhere      # (the word is no input of the result)
+        ctx.reduction, ctx.status = reduction, status      # (the word is no input of the result)
         return result
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        _refuse_captured("head_loss", ctx.elsewhere)
+        _refuse_captured("head_loss", ctx, grad.get_device())
         want_x, want_w = ctx.needs_input_grad[:2]
         dx, dw = _head_loss_grad(*ctx.saved_tensors, grad, ctx.reduction, ctx.status, want_x, want_w) if want_x or want_w else (None, None)
-        return dx, dw, None, None, None, None
+        return dx, dw, None, None, None
 
 
 def head_loss_status(device=None) -> int:

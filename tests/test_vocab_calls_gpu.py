@@ -67,3 +67,30 @@ def test_derivatives_that_there_are_none_of_are_refused():
         cb.embed_grad(grad, ids, 9)
     with torch.no_grad():
         assert torch.equal(cb.embed_grad(grad, ids, 9)[ids], grad)
+
+
+def test_a_captured_step_of_a_tied_table_beside_older_graphs():
+    """Refused while a graph of the table made on another stream lives, whatever was made since; then captured, and replayed on new tokens."""
+    V, H, n = 300, 64, 40
+    table = torch.randn(V, H, device="cuda").bfloat16().requires_grad_()
+    ids = torch.randint(0, V, (n,), device="cuda")
+
+    def step():
+        loss = cb.head_loss(cb.embed(ids, table, 2.0), table, ids.roll(-1))
+        return loss, *torch.autograd.grad(loss, table)
+
+    step()
+    kept = cb.embed(ids, table)
+    cb.head_loss(kept.detach(), table, ids)                            # dropped at once
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="still alive"):
+            step()
+    del kept
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = step()
+    for seed in (1, 2):
+        ids.copy_(torch.randint(0, V, (n,), generator=torch.Generator("cuda").manual_seed(seed), device="cuda"))
+        graph.replay()
+        want = step()
+        assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
