@@ -122,6 +122,7 @@ EXPORTS = {
                                           c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cobalt_kv4_status": (c_int, [c_void_p, POINTER(c_uint32)]),
     "cobalt_embed": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_float, c_void_p, c_int64, c_void_p]),
+    "cobalt_embed_watched": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p]),
     "cobalt_embed_grad_scratch_bytes": (c_size_t, [c_int64, c_int]),
     "cobalt_embed_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "cobalt_head_loss_scratch_bytes": (c_size_t, [c_int, c_int, c_int64]),

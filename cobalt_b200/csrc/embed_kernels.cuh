@@ -117,6 +117,7 @@ struct EmbedParams {
     int chunks, threads_per_row;           // packs of a row; a power of two
     float scale;
     bool plain;                            // scale 1: bits are copied
+    uint32_t* status;                      // or null
 };
 
 // `threads_per_row` threads a token
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(EMB_THREADS) embed_kernel(const EmbedParams P)
     if (t >= P.n) return;
     const long long id = P.ids[t];
     const bool in = id >= 0 && id < P.n_rows;
+    if (id >= P.n_rows && lane == 0 && P.status) atomicCAS(P.status, 0u, (uint32_t)DEV_OUTSIDE);
     const T* src = reinterpret_cast<const T*>(P.table) + (in ? id : 0) * P.ld;
     T* dst = reinterpret_cast<T*>(P.out) + t * P.ld_out;
     for (int c = lane; c < P.chunks; c += per) {

@@ -259,9 +259,14 @@ extern "C" {
 
 int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out, int64_t ld_out,
                  void* stream) {
+    return cobalt_embed_watched(ids, n, table, ld, type, n_rows, width, scale, out, ld_out, nullptr, stream);
+}
+
+int cobalt_embed_watched(const int64_t* ids, int64_t n, const void* table, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out, int64_t ld_out,
+                         void* status, void* stream) {
     const int size = type_bytes(type);
     if (!ids || !table || !out || !size || n <= 0 || n_rows <= 0 || width <= 0 || ld < width || ld_out < width) return COBALT_EINVAL;
-    if (((uintptr_t)ids & 7) || (((uintptr_t)table | (uintptr_t)out) & (size - 1))) return COBALT_EINVAL;
+    if (((uintptr_t)ids & 7) || (((uintptr_t)table | (uintptr_t)out) & (size - 1)) || ((uintptr_t)status & 3)) return COBALT_EINVAL;
     if (width > EMBED_MAX_WIDTH) return COBALT_ETOOBIG;
     int sms = 0;
     const int rc = sm_count(&sms);
@@ -276,6 +281,7 @@ int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, i
     while (P.threads_per_row < EMB_THREADS && P.threads_per_row < P.chunks) P.threads_per_row *= 2;
     P.scale = scale;
     P.plain = scale == 1.0f;
+    P.status = (uint32_t*)status;
     const int64_t blocks = ceil_div(n, EMB_THREADS / P.threads_per_row);
     if (blocks > 0x7FFFFFFFll) return COBALT_ETOOBIG;
     cudaStream_t st = (cudaStream_t)stream;

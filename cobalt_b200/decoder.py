@@ -155,6 +155,7 @@ class CobaltDecoder:
             raise ValueError("attention_sinks must not be negative, and needs kv_bits = 4")
         self.sinks = int(attention_sinks)
         self.prompt_status = torch.zeros(1, dtype=torch.int32, device=device)          # non-zero: a bounded wait of a prompt's attention (4-bit cache: of any) gave up
+        self.id_status = torch.zeros(1, dtype=torch.int32, device=device)              # non-zero: an id beyond the vocabulary was looked up (as zeros)
         self.score_status = torch.zeros(1, dtype=torch.int32, device=device)           # the same of the losses of score() and their gradients
         self.kv4 = [KVCache4(self.B, nkv, max_ctx, D, device, status=self.prompt_status) for _ in range(L)] if kv_bits == 4 else None
         self.k_cache = self.v_cache = None
@@ -469,7 +470,19 @@ class CobaltDecoder:
         return self._add_rmsnorm(h, self._settled(delta), self.P["model.norm.weight"], delta_w)[1]
 
     def _embed(self, ids: torch.Tensor) -> torch.Tensor:
-        return embed(ids.long(), self.P["model.embed_tokens.weight"], self.embed_factor)                    # [T, H]
+        return embed(ids.long(), self.P["model.embed_tokens.weight"], self.embed_factor, status=self.id_status)       # [T, H]
+
+    def _check_host_ids(self, ids: torch.Tensor):
+        """Refuse ids beyond the vocabulary where looking at them costs no wait; those on the device are found by the lookup."""
+        vocab = self.P["model.embed_tokens.weight"].shape[0]
+        if not ids.is_cuda and ids.numel() and int(ids.max()) >= vocab:
+            raise ValueError(f"token id {int(ids.max())} is outside the vocabulary of {vocab}")
+
+    def _check_looked_up(self):
+        """Raise if an id beyond the vocabulary was looked up; the next one is told again."""
+        if int(self.id_status.item()):
+            self.id_status.zero_()
+            raise ValueError("a token id is outside the vocabulary: what follows it was computed from zeros")
 
     def _greedy(self, rows: torch.Tensor, out: torch.Tensor):
         """``out [B]`` = the greedy token of every row of logits."""
@@ -482,7 +495,8 @@ class CobaltDecoder:
 
     def device_status(self) -> int:
         """The worst status word of everything this decoder launches (0 = healthy): modules, fused launches, prompt and one-kernel
-        attention, losses, peer all-reduce.  A launch whose bounded wait gave up leaves its output unwritten and its code here."""
+        attention, losses, peer all-reduce.  A launch whose bounded wait gave up leaves its output unwritten and its code here.  8: a token id
+        was beyond the vocabulary (it counts as padding), since the last question."""
         words = [m.device_status() for m in self.lin.values()] + [int(self.prompt_status.item()), status_word(self.att_fused)]
         words += [f.device_status() for fs in (self.qkv, self.gate_up, self.o_f, self.down) for f in fs]
         if self.head_f is not None:
@@ -491,6 +505,10 @@ class CobaltDecoder:
             words.append(self.reducer.device_status())
         if getattr(self, "score_status", None) is not None:
             words.append(int(self.score_status.item()))
+        if getattr(self, "id_status", None) is not None:
+            words.append(int(self.id_status.item()))
+            if words[-1]:
+                self.id_status.zero_()
         return max(words)
 
     def _check_prompt_attention(self):
@@ -581,7 +599,8 @@ class CobaltDecoder:
     def prefill(self, ids: torch.Tensor) -> torch.Tensor:
         """Run the prompt(s), fill the cache(s), return the logits: ``ids [T]`` -> ``[T, V]`` (sequence 0), or
         ``ids [B, T]`` (one prompt per sequence, equal lengths) -> ``[B, T, V]``.  Waits for nothing; ``device_status()`` says
-        whether the launches were healthy."""
+        whether the launches were healthy, and whether an id on the device was beyond the vocabulary (one in host memory is refused)."""
+        self._check_host_ids(ids)
         single = ids.dim() == 1
         logits = self._prefill(ids.to(self.dev).view(1, -1) if single else ids.to(self.dev), False)
         return logits[0] if single else logits
@@ -610,11 +629,12 @@ class CobaltDecoder:
     def score(self, ids: torch.Tensor, reduction: str = "none") -> torch.Tensor:
         """Negative log-likelihood (natural logarithm, fp32) of every token but the first, given those before it: ``ids [T]`` -> ``[T - 1]``,
         ``ids [B, T]`` (one text per sequence) -> ``[B, T - 1]``; with ``reduction`` ``"sum"`` or ``"mean"`` of all of them (``exp`` of the mean is the
-        perplexity).  A next token outside the vocabulary (-1: padding at the end) is not counted.  The caches are filled as by ``prefill``; no
+        perplexity).  A next token of -1 (padding at the end) is not counted; one beyond the vocabulary is refused as by ``prefill``.  The caches are filled as by ``prefill``; no
         logits are formed and none rounded, and the head is the dense one (``compress_head`` leaves its dequantised matrix there).  The blocks have no
         backward pass, but where the dense head requires a gradient, the result has one with respect to it (``head_loss``)."""
         if ids.dim() not in (1, 2) or ids.shape[-1] < 1:
             raise ValueError(f"ids must be [T] or [B, T], got {list(ids.shape)}")
+        self._check_host_ids(ids)
         ids = ids.to(self.dev, torch.int64)
         ids2 = ids.view(1, -1) if ids.dim() == 1 else ids
         with torch.no_grad():
@@ -646,6 +666,8 @@ class CobaltDecoder:
         if single and self.B != 1:
             raise ValueError("a batched decoder needs one prompt per sequence: prompt [B, T]")
         self._check_room(int(prompt.shape[-1]) + n_new)      # the captured step advances the position on the device
+        if teacher is not None:
+            self._check_host_ids(teacher[:max(n_new - 1, 0)])
         logits = self.prefill(prompt)
         last = logits[-1] if single else logits[:, -1]       # [V] or [B, V]
         first = torch.argmax(last.float(), dim=-1, keepdim=single)
@@ -676,6 +698,7 @@ class CobaltDecoder:
                 self.tok.copy_(teacher[i].reshape(-1).to(self.dev))
         toks = torch.cat(toks).cpu() if single else torch.stack(toks).cpu()
         self._check_prompt_attention()                       # the tokens are there: costs no further wait
+        self._check_looked_up()
         return toks, torch.stack(all_logits)
 
 

@@ -54,6 +54,11 @@ def _no_tangent(*tensors: torch.Tensor):
             raise RuntimeError("there are no forward-mode derivatives: a tensor that carries a tangent is not taken")
 
 
+def _check_status(status: Optional[torch.Tensor], t: torch.Tensor):
+    if status is not None and (status.dtype is not torch.int32 or status.shape != (1,) or status.device != t.device):
+        raise ValueError(f"status must be int32 [1] on {t.device}, got {status.dtype} {list(status.shape)} on {status.device}")
+
+
 def _tokens(name: str, t: torch.Tensor, index: int) -> torch.Tensor:
     if t.dtype is not torch.int64:
         raise TypeError(f"{name} must be int64, got {t.dtype}")
@@ -87,10 +92,12 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 # ----------------------------------------------------------------------------- embedding
-def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+          status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``table[ids] * scale``: rows of ``table [n_rows, width]`` (bf16, fp16 or fp32) for int64 ``ids`` of any shape, ``[*ids.shape, width]``.  The
     product is formed in fp32 and rounded once.  An id outside the table (-1: padding) reads zeros.  ``out`` (contiguous, apart from ``ids`` and
-    ``table``) receives the result.  Differentiable in ``table`` (``embed_grad``)."""
+    ``table``) receives the result.  ``status`` (int32 ``[1]``, zero) becomes 8 if an id is beyond the table's end, which no padding is.  Differentiable in
+    ``table`` (``embed_grad``)."""
     index = _gpu("table", table)
     shape, kind = table.shape, _TYPES.get(table.dtype)
     if kind is None:
@@ -99,6 +106,7 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
         raise ValueError(f"table must be [n_rows, width] with width at most {_WIDEST}, got {list(shape)}")
     ids = _tokens("ids", ids, index)
     _no_tangent(table)
+    _check_status(status, table)
     grad = torch.is_grad_enabled() and table.requires_grad
     if out is not None:
         _no_tangent(out)
@@ -109,11 +117,11 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optio
         if _overlap(out, table) or _overlap(out, ids):
             raise ValueError("out must not overlap table or ids")
     if grad:
-        return _seen(_Embed.apply(ids, table, float(scale)))
-    return _embed(ids, table, float(scale), out)
+        return _seen(_Embed.apply(ids, table, float(scale), status))
+    return _embed(ids, table, float(scale), status, out)
 
 
-def _embed(ids, table, scale, out=None):
+def _embed(ids, table, scale, status, out=None):
     n_rows, width = table.shape
     rows, apart = _matrix("table", table, width)
     n, given = ids.numel(), out is not None
@@ -122,7 +130,8 @@ def _embed(ids, table, scale, out=None):
     if n:
         if given:
             torch.autograd.graph.increment_version(out)      # who saved what it held is told, as by an operation of torch
-        _call(table.get_device(), "cobalt_embed", ids.data_ptr(), n, rows.data_ptr(), apart, _TYPES[table.dtype], n_rows, width, scale, out.data_ptr(), width)
+        _call(table.get_device(), "cobalt_embed_watched", ids.data_ptr(), n, rows.data_ptr(), apart, _TYPES[table.dtype], n_rows, width, scale, out.data_ptr(), width,
+              None if status is None else status.data_ptr())
     return out
 
 
@@ -185,16 +194,16 @@ def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float 
 
 class _Embed(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale):
+    def forward(ctx, ids, table, scale, status):
         ctx.save_for_backward(ids)
         ctx.n_rows, ctx.scale = table.shape[0], scale
-        return _embed(ids, table, scale)
+        return _embed(ids, table, scale, status)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         _refuse_captured("embed", ctx, grad.get_device())
-        return None, embed_grad(grad, ctx.saved_tensors[0], ctx.n_rows, ctx.scale), None
+        return None, embed_grad(grad, ctx.saved_tensors[0], ctx.n_rows, ctx.scale), None, None
 
 
 # ----------------------------------------------------------------------------- head loss
@@ -247,8 +256,7 @@ def _check_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, re
     if targets.shape != shape[:-1]:
         raise ValueError(f"targets must be {list(shape[:-1])}, got {list(targets.shape)}")
     _no_tangent(x, weight)
-    if status is not None and (status.dtype is not torch.int32 or status.shape != (1,) or status.get_device() != index):
-        raise ValueError(f"status must be int32 [1] on {x.device}, got {status.dtype} {list(status.shape)} on {status.device}")
+    _check_status(status, x)
     return targets
 
 

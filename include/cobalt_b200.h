@@ -393,6 +393,8 @@ int cobalt_kv4_status(void* stream, uint32_t* status_out);
  * Embedding calls: tables, rows and gradients of one type (COBALT_BF16, COBALT_FP16, COBALT_FP32), row strides ld in elements; any width
  * up to 2^28, any alignment of a value (16-byte rows are faster).  An id outside [0, n_rows) (-1: padding) reads zeros and has no gradient.
  *   cobalt_embed      : out[t] = table[ids[t]] * scale, the product in fp32, rounded once (scale 1: the bits of the table).  out overlaps neither ids nor table.
+ *   cobalt_embed_watched : the same with a status word (device memory, 4-byte aligned, zeroed by the caller; may be NULL): an id of n_rows or more leaves
+ *                       COBALT_STATUS_OUTSIDE there while it is 0 (its row of out is zeros all the same).
  *   cobalt_embed_grad : out [n_rows][width] (contiguous, 16-byte aligned, every value written) = scale * sum of the rows grad[t] with ids[t] = row, in fp32,
  *                       rounded once.  The same inputs give the same bits.  n <= 2^24.
  * Head calls: x [n][hidden] and weight [vocab][hidden] bf16 (hidden a multiple of 8, rows 16-byte aligned), l[t, v] = x[t] . weight[v] in fp32,
@@ -414,8 +416,11 @@ int cobalt_kv4_status(void* stream, uint32_t* status_out);
 #define COBALT_FP32 0
 #define COBALT_FP16 1
 #define COBALT_BF16 2
+#define COBALT_STATUS_OUTSIDE 8
 int cobalt_embed(const int64_t* ids, int64_t n, const void* table, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out,
                  int64_t ld_out, void* stream);
+int cobalt_embed_watched(const int64_t* ids, int64_t n, const void* table, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out,
+                         int64_t ld_out, void* status, void* stream);
 size_t cobalt_embed_grad_scratch_bytes(int64_t n, int width);
 int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t ld, int type, int64_t n_rows, int width, float scale, void* out,
                       void* scratch, size_t scratch_bytes, void* stream);

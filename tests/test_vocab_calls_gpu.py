@@ -3,6 +3,9 @@ import pytest
 import torch
 
 import cobalt_b200 as cb
+from cobalt_b200 import SparseQuantConfig
+from cobalt_b200.decoder import build_random_decoder
+from oracle import model_oracle as MO
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +97,48 @@ def test_a_captured_step_of_a_tied_table_beside_older_graphs():
         graph.replay()
         want = step()
         assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
+
+
+@pytest.mark.parametrize("width", [8, 33, 4096])
+def test_ids_beyond_a_table_are_told(width):
+    """-1 is padding; an id of the table's length or more comes from another vocabulary.  Both read zeros, the latter leaves its code."""
+    table = torch.randn(9, width, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ids = torch.tensor([3, -1, 8, -(2 ** 63)], device="cuda")
+    y = cb.embed(ids, table, 2.0, status=status)
+    assert int(status) == 0 and torch.equal(y[::2], table[[3, 8]] * 2) and not bool(y[1::2].any())
+    for bad in (9, 2 ** 40):
+        ids[1] = bad
+        assert torch.equal(cb.embed(ids, table.requires_grad_(), 2.0, status=status), y) and int(status) == 8
+        status.fill_(5)                                                # the first code stays
+        cb.embed(ids, table.detach(), status=status)
+        assert int(status) == 5
+        status.zero_()
+    for wrong in (torch.zeros(1, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="status"):
+            cb.embed(ids, table.detach(), status=wrong)
+
+
+def test_a_decoder_tells_ids_of_another_vocabulary():
+    """Refused at once in host memory; on the device they count as padding, and are told by device_status() and generate()."""
+    cfg = MO.llama_config(hidden=256, layers=1, heads=4, kv_heads=2, head_dim=64, inter=512, vocab=512)
+    dec = build_random_decoder(cfg, SparseQuantConfig(4, 0.5, 0.5), 64, torch.device("cuda"))
+    ids = torch.arange(20)
+    want, _ = dec.generate(ids.cuda(), 4)
+    ids[3] = 512
+    for call in (dec.prefill, dec.score, lambda i: dec.generate(i, 4)):
+        with pytest.raises(ValueError, match="512"):
+            call(ids)
+    with pytest.raises(ValueError, match="999"):
+        dec.generate(torch.arange(20), 4, teacher=torch.tensor([1, 999, 2, 3]))
+    assert dec.device_status() == 0
+    for call in (dec.prefill, dec.score):
+        call(ids.cuda())
+        assert dec.device_status() == 8 and dec.device_status() == 0
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        dec.generate(ids.cuda(), 4)
+    with pytest.raises(ValueError, match="outside the vocabulary"):    # in the captured step
+        dec.generate(torch.arange(20), 4, teacher=torch.tensor([1, 999, 2, 3], device="cuda"))
+    ids[3] = -1
+    dec.score(ids.cuda())
+    assert torch.equal(dec.generate(torch.arange(20).cuda(), 4)[0], want) and dec.device_status() == 0
