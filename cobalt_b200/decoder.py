@@ -496,19 +496,17 @@ class CobaltDecoder:
     def device_status(self) -> int:
         """The worst status word of everything this decoder launches (0 = healthy): modules, fused launches, prompt and one-kernel
         attention, losses, peer all-reduce.  A launch whose bounded wait gave up leaves its output unwritten and its code here.  8: a token id
-        was beyond the vocabulary (it counts as padding), since the last question."""
+        was beyond the vocabulary (it counts as padding).  Losses and ids: since the last question."""
         words = [m.device_status() for m in self.lin.values()] + [int(self.prompt_status.item()), status_word(self.att_fused)]
         words += [f.device_status() for fs in (self.qkv, self.gate_up, self.o_f, self.down) for f in fs]
         if self.head_f is not None:
             words += [self.head.device_status(), self.head_f.device_status()]
         if self.reducer is not None:
             words.append(self.reducer.device_status())
-        if getattr(self, "score_status", None) is not None:
-            words.append(int(self.score_status.item()))
-        if getattr(self, "id_status", None) is not None:
-            words.append(int(self.id_status.item()))
+        for word in (getattr(self, "score_status", None), getattr(self, "id_status", None)):       # told once: kernels write them while they are 0
+            words.append(0 if word is None else int(word.item()))
             if words[-1]:
-                self.id_status.zero_()
+                word.zero_()
         return max(words)
 
     def _check_prompt_attention(self):

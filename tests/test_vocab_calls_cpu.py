@@ -42,3 +42,13 @@ def test_ids_beyond_the_vocabulary_in_a_decoder():
     with pytest.raises(ValueError, match="outside the vocabulary"):
         CobaltDecoder._check_looked_up(dec)
     assert CobaltDecoder.device_status(dec) == 0
+
+
+def test_a_decoder_tells_a_loss_that_gave_up_once():
+    """The kernels write the word only while it is 0: it is cleared when it was told, so that the next one is told too.  (Set by hand: no wait is made to run out.)"""
+    word = torch.zeros(1, dtype=torch.int32)
+    dec = SimpleNamespace(score_status=word, lin={}, prompt_status=torch.zeros(1, dtype=torch.int32), att_fused=None, qkv=[], gate_up=[], o_f=[], down=[], head_f=None, reducer=None)
+    for code in (2, 4):
+        assert CobaltDecoder.device_status(dec) == 0
+        word.fill_(code)
+        assert CobaltDecoder.device_status(dec) == code and int(word) == 0

@@ -142,3 +142,11 @@ def test_a_decoder_tells_ids_of_another_vocabulary():
     ids[3] = -1
     dec.score(ids.cuda())
     assert torch.equal(dec.generate(torch.arange(20).cuda(), 4)[0], want) and dec.device_status() == 0
+
+
+@pytest.mark.parametrize("n", [20, 300])
+def test_a_healthy_call_leaves_a_status_word_alone(n):
+    x, w = torch.randn(n, 64, device="cuda").bfloat16(), torch.randn(500, 64, device="cuda").bfloat16()
+    status = torch.full((1,), 3, dtype=torch.int32, device="cuda")
+    loss, dx, dw = cb.head_loss_and_grad(x, w, torch.arange(n, device="cuda"), status=status)
+    assert int(status) == 3 and bool(loss.isfinite()) and not bool(dx.isnan().any()) and not bool(dw.isnan().any()) and cb.head_loss_status() == 0
