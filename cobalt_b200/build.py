@@ -17,6 +17,7 @@ SOURCES = ["cobalt_abi.cu", "compress_abi.cu", "kv4_abi.cu", "vocab_abi.cu"]
 HEADERS = ["common.cuh", "decode_core.cuh", "walk_kernels.cuh", "gemv_kernel.cuh", "gemm_kernel.cuh", "glue_kernels.cuh", "staged_input.cuh", "compress_kernels.cuh",
            "prompt_attn.cuh", "kv4_kernels.cuh", "kv4_attend.cuh", "kv4_prompt.cuh", "tcgen05.cuh", "embed_kernels.cuh", "head_loss.cuh", "head_few.cuh",
            os.path.join("..", "..", "include", "cobalt_b200.h")]
+FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr"]
 
 
 def _nvcc() -> str:
@@ -38,9 +39,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compile the CUDA sources into the shared library and return its path."""
     if not force and not needs_build():
         return LIB
-    cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "--expt-relaxed-constexpr", "--threads", "0", "-shared", "-Xcompiler", "-fPIC",
-           "-o", LIB] + [os.path.join(CSRC, s) for s in SOURCES]
+    cmd = [_nvcc(), *FLAGS, "--threads", "0", "-shared", "-Xcompiler", "-fPIC", "-o", LIB] + [os.path.join(CSRC, s) for s in SOURCES]
     if verbose:
         cmd.insert(1, "-Xptxas")
         cmd.insert(2, "-v")
