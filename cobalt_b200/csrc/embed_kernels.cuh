@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(EG_SUM_THREADS) embed_grad_sum_kernel(const Em
 // of long ones eight warps a part of the rows each.
 template <typename T>
 __device__ __forceinline__ void embed_grad_write(const EmbedGradParams& P, uint32_t id, int col, const float (&v)[4]) {
-    T o[4];
+    alignas(16) T o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) set_value(o[e], v[e] * P.scale);
     T* out = reinterpret_cast<T*>(P.out) + (long long)id * P.width + col;
