@@ -77,3 +77,50 @@ def test_the_hidden_gradient_over_a_large_vocabulary(n, V, H):
     slack = long_sum(mean + w[V - 1].double(), V) + w[V - 1].double() / V + want.abs() * 2.0 ** -8
     worst = ((dx.double() - want).abs() - slack).max()
     assert float(worst) <= 0, float(worst)
+
+
+def against_differences(n, which):
+    """(difference of the losses of two ends, the gradient's product with what is between them, bound).  Every value of one operand moves by one step of its
+    grid the way the gradient points, so that nothing cancels; the grid is one of multiples that bf16 holds, middle and ends alike."""
+    V, H = 500, 256
+    g = gen(100 + n)
+    x = (torch.randn(n, H, generator=g, device="cuda") * 64).round().clamp(-200, 200) / 64
+    w = (torch.randn(V, H, generator=g, device="cuda") * 64).round().clamp(-200, 200) / 1024
+    t = torch.randint(0, V, (n,), generator=g, device="cuda")
+    step = 1 / 64 if which == 0 else 1 / 1024
+    x, w = x.bfloat16(), w.bfloat16()
+    _, dx, dw = cb.head_loss_and_grad(x, w, t, "sum")
+    move = torch.sign((dx, dw)[which].double()) * step
+    ends = []
+    for s in (-1, 1):
+        moved = ((x, w)[which].double() + s * move)
+        assert torch.equal(moved.bfloat16().double(), moved)
+        ends.append(cb.head_loss(*((moved.bfloat16(), w) if which == 0 else (x, moved.bfloat16())), t, "none").double().sum())
+    xd, wd = x.double(), w.double()
+    l = xd @ wd.T
+    dl = move @ wd.T if which == 0 else xd @ move.T
+    reach = dl.amax(1) - dl.amin(1)
+    # what a central difference leaves out: a third cumulant of dl, at most sqrt(3) / 18 of its reach cubed, over 6, on either side, and a half more for what it
+    # changes along the way (reaches are far below 1)
+    left_out = (2 / 6 * 3 ** 0.5 / 18 * 1.5 * reach ** 3).sum()
+    # a loss: logits (see test_head_loss_gpu.py), exponentials, and the roundings of fp32
+    off = (2.0 ** -15.9 + 2.0 ** -24) * ((xd.abs() + move.abs() if which == 0 else xd.abs()) @ (wd.abs() if which == 0 else wd.abs() + move.abs()).T).amax(1)
+    noise = 2 * (2 * off + 2.0 ** -21 + 2.0 ** -22 * (2 * l.abs().amax(1) + 10)).sum()
+    # the gradient: d and the result rounded to bf16, 2^-8 each, and what the logits' error does to d (p times twice that, and at most 2 off of a sum over p)
+    p = torch.softmax(l, 1)
+    d = p.clone()
+    d[torch.arange(n), t] -= 1.0
+    err = d.abs() * 2.0 ** -8 + p * (4 * off[:, None] + 2.0 ** -19)
+    grad = (dx, dw)[which].double()
+    slack = (err @ wd.abs() if which == 0 else err.T @ xd.abs()) + grad.abs() * 2.0 ** -8
+    want = 2 * (grad * move).sum()
+    return float(ends[1] - ends[0]), float(want), float(left_out + noise + 2 * (slack * move.abs()).sum()), float(reach.max())
+
+
+@pytest.mark.parametrize("n", [48, 100, 300])
+@pytest.mark.parametrize("which", [0, 1])
+def test_gradients_against_differences_along_themselves(n, which):
+    """A gradient that was zero, negated or off by half would not pass."""
+    got, want, bound, reach = against_differences(n, which)
+    assert abs(got - want) <= bound, (got, want, bound)
+    assert want > 0 and bound < 0.2 * want and reach < 1, (want, bound, reach)
