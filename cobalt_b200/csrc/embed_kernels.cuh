@@ -3,21 +3,23 @@
 // An id outside the table (-1: padding) reads zeros and takes part in no sum; its row of dy is not read.
 //
 // Lookup: bound by memory.  32 bytes a thread, converted in pairs: 8192 rows of 5376 bf16 values in 25.8 us, 176 MB at 6.8 TB/s; a value
-// at a time with 16-byte loads took 50 us.
+// at a time with 16-byte loads took 50 us.  Rows off 16-byte boundaries go a value at a time: 8192 of 5375 bf16 values 98 us, 8192 of 1001 fp32 values 20.5
+// (of 1000: 9.7).
 //
-// The gradient is dense and mostly zeros: what bounds it is writing them.  It goes by sorted tokens, so that every sum has one owner and one
-// order (ascending n) and no atomics on values are needed:
-//   1. up to 6144 tokens (unless one block sorts them while a large table is cleared): every element finds its place among the sorted ones by counting those before it, while all other blocks write zeros to
-//      the whole table;
+// The gradient is dense and mostly zeros: what bounds it is writing them.  It goes by sorted tokens, so that every sum has one owner and one fixed
+// order, which the ids alone decide, and no atomics on values are needed:
+//   1. up to 6144 tokens (unless one block sorts them while a large table is cleared): every element finds its place among the sorted ones by
+//      counting those before it, while all other blocks write zeros to the whole table;
 //      more: blocks of 2048 ids sort (id, n) in registers and shared memory beside the zeros, and
 //   2. every element finds its place among those of 16 blocks by binary searches in the others' sorted ids (the rest of the zeros is written beside
 //      it), then among those of 256 blocks, and so on;
 //   3. tiles of 16 sorted tokens add up the rows of each run of equal ids (fp32) and write the table rows of runs that lie inside the tile;
 //      what a run has in tiles that it leaves or enters goes to scratch, one row at either end of a tile, and the tile where it begins to a list;
-//   4. the runs of the list add those rows in order.
+//   4. the runs of the list add those rows in order, runs of more than 64 of them in eight ranges first.
+// So a row's sum is one of fp32 partial sums over up to 16 tokens each (fewer at either end), in the tokens' order, not one chain through all of them.
 // The zeros of rows that are overwritten in 3 and 4 are written twice: a few per cent of the table, for which sorting costs nothing.
 // Zeros go out as one 32-byte store a thread of blocks that hold 32 KB each: 7.5 TB/s over 2.8 GB, where a grid that strides over the table
-// reaches 6.2 TB/s whatever the width of its stores (bulk copies from shared memory: 6.3).  16384 tokens of a table of 262144 x 5376: 436 us, of which
+// reaches 6.2 TB/s whatever the width of its stores (bulk copies from shared memory: 6.3).  16384 tokens of a table of 262144 x 5376: 438 us, of which
 // 385 write zeros, 60 add up; 2047 of 32000 x 4096: 48 us, 36 of them zeros.
 #pragma once
 #include <cuda_fp16.h>

@@ -1,10 +1,11 @@
 // The products of head_loss.cuh for few tokens (up to 128), which are bound by reading W once: the other way round.  W is the M side, 256 rows (or hidden
 // columns) a stage of 32 KB, and the tokens are the N side, 32 to 128 columns.
 //
-// In the pair kernel's tile the tokens are the 256 rows of A, most of them zeros that take half of every stage: five stages hold 70 KB of W in
-// flight, and 32000 x 4096 took 68 us for one token (3.9 TB/s).  Here six stages hold up to 192 KB: 46 us (5.7 TB/s; the loss with the kernel that joins
-// its statistics 50.4), of which 39 stream W and the rest is the start, the last unit's epilogue and the launch.  With gradients (16 tokens): logits
-// again 43 us, 40 % of them from the L2, dx 52 (one value of d), dw (head_loss.cuh) 55, 27 tiles a pair of 1 us each behind 9 us of first passes through code.
+// In the pair kernel's tile the tokens are the 256 rows of A, most of them zeros that take half of every stage: with the five stages that it had at the time
+// it held 70 KB of W in flight, and 32000 x 4096 took 68 us for one token (3.9 TB/s).  Here six stages hold up to 192 KB: 46 us (5.7 TB/s; the loss with the
+// kernel that joins its statistics 49), of which 39 stream W and the rest is the start, the last unit's epilogue and the launch.  With gradients (16 tokens):
+// logits again 40 us, 40 % of them from the L2, dx 45, dw (head_loss.cuh) 58, 27 tiles a pair of 1 us each behind 9 us of first passes through code; the loss
+// itself then takes 61, as dw's last writes leave the L2 meanwhile.
 //
 //   stats, dlogits   A = W, two blocks of up to 128 of its rows; B = x.  A unit of work is `rows` rows, so many that the units go round the CTAs evenly.
 //                    TMEM lane = row of W, column = token: a warp's statistics are reductions over its lanes, 32 tokens at a time.

@@ -12,7 +12,8 @@
 //   warps 0-7  epilogue: warp w owns TMEM lanes 32 * (w % 4).. (a thread = a row) and columns 128 * (w / 4)..
 //   warp 8     TMA         warp 9     MMA (of the pair's first CTA)        warps 10, 11     none: they fill a warpgroup
 // An epilogue thread holds 128 sums.  The 168 registers that 384 threads have each do not hold them and what belongs to them, and what is
-// spilled goes to the L2 (227 KB of shared memory leave little L1): warps 8-11 hand registers over, 216 to 72.
+// spilled goes to the L2 (227 KB of shared memory leave little L1): warps 8-11 hand registers over, 216 to 72.  48 bytes a thread are spilled all the same (12 words;
+// 148 bytes of stores and 432 of loads in the whole code).
 // Two accumulators of 256 columns: the epilogue of a tile runs under the next one's products.
 //
 // What bounds it: the tensor pipe, and behind it the power limit.  Busy (profiler, one launch): logits 87 % (2047 tokens, 32000 x 4096) to 93 % (2048 tokens,
@@ -26,10 +27,11 @@
 //
 // Precision.  The tensor core cuts every product at its running sum's last bits, always towards zero: over 5376 columns that is 1e-5 of a
 // logit, all in one direction.  So logits are summed in tensor memory over 512 columns at a time, and these sums in fp32 registers; gradients, which are
-// rounded to bf16 in the end, over 4096 tokens or rows of the vocabulary (all at once, dx of 2^19 equal weights is off by 1.2e-3 of its terms, as much as by the rounding).  d is rounded
-// to bf16 (2^-8 of an element at most, at random), because the tensor core multiplies two operands of one type: gradients are off by 1.8e-3 to 1.9e-3 in 2-norm, 1.7e-3
-// of it their own last rounding.  As hi + lo it would be 12 n V H operations instead of 8 here, where the tensor pipe is the bound; up to 64 tokens, where it
-// is not, have both (head_few.cuh).  A factor g that all tokens share
+// rounded to bf16 in the end, over 4096 tokens or rows of the vocabulary at a time (all at once, dx over 2^19 rows was off by 1.3e-3 where sums of 0.8
+// cancel).
+// d is rounded to bf16 (2^-8 of an element at most, at random), because the tensor core multiplies two operands of one type: gradients are off by 1.8e-3 to
+// 1.9e-3 in 2-norm (2.1e-3 for a few hundred tokens of small models), 1.7e-3 of it their own last rounding.  As hi + lo it would be 12 n V H operations
+// instead of 8 here, where the tensor pipe is the bound; up to 64 tokens, where it is not, have both values (head_few.cuh).  A factor g that all tokens share
 // stays out of d and multiplies the sums: -g + a little, rounded in the target's column of every token, would be off by the same for all of
 // them, while -1 + a little is not (2048 columns, 5000 rows, 600 tokens, error in 2-norm with g inside 2.6e-3).
 #pragma once

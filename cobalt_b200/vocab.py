@@ -2,7 +2,9 @@
 
 The recipe compresses the projections and leaves the embedding table and the head alone (the reference's sinq/patch_model.py:49), the largest
 tensors of a model with a large vocabulary.  ``embed`` is what a decoder begins with; ``head_loss`` scores its last hidden states without
-ever holding the logits, and both are differentiable, so the tables can be tuned after compression - a tied table through either end.
+ever holding the logits.  Both are differentiable, so a head can be tuned after compression.  A table's gradient, and that of the hidden states, is the whole
+one only where everything in between has a backward pass: compressed linears have none and end a graph without a word, so that of a model with compressed
+blocks an embedding table (and a tied table's share from that end) would see what comes by the residual stream alone.
 The kernels' contract is in ``include/cobalt_b200.h``.  There is no torch fallback: on a non-CUDA tensor every function raises.
 """
 from __future__ import annotations
@@ -168,7 +170,7 @@ def _refuse_captured(name: str, fn, index: int):
 
 def embed_grad(grad: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``embed`` with respect to its table, dense ``[n_rows, width]`` of ``grad``'s type: ``scale`` times the sum of the rows of
-    ``grad [*ids.shape, width]`` by token, in fp32 and in the tokens' order.  Tokens outside the table are left out.  No second
+    ``grad [*ids.shape, width]`` by token, in fp32 and in an order that ``ids`` alone decide (partial sums over up to 16 tokens each).  Tokens outside the table are left out.  No second
     derivatives: a ``grad`` that requires one is refused."""
     index, kind = _gpu("grad", grad), _TYPES.get(grad.dtype)
     if kind is None:
