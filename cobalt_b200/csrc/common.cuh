@@ -54,7 +54,7 @@ enum : uint32_t {
     DEV_TIMEOUT_STAGE = 5,     // GEMM: compressed tile group never arrived
     DEV_TIMEOUT_PEER = 6,      // peer all-reduce: a peer never published its partial
     DEV_TIMEOUT_ATTN = 7,      // one-kernel decode attention: a chunk of the head group never published its statistics
-    DEV_OUTSIDE = 8,           // embedding lookup: an id beyond the table (no wait: every result is written)
+    DEV_OUTSIDE = COBALT_STATUS_OUTSIDE,       // 8, embedding lookup: an id beyond the table (no wait: every result is written)
 };
 
 // ----------------------------------------------------------------------------- PTX wrappers

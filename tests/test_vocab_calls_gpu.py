@@ -150,3 +150,26 @@ def test_a_healthy_call_leaves_a_status_word_alone(n):
     status = torch.full((1,), 3, dtype=torch.int32, device="cuda")
     loss, dx, dw = cb.head_loss_and_grad(x, w, torch.arange(n, device="cuda"), status=status)
     assert int(status) == 3 and bool(loss.isfinite()) and not bool(dx.isnan().any()) and not bool(dw.isnan().any()) and cb.head_loss_status() == 0
+
+
+@pytest.mark.parametrize("n", [1, 20, 64, 65, 128])
+def test_what_does_not_count_reaches_nothing_of_few_tokens(n):
+    """Rows without a target may hold anything; if none has one, everything is zero; an infinite gradient stays in its token's row of dx."""
+    V, H = 900, 136
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x, w = torch.randn(n, H, generator=g, device="cuda").bfloat16(), (torch.randn(V, H, generator=g, device="cuda") * H ** -0.5).bfloat16()
+    t = torch.randint(0, V, (n,), generator=g, device="cuda")
+    out = torch.arange(n, device="cuda") % 3 == 1
+    t[out] = -1
+    anything = x.clone()
+    anything[out] = float("nan")
+    for reduction in ("mean", "sum", "none"):
+        want, got = cb.head_loss_and_grad(x, w, t, reduction), cb.head_loss_and_grad(anything, w, t, reduction)
+        assert all(torch.equal(a, b) for a, b in zip(want, got)) and not bool(got[1][out].any()) and bool(got[2].isfinite().all())
+        loss, dx, dw = cb.head_loss_and_grad(torch.full_like(x, float("nan")), w, torch.full_like(t, V), reduction)
+        assert not bool(loss.any()) and not bool(dx.any()) and not bool(dw.any())
+    f = torch.ones(n, device="cuda")
+    f[0] = float("inf")
+    _, dx, _ = cb.head_loss_and_grad(x, w, t, "none", f)
+    ones = cb.head_loss_and_grad(x, w, t, "none", torch.ones(n, device="cuda"))[1]
+    assert not bool(dx[0].isfinite().any()) and torch.equal(dx[1:], ones[1:])
