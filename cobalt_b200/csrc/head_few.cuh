@@ -22,9 +22,11 @@ namespace cb {
 
 constexpr int HF_TOKENS = 128;             // at most
 constexpr int HF_EPI_WARPS = 8;
-// Stages of logits that are summed in tensor memory: half of what the pair kernel takes, as the epilogue has the time here.  Error of a loss in 2-norm (16 tokens,
-// 32000 x 4096) with 2, 4, 8 stages 5.2e-7, 6.7e-7, 1.1e-6, where fp32 products summed in fp32 have 8.9e-7; 128 tokens take 62.7, 59.0, 58.0 us.
-constexpr int HF_SUM_STAGES = 4;
+// Stages of logits that are summed in tensor memory: half of what the pair kernel takes, as the epilogue has the time here, and a quarter where it has least to do.
+// Error of a loss (32000 x 4096, in 2-norm; median of 40 draws for one token) with 1, 2, 4 stages: one token 3.6e-8, 3.9e-8, 7.3e-8, where fp32 products summed
+// in fp32 have 3.2e-8; 64 tokens 7.8e-8, 6.9e-8, 9.7e-8, fp32 3.6e-7.  Time: 16 tokens 50.9, 50.7, 50.1 us, 64 tokens of 8000 x 1024 22.3,
+// 20.0, 18.4; 128 tokens with 2, 4, 8 stages 62.7, 59.0, 58.0.
+__host__ __device__ constexpr int hf_sum_stages(int n_pad) { return n_pad <= 32 ? 2 : 4; }
 constexpr int HF_THREADS = HF_EPI_WARPS * 32 + 64;
 constexpr uint32_t HF_A_BYTES = 4 * HL_BOX;
 // Up to 64 tokens d goes out as hi + lo, each rounded to bf16: 2^-16 of d is lost where one value loses 2^-8, as much as the result's own rounding (dw of one
@@ -143,6 +145,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
     const uint32_t full_mask = 0xFFFFFFFFu;
     const uint32_t s0 = (smem_u32(smem) + 1023u) & ~1023u;
     const bool logits = P.kind != HL_DX;
+    const int sum_stages = logits ? hf_sum_stages(P.n_pad) : HL_GRAD_STAGES;
     const int parts = logits ? 1 : PARTS;                  // operands of a stage's tokens' side
     const uint32_t stages = (uint32_t)hf_stages(P.n_pad, parts), stage_bytes = hf_stage_bytes(P.n_pad, parts);
     const uint32_t bars = s0 + stages * stage_bytes;
@@ -209,7 +212,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
             float acc[TOKENS];
 #pragma unroll
             for (int q = 0; q < TOKENS; ++q) acc[q] = 0.0f;
-            for (int k = k0; k < k1; k += logits ? HF_SUM_STAGES : HL_GRAD_STAGES) {
+            for (int k = k0; k < k1; k += sum_stages) {
                 if (healthy) healthy = __all_sync(full_mask, mbar_wait_bounded(hl_acc(bars, buf), ph, P.status, DEV_TIMEOUT_ACC));
                 tc_fence_after();
 #pragma unroll
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(HF_THREADS, 1) head_few_kernel(const __grid_co
         for (int u = blockIdx.x; good && u < P.units; u += gridDim.x) {
             int first, last;
             k_range(u, &first, &last);
-            good = logits ? I.unit<false, 1>(last - first, HF_SUM_STAGES) : I.unit<true, PARTS>(last - first, HL_GRAD_STAGES);
+            good = logits ? I.unit<false, 1>(last - first, sum_stages) : I.unit<true, PARTS>(last - first, sum_stages);
         }
         hl_multiplied<false>(bars, I.uses, stages, P.status);
     }
