@@ -154,6 +154,7 @@ struct EmbedGradParams {
     void* out;                             // [n_rows][width], contiguous, 16-byte aligned
     long long n, ld, n_rows;
     int width, blocks, tiles;              // blocks of ids, tiles of sorted tokens
+    int join_blocks;                       // step 4: blocks along the list
     float scale;
     uint32_t* block_ids;                   // [n] sorted within blocks of EG_BLOCK, or all of them
     uint32_t* block_pos;
@@ -323,12 +324,13 @@ __global__ void __launch_bounds__(EG_PLACE_THREADS) embed_grad_place_kernel(cons
     pos_out[place] = pos[i];
 }
 
-// Step 3.
+// Step 3.  A block takes some columns of a tile; all tiles of one range of columns come first (the grid's second dimension would end at 65535 of them).
 template <typename T, int W>
 __global__ void __launch_bounds__(EG_SUM_THREADS) embed_grad_sum_kernel(const EmbedGradParams P) {
     constexpr int N = PACK<T, W>, AHEAD = 8;               // rows in flight
     __shared__ uint32_t id_s[EG_TILE + 2], pos_s[EG_TILE];
-    const long long t0 = (long long)blockIdx.x * EG_TILE;
+    const int cols = (int)(blockIdx.x / (unsigned)P.tiles), tile = (int)(blockIdx.x - (unsigned)cols * (unsigned)P.tiles);
+    const long long t0 = (long long)tile * EG_TILE;
     const int here = (int)min((long long)EG_TILE, P.n - t0);
     if (threadIdx.x < EG_TILE + 2) {                       // the tile's ids and one on either side
         const int i = threadIdx.x;
@@ -338,12 +340,12 @@ __global__ void __launch_bounds__(EG_SUM_THREADS) embed_grad_sum_kernel(const Em
     }
     __syncthreads();
     const uint32_t tail = id_s[here];
-    if (blockIdx.y == 0 && threadIdx.x == 0 && tail != EG_NONE && id_s[here + 1] == tail && id_s[0] != tail) P.runs[1 + atomicAdd(P.runs, 1u)] = blockIdx.x;
-    const int col = ((int)blockIdx.y * EG_SUM_THREADS + (int)threadIdx.x) * N;
+    if (cols == 0 && threadIdx.x == 0 && tail != EG_NONE && id_s[here + 1] == tail && id_s[0] != tail) P.runs[1 + atomicAdd(P.runs, 1u)] = (uint32_t)tile;
+    const int col = (cols * EG_SUM_THREADS + (int)threadIdx.x) * N;
     if (col >= P.width) return;
     const T* grad = reinterpret_cast<const T*>(P.grad) + col;
     T* out = reinterpret_cast<T*>(P.out) + col;
-    float* part = P.part + (long long)blockIdx.x * 2 * P.width + col;
+    float* part = P.part + (long long)tile * 2 * P.width + col;
     float sum[N] = {};
     bool entered = id_s[0] == id_s[1];                     // the run began in an earlier tile
     for (int i0 = 0; i0 < here; i0 += AHEAD) {
@@ -419,8 +421,8 @@ template <typename T>
 __global__ void __launch_bounds__(EG_JOIN_THREADS) embed_grad_join_kernel(const EmbedGradParams P) {
     __shared__ alignas(16) float sum_s[8][EG_JOIN_COLS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col0 = (int)blockIdx.y * EG_JOIN_COLS, n_runs = (int)P.runs[0];
-    for (int k = blockIdx.x; k < n_runs; k += gridDim.x) {
+    const int cols = (int)(blockIdx.x / (unsigned)P.join_blocks), col0 = cols * EG_JOIN_COLS, n_runs = (int)P.runs[0];
+    for (int k = (int)blockIdx.x - cols * P.join_blocks; k < n_runs; k += P.join_blocks) {
         const long long a = P.runs[1 + k], end = (a + 1) * EG_TILE;
         const uint32_t id = P.ids_sorted[end];
         int rows = 0;                                      // tiles that it enters: those that begin with its id

@@ -329,7 +329,11 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
     if (!count && s.blocks > 1) P.zero_first = (P.out_bytes - std::min<int64_t>(P.out_bytes / 2, (int64_t)std::min(s.blocks, EG_GROUP) * (10 << 20))) / 32 * 32;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t zeros = ceil_div(P.zero_first, EG_ZERO_BYTES);
-    if (zeros > 0x3FFFFFFFll) return COBALT_ETOOBIG;
+    const int words = std::min(words_at_once((uintptr_t)grad | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)width * size)), 4);
+    const int64_t sums = (int64_t)s.tiles * ceil_div(width, EG_SUM_THREADS * (words ? 16 / size : 1));
+    P.join_blocks = std::min(s.tiles, EG_JOIN_GRID);
+    const int64_t joins = (int64_t)P.join_blocks * ceil_div(width, EG_JOIN_COLS);
+    if (zeros > 0x3FFFFFFFll || sums > 0x7FFFFFFFll || joins > 0x7FFFFFFFll) return COBALT_ETOOBIG;
     if (count) {
         const int ranks = (int)ceil_div(n, EG_RANK_IDS);
         embed_grad_rank_kernel<<<(unsigned)(ranks + zeros), EG_RANK_THREADS, 0, st>>>(P, ranks);
@@ -351,18 +355,13 @@ int cobalt_embed_grad(const int64_t* ids, int64_t n, const void* grad, int64_t l
         ids_to = ids_was;
         pos_to = pos_was;
     }
-    const int words = std::min(words_at_once((uintptr_t)grad | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)width * size)), 4);
-    const int per_block = EG_SUM_THREADS * (words ? 16 / size : 1);
-    if (ceil_div(width, per_block) > 65535) return COBALT_ETOOBIG;
-    const dim3 grid((unsigned)s.tiles, (unsigned)ceil_div(width, per_block));
     EMBED_TYPES(type, {
-        if (words) embed_grad_sum_kernel<T, 4><<<grid, EG_SUM_THREADS, 0, st>>>(P);
-        else embed_grad_sum_kernel<T, 0><<<grid, EG_SUM_THREADS, 0, st>>>(P);
+        if (words) embed_grad_sum_kernel<T, 4><<<(unsigned)sums, EG_SUM_THREADS, 0, st>>>(P);
+        else embed_grad_sum_kernel<T, 0><<<(unsigned)sums, EG_SUM_THREADS, 0, st>>>(P);
     });
     if ((rc = launched())) return rc;
     if (s.tiles > 1) {
-        const dim3 join((unsigned)std::min(s.tiles, EG_JOIN_GRID), (unsigned)ceil_div(width, EG_JOIN_COLS));
-        EMBED_TYPES(type, { embed_grad_join_kernel<T><<<join, EG_JOIN_THREADS, 0, st>>>(P); });
+        EMBED_TYPES(type, { embed_grad_join_kernel<T><<<(unsigned)joins, EG_JOIN_THREADS, 0, st>>>(P); });
     }
     return launched();
 }

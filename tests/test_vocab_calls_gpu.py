@@ -173,3 +173,14 @@ def test_what_does_not_count_reaches_nothing_of_few_tokens(n):
     _, dx, _ = cb.head_loss_and_grad(x, w, t, "none", f)
     ones = cb.head_loss_and_grad(x, w, t, "none", torch.ones(n, device="cuda"))[1]
     assert not bool(dx[0].isfinite().any()) and torch.equal(dx[1:], ones[1:])
+
+
+@pytest.mark.parametrize("n,V,H", [(40, 3, 65535 * 128 + 1), (20, 2, 65535 * 1024 + 8)])
+def test_the_gradient_of_very_wide_rows(n, V, H):
+    """More blocks of columns than a grid has in its second dimension, of values one by one and of 16 bytes.  Sums of small whole numbers are exact."""
+    ids = torch.arange(n, device="cuda") % V
+    ids[::7] = 0
+    grad = (torch.arange(H, device="cuda") % 13 - 6).bfloat16()[None] * (torch.arange(n, device="cuda") % 3 - 1).bfloat16()[:, None]
+    got = cb.embed_grad(grad, ids, V)
+    for v in range(V):
+        assert torch.equal(got[v], grad[ids == v].float().sum(0).bfloat16())
